@@ -442,6 +442,98 @@ xspmm_status_t xspmm_dist_gather(xspmm_dist_plan_t plan, const float* C_local, f
     int64_t N, int32_t root, int32_t timeout_ms);
 xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
 
+/* ---------------------------------------------------------------------------------------------
+ * Layer operators: what stands around the sparse product in a graph layer or a feed-forward
+ * block, in training and in serving. They have no counterpart in the reference. Rows are nodes or
+ * tokens and features are contiguous, as in B and C of the product; ld* are row strides in
+ * elements (at least the columns). Pointers need the alignment of their type only; 16-byte
+ * aligned pointers and strides take the wide loads. Asynchronous on the handle's stream; scratch
+ * comes from the device's stream-ordered pool. Results do not depend on timing (no floating-point
+ * atomics). Inputs and outputs must not overlap, except where a line below allows it.
+ *
+ * Layer norm. y = (x - mean) * rstd * weight + bias over each row's cols features, with
+ *   mean = sum(x) / cols, rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps), in fp32.
+ *   Suffixes give the types of x and y: f16f16, bf16bf16, f32f32, and f32f16 / f32bf16, which
+ *   turn the product's fp32 C into the next product's 16-bit operand. weight, bias (cols, fp32;
+ *   NULL: 1 and 0); mean, rstd (rows, fp32) are written where not NULL. y may be x (same type,
+ *   same stride).
+ * Its gradient. dy and dx have y's type (dx is then the B operand of the transposed product);
+ *   mean and rstd come from the forward pass. dweight and dbias (cols, fp32) are overwritten.
+ *   Each of dx, dweight, dbias may be NULL. rows = 0 writes zeros to dweight and dbias. dx may be
+ *   dy (same stride).
+ *
+ * Dropout. y[i] = residual[i] + (keep(i) ? x[i] / (1 - p) : 0) for n contiguous elements (residual
+ *   NULL: 0). keep(i): word i mod 4 of the Philox4x32-10 block of counter offset + i / 4 (64 bits)
+ *   and key seed is at least p * 2^32. The mask is not stored: the gradient is the same call on dy
+ *   with the same p, seed and offset and no residual. A call uses ceil(n / 4) counters: the next
+ *   one takes offset + ceil(n / 4). y may be x or residual. p in [0, 1]; p = 1 drops everything.
+ *
+ * Gated feed-forward block. y = act(x w_gate^T) * (x w_up^T), x rows x K, both weights F x K, y
+ *   rows x F; the sums are fp32. gate and up (rows x F, contiguous, or NULL) receive the two
+ *   projections, which the gradient needs. act: silu, gelu (with erf), relu or sigmoid. 16-bit
+ *   types only: fp32 rows go through a layer norm with a 16-bit y.
+ * Its gradient. dup = dy * act(gate), dgate = dy * up * act'(gate) (rounded to the 16-bit type),
+ *   dx = dgate w_gate + dup w_up, dw_gate = dgate^T x, dw_up = dup^T x (F x K, contiguous,
+ *   overwritten; zeros when rows = 0). dx may be NULL, and dw_gate and dw_up may both be.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum xspmm_activation {
+    XSPMM_ACT_SILU = 0,
+    XSPMM_ACT_GELU = 1,
+    XSPMM_ACT_RELU = 2,
+    XSPMM_ACT_SIGMOID = 3
+} xspmm_activation_t;
+
+xspmm_status_t xspmm_layer_norm_f16f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, const float* weight, const float* bias, float eps, void* y,
+    int64_t ldy, float* mean, float* rstd);
+xspmm_status_t xspmm_layer_norm_bf16bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, const float* weight, const float* bias, float eps, void* y,
+    int64_t ldy, float* mean, float* rstd);
+xspmm_status_t xspmm_layer_norm_f32f32(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, const float* weight, const float* bias, float eps, void* y,
+    int64_t ldy, float* mean, float* rstd);
+xspmm_status_t xspmm_layer_norm_f32f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, const float* weight, const float* bias, float eps, void* y,
+    int64_t ldy, float* mean, float* rstd);
+xspmm_status_t xspmm_layer_norm_f32bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, const float* weight, const float* bias, float eps, void* y,
+    int64_t ldy, float* mean, float* rstd);
+xspmm_status_t xspmm_layer_norm_backward_f16f16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+    const float* mean, const float* rstd, void* dx, int64_t lddx, float* dweight, float* dbias);
+xspmm_status_t xspmm_layer_norm_backward_bf16bf16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+    const float* mean, const float* rstd, void* dx, int64_t lddx, float* dweight, float* dbias);
+xspmm_status_t xspmm_layer_norm_backward_f32f32(xspmm_handle_t h, int64_t rows,
+    int64_t cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+    const float* mean, const float* rstd, void* dx, int64_t lddx, float* dweight, float* dbias);
+xspmm_status_t xspmm_layer_norm_backward_f32f16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+    const float* mean, const float* rstd, void* dx, int64_t lddx, float* dweight, float* dbias);
+xspmm_status_t xspmm_layer_norm_backward_f32bf16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+    const float* mean, const float* rstd, void* dx, int64_t lddx, float* dweight, float* dbias);
+xspmm_status_t xspmm_dropout_f16(xspmm_handle_t h, int64_t n, const void* x,
+    const void* residual, double p, uint64_t seed, uint64_t offset, void* y);
+xspmm_status_t xspmm_dropout_bf16(xspmm_handle_t h, int64_t n, const void* x,
+    const void* residual, double p, uint64_t seed, uint64_t offset, void* y);
+xspmm_status_t xspmm_dropout_f32(xspmm_handle_t h, int64_t n, const void* x,
+    const void* residual, double p, uint64_t seed, uint64_t offset, void* y);
+xspmm_status_t xspmm_gated_ffn_f16(xspmm_handle_t h, int64_t rows, int64_t K, int64_t F,
+    int activation, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
+    const void* w_up, int64_t ldwu, void* y, int64_t ldy, void* gate, void* up);
+xspmm_status_t xspmm_gated_ffn_bf16(xspmm_handle_t h, int64_t rows, int64_t K, int64_t F,
+    int activation, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
+    const void* w_up, int64_t ldwu, void* y, int64_t ldy, void* gate, void* up);
+xspmm_status_t xspmm_gated_ffn_backward_f16(xspmm_handle_t h, int64_t rows, int64_t K,
+    int64_t F, int activation, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+    const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu, const void* gate,
+    const void* up, void* dx, int64_t lddx, void* dw_gate, void* dw_up);
+xspmm_status_t xspmm_gated_ffn_backward_bf16(xspmm_handle_t h, int64_t rows, int64_t K,
+    int64_t F, int activation, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+    const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu, const void* gate,
+    const void* up, void* dx, int64_t lddx, void* dw_gate, void* dw_up);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

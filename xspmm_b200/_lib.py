@@ -51,6 +51,7 @@ class PlanInfo(ctypes.Structure):
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
+_U64 = ctypes.c_uint64
 _F = ctypes.c_float
 
 _lib = None
@@ -128,6 +129,20 @@ def lib():
     L.xspmm_dist_plan_execute.argtypes = [_P, _P, _P, _I64, _I32, _I32]
     L.xspmm_dist_gather.argtypes = [_P, _P, _P, _I64, _I32, _I32]
     L.xspmm_dist_plan_destroy.argtypes = [_P]
+    for t in ("f16f16", "bf16bf16", "f32f32", "f32f16", "f32bf16"):
+        getattr(L, f"xspmm_layer_norm_{t}").argtypes = [_P, _I64, _I64, _P, _I64, _P, _P, _F, _P,
+                                                        _I64, _P, _P]
+        getattr(L, f"xspmm_layer_norm_backward_{t}").argtypes = [
+            _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P]
+    for t in ("f16", "bf16", "f32"):
+        getattr(L, f"xspmm_dropout_{t}").argtypes = [_P, _I64, _P, _P, ctypes.c_double, _U64, _U64,
+                                                     _P]
+    for t in ("f16", "bf16"):
+        getattr(L, f"xspmm_gated_ffn_{t}").argtypes = [
+            _P, _I64, _I64, _I64, ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P]
+        getattr(L, f"xspmm_gated_ffn_backward_{t}").argtypes = [
+            _P, _I64, _I64, _I64, ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P,
+            _I64, _P, _P]
     _lib = L
     return L
 
