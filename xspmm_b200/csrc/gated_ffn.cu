@@ -4,130 +4,129 @@
 // du = dy * act(g), dg = dy * u * act'(g), dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x.
 // Sums are held in fp32; dg and du are rounded to the operands' 16-bit type before the products,
 // as any 16-bit matrix product's operand is.
-#include "layers.cuh"
+//
+// The products run on the tensor cores (gated_tc.cuh). TMA needs 16-byte rows: an operand whose
+// address or row stride is not is first copied to scratch with a stride that is.
+#include "gated_tc.cuh"
 
 namespace xspmm_b200 {
 namespace {
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+using namespace gated;
 
-template <Activation ACT>
-__device__ __forceinline__ float act_value(float v) {
-    if constexpr (ACT == Activation::Silu) return v * sigmoid(v);
-    else if constexpr (ACT == Activation::Gelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
-    else return sigmoid(v);
-}
-template <Activation ACT>
-__device__ __forceinline__ float act_slope(float v) {
-    if constexpr (ACT == Activation::Silu) {
-        const float s = sigmoid(v);
-        return s * (1.0f + v * (1.0f - s));
-    } else if constexpr (ACT == Activation::Gelu) {
-        return 0.5f * (1.0f + erff(v * 0.70710678118654752f)) +
-               v * __expf(-0.5f * v * v) * 0.39894228040143268f;
-    } else if constexpr (ACT == Activation::Relu) {
-        return v > 0.0f ? 1.0f : 0.0f;
-    } else {
-        const float s = sigmoid(v);
-        return s * (1.0f - s);
-    }
-}
-
-// out[i, j] = sum over the segments s and k of a_s[i, k] * b_s[k, j], any element strides.
-template <typename T>
-struct Operand {
-    const T* p;
-    int64_t si, sk;  // strides of the output index and of the summed index
-};
-constexpr int PT = 64, PK = 16;  // output tile, summed slice; 256 threads of 4 x 4 outputs
-
-template <typename T>
-__device__ void product_tile(const Operand<T>& a, const Operand<T>& b, int64_t M, int64_t N,
-                             int64_t K, int64_t i0, int64_t j0, float (&acc)[4][4]) {
-    __shared__ float sa[PK][PT + 1], sb[PK][PT + 1];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (int64_t k0 = 0; k0 < K; k0 += PK) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < PT * PK; e += 256) {
-            const int i = e / PK, k = e % PK;
-            sa[k][i] = i0 + i < M && k0 + k < K ? to_float(a.p[(i0 + i) * a.si + (k0 + k) * a.sk]) : 0.0f;
-            sb[k][i] = j0 + i < N && k0 + k < K ? to_float(b.p[(j0 + i) * b.si + (k0 + k) * b.sk]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] += sa[k][ty + 16 * i] * sb[k][tx + 16 * j];
-    }
-}
-
-template <typename T>
+// dg and du with row stride ldp. V elements a thread; dy, gate and up allow V-wide loads.
+template <typename T, Activation ACT, int V>
 __global__ void __launch_bounds__(256)
-product_kernel(Operand<T> a0, Operand<T> b0, Operand<T> a1, Operand<T> b1, int64_t M, int64_t N,
-               int64_t K, T* out, int64_t ldo) {
-    const int64_t nt = (N + PT - 1) / PT;
-    const int64_t i0 = blockIdx.x / nt * PT, j0 = blockIdx.x % nt * PT;
-    float acc[4][4] = {};
-    product_tile(a0, b0, M, N, K, i0, j0, acc);
-    if (a1.p) product_tile(a1, b1, M, N, K, i0, j0, acc);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = i0 + ty + 16 * i, c = j0 + tx + 16 * j;
-            if (r < M && c < N) out[r * ldo + c] = from_float<T>(acc[i][j]);
-        }
-}
-
-template <typename T, Activation ACT>
-__global__ void __launch_bounds__(256)
-gated_kernel(GatedArgs<T> p, T* y, int64_t ldy, T* gate, T* up) {
-    const int64_t nt = (p.F + PT - 1) / PT;
-    const int64_t i0 = blockIdx.x / nt * PT, j0 = blockIdx.x % nt * PT;
-    float g[4][4] = {}, u[4][4] = {};
-    const Operand<T> x{p.x, p.ldx, 1};
-    product_tile(x, Operand<T>{p.wg, p.ldwg, 1}, p.rows, p.F, p.K, i0, j0, g);
-    product_tile(x, Operand<T>{p.wu, p.ldwu, 1}, p.rows, p.F, p.K, i0, j0, u);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = i0 + ty + 16 * i, c = j0 + tx + 16 * j;
-            if (r >= p.rows || c >= p.F) continue;
-            y[r * ldy + c] = from_float<T>(act_value<ACT>(g[i][j]) * u[i][j]);
-            if (gate) gate[r * p.F + c] = from_float<T>(g[i][j]);
-            if (up) up[r * p.F + c] = from_float<T>(u[i][j]);
-        }
-}
-
-// dg and du, rows x F contiguous.
-template <typename T, Activation ACT>
-__global__ void __launch_bounds__(256)
-gated_slopes_kernel(int64_t rows, int64_t F, const T* dy, int64_t lddy, const T* gate, const T* up,
-                    T* dg, T* du) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * F;
+gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t lddy,
+                    const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ dg,
+                    T* __restrict__ du, int64_t ldp) {
+    const int64_t per = F / V;  // V divides F
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per;
          i += (int64_t)gridDim.x * 256) {
-        const float d = to_float(dy[i / F * lddy + i % F]), g = to_float(gate[i]);
-        du[i] = from_float<T>(d * act_value<ACT>(g));
-        dg[i] = from_float<T>(d * to_float(up[i]) * act_slope<ACT>(g));
+        const int64_t r = i / per, c = (i - r * per) * V;
+        float d[V], g[V], u[V], a[V], b[V];
+        load_pack<T, V>(dy + r * lddy + c, d);
+        load_pack<T, V>(gate + r * F + c, g);
+        load_pack<T, V>(up + r * F + c, u);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            a[e] = d[e] * u[e] * act_slope<ACT>(g[e]);
+            b[e] = d[e] * act_value<ACT>(g[e]);
+        }
+        store_pack<T, V>(dg + r * ldp + c, a);
+        store_pack<T, V>(du + r * ldp + c, b);
     }
 }
 
-template <typename F>
-void with_activation(Activation a, F&& f) {
-    switch (a) {
-        case Activation::Silu: return f(std::integral_constant<Activation, Activation::Silu>{});
-        case Activation::Gelu: return f(std::integral_constant<Activation, Activation::Gelu>{});
-        case Activation::Relu: return f(std::integral_constant<Activation, Activation::Relu>{});
-        case Activation::Sigmoid: return f(std::integral_constant<Activation, Activation::Sigmoid>{});
+// Rows of `cols` elements from stride ld to stride ldp.
+template <typename T>
+__global__ void __launch_bounds__(256)
+restride_kernel(int64_t rows, int64_t cols, const T* __restrict__ src, int64_t ld,
+                T* __restrict__ dst, int64_t ldp) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int64_t c = threadIdx.x; c < cols; c += 256) dst[r * ldp + c] = src[r * ld + c];
+}
+
+int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+
+// A matrix as TMA can read it: the caller's, or a copy in scratch.
+template <typename T>
+struct Rows {
+    const T* p;
+    int64_t ld;
+    DevBuf<T> copy;
+    Rows(Handle& h, const T* src, int64_t lds, int64_t rows, int64_t cols) : p(src), ld(lds) {
+        if (rows <= 1) ld = round8(cols);  // the stride of a single row is never taken
+        if (tma_ok(p, ld) || rows == 0 || cols == 0) return;
+        ld = round8(cols);
+        copy = DevBuf<T>((size_t)(rows * ld), h.stream);
+        const unsigned grid = (unsigned)std::min(rows, (int64_t)sm_count(h.device) * 8);
+        restride_kernel<T><<<grid, 256, 0, h.stream>>>(rows, cols, src, lds, copy.get(), ld);
+        after_launch(h, "gated_restride");
+        p = copy.get();
+    }
+};
+
+template <typename T>
+CUtensorMap map_of(const T* p, int64_t ld, int64_t rows, int64_t cols, int box_rows) {
+    return make_map_2d(p, (uint64_t)cols, (uint64_t)rows, (uint64_t)ld * 2, 64, (uint32_t)box_rows,
+                       CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Forward tile width. A tile costs its slices (the slower of the MMAs, 4 clocks per output column, and
+// the loads at about 48 bytes a clock) plus a fill and drain; tiles run in waves over the SMs.
+int forward_width(int sms, int64_t rows, int64_t K, int64_t F) {
+    const int64_t mt = ceil_div(rows, TM), steps = ceil_div(K, TK);
+    const double a_bytes = 128.0 * (double)std::min<int64_t>(rows, TM);
+    int best = 8;
+    double least = 0.0;
+    for (int bf = 8; bf <= 128; bf += 8) {
+        const int64_t waves = ceil_div(mt * ceil_div(F, bf), sms);
+        const double step = std::max(4.0 * std::max(bf, 32), (a_bytes + 256.0 * bf) / 48.0);
+        const double cost = (double)waves * ((double)steps * step + 1500.0 + 12.0 * bf);
+        if (bf == 8 || cost <= least) {
+            least = cost;
+            best = bf;
+        }
+        if (bf >= F) break;
+    }
+    return best;
+}
+
+// Tile width and number of slices of a gradient's product, by the same model: MMAs 2 clocks per column
+// and slice; a split sum adds a second kernel and its partials' trip through L2.
+void gradient_tiling(int sms, int64_t mt, int64_t N, int64_t steps, int* bn, int* splits) {
+    double least = -1.0;
+    const int widest = (int)std::min<int64_t>(256, ceil_div(N, 16) * 16);
+    for (int w = 64; w <= 256; w += 64) {
+        const int cand = std::min(w, widest);
+        const int64_t tiles = mt * ceil_div(N, cand);
+        for (int64_t sp = 1; sp <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, sms / tiles)); ++sp) {
+            const int64_t waves = ceil_div(tiles * sp, sms);
+            const double step = std::max(2.0 * std::max(cand, 64), (16384.0 + 128.0 * cand) / 48.0);
+            double cost = (double)waves * ((double)ceil_div(steps, sp) * step + 1500.0 + 6.0 * cand);
+            if (sp > 1) cost += 5000.0 + (double)(tiles * sp) * 128.0 * cand * 8.0 / 3000.0;
+            if (least < 0.0 || cost < least) {
+                least = cost;
+                *bn = cand;
+                *splits = (int)sp;
+            }
+        }
+        if (w >= widest) break;
     }
 }
 
-unsigned tile_grid(int64_t M, int64_t N) {
-    const int64_t t = ceil_div(M, PT) * ceil_div(N, PT);
-    XS_REQUIRE(t < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
-    return (unsigned)t;
+template <typename T>
+void zero_rows(Handle& h, T* p, int64_t ld, int64_t rows, int64_t cols) {
+    if (p && rows > 0 && cols > 0)
+        XS_CHECK_CUDA(cudaMemset2DAsync(p, ld * sizeof(T), 0, cols * sizeof(T), rows, h.stream));
+}
+
+template <typename T>
+void check_sizes(const GatedArgs<T>& a) {
+    const int64_t most = (int64_t(1) << 31) - 512;  // TMA coordinates are 32 bits
+    XS_REQUIRE(a.rows < most && a.K < most && a.F < most, XSPMM_STATUS_UNSUPPORTED,
+               "a dimension of the gated feed-forward block passes 2^31");
 }
 
 }  // namespace
@@ -135,43 +134,102 @@ unsigned tile_grid(int64_t M, int64_t N) {
 template <typename T>
 void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* up) {
     if (a.rows == 0 || a.F == 0) return;
-    with_activation(a.act, [&](auto act) {
-        gated_kernel<T, decltype(act)::value>
-            <<<tile_grid(a.rows, a.F), 256, 0, h.stream>>>(a, y, ldy, gate, up);
-    });
-    after_launch(h, "gated_ffn");
+    check_sizes(a);
+    if (a.K == 0) {  // sums of no terms
+        zero_rows(h, y, ldy, a.rows, a.F);
+        zero_rows(h, gate, a.F, a.rows, a.F);
+        zero_rows(h, up, a.F, a.rows, a.F);
+        return;
+    }
+    const Rows<T> x(h, a.x, a.ldx, a.rows, a.K);
+    const Rows<T> wg(h, a.wg, a.ldwg, a.F, a.K), wu(h, a.wu, a.ldwu, a.F, a.K);
+    TileArgs t = {};
+    t.M = a.rows;
+    t.N = a.F;
+    t.bn = forward_width(sm_count(h.device), a.rows, a.K, a.F);
+    t.mt = (int)ceil_div(a.rows, TM);
+    t.nt = (int)ceil_div(a.F, t.bn);
+    t.splits = 1;
+    t.ksteps = t.kseg = (int)ceil_div(a.K, TK);
+    t.a[0] = map_of(x.p, x.ld, a.rows, a.K, TM);
+    t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, t.bn);
+    t.b[1] = map_of(wu.p, wu.ld, a.F, a.K, t.bn);
+    t.act = a.act;
+    T* outs[3] = {y, gate, up};
+    for (int i = 0; i < 3; ++i) {
+        t.out[i] = outs[i];
+        t.ld[i] = i == 0 ? ldy : a.F;
+        t.vec[i] = store16_ok(outs[i], t.ld[i]);
+    }
+    launch_product<T, Product::Forward>(h, t);
 }
 
 template <typename T>
 void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t lddy, const T* gate,
                         const T* up, T* dx, int64_t lddx, T* dwg, T* dwu) {
-    const int64_t n = a.rows * a.F;
-    DevBuf<T> d(std::max<int64_t>(2 * n, 1), h.stream);
-    T *dg = d.get(), *du = d.get() + n;
-    if (n > 0) {
-        const unsigned grid = (unsigned)std::min(ceil_div(n, 256), (int64_t)sm_count(h.device) * 8);
+    check_sizes(a);
+    const int sms = sm_count(h.device);
+    if (a.rows == 0 || a.F == 0 || a.K == 0) {
+        zero_rows(h, dx, lddx, a.rows, a.K);
+        zero_rows(h, dwg, a.K, a.F, a.K);
+        zero_rows(h, dwu, a.K, a.F, a.K);
+        return;
+    }
+    if (!dx && !dwg) return;
+    const int64_t ldp = round8(a.F);
+    DevBuf<T> d((size_t)(2 * a.rows * ldp), h.stream);
+    T *dg = d.get(), *du = d.get() + a.rows * ldp;
+    {
+        const bool wide = a.F % 8 == 0 && lddy % 8 == 0 && aligned_to(dy, 16) && aligned_to(gate, 16) &&
+                          aligned_to(up, 16);
+        const int64_t n = a.rows * a.F / (wide ? 8 : 1);
+        const unsigned grid = (unsigned)std::min(ceil_div(n, 256), (int64_t)sms * 8);
         with_activation(a.act, [&](auto act) {
-            gated_slopes_kernel<T, decltype(act)::value>
-                <<<grid, 256, 0, h.stream>>>(a.rows, a.F, dy, lddy, gate, up, dg, du);
+            constexpr Activation A = decltype(act)::value;
+            auto kern = wide ? gated_slopes_kernel<T, A, 8> : gated_slopes_kernel<T, A, 1>;
+            kern<<<grid, 256, 0, h.stream>>>(a.rows, a.F, dy, lddy, gate, up, dg, du, ldp);
         });
         after_launch(h, "gated_slopes");
     }
-    const Operand<T> none{nullptr, 0, 0};
-    if (dx && a.rows > 0) {
-        product_kernel<T><<<tile_grid(a.rows, a.K), 256, 0, h.stream>>>(
-            Operand<T>{dg, a.F, 1}, Operand<T>{a.wg, 1, a.ldwg}, Operand<T>{du, a.F, 1},
-            Operand<T>{a.wu, 1, a.ldwu}, a.rows, a.K, a.F, dx, lddx);
-        after_launch(h, "gated_dx");
+    if (dx) {
+        const Rows<T> wg(h, a.wg, a.ldwg, a.F, a.K), wu(h, a.wu, a.ldwu, a.F, a.K);
+        TileArgs t = {};
+        t.M = a.rows;
+        t.N = a.K;
+        t.mt = (int)ceil_div(a.rows, TM);
+        t.kseg = (int)ceil_div(a.F, TK);
+        t.ksteps = 2 * t.kseg;
+        gradient_tiling(sms, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
+        t.nt = (int)ceil_div(a.K, t.bn);
+        t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TM);
+        t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TM);
+        t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, TK);
+        t.b[1] = map_of(wu.p, wu.ld, a.F, a.K, TK);
+        t.out[0] = dx;
+        t.ld[0] = lddx;
+        t.vec[0] = store16_ok(dx, lddx);
+        launch_product<T, Product::Dx>(h, t);
     }
-    if (dwg && a.F > 0) {
-        const T* src[2] = {dg, du};
-        T* dst[2] = {dwg, dwu};
+    if (dwg) {
+        const Rows<T> x(h, a.x, a.ldx, a.rows, a.K);
+        TileArgs t = {};
+        t.M = a.F;
+        t.N = a.K;
+        t.mt_one = (int)ceil_div(a.F, TM);
+        t.mt = 2 * t.mt_one;
+        t.kseg = t.ksteps = (int)ceil_div(a.rows, TK);
+        gradient_tiling(sms, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
+        t.nt = (int)ceil_div(a.K, t.bn);
+        t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TK);
+        t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TK);
+        t.b[0] = map_of(x.p, x.ld, a.rows, a.K, TK);
+        t.out[0] = dwg;
+        t.out[1] = dwu;
         for (int i = 0; i < 2; ++i) {
-            product_kernel<T><<<tile_grid(a.F, a.K), 256, 0, h.stream>>>(
-                Operand<T>{src[i], 1, a.F}, Operand<T>{a.x, 1, a.ldx}, none, none, a.F, a.K, a.rows,
-                dst[i], a.K);
-            after_launch(h, "gated_dw");
+            t.ld[i] = a.K;
+            t.vec[i] = store16_ok(t.out[i], a.K);
         }
+        launch_product<T, Product::Dw>(h, t);
     }
 }
 

@@ -1,0 +1,442 @@
+// gated_tc.cuh -- the matrix products of the gated feed-forward block on the 5th-generation tensor
+// cores: one persistent kernel, three products.
+//
+//   Forward   y[m, f]  = act(sum_k x[m,k] wg[f,k]) * sum_k x[m,k] wu[f,k]
+//   Dx        dx[m, k] = sum_f dg[m,f] wg[f,k] + du[m,f] wu[f,k]
+//   Dw        dw[f, k] = sum_m d[m,f] x[m,k], d = dg, then du
+//
+// An output tile is 128 rows by up to 256 accumulator columns; a summed slice is 64 deep. Operands
+// come by TMA in the SWIZZLE_128B layout, in whichever order memory has them: K-major where the
+// summed index is contiguous (x, weights of Forward; dg, du of Dx), MN-major where the output index
+// is (the others), so nothing is transposed. Forward puts bf rows of wg and the same bf rows of wu
+// one after the other in shared memory: one MMA of N = 2 bf fills both projections of bf outputs,
+// x is read once for both, and the epilogue finds g and u of an output bf columns apart in TMEM.
+// Edges need no code: TMA fills what lies outside with zeros.
+//
+// Roles (384 threads, one CTA per SM): warp 0 issues the MMAs (one lane), warp 1 the loads (one
+// lane), warp 2 allocates TMEM, warps 4..11 are the epilogue. TMEM holds two accumulators used in
+// turn, so a tile's epilogue runs under the next tile's products. The epilogue converts 32 columns
+// at a time and turns them through a warp's own piece of shared memory, so global stores are
+// 16 bytes a lane and 64 contiguous bytes a row. Every wait is bounded; a timeout sets the error
+// flag, and TMEM is freed only after the MMAs that were issued have completed.
+//
+// Where the output has too few tiles for the GPU, the sum is split: each slice's fp32 partial goes
+// to scratch and a second kernel adds them in slice order (the same order every time).
+#pragma once
+
+#include "layers.cuh"
+#include "tcgen05.cuh"
+
+namespace xspmm_b200 {
+namespace gated {
+
+enum class Product { Forward, Dx, Dw };
+
+constexpr int TM = 128;                 // tile rows (MMA M)
+constexpr int TK = 64;                  // summed slice per stage: 128 bytes of 16-bit elements
+constexpr int ACC_COLS = 256;           // TMEM columns per accumulator
+constexpr int FIRST_EPI = 4, EPI_WARPS = 8;
+constexpr int THREADS = 32 * (FIRST_EPI + EPI_WARPS);
+constexpr int A_BYTES = TM * 128;       // one stage of A
+constexpr int CHUNK = TK * 128;         // MN-major: 64 columns by TK summed rows
+constexpr int TURN_LD = 80;             // epilogue staging: 64 bytes of a row, padded off the banks
+constexpr int TURN_BYTES = EPI_WARPS * 32 * TURN_LD;
+constexpr int MAX_STAGES = 8;
+constexpr int SMEM_MAX = 232448 - 1024 - 512;  // opt-in limit less alignment and barriers
+
+struct TileArgs {
+    CUtensorMap a[2], b[2];
+    int64_t M, N;       // output rows and columns (Dw: rows of one weight)
+    int mt, nt, splits;
+    int mt_one;         // Dw: tiles of the first weight, the others belong to the second
+    int bn;             // output columns per tile
+    int acc_n;          // MMA N: 2 bn (Forward) or bn rounded up to 16
+    int ksteps, kseg;   // summed slices over all segments, and per segment
+    int stages, b_bytes;
+    uint32_t idesc;
+    Activation act;
+    void* out[3];       // Forward: y, gate, up; Dx: dx; Dw: dwg, dwu
+    int64_t ld[3];
+    int vec[3];         // 16-byte stores allowed
+    float4* partial;    // splits > 1: [split][tile][column / 4][row]
+    unsigned* err;
+};
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+
+template <Activation ACT>
+__device__ __forceinline__ float act_value(float v) {
+    if constexpr (ACT == Activation::Silu) return __fdividef(v, 1.0f + __expf(-v));
+    else if constexpr (ACT == Activation::Gelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
+    else return sigmoid(v);
+}
+template <Activation ACT>
+__device__ __forceinline__ float act_slope(float v) {
+    if constexpr (ACT == Activation::Silu) {
+        const float s = sigmoid(v);
+        return s * (1.0f + v * (1.0f - s));
+    } else if constexpr (ACT == Activation::Gelu) {
+        return 0.5f * (1.0f + erff(v * 0.70710678118654752f)) +
+               v * __expf(-0.5f * v * v) * 0.39894228040143268f;
+    } else if constexpr (ACT == Activation::Relu) {
+        return v > 0.0f ? 1.0f : 0.0f;
+    } else {
+        const float s = sigmoid(v);
+        return s * (1.0f - s);
+    }
+}
+
+template <typename F>
+__host__ __device__ __forceinline__ void with_activation(Activation a, F&& f) {
+    switch (a) {
+        case Activation::Silu: return f(std::integral_constant<Activation, Activation::Silu>{});
+        case Activation::Gelu: return f(std::integral_constant<Activation, Activation::Gelu>{});
+        case Activation::Relu: return f(std::integral_constant<Activation, Activation::Relu>{});
+        case Activation::Sigmoid: return f(std::integral_constant<Activation, Activation::Sigmoid>{});
+    }
+}
+
+// ---- device helpers -------------------------------------------------------------------------------
+// Two floats as one word of two 16-bit values, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 TMEM lanes (this warp's quarter) x 32 consecutive columns; the caller waits (tmem_wait).
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+        "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+          "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+          "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory descriptors, SWIZZLE_128B (layout 2, version 1). K-major: rows of 128 bytes, 8-row
+// atoms 1 KB apart. MN-major: 8 summed rows 1 KB apart, 64-column chunks CHUNK apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(CHUNK >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to out[row0.., col0..], `rows` x
+// `cols` of them valid, turned through the warp's staging area.
+template <typename T>
+__device__ __forceinline__ void store_group(uint8_t* turn, const uint32_t (&w)[16], T* out,
+                                            int64_t ld, int rows, int cols, bool vec) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(turn + lane * TURN_LD + i * 16) =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    __syncwarp();
+    if (vec) {
+        const int c = (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (lane >> 2) + 8 * i;
+            if (r >= rows || c >= cols) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(turn + r * TURN_LD + c * 2);
+            T* dst = out + r * ld + c;
+            if (c + 8 <= cols) {
+                *reinterpret_cast<uint4*>(dst) = v;
+            } else {
+                const T* e = reinterpret_cast<const T*>(turn + r * TURN_LD) + c;
+                for (int j = 0; j < cols - c; ++j) dst[j] = e[j];
+            }
+        }
+    } else if (lane < cols) {
+        for (int r = 0; r < rows; ++r)
+            out[r * ld + lane] = reinterpret_cast<const T*>(turn + r * TURN_LD)[lane];
+    }
+}
+
+// ---- the kernel -------------------------------------------------------------------------------------
+template <typename T, Product P>
+__global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int stage_bytes = A_BYTES + p.b_bytes;
+    uint8_t* turn = smem + p.stages * stage_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + TURN_BYTES);
+    uint64_t* empty = full + MAX_STAGES;
+    uint64_t* acc_full = empty + MAX_STAGES;  // [2]
+    uint64_t* acc_empty = acc_full + 2;       // [2]
+    uint64_t* done = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], EPI_WARPS);
+        }
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int tiles = p.mt * p.nt, work = tiles * p.splits;
+    // Tile t: rows fastest, so CTAs that run together share the columns' operand.
+    auto first_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles) / p.splits); };
+    auto last_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles + 1) / p.splits); };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int j = 0, mmas = 0;  // stages taken so far
+            bool ok = true;
+            for (int t = blockIdx.x, i = 0; t < work && ok; t += gridDim.x, ++i) {
+                const int b = i & 1;
+                if (i >= 2 && !mbar_wait(&acc_empty[b], ((i >> 1) - 1) & 1, p.err)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + (uint32_t)(b * ACC_COLS);
+                const int k0 = first_step(t), k1 = last_step(t);
+                for (int k = k0; k < k1; ++k, ++j) {
+                    const int s = j % p.stages;
+                    if (!mbar_wait(&full[s], (j / p.stages) & 1, p.err)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < TK / 16; ++q) {
+                        // 16 summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows
+                        const uint64_t da = P == Product::Dw ? desc_mn(sa + q * 2048) : desc_k(sa + q * 32);
+                        const uint64_t db = P == Product::Forward ? desc_k(sb + q * 32) : desc_mn(sb + q * 2048);
+                        tc_mma(acc, da, db, p.idesc, k > k0 || q > 0);
+                        ++mmas;
+                    }
+                    tc_commit(&empty[s]);
+                }
+                if (ok) tc_commit(&acc_full[b]);
+            }
+            if (mmas > 0) tc_commit(done);
+            else mbar_arrive(done);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int j = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < work && ok; t += gridDim.x) {
+                const int mi = t % p.mt, ni = t / p.mt % p.nt;
+                const int n0 = ni * p.bn;
+                const int k1 = last_step(t);
+                for (int k = first_step(t); k < k1; ++k, ++j) {
+                    const int s = j % p.stages;
+                    if (j >= p.stages && !mbar_wait(&empty[s], ((j / p.stages) & 1) ^ 1, p.err)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sa = smem + s * stage_bytes;
+                    uint8_t* sb = sa + A_BYTES;
+                    mbar_expect_tx(&full[s], (uint32_t)stage_bytes);
+                    if constexpr (P == Product::Forward) {
+                        tma_load_2d(sa, &p.a[0], k * TK, mi * TM, &full[s]);
+                        tma_load_2d(sb, &p.b[0], k * TK, n0, &full[s]);
+                        tma_load_2d(sb + p.bn * 128, &p.b[1], k * TK, n0, &full[s]);
+                    } else if constexpr (P == Product::Dx) {
+                        const int seg = k >= p.kseg, kk = (k - seg * p.kseg) * TK;
+                        tma_load_2d(sa, &p.a[seg], kk, mi * TM, &full[s]);
+                        for (int c = 0; c * CHUNK < p.b_bytes; ++c)
+                            tma_load_2d(sb + c * CHUNK, &p.b[seg], n0 + 64 * c, kk, &full[s]);
+                    } else {
+                        const int seg = mi >= p.mt_one, m0 = (mi - seg * p.mt_one) * TM;
+                        for (int c = 0; c < TM / 64; ++c)
+                            tma_load_2d(sa + c * CHUNK, &p.a[seg], m0 + 64 * c, k * TK, &full[s]);
+                        for (int c = 0; c * CHUNK < p.b_bytes; ++c)
+                            tma_load_2d(sb + c * CHUNK, &p.b[0], n0 + 64 * c, k * TK, &full[s]);
+                    }
+                }
+            }
+            // no load may be in flight when the CTA ends (they have all landed unless a wait ran out)
+            for (int i = max(0, j - p.stages); i < j; ++i)
+                mbar_wait(&full[i % p.stages], (i / p.stages) & 1, p.err);
+        }
+    } else if (warp >= FIRST_EPI) {
+        const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
+        uint8_t* my_turn = turn + (warp - FIRST_EPI) * 32 * TURN_LD;
+        for (int t = blockIdx.x, i = 0; t < work; t += gridDim.x, ++i) {
+            const int b = i & 1;
+            if (!mbar_wait(&acc_full[b], (i >> 1) & 1, p.err)) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * ACC_COLS);
+            const int mi = t % p.mt, ni = t / p.mt % p.nt;
+            const int seg = P == Product::Dw && mi >= p.mt_one;
+            const int64_t row0 = (int64_t)(mi - seg * p.mt_one) * TM + quarter * 32;
+            const int64_t n0 = (int64_t)ni * p.bn;
+            const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
+            const int ncols = (int)min((int64_t)p.bn, p.N - n0);
+            for (int c = half * 32; c < ncols; c += 64) {
+                const int cols = min(32, ncols - c);
+                uint32_t v[32];
+                tmem_ld32(acc + (uint32_t)c, v);
+                if constexpr (P == Product::Forward) {
+                    uint32_t u[32], w[16];
+                    tmem_ld32(acc + (uint32_t)(p.bn + c), u);
+                    tmem_wait();
+                    with_activation(p.act, [&](auto act) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float g0 = __uint_as_float(v[2 * e]), g1 = __uint_as_float(v[2 * e + 1]);
+                            w[e] = pack2(act_value<decltype(act)::value>(g0) * __uint_as_float(u[2 * e]),
+                                         act_value<decltype(act)::value>(g1) * __uint_as_float(u[2 * e + 1]),
+                                         T());
+                        }
+                    });
+                    store_group(my_turn, w, static_cast<T*>(p.out[0]) + row0 * p.ld[0] + n0 + c, p.ld[0],
+                                rows, cols, p.vec[0] != 0);
+                    if (p.out[1]) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            w[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), T());
+                        store_group(my_turn, w, static_cast<T*>(p.out[1]) + row0 * p.ld[1] + n0 + c,
+                                    p.ld[1], rows, cols, p.vec[1] != 0);
+                    }
+                    if (p.out[2]) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            w[e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), T());
+                        store_group(my_turn, w, static_cast<T*>(p.out[2]) + row0 * p.ld[2] + n0 + c,
+                                    p.ld[2], rows, cols, p.vec[2] != 0);
+                    }
+                } else {
+                    tmem_wait();
+                    if (p.splits > 1) {
+                        float4* dst = p.partial + ((int64_t)t * (ACC_COLS / 4) + c / 4) * TM + quarter * 32 + lane;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            dst[e * TM] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                                      __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+                    } else {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            w[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), T());
+                        store_group(my_turn, w, static_cast<T*>(p.out[seg]) + row0 * p.ld[seg] + n0 + c,
+                                    p.ld[seg], rows, cols, p.vec[seg] != 0);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        mbar_wait(done, 0, p.err);  // bounded; completes once the last MMA has
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+    }
+}
+
+// Adds the slices of a split sum in slice order and rounds. A warp takes 4 rows x 8 float4 columns.
+template <typename T, Product P>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileArgs p) {
+    const int tiles = p.mt * p.nt, lane = threadIdx.x & 31;
+    const int groups = (p.bn + 31) / 32;  // per tile: 32 columns each, by 32 slabs of 4 rows
+    const int64_t warps = (int64_t)tiles * groups * (TM / 4);
+    for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
+        const int slab = (int)(w % (TM / 4)), grp = (int)(w / (TM / 4) % groups);
+        const int t = (int)(w / (TM / 4) / groups);
+        const int mi = t % p.mt, ni = t / p.mt;
+        const int seg = P == Product::Dw && mi >= p.mt_one;
+        const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
+        const int64_t row = (int64_t)(mi - seg * p.mt_one) * TM + r, col = (int64_t)ni * p.bn + c4 * 4;
+        if (row >= p.M || col >= p.N || c4 * 4 >= p.bn) continue;
+        const float4* src = p.partial + ((int64_t)t * (ACC_COLS / 4) + c4) * TM + r;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < p.splits; ++i) {
+            const float4 v = src[(int64_t)i * tiles * (ACC_COLS / 4) * TM];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        T* dst = static_cast<T*>(p.out[seg]) + row * p.ld[seg] + col;
+        if (p.vec[seg] && col + 4 <= p.N) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+        } else {
+            const float e[4] = {s.x, s.y, s.z, s.w};
+            for (int i = 0; i < 4 && col + i < p.N; ++i) dst[i] = from_float<T>(e[i]);
+        }
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+// Instruction descriptor, kind::f16: fp32 accumulator, operand types and orders, N / 8, M / 16.
+inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int n) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) |
+           (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+}
+
+// Whether TMA can address rows of a 16-bit matrix: 16-byte base and row stride.
+inline bool tma_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+
+inline bool store16_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+
+// Fills the stage count and shared memory, launches, and joins the slices. `t` has the maps, sizes,
+// outputs and bn set.
+template <typename T, Product P>
+void launch_product(Handle& h, TileArgs& t) {
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    t.acc_n = P == Product::Forward ? 2 * t.bn : (t.bn + 15) / 16 * 16;
+    t.b_bytes = P == Product::Forward ? 2 * t.bn * 128 : (t.bn + 63) / 64 * CHUNK;
+    t.idesc = make_idesc(bf16, P == Product::Dw, P != Product::Forward, t.acc_n);
+    t.stages = std::min<int>(MAX_STAGES, (SMEM_MAX - TURN_BYTES) / (A_BYTES + t.b_bytes));
+    t.err = h.d_err;
+    const size_t smem = 1024 + (size_t)t.stages * (A_BYTES + t.b_bytes) + TURN_BYTES + 512;
+    const int64_t work = (int64_t)t.mt * t.nt * t.splits;
+    XS_REQUIRE(work < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
+    DevBuf<float4> ws(t.splits > 1 ? (size_t)work * (ACC_COLS / 4) * TM : 0, h.stream);
+    t.partial = ws.get();
+    auto kern = tile_kernel<T, P>;
+    XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const unsigned grid = (unsigned)std::min<int64_t>(work, sm_count(h.device));
+    kern<<<grid, THREADS, smem, h.stream>>>(t);
+    after_launch(h, "gated_product");
+    if (t.splits > 1) {
+        const int64_t warps = (int64_t)t.mt * t.nt * ((t.bn + 31) / 32) * (TM / 4);
+        const unsigned jg = (unsigned)std::min<int64_t>(ceil_div(warps, 8), (int64_t)sm_count(h.device) * 8);
+        join_kernel<T, P><<<jg, 256, 0, h.stream>>>(t);
+        after_launch(h, "gated_join");
+    }
+}
+
+}  // namespace gated
+}  // namespace xspmm_b200
