@@ -14,37 +14,58 @@ namespace {
 
 constexpr int DROP_THREADS = 256;
 
-__device__ __forceinline__ uint4 philox(uint64_t counter, uint2 key) {
+struct Keys {  // the key of each round: multiples of two constants added to the seed's halves
+    uint32_t k0[10], k1[10];
+};
+
+__device__ __forceinline__ uint4 philox(uint64_t counter, const Keys& key) {
     uint4 c = make_uint4((uint32_t)counter, (uint32_t)(counter >> 32), 0u, 0u);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t p0 = (uint64_t)0xD2511F53u * c.x, p1 = (uint64_t)0xCD9E8D57u * c.z;
-        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ key.x, (uint32_t)p1,
-                       (uint32_t)(p0 >> 32) ^ c.w ^ key.y, (uint32_t)p0);
-        key.x += 0x9E3779B9u;
-        key.y += 0xBB67AE85u;
+        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ key.k0[r], (uint32_t)p1,
+                       (uint32_t)(p0 >> 32) ^ c.w ^ key.k1[r], (uint32_t)p0);
     }
     return c;
 }
 
-template <typename T, bool RES>
+// V elements (V / 4 generator blocks) a thread; VEC: the pointers allow V-wide accesses. An element is
+// dropped iff its word is at most `last`; draw is false where p rounds to 0 and nothing is dropped.
+template <typename T, int V, bool RES, bool VEC>
 __global__ void __launch_bounds__(DROP_THREADS)
-dropout_kernel(int64_t n, const T* x, const T* res, uint32_t threshold, bool drop_all, float scale,
-               uint2 key, uint64_t offset, T* y) {
-    const int64_t blocks = (n + 3) / 4;
-    for (int64_t b = (int64_t)blockIdx.x * DROP_THREADS + threadIdx.x; b < blocks;
-         b += (int64_t)gridDim.x * DROP_THREADS) {
-        const uint4 w = philox(offset + (uint64_t)b, key);
+dropout_kernel(int64_t n, const T* x, const T* res, bool draw, uint32_t last, float scale,
+               const __grid_constant__ Keys key, uint64_t offset, T* y) {
+    const int64_t g = (int64_t)blockIdx.x * DROP_THREADS + threadIdx.x, first = g * V;
+    if (first >= n) return;
+    float v[V], r[V];
+    const bool whole = VEC && first + V <= n;
+    if (whole) {
+        load_pack<T, V>(x + first, v);
+        if (RES) load_pack<T, V>(res + first, r);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            v[e] = first + e < n ? to_float(x[first + e]) : 0.0f;
+            if (RES) r[e] = first + e < n ? to_float(res[first + e]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+        uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (draw) w = philox(offset + (uint64_t)(g * (V / 4) + q), key);
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t i = b * 4 + j;
-            if (i >= n) break;
-            const bool keep = ws[j] >= threshold && !drop_all;
-            float v = keep ? to_float(x[i]) * scale : 0.0f;
-            if (RES) v += to_float(res[i]);
-            y[i] = from_float<T>(v);
+        for (int e = 0; e < 4; ++e) {
+            const float t = !draw || ws[e] > last ? v[q * 4 + e] * scale : 0.0f;
+            v[q * 4 + e] = RES ? r[q * 4 + e] + t : t;
         }
+    }
+    if (whole) {
+        store_pack<T, V>(y + first, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (first + e < n) y[first + e] = from_float<T>(v[e]);
     }
 }
 
@@ -54,19 +75,22 @@ template <typename T>
 void dropout(Handle& h, int64_t n, const T* x, const T* residual, double p, uint64_t seed,
              uint64_t offset, T* y) {
     if (n == 0) return;
-    // keep iff word >= threshold; p = 1 gives 2^32, which no word reaches
+    // kept iff word >= threshold, which is word > threshold - 1; p = 1 gives 2^32, which no word reaches
     const uint64_t threshold = (uint64_t)std::nearbyint(p * 4294967296.0);
-    const bool all = threshold > 0xFFFFFFFFull;
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
-    const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
-    const unsigned grid = (unsigned)std::min(ceil_div(ceil_div(n, 4), DROP_THREADS),
-                                             (int64_t)sm_count(h.device) * 8);
-    if (residual)
-        dropout_kernel<T, true><<<grid, DROP_THREADS, 0, h.stream>>>(
-            n, x, residual, (uint32_t)threshold, all, scale, key, offset, y);
-    else
-        dropout_kernel<T, false><<<grid, DROP_THREADS, 0, h.stream>>>(
-            n, x, nullptr, (uint32_t)threshold, all, scale, key, offset, y);
+    Keys key;
+    for (int r = 0; r < 10; ++r) {
+        key.k0[r] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u;
+        key.k1[r] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+    }
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = aligned_to(x, 16) && aligned_to(y, 16) && aligned_to(residual, 16);
+    const int64_t grid = ceil_div(ceil_div(n, V), DROP_THREADS);
+    XS_REQUIRE(grid < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
+    auto kern = residual ? (vec ? dropout_kernel<T, V, true, true> : dropout_kernel<T, V, true, false>)
+                         : (vec ? dropout_kernel<T, V, false, true> : dropout_kernel<T, V, false, false>);
+    kern<<<(unsigned)grid, DROP_THREADS, 0, h.stream>>>(n, x, residual, threshold > 0,
+                                                        (uint32_t)(threshold - 1), scale, key, offset, y);
     after_launch(h, "dropout");
 }
 

@@ -98,16 +98,6 @@ __host__ __device__ __forceinline__ void with_activation(Activation a, F&& f) {
 }
 
 // ---- device helpers -------------------------------------------------------------------------------
-// Two floats as one word of two 16-bit values, the first in the low half.
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // 32 TMEM lanes (this warp's quarter) x 32 consecutive columns; the caller waits (tmem_wait).
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(

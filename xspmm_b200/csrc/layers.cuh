@@ -59,17 +59,51 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
     T v[V];
 };
+// Two values as one word, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {  // bf16 is fp32's high half
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// A pack's values as floats and back: one instruction per value, or per two when narrowing.
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& k, float (&out)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 f = unpack2(reinterpret_cast<const uint32_t*>(&k)[i / 2], T());
+            out[i] = f.x;
+            out[i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = to_float(k.v[i]);
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_pack(const T* p, float (&out)[V]) {
-    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = to_float(k.v[i]);
+    unpack<T, V>(*reinterpret_cast<const Pack<T, V>*>(p), out);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const float (&in)[V]) {
     Pack<T, V> k;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) k.v[i] = from_float<T>(in[i]);
+        for (int i = 0; i < V; i += 2)
+            reinterpret_cast<uint32_t*>(&k)[i / 2] = pack2(in[i], in[i + 1], T());
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) k.v[i] = from_float<T>(in[i]);
+    }
     *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
