@@ -73,8 +73,7 @@ class CudaExecutor:
 
     @property
     def handle(self):
-        lib().xspmm_set_stream(self._h, ctypes.c_void_p(
-            torch.cuda.current_stream(self.device).cuda_stream))
+        lib().xspmm_set_stream(self._h, torch._C._cuda_getCurrentRawStream(self.device_id))
         return self._h
 
     def allocate(self, nbytes: int) -> torch.Tensor:

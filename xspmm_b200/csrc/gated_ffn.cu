@@ -73,18 +73,24 @@ CUtensorMap map_of(const T* p, int64_t ld, int64_t rows, int64_t cols, int box_r
                        CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Forward tile width. A tile costs its slices (the slower of the MMAs, 4 clocks per output column, and
-// the loads at about 48 bytes a clock) plus a fill and drain; tiles run in waves over the SMs.
-int forward_width(int sms, int64_t rows, int64_t K, int64_t F) {
-    const int64_t mt = ceil_div(rows, TM), steps = ceil_div(K, TK);
+// Clocks of one 64-deep slice of a tile on one SM: the MMAs (2 clocks an accumulator column, at least 32
+// columns' worth), shared memory written and read at 128 bytes a clock, or the loads at about 48.
+double slice_clocks(int cg, int acc_n, double a_bytes) {
+    const double b_bytes = 128.0 * acc_n / cg;
+    return std::max({2.0 * std::max(acc_n, 64), 2.0 * (16384.0 + b_bytes) / 128.0, (a_bytes + b_bytes) / 48.0});
+}
+
+// Forward tile width: the cheapest by waves of tiles times slices, with a fill and drain for each tile.
+int forward_width(int sms, int cg, int64_t rows, int64_t K, int64_t F) {
+    const int64_t mt = ceil_div(rows, TM * cg), steps = ceil_div(K, TK);
     const double a_bytes = 128.0 * (double)std::min<int64_t>(rows, TM);
-    int best = 8;
+    const int unit = 8 * cg;  // MMA N = 2 bf is a multiple of 16, in a pair of 32
+    int best = unit;
     double least = 0.0;
-    for (int bf = 8; bf <= 128; bf += 8) {
-        const int64_t waves = ceil_div(mt * ceil_div(F, bf), sms);
-        const double step = std::max(4.0 * std::max(bf, 32), (a_bytes + 256.0 * bf) / 48.0);
-        const double cost = (double)waves * ((double)steps * step + 1500.0 + 12.0 * bf);
-        if (bf == 8 || cost <= least) {
+    for (int bf = unit; bf <= 128; bf += unit) {
+        const int64_t waves = ceil_div(mt * ceil_div(F, bf), sms / cg);
+        const double cost = (double)waves * ((double)steps * slice_clocks(cg, 2 * bf, a_bytes) + 1500.0 + 12.0 * bf);
+        if (bf == unit || cost <= least) {
             least = cost;
             best = bf;
         }
@@ -93,19 +99,18 @@ int forward_width(int sms, int64_t rows, int64_t K, int64_t F) {
     return best;
 }
 
-// Tile width and number of slices of a gradient's product, by the same model: MMAs 2 clocks per column
-// and slice; a split sum adds a second kernel and its partials' trip through L2.
-void gradient_tiling(int sms, int64_t mt, int64_t N, int64_t steps, int* bn, int* splits) {
+// Tile width and number of slices of a gradient's product, by the same model; a split sum adds a second
+// kernel and its partials' trip through L2.
+void gradient_tiling(int sms, int cg, int64_t mt, int64_t N, int64_t steps, int* bn, int* splits) {
     double least = -1.0;
-    const int widest = (int)std::min<int64_t>(256, ceil_div(N, 16) * 16);
+    const int unit = 16 * cg, widest = (int)std::min<int64_t>(256, ceil_div(N, unit) * unit);
     for (int w = 64; w <= 256; w += 64) {
         const int cand = std::min(w, widest);
-        const int64_t tiles = mt * ceil_div(N, cand);
-        for (int64_t sp = 1; sp <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, sms / tiles)); ++sp) {
-            const int64_t waves = ceil_div(tiles * sp, sms);
-            const double step = std::max(2.0 * std::max(cand, 64), (16384.0 + 128.0 * cand) / 48.0);
-            double cost = (double)waves * ((double)ceil_div(steps, sp) * step + 1500.0 + 6.0 * cand);
-            if (sp > 1) cost += 5000.0 + (double)(tiles * sp) * 128.0 * cand * 8.0 / 3000.0;
+        const int64_t tiles = mt * ceil_div(N, cand), slots = sms / cg;
+        for (int64_t sp = 1; sp <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, slots / tiles)); ++sp) {
+            const int64_t waves = ceil_div(tiles * sp, slots);
+            double cost = (double)waves * ((double)ceil_div(steps, sp) * slice_clocks(cg, cand, 16384.0) + 1500.0 + 6.0 * cand);
+            if (sp > 1) cost += 5000.0 + (double)(tiles * sp * cg) * 128.0 * cand * 8.0 / 3000.0;
             if (least < 0.0 || cost < least) {
                 least = cost;
                 *bn = cand;
@@ -146,8 +151,9 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
     TileArgs t = {};
     t.M = a.rows;
     t.N = a.F;
-    t.bn = forward_width(sm_count(h.device), a.rows, a.K, a.F);
-    t.mt = (int)ceil_div(a.rows, TM);
+    const int cg = a.rows > TM ? 2 : 1;
+    t.bn = forward_width(sm_count(h.device), cg, a.rows, a.K, a.F);
+    t.mt = (int)ceil_div(a.rows, TM * cg);
     t.nt = (int)ceil_div(a.F, t.bn);
     t.splits = 1;
     t.ksteps = t.kseg = (int)ceil_div(a.K, TK);
@@ -161,7 +167,8 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
         t.ld[i] = i == 0 ? ldy : a.F;
         t.vec[i] = store16_ok(outs[i], t.ld[i]);
     }
-    launch_product<T, Product::Forward>(h, t);
+    if (cg == 2) launch_product<T, Product::Forward, 2>(h, t);
+    else launch_product<T, Product::Forward, 1>(h, t);
 }
 
 template <typename T>
@@ -196,10 +203,11 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         TileArgs t = {};
         t.M = a.rows;
         t.N = a.K;
-        t.mt = (int)ceil_div(a.rows, TM);
+        const int cg = a.rows > TM ? 2 : 1;
+        t.mt = (int)ceil_div(a.rows, TM * cg);
         t.kseg = (int)ceil_div(a.F, TK);
         t.ksteps = 2 * t.kseg;
-        gradient_tiling(sms, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
+        gradient_tiling(sms, cg, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
         t.nt = (int)ceil_div(a.K, t.bn);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TM);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TM);
@@ -208,17 +216,17 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         t.out[0] = dx;
         t.ld[0] = lddx;
         t.vec[0] = store16_ok(dx, lddx);
-        launch_product<T, Product::Dx>(h, t);
+        if (cg == 2) launch_product<T, Product::Dx, 2>(h, t);
+        else launch_product<T, Product::Dx, 1>(h, t);
     }
     if (dwg) {
         const Rows<T> x(h, a.x, a.ldx, a.rows, a.K);
         TileArgs t = {};
         t.M = a.F;
         t.N = a.K;
-        t.mt_one = (int)ceil_div(a.F, TM);
-        t.mt = 2 * t.mt_one;
+        t.mt = (int)ceil_div(a.F, TM);
         t.kseg = t.ksteps = (int)ceil_div(a.rows, TK);
-        gradient_tiling(sms, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
+        gradient_tiling(sms, 2, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
         t.nt = (int)ceil_div(a.K, t.bn);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TK);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TK);
@@ -229,7 +237,7 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
             t.ld[i] = a.K;
             t.vec[i] = store16_ok(t.out[i], a.K);
         }
-        launch_product<T, Product::Dw>(h, t);
+        launch_product<T, Product::Dw, 2>(h, t);
     }
 }
 

@@ -5,20 +5,28 @@
 //   Dx        dx[m, k] = sum_f dg[m,f] wg[f,k] + du[m,f] wu[f,k]
 //   Dw        dw[f, k] = sum_m d[m,f] x[m,k], d = dg, then du
 //
-// An output tile is 128 rows by up to 256 accumulator columns; a summed slice is 64 deep. Operands
-// come by TMA in the SWIZZLE_128B layout, in whichever order memory has them: K-major where the
-// summed index is contiguous (x, weights of Forward; dg, du of Dx), MN-major where the output index
-// is (the others), so nothing is transposed. Forward puts bf rows of wg and the same bf rows of wu
-// one after the other in shared memory: one MMA of N = 2 bf fills both projections of bf outputs,
-// x is read once for both, and the epilogue finds g and u of an output bf columns apart in TMEM.
-// Edges need no code: TMA fills what lies outside with zeros.
+// A CTA's part of an output tile is 128 rows by up to 256 accumulator columns; a summed slice is 64
+// deep. Operands come by TMA in the SWIZZLE_128B layout, in whichever order memory has them: K-major
+// where the summed index is contiguous (x, weights of Forward; dg, du of Dx), MN-major where the
+// output index is (the others), so nothing is transposed. Edges need no code: TMA fills what lies
+// outside with zeros.
 //
-// Roles (384 threads, one CTA per SM): warp 0 issues the MMAs (one lane), warp 1 the loads (one
-// lane), warp 2 allocates TMEM, warps 4..11 are the epilogue. TMEM holds two accumulators used in
-// turn, so a tile's epilogue runs under the next tile's products. The epilogue converts 32 columns
-// at a time and turns them through a warp's own piece of shared memory, so global stores are
-// 16 bytes a lane and 64 contiguous bytes a row. Every wait is bounded; a timeout sets the error
-// flag, and TMEM is freed only after the MMAs that were issued have completed.
+// CG = 2: two CTAs form one MMA of 256 rows (cta_group::2). Each holds its own 128 rows of A and half
+// of B's columns in its shared memory, and all columns of its rows in its TMEM. A CTA alone has to
+// write and read 24 KB of shared memory per 16-deep MMA of 128 x 256, 192 clocks at 128 bytes a clock
+// where the MMA takes 128; in a pair it is 16 KB. Measured on 2048 tokens of 4096 x 11008, forward:
+// XX us alone, YY us paired. CG = 1 is for at most 128 rows, where the second CTA would compute padding.
+//   Forward: an MMA of N = 2 bf holds bf columns of both projections, so x is read once for both and the
+//   epilogue finds g and u of an output bf columns apart; in a pair one CTA brings wg, the other wu.
+//   Dw: the pair's first CTA computes rows of dwg, the second the same rows of dwu.
+//
+// Roles (384 threads, one CTA per SM): warp 0 of the pair's first CTA issues the MMAs (one lane), warp
+// 1 of each the loads of its own operands (one lane; they report to the first CTA's barrier), warp 2
+// allocates TMEM, warps 4..11 are the epilogue. TMEM holds two accumulators used in turn, so a tile's
+// epilogue runs under the next tile's products. The epilogue converts 32 columns at a time and turns
+// them through a warp's own piece of shared memory, so global stores are 16 bytes a lane and 64
+// contiguous bytes a row. Every wait is bounded; a timeout sets the error flag, and TMEM is freed only
+// after the MMAs that were issued have completed.
 //
 // Where the output has too few tiles for the GPU, the sum is split: each slice's fp32 partial goes
 // to scratch and a second kernel adds them in slice order (the same order every time).
@@ -47,10 +55,9 @@ constexpr int SMEM_MAX = 232448 - 1024 - 512;  // opt-in limit less alignment an
 struct TileArgs {
     CUtensorMap a[2], b[2];
     int64_t M, N;       // output rows and columns (Dw: rows of one weight)
-    int mt, nt, splits;
-    int mt_one;         // Dw: tiles of the first weight, the others belong to the second
+    int mt, nt, splits; // tiles of CG CTAs
     int bn;             // output columns per tile
-    int acc_n;          // MMA N: 2 bn (Forward) or bn rounded up to 16
+    int acc_n;          // MMA N
     int ksteps, kseg;   // summed slices over all segments, and per segment
     int stages, b_bytes;
     uint32_t idesc;
@@ -58,7 +65,7 @@ struct TileArgs {
     void* out[3];       // Forward: y, gate, up; Dx: dx; Dw: dwg, dwu
     int64_t ld[3];
     int vec[3];         // 16-byte stores allowed
-    float4* partial;    // splits > 1: [split][tile][column / 4][row]
+    float4* partial;    // splits > 1: [split][tile][CTA][column / 4][row]
     unsigned* err;
 };
 
@@ -115,6 +122,88 @@ __device__ __forceinline__ void tmem_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The forms of a pair of CTAs (CG = 2) and of a single one. Barrier addresses are shared::cluster ones.
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// `p`'s counterpart in the shared memory of the pair's first CTA.
+__device__ __forceinline__ uint32_t first_cta_addr(const void* p) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+    return a;
+}
+template <int CG>
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        tc_mma(d, a, b, idesc, accumulate);
+}
+// Arrives on the barrier at this place in every CTA of the pair once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+            " [%0], %1;" ::"r"(smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        tc_commit(bar);
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_all(uint32_t* slot) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(slot)),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(slot)),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free_all(uint32_t tmem) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(2 * ACC_COLS)
+                     : "memory");
+}
+
 // Shared-memory descriptors, SWIZZLE_128B (layout 2, version 1). K-major: rows of 128 bytes, 8-row
 // atoms 1 KB apart. MN-major: 8 summed rows 1 KB apart, 64-column chunks CHUNK apart.
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
@@ -160,8 +249,9 @@ __device__ __forceinline__ void store_group(uint8_t* turn, const uint32_t (&w)[1
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------
-template <typename T, Product P>
+template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileArgs p) {
+    static_assert(P != Product::Dw || CG == 2, "Dw: one weight a CTA");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -174,41 +264,38 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     uint64_t* done = acc_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG == 2 ? (int)cta_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 1);   // the first CTA's: its own expect_tx, both CTAs' bytes
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], EPI_WARPS);
+            mbar_init(&acc_empty[b], CG * EPI_WARPS);  // the first CTA's: both epilogues
         }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(tmem_slot)),
-                     "r"(2 * ACC_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 2) tmem_alloc_all<CG>(tmem_slot);
     tc_fence_before();
+    if constexpr (CG == 2) cluster_sync_all();  // the barriers of both CTAs are set up
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     const int tiles = p.mt * p.nt, work = tiles * p.splits;
+    const int group = blockIdx.x / CG, groups = gridDim.x / CG;
     // Tile t: rows fastest, so CTAs that run together share the columns' operand.
     auto first_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles) / p.splits); };
     auto last_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles + 1) / p.splits); };
 
     if (warp == 0) {
-        if (lane == 0) {
-            int j = 0, mmas = 0;  // stages taken so far
+        if (lane == 0 && rank == 0) {
+            int j = 0;  // stages taken so far
             bool ok = true;
-            for (int t = blockIdx.x, i = 0; t < work && ok; t += gridDim.x, ++i) {
+            for (int t = group, i = 0; t < work && ok; t += groups, ++i) {
                 const int b = i & 1;
                 if (i >= 2 && !mbar_wait(&acc_empty[b], ((i >> 1) - 1) & 1, p.err)) break;
                 tc_fence_after();
@@ -227,22 +314,21 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                         // 16 summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows
                         const uint64_t da = P == Product::Dw ? desc_mn(sa + q * 2048) : desc_k(sa + q * 32);
                         const uint64_t db = P == Product::Forward ? desc_k(sb + q * 32) : desc_mn(sb + q * 2048);
-                        tc_mma(acc, da, db, p.idesc, k > k0 || q > 0);
-                        ++mmas;
+                        pair_mma<CG>(acc, da, db, p.idesc, k > k0 || q > 0);
                     }
-                    tc_commit(&empty[s]);
+                    pair_commit<CG>(&empty[s]);
                 }
-                if (ok) tc_commit(&acc_full[b]);
+                if (ok) pair_commit<CG>(&acc_full[b]);
             }
-            if (mmas > 0) tc_commit(done);
-            else mbar_arrive(done);
+            pair_commit<CG>(done);  // arrives at once where nothing was issued
         }
     } else if (warp == 1) {
         if (lane == 0) {
             int j = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < work && ok; t += gridDim.x) {
+            for (int t = group; t < work && ok; t += groups) {
                 const int mi = t % p.mt, ni = t / p.mt % p.nt;
+                const int m0 = (P == Product::Dw ? mi : mi * CG + rank) * TM;
                 const int n0 = ni * p.bn;
                 const int k1 = last_step(t);
                 for (int k = first_step(t); k < k1; ++k, ++j) {
@@ -253,40 +339,48 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     }
                     uint8_t* sa = smem + s * stage_bytes;
                     uint8_t* sb = sa + A_BYTES;
-                    mbar_expect_tx(&full[s], (uint32_t)stage_bytes);
+                    if (rank == 0) mbar_expect_tx(&full[s], (uint32_t)(CG * stage_bytes));
+                    const uint32_t bar = CG == 2 ? first_cta_addr(&full[s]) : smem_u32(&full[s]);
                     if constexpr (P == Product::Forward) {
-                        tma_load_2d(sa, &p.a[0], k * TK, mi * TM, &full[s]);
-                        tma_load_2d(sb, &p.b[0], k * TK, n0, &full[s]);
-                        tma_load_2d(sb + p.bn * 128, &p.b[1], k * TK, n0, &full[s]);
-                    } else if constexpr (P == Product::Dx) {
-                        const int seg = k >= p.kseg, kk = (k - seg * p.kseg) * TK;
-                        tma_load_2d(sa, &p.a[seg], kk, mi * TM, &full[s]);
-                        for (int c = 0; c * CHUNK < p.b_bytes; ++c)
-                            tma_load_2d(sb + c * CHUNK, &p.b[seg], n0 + 64 * c, kk, &full[s]);
+                        pair_load<CG>(sa, &p.a[0], k * TK, m0, bar);
+                        if constexpr (CG == 2) {
+                            pair_load<CG>(sb, &p.b[rank], k * TK, n0, bar);
+                        } else {
+                            pair_load<CG>(sb, &p.b[0], k * TK, n0, bar);
+                            pair_load<CG>(sb + p.bn * 128, &p.b[1], k * TK, n0, bar);
+                        }
                     } else {
-                        const int seg = mi >= p.mt_one, m0 = (mi - seg * p.mt_one) * TM;
-                        for (int c = 0; c < TM / 64; ++c)
-                            tma_load_2d(sa + c * CHUNK, &p.a[seg], m0 + 64 * c, k * TK, &full[s]);
-                        for (int c = 0; c * CHUNK < p.b_bytes; ++c)
-                            tma_load_2d(sb + c * CHUNK, &p.b[0], n0 + 64 * c, k * TK, &full[s]);
+                        const int nb = n0 + rank * (p.acc_n / CG);  // this CTA's columns of B
+                        if constexpr (P == Product::Dx) {
+                            const int seg = k >= p.kseg, kk = (k - seg * p.kseg) * TK;
+                            pair_load<CG>(sa, &p.a[seg], kk, m0, bar);
+                            for (int c = 0; c * CHUNK < p.b_bytes; ++c)
+                                pair_load<CG>(sb + c * CHUNK, &p.b[seg], nb + 64 * c, kk, bar);
+                        } else {
+                            for (int c = 0; c < TM / 64; ++c)
+                                pair_load<CG>(sa + c * CHUNK, &p.a[rank], m0 + 64 * c, k * TK, bar);
+                            for (int c = 0; c * CHUNK < p.b_bytes; ++c)
+                                pair_load<CG>(sb + c * CHUNK, &p.b[0], nb + 64 * c, k * TK, bar);
+                        }
                     }
                 }
             }
-            // no load may be in flight when the CTA ends (they have all landed unless a wait ran out)
+            // No load may be in flight when the CTA ends. Each landed before its MMAs ran, and the commit
+            // after those freed its stage (they have all done so unless a wait ran out).
             for (int i = max(0, j - p.stages); i < j; ++i)
-                mbar_wait(&full[i % p.stages], (i / p.stages) & 1, p.err);
+                mbar_wait(&empty[i % p.stages], (i / p.stages) & 1, p.err);
         }
     } else if (warp >= FIRST_EPI) {
         const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
         uint8_t* my_turn = turn + (warp - FIRST_EPI) * 32 * TURN_LD;
-        for (int t = blockIdx.x, i = 0; t < work; t += gridDim.x, ++i) {
+        for (int t = group, i = 0; t < work; t += groups, ++i) {
             const int b = i & 1;
             if (!mbar_wait(&acc_full[b], (i >> 1) & 1, p.err)) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * ACC_COLS);
             const int mi = t % p.mt, ni = t / p.mt % p.nt;
-            const int seg = P == Product::Dw && mi >= p.mt_one;
-            const int64_t row0 = (int64_t)(mi - seg * p.mt_one) * TM + quarter * 32;
+            const int seg = P == Product::Dw ? rank : 0;
+            const int64_t row0 = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + quarter * 32;
             const int64_t n0 = (int64_t)ni * p.bn;
             const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
             const int ncols = (int)min((int64_t)p.bn, p.N - n0);
@@ -326,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 } else {
                     tmem_wait();
                     if (p.splits > 1) {
-                        float4* dst = p.partial + ((int64_t)t * (ACC_COLS / 4) + c / 4) * TM + quarter * 32 + lane;
+                        float4* dst = p.partial + (((int64_t)t * CG + rank) * (ACC_COLS / 4) + c / 4) * TM + quarter * 32 + lane;
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             dst[e * TM] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
@@ -343,39 +437,40 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            if (lane == 0) {
+                if constexpr (CG == 2) arrive_cluster(first_cta_addr(&acc_empty[b]));
+                else mbar_arrive(&acc_empty[b]);
+            }
         }
     }
     __syncwarp();
+    if (warp == 2) mbar_wait(done, 0, p.err);  // bounded; completes once the last MMA has
     tc_fence_before();
     __syncthreads();
-    if (warp == 2) {
-        mbar_wait(done, 0, p.err);  // bounded; completes once the last MMA has
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"(2 * ACC_COLS)
-                     : "memory");
-    }
+    if constexpr (CG == 2) cluster_sync_all();  // neither CTA's shared memory or TMEM is in use any more
+    tc_fence_after();
+    if (warp == 2) tmem_free_all<CG>(tmem);
 }
 
 // Adds the slices of a split sum in slice order and rounds. A warp takes 4 rows x 8 float4 columns.
-template <typename T, Product P>
+template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileArgs p) {
     const int tiles = p.mt * p.nt, lane = threadIdx.x & 31;
     const int groups = (p.bn + 31) / 32;  // per tile: 32 columns each, by 32 slabs of 4 rows
-    const int64_t warps = (int64_t)tiles * groups * (TM / 4);
+    const int64_t warps = (int64_t)tiles * CG * groups * (TM / 4);
     for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
         const int slab = (int)(w % (TM / 4)), grp = (int)(w / (TM / 4) % groups);
-        const int t = (int)(w / (TM / 4) / groups);
+        const int part = (int)(w / (TM / 4) / groups), t = part / CG, rank = part % CG;
         const int mi = t % p.mt, ni = t / p.mt;
-        const int seg = P == Product::Dw && mi >= p.mt_one;
+        const int seg = P == Product::Dw ? rank : 0;
         const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
-        const int64_t row = (int64_t)(mi - seg * p.mt_one) * TM + r, col = (int64_t)ni * p.bn + c4 * 4;
+        const int64_t row = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + r;
+        const int64_t col = (int64_t)ni * p.bn + c4 * 4;
         if (row >= p.M || col >= p.N || c4 * 4 >= p.bn) continue;
-        const float4* src = p.partial + ((int64_t)t * (ACC_COLS / 4) + c4) * TM + r;
+        const float4* src = p.partial + ((int64_t)part * (ACC_COLS / 4) + c4) * TM + r;
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int i = 0; i < p.splits; ++i) {
-            const float4 v = src[(int64_t)i * tiles * (ACC_COLS / 4) * TM];
+            const float4 v = src[(int64_t)i * tiles * CG * (ACC_COLS / 4) * TM];
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
         T* dst = static_cast<T*>(p.out[seg]) + row * p.ld[seg] + col;
@@ -390,9 +485,9 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileA
 
 // ---- host -----------------------------------------------------------------------------------------
 // Instruction descriptor, kind::f16: fp32 accumulator, operand types and orders, N / 8, M / 16.
-inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int n) {
+inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int m, int n) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) |
-           (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+           (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // Whether TMA can address rows of a 16-bit matrix: 16-byte base and row stride.
@@ -400,30 +495,47 @@ inline bool tma_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld %
 
 inline bool store16_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
 
-// Fills the stage count and shared memory, launches, and joins the slices. `t` has the maps, sizes,
-// outputs and bn set.
-template <typename T, Product P>
+// Accumulator columns (MMA N) of a tile of bn output columns: a multiple of 16, in a pair of 32.
+template <Product P, int CG>
+int acc_columns(int bn) {
+    return P == Product::Forward ? 2 * bn : (bn + 16 * CG - 1) / (16 * CG) * 16 * CG;
+}
+
+// Fills in what follows from `t`'s maps, sizes, outputs and bn, launches, and joins the slices.
+template <typename T, Product P, int CG>
 void launch_product(Handle& h, TileArgs& t) {
     constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    t.acc_n = P == Product::Forward ? 2 * t.bn : (t.bn + 15) / 16 * 16;
-    t.b_bytes = P == Product::Forward ? 2 * t.bn * 128 : (t.bn + 63) / 64 * CHUNK;
-    t.idesc = make_idesc(bf16, P == Product::Dw, P != Product::Forward, t.acc_n);
+    t.acc_n = acc_columns<P, CG>(t.bn);
+    const int own = t.acc_n / CG;  // a CTA's columns of B
+    t.b_bytes = P == Product::Forward ? own * 128 : (own + 63) / 64 * CHUNK;
+    t.idesc = make_idesc(bf16, P == Product::Dw, P != Product::Forward, TM * CG, t.acc_n);
     t.stages = std::min<int>(MAX_STAGES, (SMEM_MAX - TURN_BYTES) / (A_BYTES + t.b_bytes));
     t.err = h.d_err;
     const size_t smem = 1024 + (size_t)t.stages * (A_BYTES + t.b_bytes) + TURN_BYTES + 512;
     const int64_t work = (int64_t)t.mt * t.nt * t.splits;
-    XS_REQUIRE(work < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
-    DevBuf<float4> ws(t.splits > 1 ? (size_t)work * (ACC_COLS / 4) * TM : 0, h.stream);
+    XS_REQUIRE(work * CG < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
+    DevBuf<float4> ws(t.splits > 1 ? (size_t)work * CG * (ACC_COLS / 4) * TM : 0, h.stream);
     t.partial = ws.get();
-    auto kern = tile_kernel<T, P>;
+    auto kern = tile_kernel<T, P, CG>;
     XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const unsigned grid = (unsigned)std::min<int64_t>(work, sm_count(h.device));
-    kern<<<grid, THREADS, smem, h.stream>>>(t);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(work, sm_count(h.device) / CG) * CG));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = h.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CG > 1 ? 1 : 0;
+    XS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
     after_launch(h, "gated_product");
     if (t.splits > 1) {
-        const int64_t warps = (int64_t)t.mt * t.nt * ((t.bn + 31) / 32) * (TM / 4);
+        const int64_t warps = (int64_t)t.mt * t.nt * CG * ((t.bn + 31) / 32) * (TM / 4);
         const unsigned jg = (unsigned)std::min<int64_t>(ceil_div(warps, 8), (int64_t)sm_count(h.device) * 8);
-        join_kernel<T, P><<<jg, 256, 0, h.stream>>>(t);
+        join_kernel<T, P, CG><<<jg, 256, 0, h.stream>>>(t);
         after_launch(h, "gated_join");
     }
 }

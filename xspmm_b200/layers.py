@@ -20,30 +20,33 @@ _NORM_TYPES = ("f16f16", "bf16bf16", "f32f32", "f32f16", "f32bf16")
 
 def _matrix(exec: CudaExecutor, t: torch.Tensor, name: str, rows=None, cols=None, dtype=None):
     """Checks a matrix argument; returns its address and row stride."""
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (
-            cols is not None and t.shape[1] != cols):
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (
+            cols is not None and shape[1] != cols):
         want = ("rows" if rows is None else rows, "cols" if cols is None else cols)
-        raise ValueError(f"{name} must be {want[0]} x {want[1]}, got {tuple(t.shape)}")
+        raise ValueError(f"{name} must be {want[0]} x {want[1]}, got {tuple(shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != exec.device:
         raise ValueError(f"{name} on {t.device}, executor on {exec.device}")
-    if t.numel() == 0:
-        return None, t.shape[1]
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = shape
+    if rows == 0 or cols == 0:
+        return None, cols
+    ld, unit = t.stride()
+    if unit != 1 and cols > 1:
         raise ValueError(f"{name} must have contiguous rows")
-    if t.shape[0] == 1:
-        return t.data_ptr(), t.shape[1]
-    if t.stride(0) < t.shape[1]:
+    if rows == 1:
+        return t.data_ptr(), cols
+    if ld < cols:
         raise ValueError(f"the rows of {name} must not overlap")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), ld
 
 
 def _dense(exec: CudaExecutor, t, name: str, shape, dtype):
     """Checks a contiguous argument (or None); returns its address."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
@@ -51,7 +54,7 @@ def _dense(exec: CudaExecutor, t, name: str, shape, dtype):
         raise ValueError(f"{name} on {t.device}, executor on {exec.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr() if t.numel() else None
+    return t.data_ptr() or None
 
 
 def _norm_suffix(x: torch.Tensor, y: torch.Tensor) -> str:
