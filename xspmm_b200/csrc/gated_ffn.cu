@@ -30,8 +30,10 @@ gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t l
         load_pack<T, V>(up + r * F + c, u);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            a[e] = d[e] * u[e] * act_slope<ACT>(g[e]);
-            b[e] = d[e] * act_value<ACT>(g[e]);
+            float value, slope;
+            act_both<ACT>(g[e], &value, &slope);
+            a[e] = d[e] * u[e] * slope;
+            b[e] = d[e] * value;
         }
         store_pack<T, V>(dg + r * ldp + c, a);
         store_pack<T, V>(du + r * ldp + c, b);
@@ -73,51 +75,43 @@ CUtensorMap map_of(const T* p, int64_t ld, int64_t rows, int64_t cols, int box_r
                        CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Clocks of one 64-deep slice of a tile on one SM: the MMAs (2 clocks an accumulator column, at least 32
-// columns' worth), shared memory written and read at 128 bytes a clock, or the loads at about 48.
-double slice_clocks(int cg, int acc_n, double a_bytes) {
-    const double b_bytes = 128.0 * acc_n / cg;
-    return std::max({2.0 * std::max(acc_n, 64), 2.0 * (16384.0 + b_bytes) / 128.0, (a_bytes + b_bytes) / 48.0});
-}
-
-// Forward tile width: the cheapest by waves of tiles times slices, with a fill and drain for each tile.
-int forward_width(int sms, int cg, int64_t rows, int64_t K, int64_t F) {
-    const int64_t mt = ceil_div(rows, TM * cg), steps = ceil_div(K, TK);
-    const double a_bytes = 128.0 * (double)std::min<int64_t>(rows, TM);
-    const int unit = 8 * cg;  // MMA N = 2 bf is a multiple of 16, in a pair of 32
-    int best = unit;
-    double least = 0.0;
-    for (int bf = unit; bf <= 128; bf += unit) {
-        const int64_t waves = ceil_div(mt * ceil_div(F, bf), sms / cg);
-        const double cost = (double)waves * ((double)steps * slice_clocks(cg, 2 * bf, a_bytes) + 1500.0 + 12.0 * bf);
-        if (bf == unit || cost <= least) {
-            least = cost;
-            best = bf;
-        }
-        if (bf >= F) break;
-    }
-    return best;
-}
-
-// Tile width and number of slices of a gradient's product, by the same model; a split sum adds a second
-// kernel and its partials' trip through L2.
-void gradient_tiling(int sms, int cg, int64_t mt, int64_t N, int64_t steps, int* bn, int* splits) {
+// Picks a product's tile width, and how many slices the tiles are cut into that do not fill a wave of the
+// GPU's SMs. The model, in clocks: a 64-deep slice of a tile costs an SM the slower of its MMAs (2 per
+// accumulator column, at least 64 columns' worth), of shared memory written and read at 128 bytes a
+// clock, and of its loads at about 56 bytes a clock (measured: 2048 tokens of 4096 x 11008 forward take
+// 275 us with the loads left out and 299 with them); a tile adds a fill and drain. A split costs a
+// second kernel and its partials' trip through L2.
+template <Product P, int CG>
+void choose_tiles(Handle& h, TileArgs& t) {
+    const int slots = sm_count(h.device) / CG;
+    const int unit = P == Product::Forward ? 8 * CG : 16 * CG;  // MMA N: a multiple of 16, in a pair of 32
+    const int widest = P == Product::Forward ? 128 : 256;
+    const double a_bytes = P == Product::Dw ? A_BYTES : 128.0 * (double)std::min<int64_t>(t.M, TM);
     double least = -1.0;
-    const int unit = 16 * cg, widest = (int)std::min<int64_t>(256, ceil_div(N, unit) * unit);
-    for (int w = 64; w <= 256; w += 64) {
-        const int cand = std::min(w, widest);
-        const int64_t tiles = mt * ceil_div(N, cand), slots = sms / cg;
-        for (int64_t sp = 1; sp <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, slots / tiles)); ++sp) {
-            const int64_t waves = ceil_div(tiles * sp, slots);
-            double cost = (double)waves * ((double)ceil_div(steps, sp) * slice_clocks(cg, cand, 16384.0) + 1500.0 + 6.0 * cand);
-            if (sp > 1) cost += 5000.0 + (double)(tiles * sp * cg) * 128.0 * cand * 8.0 / 3000.0;
+    for (int bn = unit; bn <= widest; bn += unit) {
+        // Dx and Dw load whole 64-column chunks: other widths only where the output is narrower
+        if (P != Product::Forward && bn % (32 * CG) != 0 && bn < t.N) continue;
+        const int acc = acc_columns<P, CG>(bn);
+        const double b_bytes = P == Product::Forward ? 128.0 * acc / CG : (double)((acc / CG + 63) / 64 * CHUNK);
+        const double step = std::max({2.0 * std::max(acc, 64), 2.0 * (A_BYTES + b_bytes) / 128.0, (a_bytes + b_bytes) / 56.0});
+        const double ends = 1500.0 + 6.0 * acc;
+        const int64_t nt = ceil_div(t.N, bn), tiles = t.mt * nt;
+        const int64_t whole = tiles / slots * slots, rest = tiles - whole;
+        const double full = (double)(tiles / slots) * (t.ksteps * step + ends);
+        const int64_t most = rest > 0 ? std::max<int64_t>(1, std::min<int64_t>(slots / rest, t.ksteps / 4)) : 1;
+        for (int64_t sp = 1; sp <= most; ++sp) {
+            double cost = full;
+            if (rest > 0) cost += (double)ceil_div(t.ksteps, sp) * step + ends;
+            if (sp > 1) cost += 6000.0 + (double)(rest * sp) * TM * CG * acc * 8.0 / 3000.0;
             if (least < 0.0 || cost < least) {
                 least = cost;
-                *bn = cand;
-                *splits = (int)sp;
+                t.bn = bn;
+                t.nt = (int)nt;
+                t.splits = (int)sp;
+                t.whole = (int)(sp > 1 ? whole : tiles);
             }
         }
-        if (w >= widest) break;
+        if (bn >= t.N) break;
     }
 }
 
@@ -152,11 +146,11 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
     t.M = a.rows;
     t.N = a.F;
     const int cg = a.rows > TM ? 2 : 1;
-    t.bn = forward_width(sm_count(h.device), cg, a.rows, a.K, a.F);
     t.mt = (int)ceil_div(a.rows, TM * cg);
-    t.nt = (int)ceil_div(a.F, t.bn);
-    t.splits = 1;
     t.ksteps = t.kseg = (int)ceil_div(a.K, TK);
+    t.cols_first = a.rows > 2 * a.F;  // the operand of the inner index is read again and should fit L2
+    if (cg == 2) choose_tiles<Product::Forward, 2>(h, t);
+    else choose_tiles<Product::Forward, 1>(h, t);
     t.a[0] = map_of(x.p, x.ld, a.rows, a.K, TM);
     t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, t.bn);
     t.b[1] = map_of(wu.p, wu.ld, a.F, a.K, t.bn);
@@ -207,8 +201,9 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         t.mt = (int)ceil_div(a.rows, TM * cg);
         t.kseg = (int)ceil_div(a.F, TK);
         t.ksteps = 2 * t.kseg;
-        gradient_tiling(sms, cg, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
-        t.nt = (int)ceil_div(a.K, t.bn);
+        t.cols_first = a.rows > a.K;
+        if (cg == 2) choose_tiles<Product::Dx, 2>(h, t);
+        else choose_tiles<Product::Dx, 1>(h, t);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TM);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TM);
         t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, TK);
@@ -226,8 +221,8 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         t.N = a.K;
         t.mt = (int)ceil_div(a.F, TM);
         t.kseg = t.ksteps = (int)ceil_div(a.rows, TK);
-        gradient_tiling(sms, 2, t.mt, a.K, t.ksteps, &t.bn, &t.splits);
-        t.nt = (int)ceil_div(a.K, t.bn);
+        t.cols_first = 2 * a.F > a.K;
+        choose_tiles<Product::Dw, 2>(h, t);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TK);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TK);
         t.b[0] = map_of(x.p, x.ld, a.rows, a.K, TK);

@@ -28,8 +28,9 @@
 // contiguous bytes a row. Every wait is bounded; a timeout sets the error flag, and TMEM is freed only
 // after the MMAs that were issued have completed.
 //
-// Where the output has too few tiles for the GPU, the sum is split: each slice's fp32 partial goes
-// to scratch and a second kernel adds them in slice order (the same order every time).
+// Tiles that would leave part of the GPU idle (the last wave's, or all where there are few) have their
+// sum split: each slice's fp32 partial goes to scratch and a second kernel adds them in slice order (the
+// same order every time) and finishes the tile.
 #pragma once
 
 #include "layers.cuh"
@@ -55,7 +56,9 @@ constexpr int SMEM_MAX = 232448 - 1024 - 512;  // opt-in limit less alignment an
 struct TileArgs {
     CUtensorMap a[2], b[2];
     int64_t M, N;       // output rows and columns (Dw: rows of one weight)
-    int mt, nt, splits; // tiles of CG CTAs
+    int mt, nt;         // tiles of CG CTAs
+    int whole, splits;  // tiles [0, whole) are one work item each, the others `splits` items each
+    int cols_first;     // tile order: columns fastest, or rows
     int bn;             // output columns per tile
     int acc_n;          // MMA N
     int ksteps, kseg;   // summed slices over all segments, and per segment
@@ -65,11 +68,12 @@ struct TileArgs {
     void* out[3];       // Forward: y, gate, up; Dx: dx; Dw: dwg, dwu
     int64_t ld[3];
     int vec[3];         // 16-byte stores allowed
-    float4* partial;    // splits > 1: [split][tile][CTA][column / 4][row]
+    float4* partial;    // split tiles: [slice][tile][CTA][column / 4][row]
     unsigned* err;
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+// __fdividef(1, d) is 0 for d above 2^126, as the quotient nearly is.
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
 template <Activation ACT>
 __device__ __forceinline__ float act_value(float v) {
@@ -78,20 +82,47 @@ __device__ __forceinline__ float act_value(float v) {
     else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
     else return sigmoid(v);
 }
+// act(v) and act'(v).
 template <Activation ACT>
-__device__ __forceinline__ float act_slope(float v) {
+__device__ __forceinline__ void act_both(float v, float* value, float* slope) {
     if constexpr (ACT == Activation::Silu) {
         const float s = sigmoid(v);
-        return s * (1.0f + v * (1.0f - s));
+        *value = v * s;
+        *slope = s * (1.0f + v * (1.0f - s));
     } else if constexpr (ACT == Activation::Gelu) {
-        return 0.5f * (1.0f + erff(v * 0.70710678118654752f)) +
-               v * __expf(-0.5f * v * v) * 0.39894228040143268f;
+        const float half = 0.5f * (1.0f + erff(v * 0.70710678118654752f));
+        *value = v * half;
+        *slope = half + v * __expf(-0.5f * v * v) * 0.39894228040143268f;
     } else if constexpr (ACT == Activation::Relu) {
-        return v > 0.0f ? 1.0f : 0.0f;
+        *value = act_value<ACT>(v);
+        *slope = v > 0.0f ? 1.0f : 0.0f;
     } else {
         const float s = sigmoid(v);
-        return s * (1.0f - s);
+        *value = s;
+        *slope = s * (1.0f - s);
     }
+}
+
+// Work item t: a tile and the summed slices [k0, k1) of it; part < 0, or its place among the partials.
+struct Item {
+    int mi, ni, k0, k1, part;
+};
+__device__ __forceinline__ void tile_place(const TileArgs& p, int tile, int* mi, int* ni) {
+    *mi = p.cols_first ? tile / p.nt : tile % p.mt;
+    *ni = p.cols_first ? tile % p.nt : tile / p.mt;
+}
+__device__ __forceinline__ Item item_of(const TileArgs& p, int t) {
+    Item it{0, 0, 0, p.ksteps, -1};
+    int tile = t;
+    if (t >= p.whole) {
+        const int rest = p.mt * p.nt - p.whole, s = (t - p.whole) / rest;
+        it.part = t - p.whole;
+        tile = p.whole + it.part - s * rest;
+        it.k0 = (int)((int64_t)p.ksteps * s / p.splits);
+        it.k1 = (int)((int64_t)p.ksteps * (s + 1) / p.splits);
+    }
+    tile_place(p, tile, &it.mi, &it.ni);
+    return it;
 }
 
 template <typename F>
@@ -248,6 +279,24 @@ __device__ __forceinline__ void store_group(uint8_t* turn, const uint32_t (&w)[1
     }
 }
 
+// 32 accumulator columns as 16 words of the output type.
+template <typename T>
+__device__ __forceinline__ void pack_words(uint32_t (&w)[16], const uint32_t (&v)[32]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        w[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), T());
+}
+
+// The first `cols` (a multiple of 4) of 32 accumulator columns of a split tile's slice: lane = row, a
+// warp's store covers 512 contiguous bytes.
+__device__ __forceinline__ void store_partial(float4* dst, const uint32_t (&v)[32], int cols) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (4 * e < cols)
+            dst[e * TM] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                      __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+}
+
 // ---- the kernel -------------------------------------------------------------------------------------
 template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileArgs p) {
@@ -285,11 +334,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    const int tiles = p.mt * p.nt, work = tiles * p.splits;
+    const int work = p.whole + (p.mt * p.nt - p.whole) * p.splits;
     const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-    // Tile t: rows fastest, so CTAs that run together share the columns' operand.
-    auto first_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles) / p.splits); };
-    auto last_step = [&](int t) { return (int)((int64_t)p.ksteps * (t / tiles + 1) / p.splits); };
 
     if (warp == 0) {
         if (lane == 0 && rank == 0) {
@@ -300,8 +346,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 if (i >= 2 && !mbar_wait(&acc_empty[b], ((i >> 1) - 1) & 1, p.err)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + (uint32_t)(b * ACC_COLS);
-                const int k0 = first_step(t), k1 = last_step(t);
-                for (int k = k0; k < k1; ++k, ++j) {
+                const Item it = item_of(p, t);
+                for (int k = it.k0; k < it.k1; ++k, ++j) {
                     const int s = j % p.stages;
                     if (!mbar_wait(&full[s], (j / p.stages) & 1, p.err)) {
                         ok = false;
@@ -314,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                         // 16 summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows
                         const uint64_t da = P == Product::Dw ? desc_mn(sa + q * 2048) : desc_k(sa + q * 32);
                         const uint64_t db = P == Product::Forward ? desc_k(sb + q * 32) : desc_mn(sb + q * 2048);
-                        pair_mma<CG>(acc, da, db, p.idesc, k > k0 || q > 0);
+                        pair_mma<CG>(acc, da, db, p.idesc, k > it.k0 || q > 0);
                     }
                     pair_commit<CG>(&empty[s]);
                 }
@@ -327,11 +373,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             int j = 0;
             bool ok = true;
             for (int t = group; t < work && ok; t += groups) {
-                const int mi = t % p.mt, ni = t / p.mt % p.nt;
-                const int m0 = (P == Product::Dw ? mi : mi * CG + rank) * TM;
-                const int n0 = ni * p.bn;
-                const int k1 = last_step(t);
-                for (int k = first_step(t); k < k1; ++k, ++j) {
+                const Item it = item_of(p, t);
+                const int m0 = (P == Product::Dw ? it.mi : it.mi * CG + rank) * TM;
+                const int n0 = it.ni * p.bn;
+                for (int k = it.k0; k < it.k1; ++k, ++j) {
                     const int s = j % p.stages;
                     if (j >= p.stages && !mbar_wait(&empty[s], ((j / p.stages) & 1) ^ 1, p.err)) {
                         ok = false;
@@ -378,20 +423,23 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             if (!mbar_wait(&acc_full[b], (i >> 1) & 1, p.err)) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * ACC_COLS);
-            const int mi = t % p.mt, ni = t / p.mt % p.nt;
+            const Item it = item_of(p, t);
             const int seg = P == Product::Dw ? rank : 0;
-            const int64_t row0 = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + quarter * 32;
-            const int64_t n0 = (int64_t)ni * p.bn;
+            const int64_t row0 = (int64_t)(P == Product::Dw ? it.mi : it.mi * CG + rank) * TM + quarter * 32;
+            const int64_t n0 = (int64_t)it.ni * p.bn;
+            float4* partial = p.partial + ((int64_t)it.part * CG + rank) * (ACC_COLS / 4) * TM + quarter * 32 + lane;
             const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
             const int ncols = (int)min((int64_t)p.bn, p.N - n0);
             for (int c = half * 32; c < ncols; c += 64) {
                 const int cols = min(32, ncols - c);
-                uint32_t v[32];
+                uint32_t v[32], u[32], w[16];
                 tmem_ld32(acc + (uint32_t)c, v);
-                if constexpr (P == Product::Forward) {
-                    uint32_t u[32], w[16];
-                    tmem_ld32(acc + (uint32_t)(p.bn + c), u);
-                    tmem_wait();
+                if constexpr (P == Product::Forward) tmem_ld32(acc + (uint32_t)(p.bn + c), u);
+                tmem_wait();
+                if (it.part >= 0) {
+                    store_partial(partial + c / 4 * TM, v, p.bn - c);
+                    if constexpr (P == Product::Forward) store_partial(partial + (p.bn + c) / 4 * TM, u, p.bn - c);
+                } else if constexpr (P == Product::Forward) {
                     with_activation(p.act, [&](auto act) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
@@ -404,35 +452,19 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     store_group(my_turn, w, static_cast<T*>(p.out[0]) + row0 * p.ld[0] + n0 + c, p.ld[0],
                                 rows, cols, p.vec[0] != 0);
                     if (p.out[1]) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            w[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), T());
+                        pack_words<T>(w, v);
                         store_group(my_turn, w, static_cast<T*>(p.out[1]) + row0 * p.ld[1] + n0 + c,
                                     p.ld[1], rows, cols, p.vec[1] != 0);
                     }
                     if (p.out[2]) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            w[e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), T());
+                        pack_words<T>(w, u);
                         store_group(my_turn, w, static_cast<T*>(p.out[2]) + row0 * p.ld[2] + n0 + c,
                                     p.ld[2], rows, cols, p.vec[2] != 0);
                     }
                 } else {
-                    tmem_wait();
-                    if (p.splits > 1) {
-                        float4* dst = p.partial + (((int64_t)t * CG + rank) * (ACC_COLS / 4) + c / 4) * TM + quarter * 32 + lane;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            dst[e * TM] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
-                                                      __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
-                    } else {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            w[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), T());
-                        store_group(my_turn, w, static_cast<T*>(p.out[seg]) + row0 * p.ld[seg] + n0 + c,
-                                    p.ld[seg], rows, cols, p.vec[seg] != 0);
-                    }
+                    pack_words<T>(w, v);
+                    store_group(my_turn, w, static_cast<T*>(p.out[seg]) + row0 * p.ld[seg] + n0 + c,
+                                p.ld[seg], rows, cols, p.vec[seg] != 0);
                 }
             }
             tc_fence_before();
@@ -452,33 +484,54 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (warp == 2) tmem_free_all<CG>(tmem);
 }
 
-// Adds the slices of a split sum in slice order and rounds. A warp takes 4 rows x 8 float4 columns.
+// Adds the slices of the split tiles in slice order and finishes them. A warp takes 4 rows x 8 float4
+// columns.
 template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileArgs p) {
-    const int tiles = p.mt * p.nt, lane = threadIdx.x & 31;
+    const int rest = p.mt * p.nt - p.whole, lane = threadIdx.x & 31;
     const int groups = (p.bn + 31) / 32;  // per tile: 32 columns each, by 32 slabs of 4 rows
-    const int64_t warps = (int64_t)tiles * CG * groups * (TM / 4);
+    const int64_t warps = (int64_t)rest * CG * groups * (TM / 4);
+    const int64_t slice = (int64_t)rest * CG * (ACC_COLS / 4) * TM;  // float4s
     for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
         const int slab = (int)(w % (TM / 4)), grp = (int)(w / (TM / 4) % groups);
-        const int part = (int)(w / (TM / 4) / groups), t = part / CG, rank = part % CG;
-        const int mi = t % p.mt, ni = t / p.mt;
+        const int part = (int)(w / (TM / 4) / groups), rank = part % CG;
+        int mi, ni;
+        tile_place(p, p.whole + part / CG, &mi, &ni);
         const int seg = P == Product::Dw ? rank : 0;
         const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
         const int64_t row = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + r;
         const int64_t col = (int64_t)ni * p.bn + c4 * 4;
         if (row >= p.M || col >= p.N || c4 * 4 >= p.bn) continue;
-        const float4* src = p.partial + ((int64_t)part * (ACC_COLS / 4) + c4) * TM + r;
-        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int i = 0; i < p.splits; ++i) {
-            const float4 v = src[(int64_t)i * tiles * CG * (ACC_COLS / 4) * TM];
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
-        T* dst = static_cast<T*>(p.out[seg]) + row * p.ld[seg] + col;
-        if (p.vec[seg] && col + 4 <= p.N) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+        const float4* src = p.partial + (int64_t)part * (ACC_COLS / 4) * TM + r;
+        auto sum = [&](int column4) {
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int i = 0; i < p.splits; ++i) {
+                const float4 v = src[(int64_t)column4 * TM + i * slice];
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            return s;
+        };
+        auto put = [&](int o, float4 s) {
+            T* dst = static_cast<T*>(p.out[o]) + row * p.ld[o] + col;
+            if (p.vec[o] && col + 4 <= p.N) {
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+            } else {
+                const float e[4] = {s.x, s.y, s.z, s.w};
+                for (int i = 0; i < 4 && col + i < p.N; ++i) dst[i] = from_float<T>(e[i]);
+            }
+        };
+        const float4 g = sum(c4);
+        if constexpr (P == Product::Forward) {
+            const float4 u = sum(p.bn / 4 + c4);
+            with_activation(p.act, [&](auto act) {
+                constexpr Activation A = decltype(act)::value;
+                put(0, make_float4(act_value<A>(g.x) * u.x, act_value<A>(g.y) * u.y, act_value<A>(g.z) * u.z,
+                                   act_value<A>(g.w) * u.w));
+            });
+            if (p.out[1]) put(1, g);
+            if (p.out[2]) put(2, u);
         } else {
-            const float e[4] = {s.x, s.y, s.z, s.w};
-            for (int i = 0; i < 4 && col + i < p.N; ++i) dst[i] = from_float<T>(e[i]);
+            put(seg, g);
         }
     }
 }
@@ -512,9 +565,10 @@ void launch_product(Handle& h, TileArgs& t) {
     t.stages = std::min<int>(MAX_STAGES, (SMEM_MAX - TURN_BYTES) / (A_BYTES + t.b_bytes));
     t.err = h.d_err;
     const size_t smem = 1024 + (size_t)t.stages * (A_BYTES + t.b_bytes) + TURN_BYTES + 512;
-    const int64_t work = (int64_t)t.mt * t.nt * t.splits;
+    const int64_t rest = (int64_t)t.mt * t.nt - t.whole;  // split tiles
+    const int64_t work = t.whole + rest * t.splits;
     XS_REQUIRE(work * CG < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
-    DevBuf<float4> ws(t.splits > 1 ? (size_t)work * CG * (ACC_COLS / 4) * TM : 0, h.stream);
+    DevBuf<float4> ws((size_t)rest * t.splits * CG * (ACC_COLS / 4) * TM, h.stream);
     t.partial = ws.get();
     auto kern = tile_kernel<T, P, CG>;
     XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -532,8 +586,8 @@ void launch_product(Handle& h, TileArgs& t) {
     cfg.numAttrs = CG > 1 ? 1 : 0;
     XS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
     after_launch(h, "gated_product");
-    if (t.splits > 1) {
-        const int64_t warps = (int64_t)t.mt * t.nt * CG * ((t.bn + 31) / 32) * (TM / 4);
+    if (rest > 0) {
+        const int64_t warps = rest * CG * ((t.bn + 31) / 32) * (TM / 4);
         const unsigned jg = (unsigned)std::min<int64_t>(ceil_div(warps, 8), (int64_t)sm_count(h.device) * 8);
         join_kernel<T, P, CG><<<jg, 256, 0, h.stream>>>(t);
         after_launch(h, "gated_join");
