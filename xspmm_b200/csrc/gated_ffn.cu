@@ -9,6 +9,8 @@
 // address or row stride is not is first copied to scratch with a stride that is.
 #include "gated_tc.cuh"
 
+#include <initializer_list>
+
 namespace xspmm_b200 {
 namespace {
 
@@ -40,32 +42,58 @@ gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t l
     }
 }
 
-// Rows of `cols` elements from stride ld to stride ldp.
-template <typename T>
-__global__ void __launch_bounds__(256)
-restride_kernel(int64_t rows, int64_t cols, const T* __restrict__ src, int64_t ld,
-                T* __restrict__ dst, int64_t ldp) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int64_t c = threadIdx.x; c < cols; c += 256) dst[r * ldp + c] = src[r * ld + c];
-}
-
 int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 
-// A matrix as TMA can read it: the caller's, or a copy in scratch.
+// Copies of up to three matrices to row strides that TMA can take, in one launch.
 template <typename T>
-struct Rows {
-    const T* p;
-    int64_t ld;
-    DevBuf<T> copy;
-    Rows(Handle& h, const T* src, int64_t lds, int64_t rows, int64_t cols) : p(src), ld(lds) {
-        if (rows <= 1) ld = round8(cols);  // the stride of a single row is never taken
-        if (tma_ok(p, ld) || rows == 0 || cols == 0) return;
-        ld = round8(cols);
-        copy = DevBuf<T>((size_t)(rows * ld), h.stream);
-        const unsigned grid = (unsigned)std::min(rows, (int64_t)sm_count(h.device) * 8);
-        restride_kernel<T><<<grid, 256, 0, h.stream>>>(rows, cols, src, lds, copy.get(), ld);
+struct Restride {
+    struct {
+        const T* src;
+        T* dst;
+        int64_t rows, cols, ld, ldp;
+    } m[3];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) restride_kernel(const __grid_constant__ Restride<T> a) {
+    const auto& m = a.m[blockIdx.y];
+    for (int64_t r = blockIdx.x; r < m.rows; r += gridDim.x)
+#pragma unroll 4
+        for (int64_t c = threadIdx.x; c < m.cols; c += 256) m.dst[r * m.ldp + c] = m.src[r * m.ld + c];
+}
+
+// Matrices as TMA can read them: the caller's, or copies in scratch.
+template <typename T>
+struct Operands {
+    struct Rows {
+        const T* p;
+        int64_t ld, rows, cols;
+    };
+    Rows m[3];
+    DevBuf<T> copy[3];
+    Operands(Handle& h, std::initializer_list<Rows> list) {
+        Restride<T> job = {};
+        int n = 0, jobs = 0;
+        int64_t most = 0;
+        for (Rows r : list) {
+            if (r.rows <= 1) r.ld = round8(r.cols);  // the stride of a single row is never taken
+            if (!tma_ok(r.p, r.ld)) {
+                const int64_t ldp = round8(r.cols);
+                copy[n] = DevBuf<T>((size_t)(r.rows * ldp), h.stream);
+                job.m[jobs++] = {r.p, copy[n].get(), r.rows, r.cols, r.ld, ldp};
+                most = std::max(most, r.rows);
+                r.p = copy[n].get();
+                r.ld = ldp;
+            }
+            m[n++] = r;
+        }
+        if (jobs == 0) return;
+        const dim3 grid((unsigned)std::min(most, (int64_t)sm_count(h.device) * 8), (unsigned)jobs);
+        restride_kernel<T><<<grid, 256, 0, h.stream>>>(job);
         after_launch(h, "gated_restride");
-        p = copy.get();
+    }
+    CUtensorMap map(int i, int box_rows) const {
+        return make_map_2d(m[i].p, (uint64_t)m[i].cols, (uint64_t)m[i].rows, (uint64_t)m[i].ld * 2, 64,
+                           (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     }
 };
 
@@ -140,8 +168,7 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
         zero_rows(h, up, a.F, a.rows, a.F);
         return;
     }
-    const Rows<T> x(h, a.x, a.ldx, a.rows, a.K);
-    const Rows<T> wg(h, a.wg, a.ldwg, a.F, a.K), wu(h, a.wu, a.ldwu, a.F, a.K);
+    const Operands<T> in(h, {{a.x, a.ldx, a.rows, a.K}, {a.wg, a.ldwg, a.F, a.K}, {a.wu, a.ldwu, a.F, a.K}});
     TileArgs t = {};
     t.M = a.rows;
     t.N = a.F;
@@ -151,16 +178,13 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
     t.cols_first = a.rows > 2 * a.F;  // the operand of the inner index is read again and should fit L2
     if (cg == 2) choose_tiles<Product::Forward, 2>(h, t);
     else choose_tiles<Product::Forward, 1>(h, t);
-    t.a[0] = map_of(x.p, x.ld, a.rows, a.K, TM);
-    t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, t.bn);
-    t.b[1] = map_of(wu.p, wu.ld, a.F, a.K, t.bn);
+    t.a[0] = in.map(0, TM);
+    t.b[0] = in.map(1, t.bn);
+    t.b[1] = in.map(2, t.bn);
     t.act = a.act;
-    T* outs[3] = {y, gate, up};
-    for (int i = 0; i < 3; ++i) {
-        t.out[i] = outs[i];
-        t.ld[i] = i == 0 ? ldy : a.F;
-        t.vec[i] = store16_ok(outs[i], t.ld[i]);
-    }
+    set_output(t, 0, y, ldy);
+    set_output(t, 1, gate, a.F);
+    set_output(t, 2, up, a.F);
     if (cg == 2) launch_product<T, Product::Forward, 2>(h, t);
     else launch_product<T, Product::Forward, 1>(h, t);
 }
@@ -193,7 +217,7 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         after_launch(h, "gated_slopes");
     }
     if (dx) {
-        const Rows<T> wg(h, a.wg, a.ldwg, a.F, a.K), wu(h, a.wu, a.ldwu, a.F, a.K);
+        const Operands<T> in(h, {{a.wg, a.ldwg, a.F, a.K}, {a.wu, a.ldwu, a.F, a.K}});
         TileArgs t = {};
         t.M = a.rows;
         t.N = a.K;
@@ -206,16 +230,14 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         else choose_tiles<Product::Dx, 1>(h, t);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TM);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TM);
-        t.b[0] = map_of(wg.p, wg.ld, a.F, a.K, TK);
-        t.b[1] = map_of(wu.p, wu.ld, a.F, a.K, TK);
-        t.out[0] = dx;
-        t.ld[0] = lddx;
-        t.vec[0] = store16_ok(dx, lddx);
+        t.b[0] = in.map(0, TK);
+        t.b[1] = in.map(1, TK);
+        set_output(t, 0, dx, lddx);
         if (cg == 2) launch_product<T, Product::Dx, 2>(h, t);
         else launch_product<T, Product::Dx, 1>(h, t);
     }
     if (dwg) {
-        const Rows<T> x(h, a.x, a.ldx, a.rows, a.K);
+        const Operands<T> in(h, {{a.x, a.ldx, a.rows, a.K}});
         TileArgs t = {};
         t.M = a.F;
         t.N = a.K;
@@ -225,13 +247,9 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         choose_tiles<Product::Dw, 2>(h, t);
         t.a[0] = map_of<T>(dg, ldp, a.rows, a.F, TK);
         t.a[1] = map_of<T>(du, ldp, a.rows, a.F, TK);
-        t.b[0] = map_of(x.p, x.ld, a.rows, a.K, TK);
-        t.out[0] = dwg;
-        t.out[1] = dwu;
-        for (int i = 0; i < 2; ++i) {
-            t.ld[i] = a.K;
-            t.vec[i] = store16_ok(t.out[i], a.K);
-        }
+        t.b[0] = in.map(0, TK);
+        set_output(t, 0, dwg, a.K);
+        set_output(t, 1, dwu, a.K);
         launch_product<T, Product::Dw, 2>(h, t);
     }
 }

@@ -23,9 +23,8 @@
 // Roles (384 threads, one CTA per SM): warp 0 of the pair's first CTA issues the MMAs (one lane), warp
 // 1 of each the loads of its own operands (one lane; they report to the first CTA's barrier), warp 2
 // allocates TMEM, warps 4..11 are the epilogue. TMEM holds two accumulators used in turn, so a tile's
-// epilogue runs under the next tile's products. The epilogue converts 32 columns at a time and turns
-// them through a warp's own piece of shared memory, so global stores are 16 bytes a lane and 64
-// contiguous bytes a row. Every wait is bounded; a timeout sets the error flag, and TMEM is freed only
+// epilogue runs under the next tile's products. The epilogue converts 32 columns at a time and stores
+// them by TMA from a warp's own pieces of shared memory (an output that TMA cannot address: row by row). Every wait is bounded; a timeout sets the error flag, and TMEM is freed only
 // after the MMAs that were issued have completed.
 //
 // Tiles that would leave part of the GPU idle (the last wave's, or all where there are few) have their
@@ -48,8 +47,9 @@ constexpr int FIRST_EPI = 4, EPI_WARPS = 8;
 constexpr int THREADS = 32 * (FIRST_EPI + EPI_WARPS);
 constexpr int A_BYTES = TM * 128;       // one stage of A
 constexpr int CHUNK = TK * 128;         // MN-major: 64 columns by TK summed rows
-constexpr int TURN_LD = 80;             // epilogue staging: 64 bytes of a row, padded off the banks
-constexpr int TURN_BYTES = EPI_WARPS * 32 * TURN_LD;
+constexpr int TURN = 32 * 64;           // epilogue staging: 32 rows of 64 bytes, SWIZZLE_64B
+constexpr int TURNS = 3;                // pieces of it per warp, used in turn
+constexpr int TURN_BYTES = EPI_WARPS * TURNS * TURN;
 constexpr int MAX_STAGES = 8;
 constexpr int SMEM_MAX = 232448 - 1024 - 512;  // opt-in limit less alignment and barriers
 
@@ -67,11 +67,17 @@ struct TileArgs {
     Activation act;
     void* out[3];       // Forward: y, gate, up; Dx: dx; Dw: dwg, dwu
     int64_t ld[3];
-    int vec[3];         // 16-byte stores allowed
+    int tma[3];         // 16-byte stores, whole groups through omap; else element by element
+    CUtensorMap omap[3];
     float4* partial;    // split tiles: [slice][tile][CTA][column / 4][row]
     unsigned* err;
 };
 
+__device__ __forceinline__ float exp2f_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // __fdividef(1, d) is 0 for d above 2^126, as the quotient nearly is.
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
@@ -81,6 +87,23 @@ __device__ __forceinline__ float act_value(float v) {
     else if constexpr (ACT == Activation::Gelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
     else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
     else return sigmoid(v);
+}
+// act of two values. Silu's two quotients share one reciprocal, 1 / a0 = a1 / (a0 a1): the special
+// function unit (16 lanes a clock on an SM) bounds the epilogue of short sums, and this takes three of
+// its operations instead of four. The exponent is capped at 2^60, where v * 2^-60 is nothing against any
+// value it is added to, so that a0 a1 stays finite.
+template <Activation ACT>
+__device__ __forceinline__ void act_pair(float v0, float v1, float* o0, float* o1) {
+    if constexpr (ACT == Activation::Silu) {
+        const float a0 = 1.0f + exp2f_approx(fminf(v0 * -1.4426950408889634f, 60.0f));
+        const float a1 = 1.0f + exp2f_approx(fminf(v1 * -1.4426950408889634f, 60.0f));
+        const float r = __fdividef(1.0f, a0 * a1);
+        *o0 = v0 * (a1 * r);
+        *o1 = v1 * (a0 * r);
+    } else {
+        *o0 = act_value<ACT>(v0);
+        *o1 = act_value<ACT>(v1);
+    }
 }
 // act(v) and act'(v).
 template <Activation ACT>
@@ -246,36 +269,47 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to out[row0.., col0..], `rows` x
-// `cols` of them valid, turned through the warp's staging area.
+// A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to output `o` at (row0, col0), turned
+// through one of the warp's staging pieces. `rows` x `cols` of them are valid.
 template <typename T>
-__device__ __forceinline__ void store_group(uint8_t* turn, const uint32_t (&w)[16], T* out,
-                                            int64_t ld, int rows, int cols, bool vec) {
+__device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* turn, int& piece,
+                                            const uint32_t (&w)[16], int64_t row0, int64_t col0,
+                                            int rows, int cols) {
     const int lane = threadIdx.x & 31;
-    __syncwarp();
+    uint8_t* at = turn + piece * TURN;
+    piece = piece == TURNS - 1 ? 0 : piece + 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(TURNS - 1) : "memory");
+    __syncwarp();  // the piece's last store has read it
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint4*>(turn + lane * TURN_LD + i * 16) =
+        *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) =
             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    __syncwarp();
-    if (vec) {
-        const int c = (lane & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (lane >> 2) + 8 * i;
-            if (r >= rows || c >= cols) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(turn + r * TURN_LD + c * 2);
-            T* dst = out + r * ld + c;
-            if (c + 8 <= cols) {
-                *reinterpret_cast<uint4*>(dst) = v;
-            } else {
-                const T* e = reinterpret_cast<const T*>(turn + r * TURN_LD) + c;
-                for (int j = 0; j < cols - c; ++j) dst[j] = e[j];
-            }
+    if (p.tma[o] && cols == 32) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            if (rows > 0)
+                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                 reinterpret_cast<uint64_t>(&p.omap[o])),
+                             "r"((int)col0), "r"((int)row0), "r"(smem_u32(at))
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-    } else if (lane < cols) {
-        for (int r = 0; r < rows; ++r)
-            out[r * ld + lane] = reinterpret_cast<const T*>(turn + r * TURN_LD)[lane];
+    } else {
+        __syncwarp();
+        T* out = static_cast<T*>(p.out[o]) + row0 * p.ld[o] + col0;
+        if (p.tma[o]) {  // a tile's last columns, a multiple of 8: 16-byte pieces
+            const int per = cols >> 3;
+            for (int i = lane; i < rows * per; i += 32) {
+                const int r = i / per, c = i - r * per;
+                *reinterpret_cast<uint4*>(out + r * p.ld[o] + c * 8) =
+                    *reinterpret_cast<const uint4*>(at + r * 64 + ((c ^ ((r >> 1) & 3)) * 16));
+            }
+        } else if (lane < cols)
+            for (int r = 0; r < rows; ++r)
+                out[r * p.ld[o] + lane] = reinterpret_cast<const T*>(
+                    at + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16))[lane & 7];
+        __syncwarp();
     }
 }
 
@@ -417,7 +451,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp >= FIRST_EPI) {
         const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
-        uint8_t* my_turn = turn + (warp - FIRST_EPI) * 32 * TURN_LD;
+        uint8_t* my_turn = turn + (warp - FIRST_EPI) * TURNS * TURN;
+        int piece = 0;
         for (int t = group, i = 0; t < work; t += groups, ++i) {
             const int b = i & 1;
             if (!mbar_wait(&acc_full[b], (i >> 1) & 1, p.err)) break;
@@ -443,28 +478,23 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     with_activation(p.act, [&](auto act) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float g0 = __uint_as_float(v[2 * e]), g1 = __uint_as_float(v[2 * e + 1]);
-                            w[e] = pack2(act_value<decltype(act)::value>(g0) * __uint_as_float(u[2 * e]),
-                                         act_value<decltype(act)::value>(g1) * __uint_as_float(u[2 * e + 1]),
-                                         T());
+                            float a0, a1;
+                            act_pair<decltype(act)::value>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), &a0, &a1);
+                            w[e] = pack2(a0 * __uint_as_float(u[2 * e]), a1 * __uint_as_float(u[2 * e + 1]), T());
                         }
                     });
-                    store_group(my_turn, w, static_cast<T*>(p.out[0]) + row0 * p.ld[0] + n0 + c, p.ld[0],
-                                rows, cols, p.vec[0] != 0);
+                    store_group<T>(p, 0, my_turn, piece, w, row0, n0 + c, rows, cols);
                     if (p.out[1]) {
                         pack_words<T>(w, v);
-                        store_group(my_turn, w, static_cast<T*>(p.out[1]) + row0 * p.ld[1] + n0 + c,
-                                    p.ld[1], rows, cols, p.vec[1] != 0);
+                        store_group<T>(p, 1, my_turn, piece, w, row0, n0 + c, rows, cols);
                     }
                     if (p.out[2]) {
                         pack_words<T>(w, u);
-                        store_group(my_turn, w, static_cast<T*>(p.out[2]) + row0 * p.ld[2] + n0 + c,
-                                    p.ld[2], rows, cols, p.vec[2] != 0);
+                        store_group<T>(p, 2, my_turn, piece, w, row0, n0 + c, rows, cols);
                     }
                 } else {
                     pack_words<T>(w, v);
-                    store_group(my_turn, w, static_cast<T*>(p.out[seg]) + row0 * p.ld[seg] + n0 + c,
-                                p.ld[seg], rows, cols, p.vec[seg] != 0);
+                    store_group<T>(p, seg, my_turn, piece, w, row0, n0 + c, rows, cols);
                 }
             }
             tc_fence_before();
@@ -474,6 +504,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 else mbar_arrive(&acc_empty[b]);
             }
         }
+        // the stores have read the shared memory they come from before the CTA gives it up
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     __syncwarp();
     if (warp == 2) mbar_wait(done, 0, p.err);  // bounded; completes once the last MMA has
@@ -484,55 +516,67 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (warp == 2) tmem_free_all<CG>(tmem);
 }
 
-// Adds the slices of the split tiles in slice order and finishes them. A warp takes 4 rows x 8 float4
-// columns.
+// Adds the slices of the split tiles and finishes them. A CTA takes 4 rows x 32 columns; its eight warps
+// add every eighth slice, and the eight sums are added in order: one fixed order for each size.
 template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileArgs p) {
-    const int rest = p.mt * p.nt - p.whole, lane = threadIdx.x & 31;
+    __shared__ float4 red[2][8][32];
+    const int rest = p.mt * p.nt - p.whole, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int groups = (p.bn + 31) / 32;  // per tile: 32 columns each, by 32 slabs of 4 rows
-    const int64_t warps = (int64_t)rest * CG * groups * (TM / 4);
     const int64_t slice = (int64_t)rest * CG * (ACC_COLS / 4) * TM;  // float4s
-    for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
-        const int slab = (int)(w % (TM / 4)), grp = (int)(w / (TM / 4) % groups);
-        const int part = (int)(w / (TM / 4) / groups), rank = part % CG;
-        int mi, ni;
-        tile_place(p, p.whole + part / CG, &mi, &ni);
-        const int seg = P == Product::Dw ? rank : 0;
-        const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
-        const int64_t row = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + r;
-        const int64_t col = (int64_t)ni * p.bn + c4 * 4;
-        if (row >= p.M || col >= p.N || c4 * 4 >= p.bn) continue;
-        const float4* src = p.partial + (int64_t)part * (ACC_COLS / 4) * TM + r;
-        auto sum = [&](int column4) {
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int i = 0; i < p.splits; ++i) {
+    const int slab = (int)(blockIdx.x % (TM / 4)), grp = (int)(blockIdx.x / (TM / 4) % groups);
+    const int part = (int)(blockIdx.x / (TM / 4) / groups), rank = part % CG;
+    int mi, ni;
+    tile_place(p, p.whole + part / CG, &mi, &ni);
+    const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
+    const int64_t row = (int64_t)(P == Product::Dw ? mi : mi * CG + rank) * TM + r;
+    const int64_t col = (int64_t)ni * p.bn + c4 * 4;
+    const bool in = row < p.M && col < p.N && c4 * 4 < p.bn;
+    const float4* src = p.partial + (int64_t)part * (ACC_COLS / 4) * TM + r;
+    auto sum = [&](int column4) {
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (in)
+#pragma unroll 4
+            for (int i = warp; i < p.splits; i += 8) {
                 const float4 v = src[(int64_t)column4 * TM + i * slice];
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
-            return s;
-        };
-        auto put = [&](int o, float4 s) {
-            T* dst = static_cast<T*>(p.out[o]) + row * p.ld[o] + col;
-            if (p.vec[o] && col + 4 <= p.N) {
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
-            } else {
-                const float e[4] = {s.x, s.y, s.z, s.w};
-                for (int i = 0; i < 4 && col + i < p.N; ++i) dst[i] = from_float<T>(e[i]);
-            }
-        };
-        const float4 g = sum(c4);
-        if constexpr (P == Product::Forward) {
-            const float4 u = sum(p.bn / 4 + c4);
-            with_activation(p.act, [&](auto act) {
-                constexpr Activation A = decltype(act)::value;
-                put(0, make_float4(act_value<A>(g.x) * u.x, act_value<A>(g.y) * u.y, act_value<A>(g.z) * u.z,
-                                   act_value<A>(g.w) * u.w));
-            });
-            if (p.out[1]) put(1, g);
-            if (p.out[2]) put(2, u);
-        } else {
-            put(seg, g);
+        return s;
+    };
+    red[0][warp][lane] = sum(c4);
+    if (P == Product::Forward) red[1][warp][lane] = sum(p.bn / 4 + c4);
+    __syncthreads();
+    if (warp > 0 || !in) return;
+    auto total = [&](int which) {
+        float4 s = red[which][0][lane];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            const float4 v = red[which][i][lane];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
+        return s;
+    };
+    auto put = [&](int o, float4 s) {
+        T* dst = static_cast<T*>(p.out[o]) + row * p.ld[o] + col;
+        if (p.tma[o] && col + 4 <= p.N) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+        } else {
+            const float e[4] = {s.x, s.y, s.z, s.w};
+            for (int i = 0; i < 4 && col + i < p.N; ++i) dst[i] = from_float<T>(e[i]);
+        }
+    };
+    const float4 g = total(0);
+    if constexpr (P == Product::Forward) {
+        const float4 u = total(1);
+        with_activation(p.act, [&](auto act) {
+            constexpr Activation A = decltype(act)::value;
+            put(0, make_float4(act_value<A>(g.x) * u.x, act_value<A>(g.y) * u.y, act_value<A>(g.z) * u.z,
+                               act_value<A>(g.w) * u.w));
+        });
+        if (p.out[1]) put(1, g);
+        if (p.out[2]) put(2, u);
+    } else {
+        put(P == Product::Dw ? rank : 0, g);
     }
 }
 
@@ -543,10 +587,22 @@ inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int m, int n) {
            (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// Whether TMA can address rows of a 16-bit matrix: 16-byte base and row stride.
-inline bool tma_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+// Whether TMA can address rows of a 16-bit matrix: 16-byte base and row stride (below 2^40 bytes).
+inline bool tma_ok(const void* p, int64_t ld) {
+    return aligned_to(p, 16) && ld % 8 == 0 && ld < (int64_t(1) << 39);
+}
 
-inline bool store16_ok(const void* p, int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+// Sets output `i`: an M x N matrix (or none) with row stride ld. A TMA store writes whole 16-byte pieces of
+// a row, so its rows have to end on one.
+inline void set_output(TileArgs& t, int i, void* out, int64_t ld) {
+    if (out && t.M == 1) ld = t.N;  // the stride of a single row is never taken
+    t.out[i] = out;
+    t.ld[i] = ld;
+    t.tma[i] = out && t.N % 8 == 0 && tma_ok(out, ld);
+    if (t.tma[i])
+        t.omap[i] = make_map_2d(out, (uint64_t)t.N, (uint64_t)t.M, (uint64_t)ld * 2, 32, 32,
+                                CU_TENSOR_MAP_SWIZZLE_64B);
+}
 
 // Accumulator columns (MMA N) of a tile of bn output columns: a multiple of 16, in a pair of 32.
 template <Product P, int CG>
@@ -587,9 +643,8 @@ void launch_product(Handle& h, TileArgs& t) {
     XS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
     after_launch(h, "gated_product");
     if (rest > 0) {
-        const int64_t warps = rest * CG * ((t.bn + 31) / 32) * (TM / 4);
-        const unsigned jg = (unsigned)std::min<int64_t>(ceil_div(warps, 8), (int64_t)sm_count(h.device) * 8);
-        join_kernel<T, P, CG><<<jg, 256, 0, h.stream>>>(t);
+        const int64_t blocks = rest * CG * ((t.bn + 31) / 32) * (TM / 4);
+        join_kernel<T, P, CG><<<(unsigned)blocks, 256, 0, h.stream>>>(t);
         after_launch(h, "gated_join");
     }
 }
