@@ -48,7 +48,7 @@ constexpr int THREADS = 32 * (FIRST_EPI + EPI_WARPS);
 constexpr int A_BYTES = TM * 128;       // one stage of A
 constexpr int CHUNK = TK * 128;         // MN-major: 64 columns by TK summed rows
 constexpr int TURN = 32 * 64;           // epilogue staging: 32 rows of 64 bytes, SWIZZLE_64B
-constexpr int TURNS = 3;                // pieces of it per warp, used in turn
+constexpr int TURNS = 2;                // pieces of it per warp, used in turn
 constexpr int TURN_BYTES = EPI_WARPS * TURNS * TURN;
 constexpr int MAX_STAGES = 8;
 constexpr int SMEM_MAX = 232448 - 1024 - 512;  // opt-in limit less alignment and barriers
