@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <string>
 #include <stdexcept>
+#include <utility>
 
 #include "../../include/xspmm_b200.h"
 
@@ -86,6 +87,28 @@ inline void after_launch(Handle& h, const char* what) {
         throw Error(XSPMM_STATUS_CUDA_ERROR, std::string("launch of ") + what + ": " +
                                                  cudaGetErrorString(e));
     ++h.launches;
+}
+
+// Launches a kernel that calls cudaGridDependencySynchronize() before it touches memory: its launch and
+// prologue overlap the end of the stream's previous kernel.
+template <typename... P, typename... A>
+void launch_dependent(cudaStream_t stream, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster,
+                      A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    XS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
 }
 
 // Reads and clears the device error word (synchronizes the stream).

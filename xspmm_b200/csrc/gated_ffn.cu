@@ -7,6 +7,7 @@
 //
 // The products run on the tensor cores (gated_tc.cuh). TMA needs 16-byte rows: an operand whose
 // address or row stride is not is first copied to scratch with a stride that is.
+#include "gated_few.cuh"
 #include "gated_tc.cuh"
 
 #include <initializer_list>
@@ -166,6 +167,10 @@ void gated_ffn(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* 
         zero_rows(h, y, ldy, a.rows, a.F);
         zero_rows(h, gate, a.F, a.rows, a.F);
         zero_rows(h, up, a.F, a.rows, a.F);
+        return;
+    }
+    if (a.rows <= 16) {
+        few_rows(h, a, y, ldy, gate, up);
         return;
     }
     const Operands<T> in(h, {{a.x, a.ldx, a.rows, a.K}, {a.wg, a.ldwg, a.F, a.K}, {a.wu, a.ldwu, a.F, a.K}});

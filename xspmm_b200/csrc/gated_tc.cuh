@@ -367,6 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    cudaGridDependencySynchronize();  // what came before wrote the operands
 
     const int work = p.whole + (p.mt * p.nt - p.whole) * p.splits;
     const int group = blockIdx.x / CG, groups = gridDim.x / CG;
@@ -521,6 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 template <typename T, Product P, int CG>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileArgs p) {
     __shared__ float4 red[2][8][32];
+    cudaGridDependencySynchronize();
     const int rest = p.mt * p.nt - p.whole, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int groups = (p.bn + 31) / 32;  // per tile: 32 columns each, by 32 slabs of 4 rows
     const int64_t slice = (int64_t)rest * CG * (ACC_COLS / 4) * TM;  // float4s
@@ -628,23 +630,12 @@ void launch_product(Handle& h, TileArgs& t) {
     t.partial = ws.get();
     auto kern = tile_kernel<T, P, CG>;
     XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(work, sm_count(h.device) / CG) * CG));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = h.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = CG > 1 ? 1 : 0;
-    XS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
+    const unsigned grid = (unsigned)(std::min<int64_t>(work, sm_count(h.device) / CG) * CG);
+    launch_dependent(h.stream, kern, grid, THREADS, smem, CG, t);
     after_launch(h, "gated_product");
     if (rest > 0) {
         const int64_t blocks = rest * CG * ((t.bn + 31) / 32) * (TM / 4);
-        join_kernel<T, P, CG><<<(unsigned)blocks, 256, 0, h.stream>>>(t);
+        launch_dependent(h.stream, join_kernel<T, P, CG>, (unsigned)blocks, 256, 0, 1, t);
         after_launch(h, "gated_join");
     }
 }

@@ -456,26 +456,37 @@ layer_norm_grad_kernel(const TileSource<TY> dy, const TileSource<TX> x, const fl
     }
 }
 
-// out[0 | 1][column] = sum of the partials in CTA order: 32 columns, 32 strided slices of the CTAs.
-__global__ void __launch_bounds__(1024, 1)
+// out[0 | 1][column] = sum of the partials in a fixed order: 32 columns (16 bytes a lane, or with an odd D
+// one element), 32 strided slices of the CTAs.
+template <bool VEC>
+__global__ void __launch_bounds__(VEC ? 256 : 1024)
 layer_norm_join_kernel(const float* __restrict__ part, int parts, int D, float* dw, float* db) {
+    constexpr int V = VEC ? 4 : 1, LANES = 32 / V;
     __shared__ float red[32][33];
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
-    const float* src = part + (int64_t)blockIdx.y * parts * D;
-    float s = 0.0f;
+    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+    const int c = blockIdx.x * 32 + lane * V;
+    float s[V] = {};
+    cudaGridDependencySynchronize();
     if (c < D) {
-#pragma unroll 8
-        for (int i = slice; i < parts; i += 32) s += src[(int64_t)i * D + c];
+        const float* src = part + (int64_t)blockIdx.y * parts * D + c;
+#pragma unroll 4
+        for (int i = slice; i < parts; i += 32) {
+            float v[V];
+            load_pack<float, V>(src + (int64_t)i * D, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += v[e];
+        }
     }
-    red[slice][lane] = s;
+#pragma unroll
+    for (int e = 0; e < V; ++e) red[slice][lane * V + e] = s[e];
     __syncthreads();
-    if (slice == 0 && c < D) {
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && col < D) {
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) t += red[i][lane];
+        for (int i = 0; i < 32; ++i) t += red[i][threadIdx.x];
         float* out = blockIdx.y == 0 ? dw : db;
-        if (out) out[c] = t;
+        if (out) out[col] = t;
     }
 }
 
@@ -659,8 +670,10 @@ void norm_grad_launch(Handle& h, int64_t rows, int64_t D, const TY* dy, int64_t 
                                           h.d_err);
     after_launch(h, "layer_norm_grad");
     if (sums) {
-        layer_norm_join_kernel<<<dim3((unsigned)ceil_div(D, 32), 2), 1024, 0, h.stream>>>(
-            part.get(), (int)grid, (int)D, dw, db);
+        const bool vec = D % 4 == 0;
+        launch_dependent(h.stream, vec ? layer_norm_join_kernel<true> : layer_norm_join_kernel<false>,
+                         dim3((unsigned)ceil_div(D, 32), 2), vec ? 256 : 1024, 0, 1,
+                         (const float*)part.get(), (int)grid, (int)D, dw, db);
         after_launch(h, "layer_norm_join");
     }
 }
