@@ -1,5 +1,8 @@
 """CPU tests of the layer operators' argument checks (xspmm_b200/layers.py and the C entries behind
 it): what is refused is refused with a message before anything runs. No kernel is launched."""
+import os
+import subprocess
+
 import pytest
 import torch
 
@@ -102,3 +105,38 @@ def test_c_entries_reject_a_null_handle():
     assert L.xspmm_gated_ffn_backward_bf16(None, 1, 8, 8, 0, None, 8, None, 8, None, 8, None, 8, None,
                                            None, None, 8, None, None) == 1
     assert b"null handle" in L.xspmm_last_error()
+
+
+_CPP = r"""
+#include "xspmm/layers.hpp"
+using E = std::shared_ptr<const xspmm::Executor>;
+template <typename X, typename Y> void norm(E e, X* x, Y* y, float* f) {
+    xspmm::layer_norm<X, Y>(e, 4, 8, {x, 8}, f, f, 1e-5f, {y, 8}, f, f);
+    xspmm::layer_norm_backward<X, Y>(e, 4, 8, {y, 8}, {x, 8}, f, f, f, {y, 8}, f, f);
+}
+template <typename T> void drop(E e, T* x) { xspmm::dropout<T>(e, 8, x, nullptr, 0.5, 1u, 2u, x); }
+template <typename T> void gated(E e, T* t) {
+    xspmm::gated_ffn<T>(e, 4, 8, 6, xspmm::Activation::Gelu, {t, 8}, {t, 8}, {t, 8}, {t, 6}, t, t);
+    xspmm::gated_ffn_backward<T>(e, 4, 8, 6, xspmm::Activation::Silu, {t, 6}, {t, 8}, {t, 8}, {t, 8}, t, t,
+                                 {t, 8}, t, t);
+}
+template void norm(E, __half*, __half*, float*);
+template void norm(E, __nv_bfloat16*, __nv_bfloat16*, float*);
+template void norm(E, float*, float*, float*);
+template void norm(E, float*, __half*, float*);
+template void norm(E, float*, __nv_bfloat16*, float*);
+template void drop(E, __half*);
+template void drop(E, __nv_bfloat16*);
+template void drop(E, float*);
+template void gated(E, __half*);
+template void gated(E, __nv_bfloat16*);
+"""
+
+
+def test_cpp_header_instantiates_every_type(tmp_path):
+    src = tmp_path / "layers.cpp"
+    src.write_text(_CPP)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run(["g++", "-std=c++20", "-fsyntax-only", "-I" + os.path.join(root, "include"),
+                        "-I/usr/local/cuda/include", str(src)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
