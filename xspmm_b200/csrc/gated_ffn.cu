@@ -8,6 +8,7 @@
 // The products run on the tensor cores (gated_tc.cuh). TMA needs 16-byte rows: an operand whose
 // address or row stride is not is first copied to scratch with a stride that is.
 #include "gated_few.cuh"
+#include "gated_small.cuh"
 #include "gated_tc.cuh"
 
 #include <initializer_list>
@@ -206,6 +207,10 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         return;
     }
     if (!dx && !dwg) return;
+    if (small_grad_ok(a, dy, lddy, gate, up, dx, lddx, dwg)) {
+        small_grad(h, a, dy, lddy, gate, up, dx, lddx, dwg, dwu);
+        return;
+    }
     const int64_t ldp = round8(a.F);
     DevBuf<T> d((size_t)(2 * a.rows * ldp), h.stream);
     T *dg = d.get(), *du = d.get() + a.rows * ldp;

@@ -271,14 +271,14 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
 
 // A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to output `o` at (row0, col0), turned
 // through one of the warp's staging pieces. `rows` x `cols` of them are valid.
-template <typename T>
+template <typename T, int PIECES = TURNS>
 __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* turn, int& piece,
                                             const uint32_t (&w)[16], int64_t row0, int64_t col0,
                                             int rows, int cols) {
     const int lane = threadIdx.x & 31;
     uint8_t* at = turn + piece * TURN;
-    piece = piece == TURNS - 1 ? 0 : piece + 1;
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(TURNS - 1) : "memory");
+    piece = piece == PIECES - 1 ? 0 : piece + 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PIECES - 1) : "memory");
     __syncwarp();  // the piece's last store has read it
 #pragma unroll
     for (int i = 0; i < 4; ++i)
