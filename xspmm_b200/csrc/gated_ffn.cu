@@ -32,12 +32,21 @@ gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t l
         load_pack<T, V>(dy + r * lddy + c, d);
         load_pack<T, V>(gate + r * F + c, g);
         load_pack<T, V>(up + r * F + c, u);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
+        if constexpr (V == 1) {
             float value, slope;
-            act_both<ACT>(g[e], &value, &slope);
-            a[e] = d[e] * u[e] * slope;
-            b[e] = d[e] * value;
+            act_both<ACT>(g[0], &value, &slope);
+            a[0] = d[0] * u[0] * slope;
+            b[0] = d[0] * value;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                float v0, v1, s0, s1;
+                act_both_pair<ACT>(g[e], g[e + 1], &v0, &s0, &v1, &s1);
+                a[e] = d[e] * u[e] * s0;
+                a[e + 1] = d[e + 1] * u[e + 1] * s1;
+                b[e] = d[e] * v0;
+                b[e + 1] = d[e + 1] * v1;
+            }
         }
         store_pack<T, V>(dg + r * ldp + c, a);
         store_pack<T, V>(du + r * ldp + c, b);

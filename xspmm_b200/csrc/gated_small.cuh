@@ -120,10 +120,22 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_grad_kernel(const __grid_
             for (int m = 0; m < 2; ++m)
                 for (int c = 0; c < kchunks; ++c)
                     tma_load_2d(smem + SM_W + (2 * m + c) * SM_CHUNK, &p.t.b[m], 64 * c, 0, w_full);
+            // dy, gate and up of a tile, on their way to L2 while the warps have up to two tiles before it to do
+            auto prefetch = [&](const void* m, int64_t ld, int t) {
+                if (ld != p.F) return;
+                const int64_t r = (int64_t)t * TM, n = min((int64_t)TM, p.t.M - r);
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                                 static_cast<const T*>(m) + r * p.F),
+                             "r"((uint32_t)(n * p.F * sizeof(T)))
+                             : "memory");
+            };
             int i = 0;
             for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
                 const int b = i & 1;
                 if (i >= 2 && !mbar_wait(&x_empty[b], ((i >> 1) - 1) & 1, err)) break;
+                prefetch(p.dy, p.lddy, t);
+                prefetch(p.gate, p.F, t);
+                prefetch(p.up, p.F, t);
                 mbar_expect_tx(&x_full[b], (uint32_t)(kchunks * SM_CHUNK));
                 for (int c = 0; c < kchunks; ++c)
                     tma_load_2d(smem + SM_X + (2 * b + c) * SM_CHUNK, &p.t.a[0], 64 * c, t * TM, &x_full[b]);
@@ -186,32 +198,34 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_grad_kernel(const __grid_
         int i = 0, t = blockIdx.x;
         load(t);
         for (; t < p.tiles && ok; t += gridDim.x, ++i) {
-            if (i > 0 && !mbar_wait(d_empty, (i - 1) & 1, err)) {
-                ok = false;
-                break;
-            }
+            // dg into d and du into g, under the MMAs of the tile before; only the stores wait for them
             with_activation(p.t.act, [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (row[j] >= TM) continue;
-                    const uint32_t dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
-                    const uint32_t gw[4] = {g[j].x, g[j].y, g[j].z, g[j].w};
-                    const uint32_t uw[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-                    uint32_t og[4], ou[4];
+                    uint32_t* dw = reinterpret_cast<uint32_t*>(&d[j]);
+                    uint32_t* gw = reinterpret_cast<uint32_t*>(&g[j]);
+                    const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u[j]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 d2 = unpack2(dw[e], T()), g2 = unpack2(gw[e], T()), u2 = unpack2(uw[e], T());
                         float v0, v1, s0, s1;
-                        act_both<decltype(act)::value>(g2.x, &v0, &s0);
-                        act_both<decltype(act)::value>(g2.y, &v1, &s1);
-                        og[e] = pack2(d2.x * u2.x * s0, d2.y * u2.y * s1, T());
-                        ou[e] = pack2(d2.x * v0, d2.y * v1, T());
+                        act_both_pair<decltype(act)::value>(g2.x, g2.y, &v0, &s0, &v1, &s1);
+                        dw[e] = pack2(d2.x * u2.x * s0, d2.y * u2.y * s1, T());
+                        gw[e] = pack2(d2.x * v0, d2.y * v1, T());
                     }
-                    uint8_t* at = smem + SM_D + pos[j] / 8 * SM_CHUNK + row[j] * 128 + ((pos[j] ^ row[j]) & 7) * 16;
-                    *reinterpret_cast<uint4*>(at) = make_uint4(og[0], og[1], og[2], og[3]);
-                    *reinterpret_cast<uint4*>(at + 2 * SM_CHUNK) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
                 }
             });
+            if (i > 0 && !mbar_wait(d_empty, (i - 1) & 1, err)) {
+                ok = false;
+                break;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (row[j] >= TM) continue;
+                uint8_t* at = smem + SM_D + pos[j] / 8 * SM_CHUNK + row[j] * 128 + ((pos[j] ^ row[j]) & 7) * 16;
+                *reinterpret_cast<uint4*>(at) = d[j];
+                *reinterpret_cast<uint4*>(at + 2 * SM_CHUNK) = g[j];
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(d_full);

@@ -126,6 +126,24 @@ __device__ __forceinline__ void act_both(float v, float* value, float* slope) {
     }
 }
 
+// act_both of two values; silu's sigmoids share a reciprocal as in act_pair.
+template <Activation ACT>
+__device__ __forceinline__ void act_both_pair(float v0, float v1, float* value0, float* slope0, float* value1,
+                                              float* slope1) {
+    if constexpr (ACT == Activation::Silu) {
+        const float a0 = 1.0f + exp2f_approx(fminf(v0 * -1.4426950408889634f, 60.0f));
+        const float a1 = 1.0f + exp2f_approx(fminf(v1 * -1.4426950408889634f, 60.0f));
+        const float r = __fdividef(1.0f, a0 * a1), s0 = a1 * r, s1 = a0 * r;
+        *value0 = v0 * s0;
+        *value1 = v1 * s1;
+        *slope0 = s0 * (1.0f + v0 * (1.0f - s0));
+        *slope1 = s1 * (1.0f + v1 * (1.0f - s1));
+    } else {
+        act_both<ACT>(v0, value0, slope0);
+        act_both<ACT>(v1, value1, slope1);
+    }
+}
+
 // Work item t: a tile and the summed slices [k0, k1) of it; part < 0, or its place among the partials.
 struct Item {
     int mi, ni, k0, k1, part;
