@@ -64,12 +64,43 @@ struct Restride {
         int64_t rows, cols, ld, ldp;
     } m[3];
 };
+// A warp per row, 8 elements a lane: the two aligned 16-byte words that hold them, shifted together (words
+// that reach outside the matrix: element by element). The row's padding becomes zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) restride_kernel(const __grid_constant__ Restride<T> a) {
     const auto& m = a.m[blockIdx.y];
-    for (int64_t r = blockIdx.x; r < m.rows; r += gridDim.x)
-#pragma unroll 4
-        for (int64_t c = threadIdx.x; c < m.cols; c += 256) m.dst[r * m.ldp + c] = m.src[r * m.ld + c];
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(m.src);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(m.src + (m.rows - 1) * m.ld + m.cols);
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < m.rows; r += (int64_t)gridDim.x * 8) {
+        for (int64_t c = (threadIdx.x & 31) * 8; c < m.cols; c += 256) {
+            const T* src = m.src + r * m.ld + c;
+            const uintptr_t at = reinterpret_cast<uintptr_t>(src), low = at & ~uintptr_t(15);
+            const int shift = (int)(at & 15);
+            uint32_t out[4];
+            if (c + 8 <= m.cols && low >= begin && low + (shift ? 32 : 16) <= end) {
+                const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(low));
+                const uint4 v1 = shift ? __ldg(reinterpret_cast<const uint4*>(low) + 1) : v0;
+                uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                if (shift & 8)
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+                if (shift & 4)
+#pragma unroll
+                    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] = __funnelshift_r(w[i], w[i + 1], (shift & 2) * 8);
+            } else {
+                const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t lo = c + 2 * i < m.cols ? e[2 * i] : 0u;
+                    const uint32_t hi = c + 2 * i + 1 < m.cols ? e[2 * i + 1] : 0u;
+                    out[i] = lo | hi << 16;
+                }
+            }
+            *reinterpret_cast<uint4*>(m.dst + r * m.ldp + c) = make_uint4(out[0], out[1], out[2], out[3]);
+        }
+    }
 }
 
 // Matrices as TMA can read them: the caller's, or copies in scratch.
@@ -98,7 +129,7 @@ struct Operands {
             m[n++] = r;
         }
         if (jobs == 0) return;
-        const dim3 grid((unsigned)std::min(most, (int64_t)sm_count(h.device) * 8), (unsigned)jobs);
+        const dim3 grid((unsigned)std::min(ceil_div(most, 8), (int64_t)sm_count(h.device) * 8), (unsigned)jobs);
         restride_kernel<T><<<grid, 256, 0, h.stream>>>(job);
         after_launch(h, "gated_restride");
     }
