@@ -49,6 +49,7 @@ few_rows_kernel(const GatedArgs<T> p, T* y, int64_t ldy, T* gate, T* up) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int64_t f0 = (int64_t)blockIdx.x * 16;
+    cudaGridDependencySynchronize();
     const T* rows[2][2];  // a lane's two features of each weight; past the last: the last, not stored
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -112,7 +113,7 @@ void few_rows(Handle& h, const GatedArgs<T>& a, T* y, int64_t ldy, T* gate, T* u
                      tma_ok(a.x, a.rows > 1 ? a.ldx : 0);
     auto kern = a.rows <= 8 ? (vec ? few_rows_kernel<T, 1, true> : few_rows_kernel<T, 1, false>)
                             : (vec ? few_rows_kernel<T, 2, true> : few_rows_kernel<T, 2, false>);
-    kern<<<(unsigned)ceil_div(a.F, 16), 32 * FEW_WARPS, 0, h.stream>>>(a, y, ldy, gate, up);
+    launch_dependent(h.stream, kern, (unsigned)ceil_div(a.F, 16), 32 * FEW_WARPS, 0, 1, a, y, ldy, gate, up);
     after_launch(h, "gated_few_rows");
 }
 

@@ -25,6 +25,7 @@ gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t l
                     const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ dg,
                     T* __restrict__ du, int64_t ldp) {
     const int64_t per = F / V;  // V divides F
+    cudaGridDependencySynchronize();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per;
          i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per, c = (i - r * per) * V;
@@ -69,6 +70,7 @@ struct Restride {
 template <typename T>
 __global__ void __launch_bounds__(256) restride_kernel(const __grid_constant__ Restride<T> a) {
     const auto& m = a.m[blockIdx.y];
+    cudaGridDependencySynchronize();
     const uintptr_t begin = reinterpret_cast<uintptr_t>(m.src);
     const uintptr_t end = reinterpret_cast<uintptr_t>(m.src + (m.rows - 1) * m.ld + m.cols);
     for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < m.rows; r += (int64_t)gridDim.x * 8) {
@@ -130,7 +132,7 @@ struct Operands {
         }
         if (jobs == 0) return;
         const dim3 grid((unsigned)std::min(ceil_div(most, 8), (int64_t)sm_count(h.device) * 8), (unsigned)jobs);
-        restride_kernel<T><<<grid, 256, 0, h.stream>>>(job);
+        launch_dependent(h.stream, restride_kernel<T>, grid, 256, 0, 1, job);
         after_launch(h, "gated_restride");
     }
     CUtensorMap map(int i, int box_rows) const {
@@ -262,7 +264,7 @@ void gated_ffn_backward(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t l
         with_activation(a.act, [&](auto act) {
             constexpr Activation A = decltype(act)::value;
             auto kern = wide ? gated_slopes_kernel<T, A, 8> : gated_slopes_kernel<T, A, 1>;
-            kern<<<grid, 256, 0, h.stream>>>(a.rows, a.F, dy, lddy, gate, up, dg, du, ldp);
+            launch_dependent(h.stream, kern, grid, 256, 0, 1, a.rows, a.F, dy, lddy, gate, up, dg, du, ldp);
         });
         after_launch(h, "gated_slopes");
     }

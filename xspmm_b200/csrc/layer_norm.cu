@@ -310,6 +310,7 @@ layer_norm_kernel(const TileSource<TX> x, const float* __restrict__ w, const flo
     using Cols = Columns<V, CH, TAIL1, OFF>;
     constexpr int PAIRS = Cols::PAIRS;
     int phase = 0;
+    cudaGridDependencySynchronize();
     const int D = x.D, rpb = x.rpb, group = rpb == 1 ? 0 : threadIdx.x / tpr;
     const Cols cols(threadIdx.x - group * tpr, tpr, D, (int64_t)blockIdx.x * rpb + group);
     const int width = rpb == 1 ? blockDim.x : tpr;  // threads that sum a row
@@ -391,6 +392,7 @@ layer_norm_grad_kernel(const TileSource<TY> dy, const TileSource<TX> x, const fl
     using Cols = Columns<V, CH, TAIL1, false>;
     constexpr int PAIRS = Cols::PAIRS, HELD = SM ? 1 : PAIRS;
     int phase = 0;
+    cudaGridDependencySynchronize();
     const int D = x.D, rpb = x.rpb, group = rpb == 1 ? 0 : threadIdx.x / tpr;
     const Cols cols(threadIdx.x - group * tpr, tpr, D, 0);
     const int width = rpb == 1 ? blockDim.x : tpr;
@@ -704,7 +706,8 @@ void norm_launch(Handle& h, int64_t rows, int64_t D, const TX* x, int64_t ldx, c
     auto kern = tail1 ? layer_norm_kernel<TX, TY, V, E / V, RING, true, OFF>
                       : layer_norm_kernel<TX, TY, V, E / V, RING, false, OFF>;
     const unsigned grid = tile_grid(h, kern, block, smem, ceil_div(rows, src.rpb), OFF ? V : 1);
-    kern<<<grid, block, smem, h.stream>>>(src, w, b, eps, y, ldy, mean, rstd, tpr, stages, h.d_err);
+    launch_dependent(h.stream, kern, grid, block, smem, 1, src, w, b, eps, y, ldy, mean, rstd, tpr, stages,
+                     h.d_err);
     after_launch(h, "layer_norm");
 }
 
@@ -725,8 +728,8 @@ void norm_grad_launch(Handle& h, int64_t rows, int64_t D, const TY* dy, int64_t 
     const unsigned grid = tile_grid(h, kern, block, smem, ceil_div(rows, sx.rpb), 1);
     const bool sums = dw || db;
     DevBuf<float> part(sums ? (size_t)2 * grid * D : 0, h.stream);
-    kern<<<grid, block, smem, h.stream>>>(sg, sx, w, mean, rstd, dx, lddx, part.get(), tpr, stages,
-                                          h.d_err);
+    launch_dependent(h.stream, kern, grid, block, smem, 1, sg, sx, w, mean, rstd, dx, lddx, part.get(), tpr,
+                     stages, h.d_err);
     after_launch(h, "layer_norm_grad");
     if (sums) {
         const bool vec = D % 4 == 0;
