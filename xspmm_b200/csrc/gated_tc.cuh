@@ -15,7 +15,7 @@
 // of B's columns in its shared memory, and all columns of its rows in its TMEM. A CTA alone has to
 // write and read 24 KB of shared memory per 16-deep MMA of 128 x 256, 192 clocks at 128 bytes a clock
 // where the MMA takes 128; in a pair it is 16 KB. Measured on 2048 tokens of 4096 x 11008, forward:
-// XX us alone, YY us paired. CG = 1 is for at most 128 rows, where the second CTA would compute padding.
+// 354 us alone, 327 paired. CG = 1 is for at most 128 rows, where the second CTA would compute padding.
 //   Forward: an MMA of N = 2 bf holds bf columns of both projections, so x is read once for both and the
 //   epilogue finds g and u of an output bf columns apart; in a pair one CTA brings wg, the other wu.
 //   Dw: the pair's first CTA computes rows of dwg, the second the same rows of dwu.
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 
     if (warp == 0) {
         if (lane == 0 && rank == 0) {
-            int j = 0;  // stages taken so far
+            int s = 0, turn = 0;  // the next stage, and whether its ring has come round an odd number of times
             bool ok = true;
             for (int t = group, i = 0; t < work && ok; t += groups, ++i) {
                 const int b = i & 1;
@@ -400,22 +400,22 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 tc_fence_after();
                 const uint32_t acc = tmem + (uint32_t)(b * ACC_COLS);
                 const Item it = item_of(p, t);
-                for (int k = it.k0; k < it.k1; ++k, ++j) {
-                    const int s = j % p.stages;
-                    if (!mbar_wait(&full[s], (j / p.stages) & 1, p.err)) {
+                for (int k = it.k0; k < it.k1; ++k) {
+                    const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + A_BYTES;
+                    const uint64_t da = P == Product::Dw ? desc_mn(sa) : desc_k(sa);
+                    const uint64_t db = P == Product::Forward ? desc_k(sb) : desc_mn(sb);
+                    if (!mbar_wait(&full[s], turn, p.err)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + A_BYTES;
+                    // 16 summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows, in units of 16
 #pragma unroll
-                    for (int q = 0; q < TK / 16; ++q) {
-                        // 16 summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows
-                        const uint64_t da = P == Product::Dw ? desc_mn(sa + q * 2048) : desc_k(sa + q * 32);
-                        const uint64_t db = P == Product::Forward ? desc_k(sb + q * 32) : desc_mn(sb + q * 2048);
-                        pair_mma<CG>(acc, da, db, p.idesc, k > it.k0 || q > 0);
-                    }
+                    for (int q = 0; q < TK / 16; ++q)
+                        pair_mma<CG>(acc, da + q * (P == Product::Dw ? 128 : 2), db + q * (P == Product::Forward ? 2 : 128),
+                                     p.idesc, k > it.k0 || q > 0);
                     pair_commit<CG>(&empty[s]);
+                    if (++s == p.stages) s = 0, turn ^= 1;
                 }
                 if (ok) pair_commit<CG>(&acc_full[b]);
             }
@@ -423,18 +423,18 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            int j = 0;
+            int s = 0, turn = 0, held = 0;  // held: stages filled, at most all
             bool ok = true;
             for (int t = group; t < work && ok; t += groups) {
                 const Item it = item_of(p, t);
                 const int m0 = (P == Product::Dw ? it.mi : it.mi * CG + rank) * TM;
                 const int n0 = it.ni * p.bn;
-                for (int k = it.k0; k < it.k1; ++k, ++j) {
-                    const int s = j % p.stages;
-                    if (j >= p.stages && !mbar_wait(&empty[s], ((j / p.stages) & 1) ^ 1, p.err)) {
+                for (int k = it.k0; k < it.k1; ++k) {
+                    if (held == p.stages && !mbar_wait(&empty[s], turn ^ 1, p.err)) {
                         ok = false;
                         break;
                     }
+                    if (held < p.stages) ++held;
                     uint8_t* sa = smem + s * stage_bytes;
                     uint8_t* sb = sa + A_BYTES;
                     if (rank == 0) mbar_expect_tx(&full[s], (uint32_t)(CG * stage_bytes));
@@ -461,12 +461,15 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                                 pair_load<CG>(sb + c * CHUNK, &p.b[0], nb + 64 * c, k * TK, bar);
                         }
                     }
+                    if (++s == p.stages) s = 0, turn ^= 1;
                 }
             }
             // No load may be in flight when the CTA ends. Each landed before its MMAs ran, and the commit
             // after those freed its stage (they have all done so unless a wait ran out).
-            for (int i = max(0, j - p.stages); i < j; ++i)
-                mbar_wait(&empty[i % p.stages], (i / p.stages) & 1, p.err);
+            for (; held > 0; --held) {
+                if (s-- == 0) s = p.stages - 1, turn ^= 1;
+                mbar_wait(&empty[s], turn, p.err);
+            }
         }
     } else if (warp >= FIRST_EPI) {
         const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
