@@ -149,6 +149,14 @@ def test_layer_norm_row_strides(executor, tx, ty, pad):
     outside_untouched(dx, buf)
 
 
+@pytest.mark.parametrize("tx,ty", NORM_TYPES)
+@pytest.mark.parametrize("rows,cols", [(3001, 2051), (700, 4821), (601, 8191), (5, 16376), (4, 16383)])
+def test_layer_norm_long_odd_rows(executor, rows, cols, tx, ty):
+    """Rows that start off every boundary, more of them than fit the GPU at once."""
+    test_layer_norm(executor, rows, cols, tx, ty)
+    test_layer_norm_backward(executor, rows, cols, tx, ty)
+
+
 def test_layer_norm_without_parameters_in_place_and_empty(executor):
     x = rand(3, 50, 96, dtype=bf16)
     one, zero = torch.ones(96, device="cuda"), torch.zeros(96, device="cuda")
@@ -390,6 +398,14 @@ def test_gated_ffn_backward(executor, rows, K, F, act, dtype):
         close(got, ref, err, name)
     for view, b in ((dx, buf), (dwg, bg), (dwu, bu)):
         outside_untouched(view, b)
+
+
+@pytest.mark.parametrize("dtype", [f16, bf16])
+@pytest.mark.parametrize("rows,K,F", [(1100, 520, 3000), (40003, 128, 120), (30000, 64, 128), (150, 4096, 300)])
+def test_gated_ffn_several_waves(executor, rows, K, F, dtype):
+    """More tiles than the GPU takes at once, split sums, and several tiles a CTA in the one-pass gradient."""
+    test_gated_ffn(executor, rows, K, F, "silu", dtype)
+    test_gated_ffn_backward(executor, rows, K, F, "silu", dtype)
 
 
 @pytest.mark.parametrize("rows", [3, 200])
