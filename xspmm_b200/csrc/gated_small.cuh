@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_grad_kernel(const __grid_
             if (lane == 0) mbar_arrive(&dx_empty[b]);
             const int64_t row0 = (int64_t)t * TM + quarter * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, p.t.M - row0));
-            if (col0 < p.K) store_group<T, 1>(p.t, 2, turn, piece, words, row0, col0, rows, min(32, p.K - col0));
+            if (col0 < p.K) store_group<T, false, 1>(p.t, 2, turn, piece, words, row0, col0, rows, min(32, p.K - col0));
             return true;
         };
         bool ok = true;

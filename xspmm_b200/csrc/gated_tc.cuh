@@ -24,8 +24,9 @@
 // 1 of each the loads of its own operands (one lane; they report to the first CTA's barrier), warp 2
 // allocates TMEM, warps 4..11 are the epilogue. TMEM holds two accumulators used in turn, so a tile's
 // epilogue runs under the next tile's products. The epilogue converts 32 columns at a time and stores
-// them by TMA from a warp's own pieces of shared memory (an output that TMA cannot address: row by row). Every wait is bounded; a timeout sets the error flag, and TMEM is freed only
-// after the MMAs that were issued have completed.
+// them by TMA from a warp's own pieces of shared memory (an output that TMA cannot address: by one or two
+// elements a lane, in an instance of its own). Every wait is bounded; a timeout sets the error flag, and
+// TMEM is freed only after the MMAs that were issued have completed.
 //
 // Tiles that would leave part of the GPU idle (the last wave's, or all where there are few) have their
 // sum split: each slice's fp32 partial goes to scratch and a second kernel adds them in slice order (the
@@ -67,7 +68,8 @@ struct TileArgs {
     Activation act;
     void* out[3];       // Forward: y, gate, up; Dx: dx; Dw: dwg, dwu
     int64_t ld[3];
-    int tma[3];         // 16-byte stores, whole groups through omap; else element by element
+    int tma[3];         // stored by TMA (whole groups through omap) and in 16-byte words; else by store_rows,
+    int even[3];        // two elements a store
     CUtensorMap omap[3];
     float4* partial;    // split tiles: [slice][tile][CTA][column / 4][row]
     unsigned* err;
@@ -295,9 +297,37 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// The first `rows` x `cols` of a staged piece to `out` without TMA, V elements a store (1, or 2 where cols, ld and
+// the address of `out` are even). Eight reads are in flight before their stores, which the compiler would
+// not move a later read over. One copy in the program: three inlined ones do not stay in the instruction cache
+// (2^18 rows of 128 -> 127, projections kept: 120 us, inlined 199; -> 126: 104 and 131; -> 128 by TMA 58).
+// Aligned words of 4 or 8 bytes of odd rows, with their first and last elements stored singly, were slower
+// (140 us and more): a row's piece is 64 bytes in any case, and they add stores to its ends.
+template <typename T, int V>
+__device__ __noinline__ void store_rows(T* out, int64_t ld, const uint8_t* at, int rows, int cols) {
+    using Word = Pack<T, V>;
+    constexpr int PER = 32 / V;  // lanes a row
+    const int lane = threadIdx.x & 31, first = lane / PER, c = lane % PER * V;
+    if (c >= cols) return;
+    out += first * ld + c;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 8 * V) {
+        Word w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + i * V + first;
+            w[i] = *reinterpret_cast<const Word*>(at + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) * 16) + (c & 7) * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r0 + i * V + first < rows) *reinterpret_cast<Word*>(out + (int64_t)(r0 + i * V) * ld) = w[i];
+    }
+}
+
 // A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to output `o` at (row0, col0), turned
-// through one of the warp's staging pieces. `rows` x `cols` of them are valid.
-template <typename T, int PIECES = TURNS>
+// through one of the warp's staging pieces. `rows` x `cols` of them are
+// valid. ANY: outputs that TMA cannot address may be among the product's.
+template <typename T, bool ANY, int PIECES = TURNS>
 __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* turn, int& piece,
                                             const uint32_t (&w)[16], int64_t row0, int64_t col0,
                                             int rows, int cols) {
@@ -310,7 +340,7 @@ __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* t
     for (int i = 0; i < 4; ++i)
         *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) =
             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    if (p.tma[o] && cols == 32) {
+    if ((!ANY || p.tma[o]) && cols == 32) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -324,17 +354,18 @@ __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* t
     } else {
         __syncwarp();
         T* out = static_cast<T*>(p.out[o]) + row0 * p.ld[o] + col0;
-        if (p.tma[o]) {  // a tile's last columns, a multiple of 8: 16-byte pieces
+        if (!ANY || p.tma[o]) {  // a tile's last columns, a multiple of 8: 16-byte pieces
             const int per = cols >> 3;
             for (int i = lane; i < rows * per; i += 32) {
                 const int r = i / per, c = i - r * per;
                 *reinterpret_cast<uint4*>(out + r * p.ld[o] + c * 8) =
                     *reinterpret_cast<const uint4*>(at + r * 64 + ((c ^ ((r >> 1) & 3)) * 16));
             }
-        } else if (lane < cols)
-            for (int r = 0; r < rows; ++r)
-                out[r * p.ld[o] + lane] = reinterpret_cast<const T*>(
-                    at + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16))[lane & 7];
+        } else if (p.even[o]) {
+            store_rows<T, 2>(out, p.ld[o], at, rows, cols);
+        } else {
+            store_rows<T, 1>(out, p.ld[o], at, rows, cols);
+        }
         __syncwarp();
     }
 }
@@ -358,7 +389,7 @@ __device__ __forceinline__ void store_partial(float4* dst, const uint32_t (&v)[3
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------
-template <typename T, Product P, int CG>
+template <typename T, Product P, int CG, bool ANY>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileArgs p) {
     static_assert(P != Product::Dw || CG == 2, "Dw: one weight a CTA");
     extern __shared__ uint8_t smem_raw[];
@@ -514,18 +545,18 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                             w[e] = pack2(y.x, y.y, T());
                         }
                     });
-                    store_group<T>(p, 0, my_turn, piece, w, row0, n0 + c, rows, cols);
+                    store_group<T, ANY>(p, 0, my_turn, piece, w, row0, n0 + c, rows, cols);
                     if (p.out[1]) {
                         pack_words<T>(w, v);
-                        store_group<T>(p, 1, my_turn, piece, w, row0, n0 + c, rows, cols);
+                        store_group<T, ANY>(p, 1, my_turn, piece, w, row0, n0 + c, rows, cols);
                     }
                     if (p.out[2]) {
                         pack_words<T>(w, u);
-                        store_group<T>(p, 2, my_turn, piece, w, row0, n0 + c, rows, cols);
+                        store_group<T, ANY>(p, 2, my_turn, piece, w, row0, n0 + c, rows, cols);
                     }
                 } else {
                     pack_words<T>(w, v);
-                    store_group<T>(p, seg, my_turn, piece, w, row0, n0 + c, rows, cols);
+                    store_group<T, ANY>(p, seg, my_turn, piece, w, row0, n0 + c, rows, cols);
                 }
             }
             tc_fence_before();
@@ -631,6 +662,7 @@ inline void set_output(TileArgs& t, int i, void* out, int64_t ld) {
     t.out[i] = out;
     t.ld[i] = ld;
     t.tma[i] = out && t.N % 8 == 0 && tma_ok(out, ld);
+    t.even[i] = t.N % 2 == 0 && ld % 2 == 0 && aligned_to(out, 4);
     if (t.tma[i])
         t.omap[i] = make_map_2d(out, (uint64_t)t.N, (uint64_t)t.M, (uint64_t)ld * 2, 32, 32,
                                 CU_TENSOR_MAP_SWIZZLE_64B);
@@ -658,7 +690,9 @@ void launch_product(Handle& h, TileArgs& t) {
     XS_REQUIRE(work * CG < (int64_t(1) << 31), XSPMM_STATUS_UNSUPPORTED, "grid too large");
     DevBuf<float4> ws((size_t)rest * t.splits * CG * (ACC_COLS / 4) * TM, h.stream);
     t.partial = ws.get();
-    auto kern = tile_kernel<T, P, CG>;
+    bool any = false;
+    for (int i = 0; i < 3; ++i) any = any || (t.out[i] && !t.tma[i]);
+    auto kern = any ? tile_kernel<T, P, CG, true> : tile_kernel<T, P, CG, false>;
     XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const unsigned grid = (unsigned)(std::min<int64_t>(work, sm_count(h.device) / CG) * CG);
     launch_dependent(h.stream, kern, grid, THREADS, smem, CG, t);
