@@ -408,6 +408,34 @@ def test_gated_ffn_several_waves(executor, rows, K, F, dtype):
     test_gated_ffn_backward(executor, rows, K, F, "silu", dtype)
 
 
+@pytest.mark.parametrize("start,pad", [(0, 0), (1, 0), (2, 4), (0, 3), (8, 8)])
+@pytest.mark.parametrize("rows,K,F", [(130, 126, 70), (333, 134, 126), (201, 64, 133), (77, 250, 191)])
+def test_gated_ffn_odd_widths_and_addresses(executor, rows, K, F, start, pad):
+    """Outputs that start at any element with any row stride, beside kept projections, dy and weights'
+    gradients at odd addresses: every width a store can have, up to the matrix's last element."""
+    def placed(r, c, gap=0):
+        buf = torch.full((start + r * (c + gap) + 64,), 7.0, dtype=f16, device="cuda")
+        return buf.as_strided((r, c), (c + gap, 1), start), buf
+
+    x, wg, wu = ffn_problem(rows, K, F, f16, seed=9)
+    g, u, ref, eg, eu, ey = ffn_errors(x, wg, wu, "silu")
+    (y, b0), (gate, b1), (up, b2) = placed(rows, F, pad), placed(rows, F), placed(rows, F)
+    xs.gated_ffn(executor, x, wg, wu, y, "silu", gate, up)
+    for got, r, e, name in ((y, ref, ey, "y"), (gate, g, eg, "gate"), (up, u, eu, "up")):
+        close(got, r, e, name)
+    (dy, b3), (dx, b4) = placed(rows, F, pad), placed(rows, K, pad)
+    dy.copy_(rand(6, rows, F, dtype=f16))
+    (dwg, b5), (dwu, b6) = placed(F, K), placed(F, K)
+    xs.gated_ffn_backward(executor, dy, x, wg, wu, gate, up, dx, dwg, dwu)
+    for got, (r, e), name in zip((dx, dwg, dwu), grad_ref(x, wg, wu, gate, up, dy, "silu", f16),
+                                 ("dx", "dw_gate", "dw_up")):
+        close(got, r, e, name)
+    for view, buf in ((y, b0), (gate, b1), (up, b2), (dx, b4), (dwg, b5), (dwu, b6)):
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        keep.as_strided(view.shape, view.stride(), start).fill_(False)
+        assert bool((buf[keep] == 7.0).all()), "written outside the output"
+
+
 @pytest.mark.parametrize("rows", [3, 200])
 def test_gated_ffn_parts_strides_and_packed_weights(executor, rows):
     """Both weights as halves of one packed tensor with a row stride, x and y as column slices at
