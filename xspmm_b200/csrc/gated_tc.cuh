@@ -327,6 +327,8 @@ __device__ __noinline__ void store_rows(T* out, int64_t ld, const uint8_t* at, i
 // A warp's 32 rows x 32 columns (lane = row, 16 packed words each) to output `o` at (row0, col0), turned
 // through one of the warp's staging pieces. `rows` x `cols` of them are
 // valid. ANY: outputs that TMA cannot address may be among the product's.
+// Every call commits one bulk group, an empty one where it stores without TMA: the wait counts groups, and
+// the newest PIECES - 1 of them have to be those of the other pieces' last calls.
 template <typename T, bool ANY, int PIECES = TURNS>
 __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* turn, int& piece,
                                             const uint32_t (&w)[16], int64_t row0, int64_t col0,
@@ -367,6 +369,7 @@ __device__ __forceinline__ void store_group(const TileArgs& p, int o, uint8_t* t
             store_rows<T, 1>(out, p.ld[o], at, rows, cols);
         }
         __syncwarp();
+        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
 }
 
