@@ -73,14 +73,7 @@ gated_slopes_kernel(int64_t rows, int64_t F, const T* __restrict__ dy, int64_t l
         const uint4 d = load(dy, lddy, r, c), g = load(gate, F, r, c), u = load(up, F, r, c);
         const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
         uint32_t a[4], b[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 d2 = unpack2(dw[e], T()), g2 = unpack2(gw[e], T()), u2 = unpack2(uw[e], T());
-            float v0, v1, s0, s1;
-            act_both_pair<ACT>(g2.x, g2.y, &v0, &s0, &v1, &s1);
-            a[e] = pack2(d2.x * u2.x * s0, d2.y * u2.y * s1, T());
-            b[e] = pack2(d2.x * v0, d2.y * v1, T());
-        }
+        slope_words<ACT, T>(a, b, dw, gw, uw);
         *reinterpret_cast<uint4*>(dg + r * ldp + c) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(du + r * ldp + c) = make_uint4(b[0], b[1], b[2], b[3]);
     }

@@ -202,17 +202,12 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_grad_kernel(const __grid_
             with_activation(p.t.act, [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t* dw = reinterpret_cast<uint32_t*>(&d[j]);
-                    uint32_t* gw = reinterpret_cast<uint32_t*>(&g[j]);
-                    const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u[j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 d2 = unpack2(dw[e], T()), g2 = unpack2(gw[e], T()), u2 = unpack2(uw[e], T());
-                        float v0, v1, s0, s1;
-                        act_both_pair<decltype(act)::value>(g2.x, g2.y, &v0, &s0, &v1, &s1);
-                        dw[e] = pack2(d2.x * u2.x * s0, d2.y * u2.y * s1, T());
-                        gw[e] = pack2(d2.x * v0, d2.y * v1, T());
-                    }
+                    const uint32_t dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w}, gw[4] = {g[j].x, g[j].y, g[j].z, g[j].w};
+                    const uint32_t uw[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+                    uint32_t a[4], b[4];
+                    slope_words<decltype(act)::value, T>(a, b, dw, gw, uw);
+                    d[j] = make_uint4(a[0], a[1], a[2], a[3]);
+                    g[j] = make_uint4(b[0], b[1], b[2], b[3]);
                 }
             });
             if (i > 0 && !mbar_wait(d_empty, (i - 1) & 1, err)) {

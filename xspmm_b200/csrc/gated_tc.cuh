@@ -80,11 +80,27 @@ __device__ __forceinline__ float exp2f_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The larger of two values and the smaller, NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // __fdividef(1, d) is 0 for d above 2^126, as the quotient nearly is.
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
+// Where silu and its slope have reached their limits in fp32. Gates further out, infinite ones among them,
+// are taken from there: v * sigmoid(v) is 0 for v = -inf, as for every large negative v, instead of inf * 0.
+constexpr float SILU_END = 100.0f;
+
 template <Activation ACT>
 __device__ __forceinline__ float act_value(float v) {
+    if constexpr (ACT == Activation::Silu) v = max_nan(v, -SILU_END);
     if constexpr (ACT == Activation::Silu) return __fdividef(v, 1.0f + __expf(-v));
     else if constexpr (ACT == Activation::Gelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
     else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
@@ -95,31 +111,73 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The sigmoids of two values, in packed fp32. They share one reciprocal, 1 / a0 = a1 / (a0 a1): the special
-// function unit (16 lanes a clock on an SM) weighs on the epilogue of short sums, and this takes three of
-// its operations instead of four. The exponent is capped at 60, so that a0 a1 stays finite: below
-// v = -41.6 the sigmoid is 2^-60 (9e-19) where e^v is less still, an absolute error under 1e-18. Packed
-// pairs in the epilogue: 2^20 rows of 128 x 128 216 us, one value at a time 228 us.
-__device__ __forceinline__ float2 sigmoid2(float2 v) {
+// The sigmoids of two values, in packed fp32, and product = a0 a1. They share one reciprocal,
+// 1 / a0 = a1 / (a0 a1): the special function unit (16 lanes a clock on an SM) weighs on the epilogue of
+// short sums, and this takes three of its operations instead of four. They hold where the product is at most
+// PAIR_MAX, so that its reciprocal is a normal number: for gates whose negative parts add up to -86 at least.
+constexpr float PAIR_MAX = 4.2535296e37f;  // 2^125
+__device__ __forceinline__ float2 sigmoid2(float2 v, float* product) {
     const float2 x = mul2(v, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-    const float2 e = make_float2(exp2f_approx(fminf(x.x, 60.0f)), exp2f_approx(fminf(x.y, 60.0f)));
-    const float2 a = add2(e, make_float2(1.0f, 1.0f));
-    const float r = rcp_approx(a.x * a.y);
+    const float2 a = add2(make_float2(exp2f_approx(x.x), exp2f_approx(x.y)), make_float2(1.0f, 1.0f));
+    *product = a.x * a.y;
+    const float r = rcp_approx(*product);
     return mul2(make_float2(a.y, a.x), make_float2(r, r));
 }
-// act of two values.
-template <Activation ACT>
-__device__ __forceinline__ float2 act_pair(float2 v) {
-    if constexpr (ACT == Activation::Silu) return mul2(v, sigmoid2(v));
-    else return make_float2(act_value<ACT>(v.x), act_value<ACT>(v.y));
+// y = act(g) * u of the first `cols` of a row's 32 columns as 16 packed words. silu takes them in pairs (2^20
+// rows of 128 x 128, sustained: 228 us; one value at a time 240), and all of them again one at a time where a
+// pair does not hold (a NaN among them). The choice is the row's own: neither other rows nor what lies past
+// its columns enter it. The second form is a loop over copies in local memory: unrolled, its instructions
+// cost the first one 6 us.
+template <Activation ACT, typename T>
+__device__ __forceinline__ void gate_words(uint32_t (&w)[16], const uint32_t (&g)[32], const uint32_t (&u)[32], int cols) {
+    if constexpr (ACT == Activation::Silu) {
+        bool holds = true;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float2 g2 = make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
+            const float2 u2 = make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]));
+            float product;
+            const float2 y = mul2(mul2(g2, sigmoid2(g2, &product)), u2);
+            holds = holds && product <= PAIR_MAX;
+            w[e] = pack2(y.x, y.y, T());
+        }
+        if (__builtin_expect(holds, 1)) return;
+        float2 gs[16], us[16];
+        uint32_t ws[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            gs[e] = make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
+            us[e] = make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]));
+        }
+        holds = true;
+#pragma unroll 1
+        for (int e = 0; 2 * e < cols; ++e) {
+            float product;
+            sigmoid2(gs[e], &product);
+            holds = holds && product <= PAIR_MAX;
+        }
+        if (holds) return;
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e)
+            ws[e] = pack2(act_value<ACT>(gs[e].x) * us[e].x, act_value<ACT>(gs[e].y) * us[e].y, T());
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = ws[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float2 v = make_float2(act_value<ACT>(__uint_as_float(g[2 * e])), act_value<ACT>(__uint_as_float(g[2 * e + 1])));
+            const float2 y = mul2(v, make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])));
+            w[e] = pack2(y.x, y.y, T());
+        }
+    }
 }
 // act(v) and act'(v).
 template <Activation ACT>
 __device__ __forceinline__ void act_both(float v, float* value, float* slope) {
     if constexpr (ACT == Activation::Silu) {
-        const float s = sigmoid(v);
-        *value = v * s;
-        *slope = s * (1.0f + v * (1.0f - s));
+        const float low = max_nan(v, -SILU_END), s = sigmoid(low);
+        *value = low * s;
+        *slope = s * (1.0f + min_nan(low, SILU_END) * (1.0f - s));
     } else if constexpr (ACT == Activation::Gelu) {
         const float half = 0.5f * (1.0f + erff(v * 0.70710678118654752f));
         *value = v * half;
@@ -134,24 +192,41 @@ __device__ __forceinline__ void act_both(float v, float* value, float* slope) {
     }
 }
 
-// act_both of two values; silu's sigmoids share a reciprocal as in sigmoid2. One value at a time here: packed
-// pairs need aligned register pairs, and the one-pass gradient, which has no register to spare, spills for
-// them (2^20 rows of 128: 329 us here, 351 us packed).
-template <Activation ACT>
-__device__ __forceinline__ void act_both_pair(float v0, float v1, float* value0, float* slope0, float* value1,
-                                              float* slope1) {
+// dg = dy * up * act'(gate) and du = dy * act(gate) of 8 packed values. silu's sigmoids share a reciprocal by
+// twos as in sigmoid2, and all 8 are taken again one at a time where a pair does not hold. In its slope
+// 1 - s = e^-v s, which does not cancel. The arithmetic is on single values: packed fp32 needs aligned
+// register pairs, and the one-pass gradient, which has no register to spare, spills for them (2^20 rows of
+// 128: 329 us here, 351 us packed).
+template <Activation ACT, typename T>
+__device__ __forceinline__ void slope_words(uint32_t (&dg)[4], uint32_t (&du)[4], const uint32_t (&dy)[4],
+                                            const uint32_t (&gate)[4], const uint32_t (&up)[4]) {
+    auto words = [&](auto both) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 d = unpack2(dy[e], T()), g = unpack2(gate[e], T()), u = unpack2(up[e], T());
+            float2 v, s;
+            both(g, &v, &s);
+            dg[e] = pack2(d.x * u.x * s.x, d.y * u.y * s.y, T());
+            du[e] = pack2(d.x * v.x, d.y * v.y, T());
+        }
+    };
     if constexpr (ACT == Activation::Silu) {
-        const float a0 = 1.0f + exp2f_approx(fminf(v0 * -1.4426950408889634f, 60.0f));
-        const float a1 = 1.0f + exp2f_approx(fminf(v1 * -1.4426950408889634f, 60.0f));
-        const float r = __fdividef(1.0f, a0 * a1), s0 = a1 * r, s1 = a0 * r;
-        *value0 = v0 * s0;
-        *value1 = v1 * s1;
-        *slope0 = s0 * (1.0f + v0 * (1.0f - s0));
-        *slope1 = s1 * (1.0f + v1 * (1.0f - s1));
-    } else {
-        act_both<ACT>(v0, value0, slope0);
-        act_both<ACT>(v1, value1, slope1);
+        bool holds = true;
+        words([&](float2 g, float2* value, float2* slope) {
+            const float e0 = exp2f_approx(g.x * -1.4426950408889634f), e1 = exp2f_approx(g.y * -1.4426950408889634f);
+            const float a0 = 1.0f + e0, a1 = 1.0f + e1, product = a0 * a1;
+            const float r = rcp_approx(product), s0 = a1 * r, s1 = a0 * r;
+            holds = holds && product <= PAIR_MAX;
+            *value = make_float2(g.x * s0, g.y * s1);
+            *slope = make_float2(s0 * (1.0f + fminf(g.x, SILU_END) * (e0 * s0)),
+                                 s1 * (1.0f + fminf(g.y, SILU_END) * (e1 * s1)));
+        });
+        if (holds) return;
     }
+    words([](float2 g, float2* value, float2* slope) {
+        act_both<ACT>(g.x, &value->x, &slope->x);
+        act_both<ACT>(g.y, &value->y, &slope->y);
+    });
 }
 
 // Work item t: a tile and the summed slices [k0, k1) of it; part < 0, or its place among the partials.
@@ -539,15 +614,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     store_partial(partial + c / 4 * TM, v, p.bn - c);
                     if constexpr (P == Product::Forward) store_partial(partial + (p.bn + c) / 4 * TM, u, p.bn - c);
                 } else if constexpr (P == Product::Forward) {
-                    with_activation(p.act, [&](auto act) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 g2 = make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-                            const float2 u2 = make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]));
-                            const float2 y = mul2(act_pair<decltype(act)::value>(g2), u2);
-                            w[e] = pack2(y.x, y.y, T());
-                        }
-                    });
+                    with_activation(p.act, [&](auto act) { gate_words<decltype(act)::value, T>(w, v, u, cols); });
                     store_group<T, ANY>(p, 0, my_turn, piece, w, row0, n0 + c, rows, cols);
                     if (p.out[1]) {
                         pack_words<T>(w, v);
