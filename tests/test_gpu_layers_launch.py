@@ -1,9 +1,15 @@
-"""GPU tests of the layer operators' launches: shared memory at the edges of what a launch may take unasked."""
+"""GPU tests of the layer operators' launches: shared memory at the edges of what a launch may take unasked,
+and launches of one kernel from several threads."""
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
+import torch
+
+import xspmm_b200 as xs
+from xspmm_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +64,49 @@ print("done")
 def test_rings_of_a_little_less_than_48_kb(executor):
     r = subprocess.run([sys.executable, "-c", _WIDTHS], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+def _gated(handle, rows, K, F):
+    x, wg, wu = (torch.ones(r, K, dtype=torch.bfloat16, device="cuda") for r in (rows, F, F))
+    y = torch.empty(rows, F, dtype=torch.bfloat16, device="cuda")
+    args = (handle, rows, K, F, 2, x.data_ptr(), K, wg.data_ptr(), K, wu.data_ptr(), K, y.data_ptr(), F, None, None)
+    return _lib.lib().xspmm_gated_ffn_bf16, args, y, float(K * K), (x, wg, wu)
+
+
+def _norm(handle, cols):
+    x, bias = torch.ones(2, cols, device="cuda"), torch.full((cols,), 0.75, device="cuda")
+    y = torch.empty_like(x)
+    args = (handle, 2, cols, x.data_ptr(), cols, None, bias.data_ptr(), 1e-5, y.data_ptr(), cols, None, None)
+    return _lib.lib().xspmm_layer_norm_f32f32, args, y, 0.75, (x, bias)
+
+
+# shapes of one kernel instance whose shared memory differs
+@pytest.mark.parametrize("shapes", [[(_gated, 300, 32, 16), (_gated, 20000, 64, 256)],
+                                    [(_gated, 100, 32, 8), (_gated, 100, 64, 20000)],
+                                    [(_norm, 6300), (_norm, 8192)]])
+def test_threads_with_their_own_executors(executor, shapes):
+    """Each thread has its handle, stream and tensors; every call has to launch whatever size the others use.
+    The entries are called without the Python checks between them, so that calls overlap."""
+    failures = []
+    start = threading.Barrier(2 * len(shapes))
+
+    def work(make, *size):
+        ex, stream = xs.CudaExecutor(0), torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            call, args, y, want, _inputs = make(ex.handle, *size)
+            torch.cuda.current_stream().synchronize()
+            start.wait(timeout=60)
+            for _ in range(8000):
+                if call(*args):
+                    failures.append((make.__name__, size, _lib.lib().xspmm_last_error()))
+                    break
+            stream.synchronize()
+            if not bool((y == want).all()):
+                failures.append((make.__name__, size, "wrong result"))
+
+    threads = [threading.Thread(target=work, args=s) for s in shapes for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures

@@ -89,6 +89,16 @@ inline void after_launch(Handle& h, const char* what) {
     ++h.launches;
 }
 
+// Dynamic shared memory that a kernel with at most 2 KB of its own static may be launched with (of 227 KB).
+constexpr size_t DYNAMIC_SMEM = 232448 - 2048;
+// Lets `kern` be launched with up to `most` bytes of dynamic shared memory. The limit belongs to the kernel and
+// not to the launch, and threads with other handles launch the same kernel: `most` is one constant for each, so
+// that no call lowers the limit between another's call and its launch.
+template <typename K>
+void allow_smem(K kern, size_t most = DYNAMIC_SMEM) {
+    XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+}
+
 // Launches a kernel that calls cudaGridDependencySynchronize() before it touches memory: its launch and
 // prologue overlap the end of the stream's previous kernel.
 template <typename... P, typename... A>

@@ -290,7 +290,7 @@ void small_grad(Handle& h, const GatedArgs<T>& a, const T* dy, int64_t lddy, con
     set_output(t, 2, dx, lddx);
     DevBuf<float4> ws((size_t)grid * 2 * (ACC_COLS / 4) * TM, h.stream);
     t.partial = ws.get();
-    XS_CHECK_CUDA(cudaFuncSetAttribute(small_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM_BYTES));
+    allow_smem(small_grad_kernel<T>, SM_BYTES);
     launch_dependent(h.stream, small_grad_kernel<T>, (unsigned)grid, SM_THREADS, SM_BYTES, 1, s);
     after_launch(h, "gated_small_grad");
     // one shared tile for each weight, a slice a CTA

@@ -763,7 +763,7 @@ void launch_product(Handle& h, TileArgs& t) {
     bool any = false;
     for (int i = 0; i < 3; ++i) any = any || (t.out[i] && !t.tma[i]);
     auto kern = any ? tile_kernel<T, P, CG, true> : tile_kernel<T, P, CG, false>;
-    XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    allow_smem(kern, 1024 + SMEM_MAX + 512);
     const unsigned grid = (unsigned)(std::min<int64_t>(work, sm_count(h.device) / CG) * CG);
     launch_dependent(h.stream, kern, grid, THREADS, smem, CG, t);
     after_launch(h, "gated_product");

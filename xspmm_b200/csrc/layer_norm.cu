@@ -663,8 +663,7 @@ template <typename K>
 unsigned tile_grid(Handle& h, K kern, int block, size_t smem, int64_t tiles, int multiple) {
     const int sms = sm_count(h.device);
     // a launch may take 48 KB unasked, the kernel's static shared memory (below 2 KB here) among them
-    if (smem > 46 * 1024)
-        XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 46 * 1024) allow_smem(kern);
     if (tiles <= sms) return (unsigned)tiles;  // each has its own
     int per_sm = 0;
     XS_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, block, smem));
