@@ -1,5 +1,5 @@
 """GPU tests of the layer operators' launches: shared memory at the edges of what a launch may take unasked,
-and launches of one kernel from several threads."""
+launches of one kernel from several threads, and a thread whose first CUDA call is one of them."""
 import os
 import subprocess
 import sys
@@ -110,3 +110,16 @@ def test_threads_with_their_own_executors(executor, shapes):
     for t in threads:
         t.join()
     assert not failures, failures
+
+
+def test_a_threads_first_cuda_call(executor):
+    """A host thread that has not touched the GPU yet has no context of its own to encode tensor maps in."""
+    call, args, y, want, _inputs = _gated(executor.handle, 300, 32, 64)
+    torch.cuda.synchronize()
+    results = []
+    thread = threading.Thread(target=lambda: results.append((call(*args), _lib.lib().xspmm_last_error())))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert results[0][0] == 0, results
+    assert bool((y == want).all())

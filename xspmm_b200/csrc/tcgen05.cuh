@@ -137,10 +137,18 @@ inline CUtensorMap make_map_2d(const void* base, uint64_t inner, uint64_t outer,
     const cuuint64_t strides[1] = {row_bytes};
     const cuuint32_t box[2] = {box_inner, box_outer};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
-                                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // the thread's first CUDA call: it has a device, but no context yet
+        int device = 0;
+        XS_CHECK_CUDA(cudaGetDevice(&device));
+        XS_CHECK_CUDA(cudaSetDevice(device));
+        r = encode();
+    }
     XS_REQUIRE(r == CUDA_SUCCESS, XSPMM_STATUS_CUDA_ERROR,
                "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
     return m;
