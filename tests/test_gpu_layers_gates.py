@@ -139,3 +139,55 @@ def test_silu_gradient_far_from_zero(executor, n, dtype, odd):
     keep = (v != torch.inf).all(1)
     dwu, v = dwu[keep], v[keep]
     close(dwu, 0.5 * silu(v), 0.5 * silu_error(v), "dup")
+
+
+# ---- gelu -------------------------------------------------------------------------------------------
+# gelu = v * erfc(-v / sqrt 2) / 2. The tail's formula is within 2^-20 of itself with its roundings; e^(-v^2 / 2)
+# carries the roundings of its argument (three of 2^-24 times v^2 / 2) and the exponential's own. (v^2 + 16) * 2^-22
+# of each term covers them with the products after it. Values below 16 * 2^-126 may be 0.
+
+TAIL = {bf16: [-1e20, -1e4, -100.0, -16.0, -12.0, -11.0, -10.0, -9.0, -8.0, -7.0, -6.0, -5.5, -5.0, -4.5, -4.0, -3.0,
+               -2.0, -1.0, -0.25, 0.0, 0.5, 1.0, 3.0, 6.0, 20.0, 1e4],
+        f16: [-6e4, -100.0, -16.0, -8.0, -6.5, -6.0, -5.75, -5.5, -5.25, -5.0, -4.75, -4.5, -4.25, -4.0, -3.0, -2.0,
+              -1.0, 0.0, 1.0, 3.0, 6.0]}
+
+
+def tail(n, dtype):
+    return torch.tensor([TAIL[dtype][i % len(TAIL[dtype])] for i in range(n)], device="cuda").to(dtype)
+
+
+def gelu_terms(v):
+    """gelu(v), its slope's two terms, and the relative error of each."""
+    v = v.clamp(min=-1e3)
+    half = 0.5 * torch.special.erfc(-v * 0.5 ** 0.5)
+    c = v.clamp(max=1e3)
+    return v * half, half, c * torch.exp(-0.5 * c * c) * (2 * torch.pi) ** -0.5, (v.abs().clamp(max=20) ** 2 + 16) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("dtype", [f16, bf16])
+@pytest.mark.parametrize("rows,K", PATHS)
+def test_gelu_of_negative_gates(executor, rows, K, dtype):
+    v = tail(200, dtype)
+    y, _, _ = forward(executor, rows, K, v, 1024.0, "gelu")
+    value, _, _, rel = gelu_terms(v.double())
+    close(y, (1024 * value).expand(rows, -1), 1024 * (value.abs() * rel + 16 * 2.0 ** -126), "y")
+
+
+@pytest.mark.parametrize("dtype", [f16, bf16])
+@pytest.mark.parametrize("n", [64, 128, 191, 200])
+@pytest.mark.parametrize("odd", [None, torch.inf, -torch.inf])
+def test_gelu_gradient_of_negative_gates(executor, n, dtype, odd):
+    eye = torch.eye(n, dtype=dtype, device="cuda")
+    zero = torch.zeros_like(eye)
+    gate = tail(n * n, dtype)
+    if odd is not None:
+        gate[5::37] = odd
+    gate = gate.view(n, n)
+    dy, up = torch.full_like(eye, 64.0), torch.full_like(eye, 64.0)
+    dx, dwg, dwu = torch.empty_like(eye), torch.empty_like(eye), torch.empty_like(eye)
+    xs.gated_ffn_backward(executor, dy, eye, zero, zero, gate, up, dx, dwg, dwu, activation="gelu")
+    v = gate.double().t()
+    value, half, bell, rel = gelu_terms(v)
+    close(dwg, 4096 * (half + bell), 4096 * ((half + bell.abs()) * rel + 16 * 2.0 ** -126), "dgate")
+    keep = (v != torch.inf).all(1)
+    close(dwu[keep], 64 * value[keep], 64 * (value.abs() * rel + 16 * 2.0 ** -126)[keep], "dup")

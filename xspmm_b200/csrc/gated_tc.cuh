@@ -98,18 +98,53 @@ __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f
 // are taken from there: v * sigmoid(v) is 0 for v = -inf, as for every large negative v, instead of inf * 0.
 constexpr float SILU_END = 100.0f;
 
-template <Activation ACT>
-__device__ __forceinline__ float act_value(float v) {
-    if constexpr (ACT == Activation::Silu) v = max_nan(v, -SILU_END);
-    if constexpr (ACT == Activation::Silu) return __fdividef(v, 1.0f + __expf(-v));
-    else if constexpr (ACT == Activation::Gelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
-    else return sigmoid(v);
-}
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// gelu(v) = v Phi(v), Phi the normal distribution, from its upper tail Q(z) = erfc(z / sqrt 2) / 2 at z = |v|:
+// v Phi(v) = max(v, 0) - z Q(z), which does not cancel for negative v as v (1 + erf(v / sqrt 2)) / 2 does (at
+// v = -5.5 that sum is a rounding error). Q(z) = e^(-z^2 / 2) P(t), P a polynomial in t = 1 / (1 + p z) without a
+// constant term: the form of Hastings, Approximations for Digital Computers (1955), with p and the coefficients
+// fitted here for the least relative error on [0, GELU_END], 7e-7 (1.0e-6 with fp32's roundings). The slope,
+// Phi(v) + v e^(-v^2 / 2) / sqrt(2 pi), has the same exponential. From GELU_END on Q is 0 in fp32.
+constexpr float GELU_END = 16.0f, GELU_P = 0.2658f;
+__device__ constexpr float GELU_Q[7] = {0.105937719f,   0.107884675f, 0.084771432f,  0.137925252f,
+                                        -0.0588914752f, 0.189003125f, -0.0666310787f};
+// Q(z) for z in [0, GELU_END], and e^(-z^2 / 2).
+__device__ __forceinline__ float normal_tail(float z, float* bell) {
+    const float t = rcp_approx(fmaf(GELU_P, z, 1.0f));
+    float q = GELU_Q[6];
+#pragma unroll
+    for (int i = 5; i >= 0; --i) q = fmaf(q, t, GELU_Q[i]);
+    *bell = exp2f_approx(z * z * -0.72134752044448170f);
+    return q * t * *bell;
+}
+// gelu of two values in packed fp32, with one reciprocal for both: 1 / a0 = a1 / (a0 a1).
+__device__ __forceinline__ float2 gelu2(float2 v) {
+    const float2 z = make_float2(fminf(fabsf(v.x), GELU_END), fminf(fabsf(v.y), GELU_END));  // NaN: GELU_END
+    const float2 a = fma2(z, make_float2(GELU_P, GELU_P), make_float2(1.0f, 1.0f));
+    const float r = rcp_approx(a.x * a.y);
+    const float2 t = mul2(make_float2(a.y, a.x), make_float2(r, r));
+    float2 q = make_float2(GELU_Q[6], GELU_Q[6]);
+#pragma unroll
+    for (int i = 5; i >= 0; --i) q = fma2(q, t, make_float2(GELU_Q[i], GELU_Q[i]));
+    const float2 x = mul2(mul2(z, z), make_float2(-0.72134752044448170f, -0.72134752044448170f));
+    q = mul2(mul2(q, t), make_float2(exp2f_approx(x.x), exp2f_approx(x.y)));
+    return fma2(make_float2(-z.x, -z.y), q, make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f)));
+}
+
+template <Activation ACT>
+__device__ __forceinline__ float act_value(float v) {
+    if constexpr (ACT == Activation::Silu) v = max_nan(v, -SILU_END);
+    if constexpr (ACT == Activation::Silu) return __fdividef(v, 1.0f + __expf(-v));
+    else if constexpr (ACT == Activation::Gelu) {
+        const float z = min_nan(fabsf(v), GELU_END);
+        float bell;
+        return fmaf(-z, normal_tail(z, &bell), fmaxf(v, 0.0f));
+    } else if constexpr (ACT == Activation::Relu) return v > 0.0f ? v : (v != v ? v : 0.0f);
+    else return sigmoid(v);
 }
 // The sigmoids of two values, in packed fp32, and product = a0 a1. They share one reciprocal,
 // 1 / a0 = a1 / (a0 a1): the special function unit (16 lanes a clock on an SM) weighs on the epilogue of
@@ -165,7 +200,10 @@ __device__ __forceinline__ void gate_words(uint32_t (&w)[16], const uint32_t (&g
     } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float2 v = make_float2(act_value<ACT>(__uint_as_float(g[2 * e])), act_value<ACT>(__uint_as_float(g[2 * e + 1])));
+            const float2 g2 = make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
+            float2 v;
+            if constexpr (ACT == Activation::Gelu) v = gelu2(g2);
+            else v = make_float2(act_value<ACT>(g2.x), act_value<ACT>(g2.y));
             const float2 y = mul2(v, make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])));
             w[e] = pack2(y.x, y.y, T());
         }
@@ -179,9 +217,11 @@ __device__ __forceinline__ void act_both(float v, float* value, float* slope) {
         *value = low * s;
         *slope = s * (1.0f + min_nan(low, SILU_END) * (1.0f - s));
     } else if constexpr (ACT == Activation::Gelu) {
-        const float half = 0.5f * (1.0f + erff(v * 0.70710678118654752f));
-        *value = v * half;
-        *slope = half + v * __expf(-0.5f * v * v) * 0.39894228040143268f;
+        const float z = min_nan(fabsf(v), GELU_END);
+        float bell;
+        const float tail = normal_tail(z, &bell);
+        *value = fmaf(-z, tail, fmaxf(v, 0.0f));
+        *slope = fmaf(copysignf(z, v) * 0.39894228040143268f, bell, v > 0.0f ? 1.0f - tail : tail);
     } else if constexpr (ACT == Activation::Relu) {
         *value = act_value<ACT>(v);
         *slope = v > 0.0f ? 1.0f : 0.0f;
