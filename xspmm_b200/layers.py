@@ -5,9 +5,12 @@ Rows are nodes or tokens and features are contiguous, as in B and C of `spmm`. M
 device tensors whose last dimension has stride 1; their row stride is free (a slice of columns of
 a wider tensor is taken as it is), except where a function says contiguous. Outputs are the
 caller's tensors and are overwritten. Work is enqueued on torch's current stream; nothing
-synchronizes. Wrong shapes, types, strides or devices raise ValueError before anything runs.
+synchronizes. Wrong shapes, types, strides, devices or values and missing inputs raise ValueError
+before anything runs.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -57,6 +60,21 @@ def _dense(exec: CudaExecutor, t, name: str, shape, dtype):
     return t.data_ptr() or None
 
 
+def _needed(exec: CudaExecutor, t, name: str, shape, dtype):
+    """Checks a contiguous argument that may not be None; returns its address."""
+    if t is None:
+        raise ValueError(f"{name} is needed")
+    return _dense(exec, t, name, shape, dtype)
+
+
+def _norm_rows(exec: CudaExecutor, t: torch.Tensor, name: str):
+    """Checks the first matrix of a layer norm, which has to have features; returns _matrix's."""
+    found = _matrix(exec, t, name)
+    if t.shape[1] == 0:
+        raise ValueError(f"{name} must have at least one column")
+    return found
+
+
 def _norm_suffix(x: torch.Tensor, y: torch.Tensor) -> str:
     suffix = _VAL.get(x.dtype, "?") + _VAL.get(y.dtype, "?")
     if suffix not in _NORM_TYPES:
@@ -70,7 +88,9 @@ def layer_norm(exec: CudaExecutor, x: torch.Tensor, weight, bias, eps: float, y:
     y 16 bits. weight and bias: float32 (cols) or None. mean, rstd: float32 (rows), written where
     given. y may be x."""
     suffix = _norm_suffix(x, y)
-    px, ldx = _matrix(exec, x, "x")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and non-negative")
+    px, ldx = _norm_rows(exec, x, "x")
     rows, cols = x.shape
     py, ldy = _matrix(exec, y, "y", rows, cols)
     f32 = torch.float32
@@ -86,13 +106,13 @@ def layer_norm_backward(exec: CudaExecutor, dy: torch.Tensor, x: torch.Tensor, w
     """Gradients of layer_norm from the forward pass's mean and rstd. dy and dx have the type of y;
     dweight and dbias are float32 (cols). Outputs that are None are not computed. dx may be dy."""
     suffix = _norm_suffix(x, dy)
-    pdy, lddy = _matrix(exec, dy, "dy")
+    pdy, lddy = _norm_rows(exec, dy, "dy")
     rows, cols = dy.shape
     px, ldx = _matrix(exec, x, "x", rows, cols)
     pdx, lddx = (None, cols) if dx is None else _matrix(exec, dx, "dx", rows, cols, dy.dtype)
     f32 = torch.float32
     pw = _dense(exec, weight, "weight", (cols,), f32)
-    pm, pr = _dense(exec, mean, "mean", (rows,), f32), _dense(exec, rstd, "rstd", (rows,), f32)
+    pm, pr = _needed(exec, mean, "mean", (rows,), f32), _needed(exec, rstd, "rstd", (rows,), f32)
     pdw = _dense(exec, dweight, "dweight", (cols,), f32)
     pdb = _dense(exec, dbias, "dbias", (cols,), f32)
     check(getattr(lib(), "xspmm_layer_norm_backward_" + suffix)(
@@ -157,11 +177,13 @@ def gated_ffn_backward(exec: CudaExecutor, dy: torch.Tensor, x: torch.Tensor, w_
     and dw_up (F x K, contiguous) are both given or both None. All of x's type."""
     rows, K, F, operands = _gated(exec, x, w_gate, w_up, activation)
     pdy, lddy = _matrix(exec, dy, "dy", rows, F, x.dtype)
-    pg = _dense(exec, gate, "gate", (rows, F), x.dtype)
-    pu = _dense(exec, up, "up", (rows, F), x.dtype)
+    pg = _needed(exec, gate, "gate", (rows, F), x.dtype)
+    pu = _needed(exec, up, "up", (rows, F), x.dtype)
     pdx, lddx = (None, K) if dx is None else _matrix(exec, dx, "dx", rows, K, x.dtype)
     pdg = _dense(exec, dw_gate, "dw_gate", (F, K), x.dtype)
     pdu = _dense(exec, dw_up, "dw_up", (F, K), x.dtype)
+    if (dw_gate is None) != (dw_up is None):
+        raise ValueError("dw_gate and dw_up are given both or neither")
     check(getattr(lib(), "xspmm_gated_ffn_backward_" + _VAL[x.dtype])(
         exec.handle, rows, K, F, _ACT[activation], pdy, lddy, *operands, pg, pu, pdx, lddx, pdg,
         pdu))
