@@ -191,3 +191,26 @@ def test_gelu_gradient_of_negative_gates(executor, n, dtype, odd):
     close(dwg, 4096 * (half + bell), 4096 * ((half + bell.abs()) * rel + 16 * 2.0 ** -126), "dgate")
     keep = (v != torch.inf).all(1)
     close(dwu[keep], 64 * value[keep], 64 * (value.abs() * rel + 16 * 2.0 ** -126)[keep], "dup")
+
+
+# ---- sigmoid ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [f16, bf16])
+@pytest.mark.parametrize("n", [64, 191, 200])
+@pytest.mark.parametrize("odd", [None, torch.inf, -torch.inf])
+def test_sigmoid_gradient_far_from_zero(executor, n, dtype, odd):
+    """s (1 - s) falls off as e^-|v| on both sides. The errors are those of silu's sigmoid."""
+    v = [0.0, 1.0, 3.0, 6.0, 8.0, 10.0, 11.0, 12.0, 14.0, 16.0, 18.0, 20.0, 30.0, 60.0, 100.0, 6e4]
+    v = torch.tensor((v + [-a for a in v]) * (n * n // 32 + 1), device="cuda")[:n * n].to(dtype)
+    if odd is not None:
+        v[5::37] = odd
+    eye = torch.eye(n, dtype=dtype, device="cuda")
+    zero = torch.zeros_like(eye)
+    dy, up = torch.full_like(eye, 64.0), torch.full_like(eye, 64.0)
+    dx, dwg, dwu = torch.empty_like(eye), torch.empty_like(eye), torch.empty_like(eye)
+    xs.gated_ffn_backward(executor, dy, eye, zero, zero, v.view(n, n), up, dx, dwg, dwu, activation="sigmoid")
+    v = v.view(n, n).t().double()
+    s, c = torch.sigmoid(v), torch.sigmoid(-v)
+    rel = (v.abs().clamp(max=100) + 16) * 2.0 ** -22
+    close(dwg, 4096 * s * c, 4096 * (s * c * rel + 2.0 ** -126), "dgate")
+    close(dwu, 64 * s, 64 * (s * rel + 2.0 ** -126), "dup")

@@ -226,9 +226,10 @@ __device__ __forceinline__ void act_both(float v, float* value, float* slope) {
         *value = act_value<ACT>(v);
         *slope = v > 0.0f ? 1.0f : 0.0f;
     } else {
-        const float s = sigmoid(v);
-        *value = s;
-        *slope = s * (1.0f - s);
+        // s(|v|) and s(-|v|) from one exponential: 1 - s would cancel for large positive v
+        const float e = exp2f_approx(fabsf(v) * -1.4426950408889634f), high = rcp_approx(1.0f + e), low = e * high;
+        *value = v < 0.0f ? low : high;
+        *slope = high * low;
     }
 }
 
