@@ -159,10 +159,11 @@ __device__ __forceinline__ float2 sigmoid2(float2 v, float* product) {
     return mul2(make_float2(a.y, a.x), make_float2(r, r));
 }
 // y = act(g) * u of the first `cols` of a row's 32 columns as 16 packed words. silu takes them in pairs (2^20
-// rows of 128 x 128, sustained: 228 us; one value at a time 240), and all of them again one at a time where a
+// rows of 128 x 128, sustained: 216 us; one value at a time 229), and all of them again one at a time where a
 // pair does not hold (a NaN among them). The choice is the row's own: neither other rows nor what lies past
-// its columns enter it. The second form is a loop over copies in local memory: unrolled, its instructions
-// cost the first one 6 us.
+// its columns enter it. The second form is a loop over copies in local memory, two pairs at a time:
+// unrolled, its instructions cost the first one 6 us, by four 1 us. All gates below -43: 485 us (648 by one pair,
+// 415 by four).
 template <Activation ACT, typename T>
 __device__ __forceinline__ void gate_words(uint32_t (&w)[16], const uint32_t (&g)[32], const uint32_t (&u)[32], int cols) {
     if constexpr (ACT == Activation::Silu) {
@@ -184,15 +185,17 @@ __device__ __forceinline__ void gate_words(uint32_t (&w)[16], const uint32_t (&g
             gs[e] = make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
             us[e] = make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]));
         }
-        holds = true;
+        if (cols < 32) {
+            holds = true;
 #pragma unroll 1
-        for (int e = 0; 2 * e < cols; ++e) {
-            float product;
-            sigmoid2(gs[e], &product);
-            holds = holds && product <= PAIR_MAX;
+            for (int e = 0; 2 * e < cols; ++e) {
+                float product;
+                sigmoid2(gs[e], &product);
+                holds = holds && product <= PAIR_MAX;
+            }
+            if (holds) return;
         }
-        if (holds) return;
-#pragma unroll 1
+#pragma unroll 2
         for (int e = 0; e < 16; ++e)
             ws[e] = pack2(act_value<ACT>(gs[e].x) * us[e].x, act_value<ACT>(gs[e].y) * us[e].y, T());
 #pragma unroll
