@@ -473,7 +473,8 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   projections, which the gradient needs. act: silu, gelu (with erf), relu or sigmoid; silu of
  *   -inf and its slope there are 0, as for every large negative gate. 16-bit types only: fp32 rows
  *   go through a layer norm with a 16-bit y.
- * Its gradient. dup = dy * act(gate), dgate = dy * up * act'(gate) (rounded to the 16-bit type),
+ * Its gradient. dup = dy * act(gate), dgate = dy * up * act'(gate) (rounded to the 16-bit type,
+ *   infinite past its range),
  *   dx = dgate w_gate + dup w_up, dw_gate = dgate^T x, dw_up = dup^T x (F x K, contiguous,
  *   overwritten; zeros when rows = 0). dx may be NULL, and dw_gate and dw_up may both be.
  * ------------------------------------------------------------------------------------------- */

@@ -99,8 +99,10 @@ void allow_smem(K kern, size_t most = DYNAMIC_SMEM) {
     XS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
 }
 
-// Launches a kernel that calls cudaGridDependencySynchronize() before it touches memory: its launch and
-// prologue overlap the end of the stream's previous kernel.
+// Launches a kernel that calls cudaGridDependencySynchronize() before it touches memory. No kernel here triggers
+// its dependents early, so its CTAs start once the stream's previous kernel has none left to start or run: the
+// launch is hidden, and the prologue runs while that kernel's results settle, not under its work (4096 x 4096
+// bf16 norm gradient, two kernels: 33 us without, 30 with).
 template <typename... P, typename... A>
 void launch_dependent(cudaStream_t stream, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster,
                       A&&... args) {

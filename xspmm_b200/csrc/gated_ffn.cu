@@ -3,7 +3,9 @@
 // Forward: g = x wg^T, u = x wu^T, y = act(g) * u. Backward, from dy and the kept g and u:
 // du = dy * act(g), dg = dy * u * act'(g), dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x.
 // Sums are held in fp32; dg and du are rounded to the operands' 16-bit type before the products,
-// as any 16-bit matrix product's operand is.
+// as any 16-bit matrix product's operand is. Where the terms of a sum are independent that makes a gradient's
+// error sqrt 2 times its own rounding's; where they cancel, more; and an fp16 dg or du past 65504 is infinite.
+// Products of what the rounding leaves off, added on, would take as long again as the products themselves.
 //
 // The products run on the tensor cores (gated_tc.cuh). TMA needs 16-byte rows: an operand whose
 // address or row stride is not is first copied to scratch with a stride that is.
