@@ -1,6 +1,8 @@
 // xspmm/layers.hpp -- the operators of the layer around the sparse product, over the C ABI: layer norm,
-// dropout and the gated feed-forward block, each with its gradient (xspmm_layer_norm_*, xspmm_dropout_*,
-// xspmm_gated_ffn_* in include/xspmm_b200.h, which states what each computes). The reference has none.
+// group norm, dropout and the gated feed-forward block, each with its gradient, 8-bit rows and their product,
+// and the orthogonalised update of a weight (xspmm_layer_norm_*, xspmm_group_norm_*, xspmm_dropout_*,
+// xspmm_gated_ffn_*, xspmm_quantize_rows_*, xspmm_linear_int8_*, xspmm_orthogonalize_* in
+// include/xspmm_b200.h, which states what each computes). The reference has none.
 //
 // Rows are nodes or tokens, features are contiguous; a Rows<T> is a device matrix with its row stride in
 // elements. Calls enqueue on the executor's stream and throw as the other calls do.
@@ -14,7 +16,7 @@
 
 namespace xspmm {
 
-enum class Activation { Silu = XSPMM_ACT_SILU, Gelu = XSPMM_ACT_GELU, Relu = XSPMM_ACT_RELU, Sigmoid = XSPMM_ACT_SIGMOID };
+enum class Activation { Silu = XSPMM_ACT_SILU, Gelu = XSPMM_ACT_GELU, Relu = XSPMM_ACT_RELU, Sigmoid = XSPMM_ACT_SIGMOID, None = XSPMM_ACT_NONE };
 
 template <typename T>
 struct Rows {
@@ -31,6 +33,8 @@ struct NormAbi;
     struct NormAbi<X, Y> {                                                       \
         static constexpr auto forward = xspmm_layer_norm_##S;                    \
         static constexpr auto backward = xspmm_layer_norm_backward_##S;          \
+        static constexpr auto group_forward = xspmm_group_norm_##S;              \
+        static constexpr auto group_backward = xspmm_group_norm_backward_##S;    \
     };
 XSPMM_NORM_ROW(__half, __half, f16f16)
 XSPMM_NORM_ROW(__nv_bfloat16, __nv_bfloat16, bf16bf16)
@@ -55,6 +59,28 @@ template <> struct GatedAbi<__nv_bfloat16> {
     static constexpr auto forward = xspmm_gated_ffn_bf16;
     static constexpr auto backward = xspmm_gated_ffn_backward_bf16;
 };
+
+template <typename T>
+struct Int8Abi;
+template <> struct Int8Abi<__half> {
+    static constexpr auto quantize = xspmm_quantize_rows_f16;
+    static constexpr auto linear = xspmm_linear_int8_f16;
+};
+template <> struct Int8Abi<__nv_bfloat16> {
+    static constexpr auto quantize = xspmm_quantize_rows_bf16;
+    static constexpr auto linear = xspmm_linear_int8_bf16;
+};
+template <> struct Int8Abi<float> {
+    static constexpr auto quantize = xspmm_quantize_rows_f32;
+    static constexpr auto linear = xspmm_linear_int8_f32;
+};
+
+template <typename X, typename Y>
+struct UpdateAbi;
+template <> struct UpdateAbi<__half, __half> { static constexpr auto call = xspmm_orthogonalize_f16f16; };
+template <> struct UpdateAbi<__nv_bfloat16, __nv_bfloat16> { static constexpr auto call = xspmm_orthogonalize_bf16bf16; };
+template <> struct UpdateAbi<float, __half> { static constexpr auto call = xspmm_orthogonalize_f32f16; };
+template <> struct UpdateAbi<float, __nv_bfloat16> { static constexpr auto call = xspmm_orthogonalize_f32bf16; };
 
 }  // namespace detail
 
@@ -102,6 +128,60 @@ void gated_ffn_backward(std::shared_ptr<const Executor> exec, int64_t rows, int6
     detail::check(detail::GatedAbi<T>::backward(detail::handle_of(exec), rows, K, F, static_cast<int>(act),
                                                 dy.data, dy.ld, x.data, x.ld, w_gate.data, w_gate.ld,
                                                 w_up.data, w_up.ld, gate, up, dx.data, dx.ld, dw_gate, dw_up));
+}
+
+// A packed batch for the group norm: sample i is rows [offsets[i], offsets[i + 1]) (device, samples + 1).
+// The default is one sample of all rows.
+struct Samples {
+    int64_t count = 1;
+    const int64_t* offsets = nullptr;
+};
+
+// y = act((x - mean) * rstd * weight + bias) over each sample's rows and group of neighbouring channels.
+// weight, bias, mean, rstd may be null.
+template <typename X, typename Y>
+void group_norm(std::shared_ptr<const Executor> exec, int64_t rows, int64_t cols, int64_t groups, Samples samples,
+                Rows<const X> x, const float* weight, const float* bias, float eps, Activation act, Rows<Y> y,
+                float* mean = nullptr, float* rstd = nullptr) {
+    detail::check(detail::NormAbi<X, Y>::group_forward(detail::handle_of(exec), rows, cols, groups, samples.count,
+                                                       samples.offsets, x.data, x.ld, weight, bias, eps,
+                                                       static_cast<int>(act), y.data, y.ld, mean, rstd));
+}
+
+// Gradients of group_norm; outputs that are null are not computed.
+template <typename X, typename Y>
+void group_norm_backward(std::shared_ptr<const Executor> exec, int64_t rows, int64_t cols, int64_t groups,
+                         Samples samples, Rows<const Y> dy, Rows<const X> x, const float* weight, const float* bias,
+                         const float* mean, const float* rstd, Activation act, Rows<Y> dx, float* dweight,
+                         float* dbias) {
+    detail::check(detail::NormAbi<X, Y>::group_backward(detail::handle_of(exec), rows, cols, groups, samples.count,
+                                                        samples.offsets, dy.data, dy.ld, x.data, x.ld, weight, bias,
+                                                        mean, rstd, static_cast<int>(act), dx.data, dx.ld, dweight,
+                                                        dbias));
+}
+
+// Rows of x as 8-bit integers q with a scale each.
+template <typename T>
+void quantize_rows(std::shared_ptr<const Executor> exec, int64_t rows, int64_t cols, Rows<const T> x, Rows<int8_t> q,
+                   float* scale) {
+    detail::check(detail::Int8Abi<T>::quantize(detail::handle_of(exec), rows, cols, x.data, x.ld, q.data, q.ld, scale));
+}
+
+// y = x_scale * w_scale * (x w^T) + bias of 8-bit x (rows x K) and w (F x K); bias may be null.
+template <typename T>
+void linear_int8(std::shared_ptr<const Executor> exec, int64_t rows, int64_t K, int64_t F, Rows<const int8_t> x,
+                 const float* x_scale, Rows<const int8_t> w, const float* w_scale, Rows<T> y,
+                 const float* bias = nullptr) {
+    detail::check(detail::Int8Abi<T>::linear(detail::handle_of(exec), rows, K, F, x.data, x.ld, x_scale, w.data, w.ld,
+                                             w_scale, bias, y.data, y.ld));
+}
+
+// The orthogonalised update y of a weight matrix from its gradient or momentum g.
+template <typename X, typename Y>
+void orthogonalize(std::shared_ptr<const Executor> exec, int64_t rows, int64_t cols, Rows<const X> g, Rows<Y> y,
+                   int steps = 5, float eps = 1e-7f) {
+    detail::check(detail::UpdateAbi<X, Y>::call(detail::handle_of(exec), rows, cols, g.data, g.ld, steps, eps, y.data,
+                                                y.ld));
 }
 
 }  // namespace xspmm

@@ -477,12 +477,46 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   infinite past its range),
  *   dx = dgate w_gate + dup w_up, dw_gate = dgate^T x, dw_up = dup^T x (F x K, contiguous,
  *   overwritten; zeros when rows = 0). dx may be NULL, and dw_gate and dw_up may both be.
+ *
+ * Group norm with an activation, channels contiguous. x is rows x cols; offsets (samples + 1, int64,
+ *   device) cuts the rows into samples, sample i being rows [offsets[i], offsets[i + 1]): the graphs of
+ *   a packed batch. offsets NULL (samples = 1): one sample of all rows. Rows before the first offset and
+ *   behind the last are not read and their outputs are left as they were; a sample may have no rows.
+ *   Offsets must not decrease and lie in [0, rows]; others are taken as the nearest that does (samples
+ *   then overlap or are empty, and nothing out of range is touched). groups divides cols, cols / groups
+ *   is at most 16384. Over a sample's rows and a group's n values,
+ *   mean = sum(x) / n, rstd = 1 / sqrt(sum((x - mean)^2) / n + eps) (no values: 0 and 1 / sqrt(eps)),
+ *   z = ((x - mean) * rstd) * weight + bias, y = act(z); activation as below or XSPMM_ACT_NONE (y = z).
+ *   All in fp32, z with each operation rounded by itself. Types as for the layer norm; weight, bias
+ *   (cols, fp32; NULL: 1 and 0); mean, rstd (samples x groups, fp32) are written where not NULL. y may
+ *   be x (same type and stride).
+ * Its gradient. dz = dy * act'(z) with z as above (relu: 1 where z > 0), t = dz * weight,
+ *   dx = rstd * (t - mean(t) - xh * mean(t * xh)), xh = (x - mean) * rstd, the means over the sample's
+ *   group; dweight = sum of dz * xh, dbias = sum of dz over all samples' rows (cols, fp32, overwritten).
+ *   dy and dx have y's type. Each of dx, dweight, dbias may be NULL. dx may be dy (same stride).
+ *
+ * Rows in 8-bit integers. scale[r] = max|x| / 127 over row r and q = 127 x / max|x| rounded to the
+ *   nearest whole number (ties to even) of the exact quotient, so q * scale stands for x. A row of zeros
+ *   has scale 0; a row that holds an infinity or NaN has scale NaN and q = 0, so that products of it are
+ *   NaN. q (rows x cols, int8), scale (rows, fp32).
+ * Product of 8-bit rows. y[r, f] = x_scale[r] * w_scale[f] * sum_k x[r, k] w[f, k] + bias[f], x rows x K
+ *   and w F x K of int8, the sum exact (32-bit integers, K at most 131071), the rest in fp32; y (rows x
+ *   F) fp16, bf16 or fp32; bias (F, fp32) may be NULL. K = 0: y = bias.
+ *
+ * Orthogonalised update. y = X_steps for a matrix g: X_0 = g / (|g| + eps), |g| the root of the sum of
+ *   squares, X_{i+1} = a X_i + (b A + c A A) X_i, A = X_i X_i^T, (a, b, c) = (3.4445, -4.7750, 2.0315):
+ *   an odd polynomial of the singular values that drives them to about 1 (0.68 to 1.2 after 5 steps,
+ *   where they were not tiny). g fp16, bf16 or fp32; y fp16 or bf16 (the type of a 16-bit g). Products
+ *   of 22-bit operands (two fp16 parts each) with fp32 sums: the error is a small part of y's rounding.
+ *   0 <= steps <= 100; steps = 0: y = X_0. An infinity or NaN in g makes y NaN (steps >= 1). y may be g
+ *   (same type and stride).
  * ------------------------------------------------------------------------------------------- */
 typedef enum xspmm_activation {
     XSPMM_ACT_SILU = 0,
     XSPMM_ACT_GELU = 1,
     XSPMM_ACT_RELU = 2,
-    XSPMM_ACT_SIGMOID = 3
+    XSPMM_ACT_SIGMOID = 3,
+    XSPMM_ACT_NONE = -1 /* group norm only */
 } xspmm_activation_t;
 
 xspmm_status_t xspmm_layer_norm_f16f16(xspmm_handle_t h, int64_t rows, int64_t cols,
@@ -535,6 +569,74 @@ xspmm_status_t xspmm_gated_ffn_backward_bf16(xspmm_handle_t h, int64_t rows, int
     int64_t F, int activation, const void* dy, int64_t lddy, const void* x, int64_t ldx,
     const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu, const void* gate,
     const void* up, void* dx, int64_t lddx, void* dw_gate, void* dw_up);
+xspmm_status_t xspmm_group_norm_f16f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    int64_t groups, int64_t samples, const int64_t* offsets, const void* x, int64_t ldx,
+    const float* weight, const float* bias, float eps, int activation, void* y, int64_t ldy,
+    float* mean, float* rstd);
+xspmm_status_t xspmm_group_norm_bf16bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    int64_t groups, int64_t samples, const int64_t* offsets, const void* x, int64_t ldx,
+    const float* weight, const float* bias, float eps, int activation, void* y, int64_t ldy,
+    float* mean, float* rstd);
+xspmm_status_t xspmm_group_norm_f32f32(xspmm_handle_t h, int64_t rows, int64_t cols,
+    int64_t groups, int64_t samples, const int64_t* offsets, const void* x, int64_t ldx,
+    const float* weight, const float* bias, float eps, int activation, void* y, int64_t ldy,
+    float* mean, float* rstd);
+xspmm_status_t xspmm_group_norm_f32f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    int64_t groups, int64_t samples, const int64_t* offsets, const void* x, int64_t ldx,
+    const float* weight, const float* bias, float eps, int activation, void* y, int64_t ldy,
+    float* mean, float* rstd);
+xspmm_status_t xspmm_group_norm_f32bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    int64_t groups, int64_t samples, const int64_t* offsets, const void* x, int64_t ldx,
+    const float* weight, const float* bias, float eps, int activation, void* y, int64_t ldy,
+    float* mean, float* rstd);
+xspmm_status_t xspmm_group_norm_backward_f16f16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, int64_t groups, int64_t samples, const int64_t* offsets, const void* dy,
+    int64_t lddy, const void* x, int64_t ldx, const float* weight, const float* bias,
+    const float* mean, const float* rstd, int activation, void* dx, int64_t lddx, float* dweight,
+    float* dbias);
+xspmm_status_t xspmm_group_norm_backward_bf16bf16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, int64_t groups, int64_t samples, const int64_t* offsets, const void* dy,
+    int64_t lddy, const void* x, int64_t ldx, const float* weight, const float* bias,
+    const float* mean, const float* rstd, int activation, void* dx, int64_t lddx, float* dweight,
+    float* dbias);
+xspmm_status_t xspmm_group_norm_backward_f32f32(xspmm_handle_t h, int64_t rows,
+    int64_t cols, int64_t groups, int64_t samples, const int64_t* offsets, const void* dy,
+    int64_t lddy, const void* x, int64_t ldx, const float* weight, const float* bias,
+    const float* mean, const float* rstd, int activation, void* dx, int64_t lddx, float* dweight,
+    float* dbias);
+xspmm_status_t xspmm_group_norm_backward_f32f16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, int64_t groups, int64_t samples, const int64_t* offsets, const void* dy,
+    int64_t lddy, const void* x, int64_t ldx, const float* weight, const float* bias,
+    const float* mean, const float* rstd, int activation, void* dx, int64_t lddx, float* dweight,
+    float* dbias);
+xspmm_status_t xspmm_group_norm_backward_f32bf16(xspmm_handle_t h, int64_t rows,
+    int64_t cols, int64_t groups, int64_t samples, const int64_t* offsets, const void* dy,
+    int64_t lddy, const void* x, int64_t ldx, const float* weight, const float* bias,
+    const float* mean, const float* rstd, int activation, void* dx, int64_t lddx, float* dweight,
+    float* dbias);
+xspmm_status_t xspmm_quantize_rows_f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale);
+xspmm_status_t xspmm_quantize_rows_bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale);
+xspmm_status_t xspmm_quantize_rows_f32(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale);
+xspmm_status_t xspmm_linear_int8_f16(xspmm_handle_t h, int64_t rows, int64_t K, int64_t F,
+    const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+    const float* w_scale, const float* bias, void* y, int64_t ldy);
+xspmm_status_t xspmm_linear_int8_bf16(xspmm_handle_t h, int64_t rows, int64_t K, int64_t F,
+    const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+    const float* w_scale, const float* bias, void* y, int64_t ldy);
+xspmm_status_t xspmm_linear_int8_f32(xspmm_handle_t h, int64_t rows, int64_t K, int64_t F,
+    const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+    const float* w_scale, const float* bias, void* y, int64_t ldy);
+xspmm_status_t xspmm_orthogonalize_f16f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* g, int64_t ldg, int steps, float eps, void* y, int64_t ldy);
+xspmm_status_t xspmm_orthogonalize_bf16bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* g, int64_t ldg, int steps, float eps, void* y, int64_t ldy);
+xspmm_status_t xspmm_orthogonalize_f32f16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* g, int64_t ldg, int steps, float eps, void* y, int64_t ldy);
+xspmm_status_t xspmm_orthogonalize_f32bf16(xspmm_handle_t h, int64_t rows, int64_t cols,
+    const void* g, int64_t ldg, int steps, float eps, void* y, int64_t ldy);
 
 #ifdef __cplusplus
 } /* extern "C" */

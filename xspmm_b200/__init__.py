@@ -4,7 +4,8 @@ Tier-1 BCSR 16x16 block SpMM on tensor cores and the Tier-2 pipeline around it (
 Jaccard row clustering, CSR row permutation, CSR->BCSR conversion, unpermute), all on the device,
 behind the C ABI in include/xspmm_b200.h (libxspmm_b200.so). This package is the Python view of
 that ABI, mirroring the reference's API names. Next to the product stand the operators of the layer around
-it, forward and backward: layer norm, dropout and the gated feed-forward block (layers.py).
+it: layer norm, group norm, dropout and the gated feed-forward block, forward and backward, 8-bit rows and
+their product, and the orthogonalised update of a weight (layers.py).
 """
 from .api import (  # noqa: F401
     BCSRMatrix,
@@ -23,7 +24,12 @@ from .layers import (  # noqa: F401
     dropout_backward,
     gated_ffn,
     gated_ffn_backward,
+    group_norm,
+    group_norm_backward,
     layer_norm,
     layer_norm_backward,
+    linear_int8,
+    orthogonalize,
+    quantize_rows,
 )
 from ._lib import XSpMMError, lib  # noqa: F401

@@ -134,9 +134,20 @@ def lib():
                                                         _I64, _P, _P]
         getattr(L, f"xspmm_layer_norm_backward_{t}").argtypes = [
             _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P]
+        getattr(L, f"xspmm_group_norm_{t}").argtypes = [
+            _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _F, ctypes.c_int, _P, _I64, _P, _P]
+        getattr(L, f"xspmm_group_norm_backward_{t}").argtypes = [
+            _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, ctypes.c_int, _P,
+            _I64, _P, _P]
+    for t in ("f16f16", "bf16bf16", "f32f16", "f32bf16"):
+        getattr(L, f"xspmm_orthogonalize_{t}").argtypes = [
+            _P, _I64, _I64, _P, _I64, ctypes.c_int, _F, _P, _I64]
     for t in ("f16", "bf16", "f32"):
         getattr(L, f"xspmm_dropout_{t}").argtypes = [_P, _I64, _P, _P, ctypes.c_double, _U64, _U64,
                                                      _P]
+        getattr(L, f"xspmm_quantize_rows_{t}").argtypes = [_P, _I64, _I64, _P, _I64, _P, _I64, _P]
+        getattr(L, f"xspmm_linear_int8_{t}").argtypes = [
+            _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64]
     for t in ("f16", "bf16"):
         getattr(L, f"xspmm_gated_ffn_{t}").argtypes = [
             _P, _I64, _I64, _I64, ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P]

@@ -1,5 +1,6 @@
 // layers.cuh -- internal host entry points of the layer operators that stand next to the sparse
-// product (layer norm, dropout, gated feed-forward) and the device pieces they share. Rows are
+// product (layer norm, group norm, dropout, gated feed-forward, 8-bit rows and their product,
+// orthogonalised updates) and the device pieces they share. Rows are
 // nodes or tokens, features are contiguous; ld* are row strides in elements.
 #pragma once
 
@@ -17,13 +18,56 @@ void layer_norm_backward(Handle& h, int64_t rows, int64_t D, const TY* dy, int64
                          const TX* x, int64_t ldx, const float* w, const float* mean,
                          const float* rstd, TY* dx, int64_t lddx, float* dw, float* db);
 
+// Group norm with an activation (group_norm.cu). Channels are contiguous; sample i is rows
+// [offsets[i], offsets[i + 1]), all rows where offsets is null (samples is 1 then).
+enum class Activation { None = -1, Silu = 0, Gelu = 1, Relu = 2, Sigmoid = 3 };
+template <typename TX>
+struct GroupNormArgs {
+    int64_t rows, C, groups, samples;
+    const int64_t* offsets;
+    const TX* x;
+    int64_t ldx;
+    const float *w, *b;  // C, or null
+    Activation act;
+};
+constexpr int64_t GROUP_NORM_MAX_WIDTH = 16384;  // channels of a group
+// mean and rstd (samples x groups) may be null.
+template <typename TX, typename TY>
+void group_norm(Handle& h, const GroupNormArgs<TX>& a, float eps, TY* y, int64_t ldy, float* mean, float* rstd);
+// Its gradient; any of dx, dw, db may be null.
+template <typename TX, typename TY>
+void group_norm_backward(Handle& h, const GroupNormArgs<TX>& a, const TY* dy, int64_t lddy, const float* mean,
+                         const float* rstd, TY* dx, int64_t lddx, float* dw, float* db);
+
+// Rows in 8-bit integers with a scale each (int8.cu).
+template <typename T>
+void quantize_rows(Handle& h, int64_t rows, int64_t cols, const T* x, int64_t ldx, int8_t* q, int64_t ldq,
+                   float* scale);
+// y[r, f] = xs[r] * ws[f] * sum_k x[r, k] w[f, k] + bias[f]; bias may be null.
+constexpr int64_t INT8_MAX_K = 131071;  // 2^14 K stays below 2^31
+struct Int8Args {
+    int64_t rows, K, F;
+    const int8_t* x;
+    int64_t ldx;
+    const float* xs;
+    const int8_t* w;
+    int64_t ldw;
+    const float *ws, *bias;
+};
+template <typename T>
+void linear_int8(Handle& h, const Int8Args& a, T* y, int64_t ldy);
+
+// The orthogonalised update of a weight matrix (orthogonalize.cu).
+template <typename TX, typename TY>
+void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t ldg, int steps, float eps, TY* y,
+                   int64_t ldy);
+
 // y = residual + keep * x / (1 - p) over n contiguous elements (dropout.cu).
 template <typename T>
 void dropout(Handle& h, int64_t n, const T* x, const T* residual, double p, uint64_t seed,
              uint64_t offset, T* y);
 
 // Gated feed-forward block (gated_ffn.cu).
-enum class Activation { Silu = 0, Gelu = 1, Relu = 2, Sigmoid = 3 };
 template <typename T>
 struct GatedArgs {
     int64_t rows, K, F;  // x is rows x K, the weights F x K, the block's output rows x F

@@ -1,5 +1,6 @@
-"""The operators of the layer around the sparse product, over the C ABI: layer norm, dropout and the
-gated feed-forward block, each with its gradient.
+"""The operators of the layer around the sparse product, over the C ABI: layer norm, group norm with an
+activation, dropout and the gated feed-forward block, each with its gradient; rows in 8-bit integers and
+their product, for serving; the orthogonalised update of a weight matrix, for training.
 
 Rows are nodes or tokens and features are contiguous, as in B and C of `spmm`. Matrices are 2-D
 device tensors whose last dimension has stride 1; their row stride is free (a slice of columns of
@@ -18,6 +19,8 @@ from ._lib import check, lib
 from .api import _VAL, CudaExecutor
 
 _ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+_GROUP_ACT = {None: -1, **_ACT}
+_MAX_GROUP, _MAX_INT8_K = 16384, 131071
 _NORM_TYPES = ("f16f16", "bf16bf16", "f32f32", "f32f16", "f32bf16")
 
 
@@ -187,3 +190,122 @@ def gated_ffn_backward(exec: CudaExecutor, dy: torch.Tensor, x: torch.Tensor, w_
     check(getattr(lib(), "xspmm_gated_ffn_backward_" + _VAL[x.dtype])(
         exec.handle, rows, K, F, _ACT[activation], pdy, lddy, *operands, pg, pu, pdx, lddx, pdg,
         pdu))
+
+
+def _group_norm(exec, x, y, y_name, groups, weight, bias, offsets, activation):
+    """Checks what group_norm and its gradient have in common; returns the C arguments before and
+    after x's address and stride, and the shape of the statistics."""
+    suffix = _VAL.get(x.dtype, "?") + _VAL.get(y.dtype, "?")
+    if suffix not in _NORM_TYPES:
+        raise ValueError(f"group norm takes {x.dtype} to no {y.dtype}")
+    if activation not in _GROUP_ACT:
+        raise ValueError(f"activation must be None or one of {', '.join(_ACT)}, not {activation!r}")
+    found = _norm_rows(exec, x, "x")
+    rows, cols = x.shape
+    if not (isinstance(groups, int) and groups >= 1 and cols % groups == 0):
+        raise ValueError(f"groups must be a whole number that divides {cols}, not {groups!r}")
+    if cols // groups > _MAX_GROUP:
+        raise ValueError(f"a group has at most {_MAX_GROUP} channels, not {cols // groups}")
+    samples = 1
+    if offsets is not None:
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must hold one more value than there are samples")
+        samples = offsets.numel() - 1
+    po = _dense(exec, offsets, "offsets", (samples + 1,), torch.int64)
+    out = _matrix(exec, y, y_name, rows, cols)
+    pw = _dense(exec, weight, "weight", (cols,), torch.float32)
+    pb = _dense(exec, bias, "bias", (cols,), torch.float32)
+    return suffix, (rows, cols, groups, samples, po), found, out, (pw, pb), (samples, groups)
+
+
+def group_norm(exec: CudaExecutor, x: torch.Tensor, groups: int, weight, bias, eps: float,
+               y: torch.Tensor, offsets=None, activation=None, mean=None, rstd=None) -> None:
+    """y = act((x - mean) * rstd * weight + bias) with the statistics of each sample's rows and each of
+    `groups` groups of neighbouring channels. offsets (int64, samples + 1): sample i is rows
+    [offsets[i], offsets[i + 1]); rows outside all of them are left as they were in y, and a sample may be
+    empty. None: all rows are one sample. activation: None, silu, gelu (erf), relu or sigmoid. x and y of
+    one type, or x float32 and y 16 bits. weight and bias: float32 (cols) or None. mean, rstd: float32
+    (samples, groups), written where given. y may be x. The offsets' values are not checked: see the C
+    header for what those out of order mean."""
+    suffix, sizes, (px, ldx), (py, ldy), wb, shape = _group_norm(
+        exec, x, y, "y", groups, weight, bias, offsets, activation)
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and non-negative")
+    pm = _dense(exec, mean, "mean", shape, torch.float32)
+    pr = _dense(exec, rstd, "rstd", shape, torch.float32)
+    check(getattr(lib(), "xspmm_group_norm_" + suffix)(
+        exec.handle, *sizes, px, ldx, *wb, eps, _GROUP_ACT[activation], py, ldy, pm, pr))
+
+
+def group_norm_backward(exec: CudaExecutor, dy: torch.Tensor, x: torch.Tensor, groups: int, weight,
+                        bias, mean: torch.Tensor, rstd: torch.Tensor, dx=None, dweight=None,
+                        dbias=None, offsets=None, activation=None) -> None:
+    """Gradients of group_norm from the forward pass's mean and rstd, with its weight, bias, offsets and
+    activation. dy and dx have the type of y; dweight and dbias are float32 (cols). Outputs that are None
+    are not computed. dx may be dy."""
+    suffix, sizes, (px, ldx), (pdy, lddy), wb, shape = _group_norm(
+        exec, x, dy, "dy", groups, weight, bias, offsets, activation)
+    rows, cols = x.shape
+    pdx, lddx = (None, cols) if dx is None else _matrix(exec, dx, "dx", rows, cols, dy.dtype)
+    f32 = torch.float32
+    pm, pr = _needed(exec, mean, "mean", shape, f32), _needed(exec, rstd, "rstd", shape, f32)
+    pdw = _dense(exec, dweight, "dweight", (cols,), f32)
+    pdb = _dense(exec, dbias, "dbias", (cols,), f32)
+    check(getattr(lib(), "xspmm_group_norm_backward_" + suffix)(
+        exec.handle, *sizes, pdy, lddy, px, ldx, *wb, pm, pr, _GROUP_ACT[activation], pdx, lddx, pdw,
+        pdb))
+
+
+def quantize_rows(exec: CudaExecutor, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """Rows of x in 8-bit integers: scale = max|x| / 127 of each row (float32), q = x / scale rounded to
+    the nearest (int8, of x's shape). A row of zeros has scale 0, one with an infinity or NaN scale NaN."""
+    if x.dtype not in _VAL:
+        raise ValueError(f"quantize_rows takes no {x.dtype}")
+    px, ldx = _matrix(exec, x, "x")
+    rows, cols = x.shape
+    pq, ldq = _matrix(exec, q, "q", rows, cols, torch.int8)
+    ps = _needed(exec, scale, "scale", (rows,), torch.float32)
+    check(getattr(lib(), "xspmm_quantize_rows_" + _VAL[x.dtype])(
+        exec.handle, rows, cols, px, ldx, pq, ldq, ps))
+
+
+def linear_int8(exec: CudaExecutor, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor,
+                w_scale: torch.Tensor, y: torch.Tensor, bias=None) -> None:
+    """y = (x @ w.T) * x_scale[:, None] * w_scale + bias: x (rows x K) and w (F x K) int8, as
+    quantize_rows makes them of activations and of a weight; the sum is exact. y (rows x F) float16,
+    bfloat16 or float32; x_scale (rows), w_scale (F) and bias (F, or None) float32."""
+    if y.dtype not in _VAL:
+        raise ValueError(f"linear_int8 gives no {y.dtype}")
+    px, ldx = _matrix(exec, x, "x", None, None, torch.int8)
+    rows, K = x.shape
+    if K > _MAX_INT8_K:
+        raise ValueError(f"x has at most {_MAX_INT8_K} columns, not {K}")
+    pw, ldw = _matrix(exec, w, "w", None, K, torch.int8)
+    F = w.shape[0]
+    f32 = torch.float32
+    pxs = _needed(exec, x_scale, "x_scale", (rows,), f32)
+    pws = _needed(exec, w_scale, "w_scale", (F,), f32)
+    pb = _dense(exec, bias, "bias", (F,), f32)
+    py, ldy = _matrix(exec, y, "y", rows, F)
+    check(getattr(lib(), "xspmm_linear_int8_" + _VAL[y.dtype])(
+        exec.handle, rows, K, F, px, ldx, pxs, pw, ldw, pws, pb, py, ldy))
+
+
+def orthogonalize(exec: CudaExecutor, g: torch.Tensor, y: torch.Tensor, steps: int = 5,
+                  eps: float = 1e-7) -> None:
+    """The update of a weight matrix from its gradient or momentum g with every singular value driven to
+    about 1, by Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T, from X = g / (|g| + eps),
+    (a, b, c) = (3.4445, -4.7750, 2.0315). g float16, bfloat16 or float32; y float16 or bfloat16, g's
+    type where that is 16 bits. y may be g."""
+    suffix = _VAL.get(g.dtype, "?") + _VAL.get(y.dtype, "?")
+    if suffix not in ("f16f16", "bf16bf16", "f32f16", "f32bf16"):
+        raise ValueError(f"orthogonalize takes {g.dtype} to no {y.dtype}")
+    if not (isinstance(steps, int) and 0 <= steps <= 100):
+        raise ValueError("steps must be a whole number in [0, 100]")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and non-negative")
+    pg, ldg = _matrix(exec, g, "g")
+    rows, cols = g.shape
+    py, ldy = _matrix(exec, y, "y", rows, cols)
+    check(getattr(lib(), "xspmm_orthogonalize_" + suffix)(
+        exec.handle, rows, cols, pg, ldg, steps, eps, py, ldy))
