@@ -113,7 +113,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// ---- host: 2-D tensor maps of 16-bit elements -------------------------------------------------------
+// ---- host: 2-D tensor maps, of 16-bit elements unless another type is given -------------------------------------------------------
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -130,7 +130,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 inline CUtensorMap make_map_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
-                        uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw) {
+                        uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
+                        CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16) {
     CUtensorMap m;
     std::memset(&m, 0, sizeof(m));
     const cuuint64_t dims[2] = {inner, outer};
@@ -138,7 +139,7 @@ inline CUtensorMap make_map_2d(const void* base, uint64_t inner, uint64_t outer,
     const cuuint32_t box[2] = {box_inner, box_outer};
     const cuuint32_t estr[2] = {1, 1};
     auto encode = [&] {
-        return encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+        return encode_fn()(&m, type, 2, const_cast<void*>(base), dims, strides, box,
                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
