@@ -385,3 +385,38 @@ def test_streams_graphs_and_repeats(executor):
         assert torch.equal(a, o)
     for a, o, p in zip(again, replayed, spare):
         assert torch.equal(a, o) and torch.equal(a, p)
+
+
+def mixed(cols, size):
+    """Offsets of 3000 samples: mostly a few rows, some empty, one of more than a warp takes, one of more than a CTA."""
+    lengths = [(7 * i) % 11 for i in range(3000)]
+    lengths[100], lengths[1234], lengths[2990] = 70_000 // (cols * size) + 50, 400_000 // (cols * size) + 300, 40
+    ends = torch.tensor([3] + lengths).cumsum(0).tolist()
+    return ends, ends[-1] + 5
+
+
+@pytest.mark.parametrize("tx,ty", TYPES)
+@pytest.mark.parametrize("cols,groups", [(64, 8), (33, 11), (30, 1), (264, 2), (520, 1)])
+def test_many_samples(executor, cols, groups, tx, ty):
+    """Short samples by a warp each, middle ones by a CTA, long ones by all, side by side."""
+    offsets, rows = mixed(cols, 2)
+    x, dy = rand(21, rows, cols, dtype=tx, shift=0.5), rand(22, rows, cols, dtype=ty)
+    w, b = rand(23, cols, scale=0.2, shift=1.0), rand(24, cols, scale=0.1)
+    y, ybuf = guarded(rows, cols, ty)
+    check_forward(executor, x, groups, w, b, 1e-5, y, offsets, "silu", ybuf)
+    dx, dbuf = guarded(rows, cols, ty)
+    check_backward(executor, dy, x, groups, w, b, offsets, "silu", dx, dbuf)
+
+
+@pytest.mark.parametrize("tx,ty", TYPES)
+@pytest.mark.parametrize("rows,cols,groups,offsets", [
+    (30000, 128, 32, None), (30000, 33, 3, [0, 9000, 9000, 9001, 21000, 29999]), (9000, 640, 1, [5, 4000, 8990]),
+    (40000, 8, 2, [1, 20000, 20001, 40000])])
+def test_long_samples(executor, rows, cols, groups, offsets, tx, ty):
+    """Samples cut into chunks, which begin and end inside them."""
+    x, dy = rand(31, rows, cols, dtype=tx, shift=0.5), rand(32, rows, cols, dtype=ty)
+    w, b = rand(33, cols, scale=0.2, shift=1.0), rand(34, cols, scale=0.1)
+    y, ybuf = guarded(rows, cols, ty)
+    check_forward(executor, x, groups, w, b, 1e-5, y, offsets, "gelu", ybuf)
+    dx, dbuf = guarded(rows, cols, ty)
+    check_backward(executor, dy, x, groups, w, b, offsets, "gelu", dx, dbuf)

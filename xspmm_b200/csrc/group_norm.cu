@@ -1,171 +1,400 @@
-// group_norm.cu -- group norm with an activation over the samples of a packed batch, forward and backward.
+// group_norm.cu -- group norm with an activation over the samples of a packed batch.
 //
-// Forward: over the n values of a sample's rows and a group's channels, mean = sum(x) / n,
-// var = sum((x - mean)^2) / n, rstd = 1 / sqrt(var + eps); z = ((x - mean) * rstd) * w + b, y = act(z).
-// Backward: dz = dy * act'(z), t = dz * w, dx = rstd * (t - mean(t) - xh * mean(t * xh)), dw = sum of dz * xh,
-// db = sum of dz over all samples' rows.
+// Over the n values of a sample's rows and a group's channels, mean = sum(x) / n, var = sum((x - mean)^2) / n,
+// rstd = 1 / sqrt(var + eps); z = ((x - mean) * rstd) * w + b, y = act(z).
 //
-// One CTA per sample and group, which reads the group's values three times.
-#include "gated_tc.cuh"
+// The pass is bound by memory: x has to be read and y written once, and where a sample does not fit on chip x is read
+// a second time, from L2 as far as it is still there. The host does not know the samples' lengths, so each launch
+// decides on the device who takes what:
+//   * short samples (a few tens of KB of a column tile) by a warp each, eight to a CTA; where there are too few to
+//     fill the GPU with warps, by a CTA each;
+//   * samples of up to Chunks::longest rows by a CTA, which reads them twice;
+//   * longer ones in chunks of rows by all CTAs: moments of each chunk, a second kernel that joins them, a third that
+//     applies them, from the last chunk to the first, since the last ones read are still in L2. These two are not
+//     launched where no sample can be long.
+// Moments are joined from those of batches of rows that a thread holds in registers, each taken about its own mean, so
+// neither a large mean nor rows far from the others cost accuracy; all orders are fixed by the sizes and offsets.
+#include "group_norm.cuh"
 
 namespace xspmm_b200 {
 namespace {
 
-constexpr int GN_THREADS = 256;
+using namespace group;
 
-// A CTA's sum, the same in all its threads.
-__device__ __forceinline__ float cta_sum(float v) {
-    __shared__ float part[GN_THREADS / 32];
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int i = 0; i < GN_THREADS / 32; ++i) v += part[i];
-    return v;
-}
-
-// Sample s's rows, within the matrix whatever the offsets hold.
-struct Span {
-    int64_t begin, end;
+template <typename TX, typename TY>
+struct Forward {
+    GroupNormArgs<TX> a;
+    Tiling t;
+    Chunks ch;
+    int each;         // samples that a CTA of short samples takes: WARPS or 1
+    int64_t warp_rows;  // most rows that a warp takes
+    float eps;
+    TY* y;
+    int64_t ldy;
+    float *mean, *rstd;  // or null
+    float2* part;        // [slot][chunk][group or tile of it]: mean and sum of squares about it
+    float2* fin;         // [chunk][group]: mean and rstd of the long sample that begins in the chunk
+    int2* found;         // [chunk]: the long samples with rows in it
 };
-__device__ __forceinline__ Span span_of(const int64_t* offsets, int64_t s, int64_t rows) {
-    if (!offsets) return {0, rows};
-    const int64_t b = max((int64_t)0, min(rows, offsets[s]));
-    return {b, max(b, min(rows, offsets[s + 1]))};
-}
 
-// z, each operation rounded by itself: the sign of z, which decides relu's slope, is then the same however the
-// compiler orders the code around it.
-__device__ __forceinline__ float affine(float xh, float w, float b) { return __fadd_rn(__fmul_rn(xh, w), b); }
-__device__ __forceinline__ float centred(float x, float mean, float rstd) {
-    return __fmul_rn(__fsub_rn(x, mean), rstd);
-}
+template <int E>
+struct Moments {
+    float n = 0.0f, mean[E] = {}, m2[E] = {};
+};
 
-// act(z) and its slope. 16-bit outputs take the block's approximate forms (errors far below their rounding),
-// fp32 ones CUDA's accurate functions.
-template <typename TY>
-__device__ __forceinline__ float act_of(Activation act, float z) {
-    constexpr bool FINE = sizeof(TY) == 4;
-    if constexpr (FINE) {
-        switch (act) {
-            case Activation::Silu: return z > -gated::SILU_END ? z / (1.0f + expf(-z)) : (z != z ? z : 0.0f);
-            case Activation::Gelu: return z > -gated::GELU_END ? z * normcdff(z) : (z != z ? z : 0.0f);
-            case Activation::Sigmoid: return 1.0f / (1.0f + expf(-z));
-            case Activation::Relu: return z > 0.0f ? z : (z != z ? z : 0.0f);
-            default: return z;
-        }
-    } else {
-        float v = z;
-        if (act != Activation::None)
-            gated::with_activation(act, [&](auto a) { v = gated::act_value<decltype(a)::value>(z); });
-        return v;
+// Adds the first `count` rows of a batch.
+template <int B, typename TX, int V, int U>
+__device__ __forceinline__ void add_rows(Moments<V * U>& m, const Pack<TX, V> (&raw)[B][U], int count) {
+    constexpr int E = V * U;
+    float s[E], q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = q[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {  // rows past the last are zeros
+        float v[E];
+        Place<V, U>::values(raw[i], v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] += v[e];
     }
-}
-template <typename TY>
-__device__ __forceinline__ float slope_of(Activation act, float z) {
-    constexpr bool FINE = sizeof(TY) == 4;
-    if (act == Activation::None) return 1.0f;
-    if constexpr (FINE) {
-        switch (act) {
-            case Activation::Silu: {
-                const float low = fmaxf(fminf(z, gated::SILU_END), -gated::SILU_END);
-                const float e = expf(-low), s = 1.0f / (1.0f + e);
-                return z != z ? z : s * (1.0f + low * (e * s));
-            }
-            case Activation::Gelu: {
-                const float low = fmaxf(fminf(z, gated::GELU_END), -gated::GELU_END);
-                return z != z ? z : normcdff(low) + low * 0.39894228040143268f * expf(-0.5f * low * low);
-            }
-            case Activation::Sigmoid: {
-                const float e = expf(-fabsf(z)), high = 1.0f / (1.0f + e);
-                return high * (e * high);
-            }
-            default: return z > 0.0f ? 1.0f : 0.0f;
+    const float n = (float)count, per = count == B ? 1.0f / B : 1.0f / n;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] *= per;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        if (i >= count) break;
+        float v[E];
+        Place<V, U>::values(raw[i], v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = v[e] - s[e];
+            q[e] = fmaf(d, d, q[e]);
         }
-    } else {
-        float v = 1.0f, value;
-        gated::with_activation(act, [&](auto a) { gated::act_both<decltype(a)::value>(z, &value, &v); });
-        return v;
     }
+    const float total = m.n + n, fb = n / total, f = m.n * fb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float d = s[e] - m.mean[e];
+        m.mean[e] = fmaf(d, fb, m.mean[e]);
+        m.m2[e] += fmaf(d * d, f, q[e]);
+    }
+    m.n = total;
 }
 
-template <typename TX, typename TY>
-__global__ void __launch_bounds__(GN_THREADS)
-group_norm_kernel(const GroupNormArgs<TX> a, float eps, TY* y, int64_t ldy, float* mean, float* rstd) {
-    const int64_t s = blockIdx.x / a.groups, g = blockIdx.x % a.groups, width = a.C / a.groups;
-    const Span rows = span_of(a.offsets, s, a.rows);
-    const int64_t n = (rows.end - rows.begin) * width;
-    auto each = [&](auto&& f) {
-        for (int64_t i = threadIdx.x; i < n; i += GN_THREADS) f(rows.begin + i / width, g * width + i % width);
+// Moments of the tile's groups over rows [begin, end) of x (its first channel): f(group of the tile, mean, sum of
+// squares), called by one thread a group. The strips may be written again after a team_sync.
+template <bool CTA, int B, typename TX, int V, int U, typename F>
+__device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const TX* x, int64_t ldx, int64_t begin,
+                                              int64_t end, const Tile& k, Strips& sh, F&& f) {
+    constexpr int E = V * U;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Moments<E> m;
+    for (int64_t r = begin + tm.rl; r < end; r += (int64_t)tm.step * B) {
+        Pack<TX, V> raw[B][U];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int64_t row = r + (int64_t)i * tm.step;
+            if (row < end) tm.at.load(raw[i], x + row * ldx);
+            else
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[i][u] = Pack<TX, V>{};
+        }
+        add_rows(m, raw, (int)min((int64_t)B, (end - r + tm.step - 1) / tm.step));
+    }
+    auto weights = [](float na, float nb, float* fb, float* f) {
+        const float n = na + nb;
+        *fb = n > 0.0f ? nb / n : 0.0f;
+        *f = na * *fb;
+        return n;
     };
-    float v = 0.0f;
-    each([&](int64_t r, int64_t c) { v += to_float(a.x[r * a.ldx + c]); });
-    const float m = n ? cta_sum(v) / (float)n : 0.0f;
-    v = 0.0f;
-    each([&](int64_t r, int64_t c) {
-        const float d = to_float(a.x[r * a.ldx + c]) - m;
-        v = fmaf(d, d, v);
+    for (int o = 16; o >= tm.at.lpr; o >>= 1) {
+        // both of a pair take the lower lane's moments first, so that they end with the same numbers
+        const bool low = (lane & o) == 0;
+        const float other = __shfl_xor_sync(0xffffffffu, m.n, o);
+        float fb, g;
+        const float n = weights(low ? m.n : other, low ? other : m.n, &fb, &g);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float mo = __shfl_xor_sync(0xffffffffu, m.mean[e], o), so = __shfl_xor_sync(0xffffffffu, m.m2[e], o);
+            float ma = low ? m.mean[e] : mo, sa = low ? m.m2[e] : so;
+            join_moments(ma, sa, low ? mo : m.mean[e], low ? so : m.m2[e], fb, g);
+            m.mean[e] = ma;
+            m.m2[e] = sa;
+        }
+        m.n = n;
+    }
+    team_sync<CTA>();
+    if (lane < tm.at.lpr)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (tm.at.in(u))
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    sh.v[warp][0][tm.at.col(u) + e] = m.mean[u * V + e];
+                    sh.v[warp][1][tm.at.col(u) + e] = m.m2[u * V + e];
+                }
+    if (lane == 0) sh.n[warp] = m.n;
+    team_sync<CTA>();
+    if constexpr (CTA) {
+        const int c = threadIdx.x;
+        if (c < k.cols) {
+            float n = sh.n[0], ma = sh.v[0][0][c], sa = sh.v[0][1][c];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) {
+                float fb, g;
+                n = weights(n, sh.n[w], &fb, &g);
+                join_moments(ma, sa, sh.v[w][0][c], sh.v[w][1][c], fb, g);
+            }
+            sh.v[0][0][c] = ma;
+            sh.v[0][1][c] = sa;
+        }
+        __syncthreads();
+    }
+    // every channel has the same number of values
+    const float* cm = sh.v[CTA ? 0 : warp][0];
+    const float* cs = sh.v[CTA ? 0 : warp][1];
+    const float n = (float)(end - begin);
+    each_group<CTA>(k.ng, [&](int g, int j, int l, bool live) {
+        float s = 0.0f;
+        if (live)
+            for (int c = j; c < k.lw; c += l) s += cm[g * k.lw + c];
+        const float mean = group_sum(s, l) / (float)k.lw;
+        s = 0.0f;
+        if (live)
+            for (int c = j; c < k.lw; c += l) {
+                const float d = cm[g * k.lw + c] - mean;
+                s += fmaf(n * d, d, cs[g * k.lw + c]);
+            }
+        s = group_sum(s, l);
+        if (live && j == 0) f(g, mean, s);
     });
-    const float rs = 1.0f / sqrtf((n ? cta_sum(v) / (float)n : 0.0f) + eps);
-    each([&](int64_t r, int64_t c) {
-        const float xh = centred(to_float(a.x[r * a.ldx + c]), m, rs);
-        y[r * ldy + c] = from_float<TY>(act_of<TY>(a.act, affine(xh, a.w ? a.w[c] : 1.0f, a.b ? a.b[c] : 0.0f)));
-    });
-    if (threadIdx.x == 0) {
-        if (mean) mean[blockIdx.x] = m;
-        if (rstd) rstd[blockIdx.x] = rs;
+}
+
+// y of rows [begin, end) from the groups' mean and rstd at st[group of the tile].
+template <bool CTA, int B, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void apply(const Team<CTA, V, U>& tm, const TX* x, int64_t ldx, TY* y, int64_t ldy,
+                                      int64_t begin, int64_t end, const Tile& k, const float* gm, const float* gr,
+                                      const float (&w)[V * U], const float (&b)[V * U], Activation act) {
+    constexpr int E = V * U;
+    float m[E], rs[E];
+    tm.of_groups(m, gm, k);
+    tm.of_groups(rs, gr, k);
+    for (int64_t r = begin + tm.rl; r < end; r += (int64_t)tm.step * B) {
+        Pack<TX, V> raw[B][U];
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (r + (int64_t)i * tm.step < end) tm.at.load(raw[i], x + (r + (int64_t)i * tm.step) * ldx);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int64_t row = r + (int64_t)i * tm.step;
+            if (row >= end) break;
+            float v[E];
+            Place<V, U>::values(raw[i], v);
+            with_act(act, [&](auto a) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    v[e] = act_one<sizeof(TY) == 4, decltype(a)::value>(affine(centred(v[e], m[e], rs[e]), w[e], b[e]));
+            });
+            tm.at.store(y + row * ldy, v);
+        }
     }
 }
 
-template <typename TX, typename TY>
-__global__ void __launch_bounds__(GN_THREADS)
-group_norm_grad_kernel(const GroupNormArgs<TX> a, const TY* dy, int64_t lddy, const float* mean, const float* rstd,
-                       TY* dx, int64_t lddx) {
-    const int64_t s = blockIdx.x / a.groups, g = blockIdx.x % a.groups, width = a.C / a.groups;
-    const Span rows = span_of(a.offsets, s, a.rows);
-    const int64_t n = (rows.end - rows.begin) * width;
-    const float m = mean[blockIdx.x], rs = rstd[blockIdx.x];
-    auto each = [&](auto&& f) {
-        for (int64_t i = threadIdx.x; i < n; i += GN_THREADS) {
-            const int64_t r = rows.begin + i / width, c = g * width + i % width;
-            const float xh = centred(to_float(a.x[r * a.ldx + c]), m, rs), w = a.w ? a.w[c] : 1.0f;
-            const float z = affine(xh, w, a.b ? a.b[c] : 0.0f);
-            f(r, c, xh, to_float(dy[r * lddy + c]) * slope_of<TY>(a.act, z) * w);
+// A sample by a team: all tiles of the block twice.
+template <bool CTA, int B, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void whole_sample(const Forward<TX, TY>& p, int s, Span rows, int block, Strips& sh,
+                                             float* gm, float* gr) {
+    const int t0 = block * p.t.tpg;
+    const float n = (float)(rows.end - rows.begin);
+    for (int j = 0; j < p.t.tpg; ++j) {
+        const Tile k = tile_of(p.t, t0 + j);
+        const Team<CTA, V, U> tm(p.t, k.cols);
+        group_moments<CTA, B>(tm, p.a.x + k.c0, p.a.ldx, rows.begin, rows.end, k, sh, [&](int g, float mean, float m2) {
+            if (j > 0) {  // the same thread's sums of the tiles before
+                const float na = n * (float)(j * p.t.max_cols), nb = n * (float)k.lw, fb = nb / (na + nb);
+                float ma = gm[g], sa = gr[g];
+                join_moments(ma, sa, mean, m2, fb, na * fb);
+                mean = ma;
+                m2 = sa;
+            }
+            if (j + 1 == p.t.tpg) {
+                const float count = n * (float)p.t.width;
+                m2 = 1.0f / sqrtf(m2 / count + p.eps);
+                const int64_t at = (int64_t)s * p.t.groups + k.g0 + g;
+                if (p.mean) p.mean[at] = mean;
+                if (p.rstd) p.rstd[at] = m2;
+            }
+            gm[g] = mean;
+            gr[g] = m2;
+        });
+        team_sync<CTA>();
+    }
+    for (int j = 0; j < p.t.tpg; ++j) {
+        const Tile k = tile_of(p.t, t0 + j);
+        const Team<CTA, V, U> tm(p.t, k.cols);
+        float w[V * U], b[V * U];
+        tm.at.param(w, p.a.w, k.c0, 1.0f);
+        tm.at.param(b, p.a.b, k.c0, 0.0f);
+        apply<CTA, B>(tm, p.a.x + k.c0, p.a.ldx, p.y + k.c0, p.ldy, rows.begin, rows.end, k, gm, gr, w, b, p.a.act);
+    }
+    team_sync<CTA>();
+}
+
+// CTAs [0, chunks x tiles): moments of the long samples' chunks. The others: short and middle samples.
+template <typename TX, typename TY, int V, int U, int B>
+__global__ void __launch_bounds__(THREADS) group_norm_kernel(const __grid_constant__ Forward<TX, TY> p) {
+    __shared__ Strips sh;
+    __shared__ float gm[WARPS][MAX_TILE], gr[WARPS][MAX_TILE];
+    cudaGridDependencySynchronize();
+    const int chunked = p.ch.count * p.t.tiles;
+    if ((int)blockIdx.x < chunked) {
+        const int i = blockIdx.x / p.t.tiles, tile = blockIdx.x - i * p.t.tiles;
+        const int2 found = long_samples(p.a.offsets, (int)p.a.samples, p.a.rows, p.ch, i);
+        if (tile == 0 && threadIdx.x == 0) p.found[i] = found;
+        const Tile k = tile_of(p.t, tile);
+        const Team<true, V, U> tm(p.t, k.cols);
+        const int64_t r0 = i * p.ch.rows, r1 = min(p.a.rows, r0 + p.ch.rows), slots = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
+        for (int slot = 0; slot < 2; ++slot) {
+            const int s = slot ? found.y : found.x;
+            if (s < 0) continue;
+            const Span sp = span_of(p.a.offsets, s, p.a.rows);
+            float2* out = p.part + ((int64_t)slot * p.ch.count + i) * slots + part_slot(p.t, tile, k);
+            group_moments<true, B>(tm, p.a.x + k.c0, p.a.ldx, max(r0, sp.begin), min(r1, sp.end), k, sh,
+                                   [&](int g, float mean, float m2) { out[g] = make_float2(mean, m2); });
+            __syncthreads();
+        }
+        return;
+    }
+    const int warp = threadIdx.x >> 5;
+    const int64_t at = blockIdx.x - chunked;
+    const int block = (int)(at % p.t.blocks);
+    const int64_t s0 = at / p.t.blocks * p.each;
+    auto rows_of = [&](int64_t s) { return span_of(p.a.offsets, s, p.a.rows); };
+    // a sample without rows has statistics all the same
+    auto empty = [&](int64_t s) {
+        const Tile first = tile_of(p.t, block * p.t.tpg);
+        const float rs = 1.0f / sqrtf(p.eps);
+        for (int g = threadIdx.x & 31; g < first.ng; g += 32) {
+            const int64_t o = s * p.t.groups + first.g0 + g;
+            if (p.mean) p.mean[o] = 0.0f;
+            if (p.rstd) p.rstd[o] = rs;
         }
     };
-    float s1 = 0.0f, s2 = 0.0f;
-    each([&](int64_t, int64_t, float xh, float t) { s1 += t, s2 = fmaf(t, xh, s2); });
-    if (n == 0) return;
-    s1 = cta_sum(s1) / (float)n;
-    s2 = cta_sum(s2) / (float)n;
-    each([&](int64_t r, int64_t c, float xh, float t) { dx[r * lddx + c] = from_float<TY>(rs * (t - s1 - xh * s2)); });
+    if (p.each > 1) {
+        const int64_t s = s0 + warp;
+        if (s < p.a.samples) {
+            const Span sp = rows_of(s);
+            const int64_t n = sp.end - sp.begin;
+            if (n == 0) empty(s);
+            else if (n <= p.warp_rows) whole_sample<false, B, TX, TY, V, U>(p, (int)s, sp, block, sh, gm[warp], gr[warp]);
+        }
+        __syncthreads();
+    }
+    for (int j = 0; j < p.each; ++j) {
+        const int64_t s = s0 + j;
+        if (s >= p.a.samples) break;
+        const Span sp = rows_of(s);
+        const int64_t n = sp.end - sp.begin;
+        if (n == 0 && p.each == 1 && warp == 0) empty(s);
+        if (n > 0 && n <= p.ch.longest && (p.each == 1 || n > p.warp_rows))
+            whole_sample<true, B, TX, TY, V, U>(p, (int)s, sp, block, sh, gm[0], gr[0]);
+    }
 }
 
-// A CTA per channel.
+// Mean and rstd of the long samples: a warp for each chunk and group, whose lanes take every 32nd of the parts. A sample
+// belongs to the chunk it begins in.
 template <typename TX, typename TY>
-__global__ void __launch_bounds__(GN_THREADS)
-group_norm_weight_kernel(const GroupNormArgs<TX> a, const TY* dy, int64_t lddy, const float* mean, const float* rstd,
-                         float* dw, float* db) {
-    const int64_t c = blockIdx.x, g = c / (a.C / a.groups);
-    const float w = a.w ? a.w[c] : 1.0f, b = a.b ? a.b[c] : 0.0f;
-    float sw = 0.0f, sb = 0.0f;
-    for (int64_t s = 0; s < a.samples; ++s) {
-        const Span rows = span_of(a.offsets, s, a.rows);
-        const float m = mean[s * a.groups + g], rs = rstd[s * a.groups + g];
-        for (int64_t r = rows.begin + threadIdx.x; r < rows.end; r += GN_THREADS) {
-            const float xh = centred(to_float(a.x[r * a.ldx + c]), m, rs);
-            const float dz = to_float(dy[r * lddy + c]) * slope_of<TY>(a.act, affine(xh, w, b));
-            sw = fmaf(dz, xh, sw);
-            sb += dz;
+__global__ void __launch_bounds__(THREADS) group_norm_join_kernel(const __grid_constant__ Forward<TX, TY> p) {
+    cudaGridDependencySynchronize();
+    const int i = blockIdx.x, s = p.found[i].y, g = blockIdx.y * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (s < 0 || g >= p.t.groups) return;
+    const Span sp = span_of(p.a.offsets, s, p.a.rows);
+    const int last = (int)((sp.end - 1) / p.ch.rows), tpg = p.t.tpg, parts = (last - i + 1) * tpg;
+    const int64_t slots = tpg == 1 ? p.t.groups : p.t.tiles;
+    float n = 0.0f, mean = 0.0f, m2 = 0.0f;
+    auto join = [&](float nb, float mb, float sb) {
+        const float total = n + nb, fb = total > 0.0f ? nb / total : 0.0f;
+        join_moments(mean, m2, mb, sb, fb, n * fb);
+        n = total;
+    };
+#pragma unroll 4
+    for (int q = lane; q < parts; q += 32) {
+        const int c = i + q / tpg, part = q % tpg;
+        const int64_t rows = min(sp.end, (c + 1) * p.ch.rows) - max(sp.begin, c * p.ch.rows);
+        const int lw = tpg == 1 ? p.t.width : min(p.t.max_cols, p.t.width - part * p.t.max_cols);
+        const float2 v = p.part[((int64_t)(c == i) * p.ch.count + c) * slots + g * tpg + part];
+        join((float)rows * (float)lw, v.x, v.y);
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool low = (lane & o) == 0;
+        float nb = __shfl_xor_sync(0xffffffffu, n, o), mb = __shfl_xor_sync(0xffffffffu, mean, o);
+        float sb = __shfl_xor_sync(0xffffffffu, m2, o);
+        if (!low) {
+            float x;
+            x = n, n = nb, nb = x;
+            x = mean, mean = mb, mb = x;
+            x = m2, m2 = sb, sb = x;
         }
+        join(nb, mb, sb);
     }
-    sw = cta_sum(sw);
-    sb = cta_sum(sb);
-    if (threadIdx.x == 0) {
-        if (dw) dw[c] = sw;
-        if (db) db[c] = sb;
+    if (lane == 0) {
+        const float rs = 1.0f / sqrtf(m2 / n + p.eps);
+        p.fin[(int64_t)i * p.t.groups + g] = make_float2(mean, rs);
+        if (p.mean) p.mean[(int64_t)s * p.t.groups + g] = mean;
+        if (p.rstd) p.rstd[(int64_t)s * p.t.groups + g] = rs;
     }
+}
+
+template <typename TX, typename TY, int V, int U, int B>
+__global__ void __launch_bounds__(THREADS) group_norm_apply_kernel(const __grid_constant__ Forward<TX, TY> p) {
+    __shared__ float gm[MAX_TILE], gr[MAX_TILE];
+    cudaGridDependencySynchronize();
+    const int i = p.ch.count - 1 - blockIdx.x / p.t.tiles, tile = blockIdx.x % p.t.tiles;
+    const int2 found = p.found[i];
+    if (found.x < 0 && found.y < 0) return;
+    const Tile k = tile_of(p.t, tile);
+    const Team<true, V, U> tm(p.t, k.cols);
+    const int64_t r0 = i * p.ch.rows, r1 = min(p.a.rows, r0 + p.ch.rows);
+    float w[V * U], b[V * U];
+    tm.at.param(w, p.a.w, k.c0, 1.0f);
+    tm.at.param(b, p.a.b, k.c0, 0.0f);
+    for (int slot = 0; slot < 2; ++slot) {
+        const int s = slot ? found.y : found.x;
+        if (s < 0) continue;
+        const Span sp = span_of(p.a.offsets, s, p.a.rows);
+        __syncthreads();
+        if ((int)threadIdx.x < k.ng) {
+            const float2 v = p.fin[sp.begin / p.ch.rows * p.t.groups + k.g0 + threadIdx.x];
+            gm[threadIdx.x] = v.x;
+            gr[threadIdx.x] = v.y;
+        }
+        __syncthreads();
+        apply<true, B>(tm, p.a.x + k.c0, p.a.ldx, p.y + k.c0, p.ldy, max(r0, sp.begin), min(r1, sp.end), k, gm, gr, w, b, p.a.act);
+    }
+}
+
+template <typename TX, typename TY, int V, int U, int B>
+void forward(Handle& h, Forward<TX, TY>& p) {
+    const int sms = sm_count(h.device);
+    const Cut cut = make_cut(p.a, p.t, (int)sizeof(TX), sms);
+    p.ch = cut.ch;
+    p.each = cut.each;
+    p.warp_rows = cut.warp_rows;
+    DevBuf<float2> ws((size_t)p.ch.count * (2 * part_slots(p.t) + p.t.groups), h.stream);
+    DevBuf<int2> found((size_t)p.ch.count, h.stream);
+    p.part = ws.get();
+    p.fin = ws.get() + (int64_t)p.ch.count * 2 * part_slots(p.t);
+    p.found = found.get();
+    const int64_t chunked = (int64_t)p.ch.count * p.t.tiles;
+    const int64_t grid = chunked + (cut.only_long ? 0 : ceil_div(p.a.samples, p.each) * p.t.blocks);
+    XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "too many samples and groups");
+    launch_dependent(h.stream, group_norm_kernel<TX, TY, V, U, B>, (unsigned)grid, THREADS, 0, 1, p);
+    after_launch(h, "group_norm");
+    if (p.ch.count == 0) return;
+    launch_dependent(h.stream, group_norm_join_kernel<TX, TY>, dim3((unsigned)p.ch.count, (unsigned)ceil_div(p.t.groups, WARPS)),
+                     THREADS, 0, 1, p);
+    after_launch(h, "group_norm_join");
+    launch_dependent(h.stream, group_norm_apply_kernel<TX, TY, V, U, B>, (unsigned)chunked, THREADS, 0, 1, p);
+    after_launch(h, "group_norm_apply");
 }
 
 }  // namespace
@@ -173,30 +402,28 @@ group_norm_weight_kernel(const GroupNormArgs<TX> a, const TY* dy, int64_t lddy, 
 template <typename TX, typename TY>
 void group_norm(Handle& h, const GroupNormArgs<TX>& a, float eps, TY* y, int64_t ldy, float* mean, float* rstd) {
     if (a.samples == 0) return;
-    XS_REQUIRE(a.samples * a.groups < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "too many samples and groups");
-    group_norm_kernel<TX, TY><<<(unsigned)(a.samples * a.groups), GN_THREADS, 0, h.stream>>>(a, eps, y, ldy, mean, rstd);
-    after_launch(h, "group_norm");
+    Forward<TX, TY> p = {};
+    p.a = a;
+    p.eps = eps;
+    p.y = y;
+    p.ldy = ldy;
+    p.mean = mean;
+    p.rstd = rstd;
+    constexpr int V = 16 / sizeof(TX);
+    const bool wide = a.C % V == 0 && (a.rows <= 1 || (a.ldx % V == 0 && ldy % V == 0)) && aligned_to(a.x, 16) &&
+                      aligned_to(y, std::min<size_t>(16, V * sizeof(TY)));
+    if (wide && make_tiling(p.t, a.C, a.groups, V, 1, 32 * V)) return forward<TX, TY, V, 1, 8>(h, p);
+    if (a.C <= 32) {
+        make_tiling(p.t, a.C, a.groups, 1, 1, 32);
+        forward<TX, TY, 1, 1, 8>(h, p);
+    } else {
+        make_tiling(p.t, a.C, a.groups, 1, 8, MAX_TILE);
+        forward<TX, TY, 1, 8, 2>(h, p);
+    }
 }
 
-template <typename TX, typename TY>
-void group_norm_backward(Handle& h, const GroupNormArgs<TX>& a, const TY* dy, int64_t lddy, const float* mean,
-                         const float* rstd, TY* dx, int64_t lddx, float* dw, float* db) {
-    XS_REQUIRE(a.samples * a.groups < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "too many samples and groups");
-    if (dw || db) {
-        group_norm_weight_kernel<TX, TY><<<(unsigned)a.C, GN_THREADS, 0, h.stream>>>(a, dy, lddy, mean, rstd, dw, db);
-        after_launch(h, "group_norm_weight");
-    }
-    if (dx && a.samples > 0) {
-        group_norm_grad_kernel<TX, TY>
-            <<<(unsigned)(a.samples * a.groups), GN_THREADS, 0, h.stream>>>(a, dy, lddy, mean, rstd, dx, lddx);
-        after_launch(h, "group_norm_grad");
-    }
-}
-
-#define XS_INST_GROUP_NORM(TX, TY)                                                                              \
-    template void group_norm<TX, TY>(Handle&, const GroupNormArgs<TX>&, float, TY*, int64_t, float*, float*);    \
-    template void group_norm_backward<TX, TY>(Handle&, const GroupNormArgs<TX>&, const TY*, int64_t,             \
-                                              const float*, const float*, TY*, int64_t, float*, float*);
+#define XS_INST_GROUP_NORM(TX, TY) \
+    template void group_norm<TX, TY>(Handle&, const GroupNormArgs<TX>&, float, TY*, int64_t, float*, float*);
 XS_INST_GROUP_NORM(__half, __half)
 XS_INST_GROUP_NORM(__nv_bfloat16, __nv_bfloat16)
 XS_INST_GROUP_NORM(float, float)
