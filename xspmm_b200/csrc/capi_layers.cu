@@ -43,12 +43,13 @@ GroupNormArgs<TX> group_norm_args(int64_t rows, int64_t C, int64_t groups, int64
                                   const void* x, int64_t ldx, const float* w, const float* b, int act) {
     need(rows >= 0 && C >= 1, "rows must be non-negative and cols positive");
     need(groups >= 1 && C % groups == 0, "groups must divide cols");
-    need(samples >= 0 && samples < INT32_MAX, "samples out of range");
+    need(samples >= 0, "negative dimension");
     need(offsets != nullptr || samples == 1, "null offsets: samples must be 1");
     need(aligned_to(offsets, sizeof(int64_t)), "offsets not aligned to its type");
     need(act >= XSPMM_ACT_NONE && act <= XSPMM_ACT_SIGMOID, "unknown activation");
     XS_REQUIRE(C / groups <= GROUP_NORM_MAX_WIDTH, XSPMM_STATUS_UNSUPPORTED, "more than 16384 channels a group");
-    XS_REQUIRE(rows < INT32_MAX && C < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "a dimension passes 2^31");
+    constexpr int64_t most = INT32_MAX - (1 << 24);  // sums of an index and a chunk of rows stay within 32 bits
+    XS_REQUIRE(rows < most && C < most && samples < most, XSPMM_STATUS_UNSUPPORTED, "a dimension passes 2^31");
     return GroupNormArgs<TX>{rows, C, groups, samples, offsets, matrix<TX>(x, rows, C, ldx, "x"), ldx,
                              vec(w, "weight"), vec(b, "bias"), static_cast<Activation>(act)};
 }

@@ -7,8 +7,17 @@
 namespace xspmm_b200 {
 namespace group {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int MAX_TILE = 256;  // channels of a column tile
+constexpr int WARPS_LOG = 2, WARPS = 1 << WARPS_LOG, THREADS = 32 * WARPS;
+constexpr int PER = 4;         // channels a thread holds of a row
+constexpr int MAX_TILE = 32 * PER;  // channels of a column tile
+
+// Two fp32 operations in one instruction. The compiler's own, not layers.cuh's inline assembly: it then keeps pairs in
+// aligned registers through a whole loop (2^20 x 128 fp32 to fp16 with silu, second pass: 27 instructions a value with
+// the assembly).
+__device__ __forceinline__ float2 pair_add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 pair_mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 pair_fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // Channels are cut into column tiles: whole groups side by side (gpt of them), or, where a group is wider than a
 // tile, tpg tiles to a group. A block is a tile, or all tiles of a wide group: what shares statistics.
@@ -16,12 +25,15 @@ struct Tiling {
     int groups, width;  // width: channels of a group
     int gpt, tpg, tiles, blocks;
     int max_cols;       // channels of the widest tile
-    int lpr;            // threads side by side in a row, a power of two up to 32
+    int lpr, lpr_log;   // threads side by side in a row, a power of two up to 32
+    uint32_t inv;       // 2^16 / width rounded up (groups within a tile)
 };
 struct Tile {
     int c0, cols;  // channels [c0, c0 + cols)
     int g0, ng;    // groups [g0, g0 + ng)
     int lw;        // channels of each of them in the tile
+    uint32_t inv;  // 2^16 / lw rounded up: exact for the channels of a tile
+    __device__ int group(int c) const { return (int)(c * inv >> 16); }
 };
 __device__ __forceinline__ Tile tile_of(const Tiling& t, int i) {
     Tile k;
@@ -38,6 +50,7 @@ __device__ __forceinline__ Tile tile_of(const Tiling& t, int i) {
         k.c0 = k.g0 * t.width + off;
         k.lw = k.cols = min(t.max_cols, t.width - off);
     }
+    k.inv = t.tpg == 1 ? t.inv : 0;
     return k;
 }
 // Slot of a tile's first group among the partial sums of a chunk of rows: one a group, or one a tile of it.
@@ -48,19 +61,19 @@ inline int part_slots(const Tiling& t) { return t.tpg == 1 ? t.groups : t.tiles;
 // itself; a chunk is no longer, so at most two long samples have rows in one: one that began before it (slot 0)
 // and one that begins in it (slot 1).
 struct Chunks {
-    int64_t rows;     // of a chunk
-    int64_t longest;
-    int count;        // 0: no sample can be long
+    int rows;     // of a chunk
+    int longest;
+    int count;    // 0: no sample can be long
 };
 
 struct Span {
-    int64_t begin, end;
+    int begin, end;
 };
 // Sample s's rows, within the matrix whatever the offsets hold.
-__device__ __forceinline__ Span span_of(const int64_t* offsets, int64_t s, int64_t rows) {
+__device__ __forceinline__ Span span_of(const int64_t* offsets, int s, int rows) {
     if (!offsets) return {0, rows};
-    const int64_t b = max((int64_t)0, min(rows, offsets[s]));
-    return {b, max(b, min(rows, offsets[s + 1]))};
+    const int b = (int)max((int64_t)0, min((int64_t)rows, offsets[s]));
+    return {b, max(b, (int)max((int64_t)0, min((int64_t)rows, offsets[s + 1])))};
 }
 // The last sample that begins at or before row r, -1 if none does. A warp's threads call it together and probe 32
 // offsets at a time.
@@ -78,10 +91,23 @@ __device__ __forceinline__ int last_begun(const int64_t* offsets, int samples, i
     }
     return lo - 1;
 }
+// A long sample's chunks: it belongs to the one it begins in, where its part is in slot 1; in the others it is in slot 0.
+struct Parts {
+    int first, count;       // chunks first ... first + count - 1
+    int64_t slots, chunks;  // parts[slot][part of the tile's groups][chunk]
+    __device__ Parts(const Span& sp, const Chunks& ch, int64_t slots_) : slots(slots_), chunks(ch.count) {
+        first = sp.begin / ch.rows;
+        count = (sp.end - 1) / ch.rows - first + 1;
+    }
+    __device__ float2 get(const float2* part, int64_t slot, int i) const {
+        return part[((int64_t)(i == 0) * slots + slot) * chunks + first + i];
+    }
+};
+
 // The long samples with rows in chunk i, -1 where there is none; the same in all threads.
-__device__ __forceinline__ int2 long_samples(const int64_t* offsets, int samples, int64_t rows, const Chunks& ch, int i) {
+__device__ __forceinline__ int2 long_samples(const int64_t* offsets, int samples, int rows, const Chunks& ch, int i) {
     __shared__ int found[2];
-    const int64_t r0 = i * ch.rows, r1 = min(rows, r0 + ch.rows);
+    const int r0 = i * ch.rows, r1 = r0 + min(ch.rows, rows - r0);
     const int warp = threadIdx.x >> 5;
     if (warp < 2) {
         int s = last_begun(offsets, samples, warp == 0 ? r0 : r1 - 1);
@@ -95,7 +121,8 @@ __device__ __forceinline__ int2 long_samples(const int64_t* offsets, int samples
     return make_int2(found[0], found[1]);
 }
 
-// A thread's channels of a tile: V consecutive ones at each of U places, lpr * V apart.
+// A thread's channels of a tile: V consecutive ones at each of U places, lpr * V apart. Pointers to rows are at the
+// thread's first channel.
 template <int V, int U>
 struct Place {
     int lane, lpr, cols;
@@ -106,35 +133,46 @@ struct Place {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             raw[u] = Pack<T, V>{};
-            if (in(u)) raw[u] = *reinterpret_cast<const Pack<T, V>*>(row + col(u));
+            if (U == 1 || in(u)) raw[u] = *reinterpret_cast<const Pack<T, V>*>(row + u * lpr * V);
         }
     }
     template <typename T>
-    static __device__ void values(const Pack<T, V> (&raw)[U], float (&v)[V * U]) {
+    static __device__ void values(const Pack<T, V> (&raw)[U], float2 (&v)[V * U / 2]) {
+        if constexpr (V == 1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float f[V];
-            unpack<T, V>(raw[u], f);
+            for (int u = 0; u < U; u += 2) v[u / 2] = make_float2(to_float(raw[u].v[0]), to_float(raw[u + 1].v[0]));
+        } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[u * V + e] = f[e];
+            for (int u = 0; u < U; ++u) {
+                float f[V];
+                unpack<T, V>(raw[u], f);
+#pragma unroll
+                for (int e = 0; e < V; e += 2) v[(u * V + e) / 2] = make_float2(f[e], f[e + 1]);
+            }
         }
     }
     template <typename T>
-    __device__ void store(T* row, const float (&v)[V * U]) const {
+    __device__ void store(T* row, const float2 (&v)[V * U / 2]) const {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[e] = v[u * V + e];
-            if (in(u)) store_pack<T, V>(row + col(u), f);
+            for (int e = 0; e < V; ++e) f[e] = (u * V + e) % 2 ? v[(u * V + e) / 2].y : v[(u * V + e) / 2].x;
+            if (U == 1 || in(u)) store_pack<T, V>(row + u * lpr * V, f);
+        }
+    }
+    // f(channel of the tile, whether it is one of its) for each of the thread's channels, as pairs.
+    template <typename F>
+    __device__ void each(float2 (&v)[V * U / 2], F&& f) const {
+#pragma unroll
+        for (int i = 0; i < V * U; i += 2) {
+            v[i / 2].x = f(col(i / V) + i % V, in(i / V));
+            v[i / 2].y = f(col((i + 1) / V) + (i + 1) % V, in((i + 1) / V));
         }
     }
     // A parameter vector's values at the tile's channels, `none` where it is absent.
-    __device__ void param(float (&v)[V * U], const float* p, int c0, float none) const {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[u * V + e] = p && in(u) ? __ldg(p + c0 + col(u) + e) : none;
+    __device__ void param(float2 (&v)[V * U / 2], const float* p, int c0, float none) const {
+        each(v, [&](int c, bool mine) { return p && mine ? __ldg(p + c0 + c) : none; });
     }
 };
 
@@ -149,23 +187,57 @@ __device__ __forceinline__ void team_sync() {
 template <bool CTA, int V, int U>
 struct Team {
     Place<V, U> at;
-    int rl, step;
+    int rl, step, step_log;
     __device__ Team(const Tiling& t, int cols) {
         const int id = CTA ? threadIdx.x : threadIdx.x & 31;
         at.lpr = t.lpr;
         at.cols = cols;
         at.lane = id & (t.lpr - 1);
-        rl = id / t.lpr;
-        step = (CTA ? THREADS : 32) / t.lpr;
+        rl = id >> t.lpr_log;
+        step_log = (CTA ? 5 + WARPS_LOG : 5) - t.lpr_log;
+        step = 1 << step_log;
+    }
+    // This thread's number of rows among n; none where it has no channels.
+    __device__ int rows(int n) const { return at.in(0) && rl < n ? (n - rl + step - 1) >> step_log : 0; }
+    // Where its first row and channel are, in a matrix whose row `begin` of the tile is at `p`.
+    template <typename T>
+    __device__ T* first(T* p, int64_t begin, int64_t ld) const {
+        return p + (begin + rl) * ld + at.lane * V;
     }
     // The values of the tile's groups at this thread's channels.
-    __device__ void of_groups(float (&v)[V * U], const float* g, const Tile& k) const {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[u * V + e] = g[at.in(u) ? (at.col(u) + e) / k.lw : 0];
+    __device__ void of_groups(float2 (&v)[V * U / 2], const float* g, const Tile& k) const {
+        at.each(v, [&](int c, bool mine) { return g[mine ? k.group(c) : 0]; });
     }
 };
+
+// A thread's rows in batches of B, the next batch's loads before the work on this one: load(full, batch, i, n) fetches rows
+// i, i + 1, ... of the n > i there are, use(full, batch, i, n) works on them. full (a constant) says that there are B: the
+// rows of a whole batch are one run of instructions without branches between them.
+template <int B, typename Batch, typename L, typename F>
+__device__ __forceinline__ void batches(int n, L&& load, F&& use) {
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    Batch a, b;
+    auto fetch = [&](Batch& t, int i) {
+        if (i + B <= n) load(yes, t, i, n);
+        else if (i < n) load(no, t, i, n);
+    };
+    fetch(a, 0);
+    int i = 0;
+    for (; i + 2 * B <= n; i += 2 * B) {
+        fetch(b, i + B);
+        use(yes, a, i, n);
+        fetch(a, i + 2 * B);
+        use(yes, b, i + B, n);
+    }
+    if (i + B <= n) {
+        fetch(b, i + B);
+        use(yes, a, i, n);
+        i += B;
+        a = b;
+    }
+    if (i < n) use(no, a, i, n);
+}
 
 // Shared memory of a team's sums over rows: two values a channel, for each warp.
 struct Strips {
@@ -181,28 +253,36 @@ __device__ __forceinline__ void join_moments(float& ma, float& sa, float mb, flo
     sa += fmaf(d * d, f, sb);
 }
 
+// A thread's two values a channel to a warp's strips.
+template <int V, int U>
+__device__ __forceinline__ void put_channels(const float2 (&a)[V * U / 2], const float2 (&b)[V * U / 2], const Place<V, U>& at,
+                                             float (&strips)[2][MAX_TILE]) {
+#pragma unroll
+    for (int i = 0; i < V * U; ++i)
+        if (at.in(i / V)) {
+            const int c = at.col(i / V) + i % V;
+            strips[0][c] = i % 2 ? a[i / 2].y : a[i / 2].x;
+            strips[1][c] = i % 2 ? b[i / 2].y : b[i / 2].x;
+        }
+}
+
 // The sums over a team's threads of two values a channel, at `out` (strips of this warp, or of the CTA's first) by
 // channel of the tile. Every thread of the team has the result on return and may not write the strips before its next
 // team_sync.
 template <bool CTA, int V, int U>
-__device__ __forceinline__ void sum_channels(float (&a)[V * U], float (&b)[V * U], const Place<V, U>& at, Strips& sh) {
+__device__ __forceinline__ void sum_channels(float2 (&a)[V * U / 2], float2 (&b)[V * U / 2], const Place<V, U>& at, Strips& sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto from = [](float2 v, int o) {
+        return make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o));
+    };
     for (int o = 16; o >= at.lpr; o >>= 1)
 #pragma unroll
-        for (int e = 0; e < V * U; ++e) {
-            a[e] += __shfl_xor_sync(0xffffffffu, a[e], o);
-            b[e] += __shfl_xor_sync(0xffffffffu, b[e], o);
+        for (int i = 0; i < V * U / 2; ++i) {
+            a[i] = pair_add(a[i], from(a[i], o));
+            b[i] = pair_add(b[i], from(b[i], o));
         }
     team_sync<CTA>();
-    if (lane < at.lpr)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (at.in(u))
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    sh.v[warp][0][at.col(u) + e] = a[u * V + e];
-                    sh.v[warp][1][at.col(u) + e] = b[u * V + e];
-                }
+    if (lane < at.lpr) put_channels(a, b, at, sh.v[warp]);
     team_sync<CTA>();
     if constexpr (CTA) {
         if ((int)threadIdx.x < at.cols) {
@@ -216,21 +296,16 @@ __device__ __forceinline__ void sum_channels(float (&a)[V * U], float (&b)[V * U
     }
 }
 
-// Threads of a team that sum one of ng groups: a power of two up to 32.
-template <bool CTA>
-__device__ __forceinline__ int threads_a_group(int ng) {
-    int l = 32;
-    while (l > 1 && l * ng > (CTA ? THREADS : 32)) l >>= 1;
-    return l;
-}
 // f(group of the tile, thread of the group, threads a group) for every group, all the group's threads together in a
-// warp; groups past the last are called with live = false.
+// warp: a power of two up to 32. Groups past the last are called with live = false.
 template <bool CTA, typename F>
 __device__ __forceinline__ void each_group(int ng, F&& f) {
-    const int l = threads_a_group<CTA>(ng), t = CTA ? threadIdx.x : threadIdx.x & 31, step = (CTA ? THREADS : 32) / l;
-    for (int base = 0; base < ng; base += step) {
-        const int i = base + t / l;
-        f(i, t % l, l, i < ng);
+    constexpr int TEAM_LOG = CTA ? 5 + WARPS_LOG : 5;
+    const int log = max(0, min(5, TEAM_LOG - (ng > 1 ? 32 - __clz(ng - 1) : 0))), l = 1 << log;
+    const int t = CTA ? threadIdx.x : threadIdx.x & 31;
+    for (int base = 0; base < ng; base += 1 << (TEAM_LOG - log)) {
+        const int i = base + (t >> log);
+        f(i, t & (l - 1), l, i < ng);
     }
 }
 __device__ __forceinline__ float group_sum(float v, int l) {
@@ -240,8 +315,8 @@ __device__ __forceinline__ float group_sum(float v, int l) {
 
 // z, each operation rounded by itself: the sign of z, which decides relu's slope, is then the same in the forward
 // and the backward pass and however the compiler orders the code around it.
-__device__ __forceinline__ float centred(float x, float mean, float rstd) { return __fmul_rn(__fsub_rn(x, mean), rstd); }
-__device__ __forceinline__ float affine(float xh, float w, float b) { return __fadd_rn(__fmul_rn(xh, w), b); }
+__device__ __forceinline__ float2 centred(float2 x, float2 neg_mean, float2 rstd) { return pair_mul(pair_add(x, neg_mean), rstd); }
+__device__ __forceinline__ float2 affine(float2 xh, float2 w, float2 b) { return pair_add(pair_mul(xh, w), b); }
 
 // act(z) of a row's values and its slope. 16-bit outputs take the gated block's approximate forms (errors far below
 // their rounding), fp32 ones CUDA's accurate functions.
@@ -276,6 +351,74 @@ __device__ __forceinline__ float slope_one(float z) {
         return high * (e * high);
     }
 }
+// A row's four values one at a time: where a pair's shared reciprocal does not hold.
+template <bool SLOPE, Activation ACT>
+__device__ __noinline__ float4 singly(float4 z) {
+    auto one = [](float v) { return SLOPE ? slope_one<false, ACT>(v) : act_one<false, ACT>(v); };
+    return make_float4(one(z.x), one(z.y), one(z.z), one(z.w));
+}
+// act of a row's values, or its slope, in place of them. 16-bit silu and sigmoid take one reciprocal for two values
+// where its product holds (gated_tc.cuh), 16-bit gelu its packed form.
+template <bool SLOPE, bool FINE, Activation ACT>
+__device__ __forceinline__ void act_row(float2 (&z)[PER / 2]) {
+    constexpr int P = PER / 2;
+    if constexpr (ACT == Activation::None) {
+        if (SLOPE)
+#pragma unroll
+            for (int i = 0; i < P; ++i) z[i] = both(1.0f);
+    } else if constexpr (!FINE && (ACT == Activation::Silu || ACT == Activation::Sigmoid)) {
+        bool holds = true;
+        float2 v[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const float2 x = pair_mul(z[i], both(-1.4426950408889634f));
+            const float2 e = make_float2(gated::exp2f_approx(x.x), gated::exp2f_approx(x.y)), a = pair_add(e, both(1.0f));
+            const float product = a.x * a.y;
+            holds = holds && product <= gated::PAIR_MAX;
+            const float2 s = pair_mul(make_float2(a.y, a.x), both(gated::rcp_approx(product)));
+            if constexpr (!SLOPE) {
+                v[i] = ACT == Activation::Silu ? pair_mul(z[i], s) : s;
+            } else {
+                const float2 tail = pair_mul(e, s);  // 1 - s without cancelling
+                if constexpr (ACT == Activation::Sigmoid) v[i] = pair_mul(s, tail);
+                else v[i] = pair_mul(s, pair_fma(make_float2(fminf(z[i].x, gated::SILU_END), fminf(z[i].y, gated::SILU_END)), tail, both(1.0f)));
+            }
+        }
+        if (__builtin_expect(!holds, 0)) {
+            const float4 t = singly<SLOPE, ACT>(make_float4(z[0].x, z[0].y, z[1].x, z[1].y));
+            v[0] = make_float2(t.x, t.y);
+            v[1] = make_float2(t.z, t.w);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) z[i] = v[i];
+    } else if constexpr (!FINE && ACT == Activation::Gelu) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {  // gated::gelu2 and act_both's slope, packed
+            const float2 t = make_float2(fminf(fabsf(z[i].x), gated::GELU_END), fminf(fabsf(z[i].y), gated::GELU_END));
+            const float2 a = pair_fma(t, both(gated::GELU_P), both(1.0f));
+            const float2 r = pair_mul(make_float2(a.y, a.x), both(gated::rcp_approx(a.x * a.y)));
+            float2 q = both(gated::GELU_Q[6]);
+#pragma unroll
+            for (int j = 5; j >= 0; --j) q = pair_fma(q, r, both(gated::GELU_Q[j]));
+            const float2 x = pair_mul(pair_mul(t, t), both(-0.72134752044448170f));
+            const float2 bell = make_float2(gated::exp2f_approx(x.x), gated::exp2f_approx(x.y));
+            q = pair_mul(pair_mul(q, r), bell);
+            if constexpr (!SLOPE) {
+                z[i] = pair_fma(make_float2(-t.x, -t.y), q, make_float2(gated::max_nan(z[i].x, 0.0f), gated::max_nan(z[i].y, 0.0f)));
+            } else {
+                const float2 side = pair_mul(make_float2(copysignf(t.x, z[i].x), copysignf(t.y, z[i].y)), both(0.39894228040143268f));
+                const float2 low = make_float2(z[i].x > 0.0f ? 1.0f - q.x : q.x, z[i].y > 0.0f ? 1.0f - q.y : q.y);
+                const float2 s = pair_fma(side, bell, low);
+                z[i] = make_float2(z[i].x != z[i].x ? z[i].x : s.x, z[i].y != z[i].y ? z[i].y : s.y);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            z[i] = SLOPE ? make_float2(slope_one<FINE, ACT>(z[i].x), slope_one<FINE, ACT>(z[i].y))
+                         : make_float2(act_one<FINE, ACT>(z[i].x), act_one<FINE, ACT>(z[i].y));
+    }
+}
 // One branch for a row's values.
 template <typename F>
 __device__ __forceinline__ void with_act(Activation act, F&& f) {
@@ -283,56 +426,64 @@ __device__ __forceinline__ void with_act(Activation act, F&& f) {
     else gated::with_activation(act, f);
 }
 
+constexpr int64_t SMALL = 1 << 18;  // elements
+
 // ---- host ---------------------------------------------------------------------------------------------
-// Column tiles of `vec` elements a thread and at most `most` channels a tile. A tile that starts within a 16-byte
-// word cannot take wide loads: false where the groups' width allows none that does not.
-inline bool make_tiling(Tiling& t, int64_t C, int64_t groups, int vec, int places, int most) {
-    t.groups = (int)groups;
-    t.width = (int)(C / groups);
-    if (t.width > most) {
+// Column tiles of `places` times `vec` channels a thread: as wide as may be; in a small call, where there would be fewer
+// tiles of samples than two for every SM, narrower, down to 32 bytes of a row. A tile that starts within a word of `vec`
+// elements cannot take wide loads: false where the groups' width allows none that does not.
+template <typename TX>
+bool make_tiling(Tiling& t, const GroupNormArgs<TX>& a, int vec, int places, int sms) {
+    t.groups = (int)a.groups;
+    t.width = (int)(a.C / a.groups);
+    int unit = 1;  // groups that make whole words
+    while (unit < t.groups && unit * t.width % vec != 0) unit *= 2;
+    unit = std::min(unit, t.groups);
+    if (t.width > MAX_TILE) {
         if (t.width % vec != 0) return false;
         t.gpt = 1;
-        t.tpg = (int)ceil_div(t.width, most);
-        t.max_cols = most;
+        t.tpg = (int)ceil_div(t.width, MAX_TILE);
+        t.max_cols = MAX_TILE;
         t.tiles = t.groups * t.tpg;
         t.blocks = t.groups;
     } else {
-        int unit = 1;  // groups that make whole words
-        while (unit * t.width % vec != 0) unit *= 2;
-        if (unit * t.width > most && unit < groups) return false;
-        t.gpt = (int)std::min<int64_t>(groups, std::max(1, most / t.width / unit) * unit);
+        if (unit * t.width > MAX_TILE) return false;
+        int most = MAX_TILE;
+        const int64_t least = std::max<int64_t>(1, std::min(a.samples, a.rows));
+        while (a.rows * a.C <= SMALL && most * sizeof(TX) > 32 && least * ceil_div(a.C, most) < 2 * sms) most /= 2;
+        t.gpt = std::min(t.groups, std::max(1, most / t.width / unit) * unit);
         t.tpg = 1;
         t.max_cols = t.gpt * t.width;
-        if (t.max_cols > most) return false;
-        t.tiles = t.blocks = (int)ceil_div(groups, t.gpt);
+        t.tiles = t.blocks = (int)ceil_div(t.groups, t.gpt);
     }
+    t.inv = (uint32_t)ceil_div(65536, t.width);
     t.lpr = 1;
-    while (t.lpr < 32 && t.lpr * vec * places < t.max_cols) t.lpr *= 2;
+    t.lpr_log = 0;
+    while (t.lpr < 32 && t.lpr * vec * places < t.max_cols) t.lpr *= 2, ++t.lpr_log;
     return true;
 }
 
-// Who takes which samples. `longest`: 256 KB of a tile's columns, which the CTAs of a wave hold in L2 between their
-// two reads. Chunks: about four a wave's CTA, at least 64 rows. Short samples go to warps where that leaves every
-// SM 16 of them at least; a warp takes up to 64 KB.
+// Who takes which samples. Chunks: one for each CTA of a wave (per_sm an SM), at least 64 rows. `longest`: 512 KB of a
+// tile's columns, or a chunk. Samples of less than 4 KB of a tile on the average go to warps, up to 16 KB each: a CTA's
+// threads would have a row or two.
 struct Cut {
     Chunks ch;
-    int each;
-    int64_t warp_rows;
+    bool by_warp;
+    int warp_rows;
     bool only_long;  // all rows are one sample, and it is long
 };
 template <typename TX>
-Cut make_cut(const GroupNormArgs<TX>& a, const Tiling& t, int bytes, int sms) {
-    const int64_t rows = a.rows, samples = a.samples;
+Cut make_cut(const GroupNormArgs<TX>& a, const Tiling& t, int bytes, int sms, int per_sm) {
     Cut c = {};
-    const int64_t row = (int64_t)t.max_cols * bytes;
-    c.ch.longest = std::max<int64_t>(256, (256 << 10) / row);
-    if (rows > c.ch.longest) {
-        c.ch.rows = std::min(c.ch.longest, std::max<int64_t>(64, ceil_div(rows * t.tiles, 16 * sms)));
-        c.ch.count = (int)ceil_div(rows, c.ch.rows);
+    const int64_t row = (int64_t)t.max_cols * bytes, share = std::max<int64_t>(64, ceil_div(a.rows * t.tiles, per_sm * sms));
+    c.ch.longest = (int)std::max(share, (512 << 10) / row);
+    if (a.rows > c.ch.longest) {
+        c.ch.rows = (int)share;
+        c.ch.count = (int)ceil_div(a.rows, share);
     }
-    c.each = samples * t.blocks >= 16 * sms && t.tpg == 1 ? WARPS : 1;
-    c.warp_rows = std::max<int64_t>(1, (64 << 10) / row);
-    c.only_long = !a.offsets && rows > c.ch.longest;
+    c.by_warp = a.samples >= WARPS && a.rows * row < a.samples * (4 << 10) && t.tpg == 1;
+    c.warp_rows = (int)std::max<int64_t>(1, (16 << 10) / row);
+    c.only_long = !a.offsets && a.rows > c.ch.longest;
     return c;
 }
 

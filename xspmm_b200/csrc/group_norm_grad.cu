@@ -5,9 +5,9 @@
 // values are m1 = sum_c w A / n and m2 = sum_c w B / n, and dx = rstd * (t - m1 - xh * m2). So one pass over x and dy
 // for A and B serves the weights and the groups, and a second one gives dx.
 //
-// Who takes which samples is decided as in the forward pass (group_norm.cu). The sums for the weights' gradients stay
-// in a thread's registers over all samples that its CTA takes and leave as one row a CTA (or chunk), added in order
-// by the last kernel; a group wider than a tile has no registers for them and adds them to its CTA's row as it goes.
+// Who takes which samples is decided as in the forward pass (group_norm.cu). The sums for the weights' gradients are
+// kept for each thread over all samples that its CTA takes and leave as one row a CTA (or chunk), added in order by the
+// last kernel; a block of several tiles has no room for them and adds them to its CTA's row as it goes.
 #include "group_norm.cuh"
 
 namespace xspmm_b200 {
@@ -15,98 +15,126 @@ namespace {
 
 using namespace group;
 
+constexpr int CTAS = 4;  // that an SM should hold: 128 registers a thread
+
 template <typename TX, typename TY>
 struct Backward {
     GroupNormArgs<TX> a;
     Tiling t;
     Chunks ch;
-    int each;           // samples of a work item: WARPS or 1
-    int walkers;        // CTAs a block that walk the work items, 0 where all samples are long
-    int64_t warp_rows;  // most rows that a warp takes
+    int walkers;        // CTAs a block that walk over samples, 0 where all samples are long
+    int each;           // neighbouring samples that one of them takes
+    int warp_rows;      // most rows that a warp takes, 0: none
     const TY* dy;
     int64_t lddy;
     const float *mean, *rstd;
     TY* dx;  // or null
     int64_t lddx;
     float* weights;  // [walker, then chunk][2][channel]: sums of dz * xh and dz, or null
-    float2* part;    // [slot][chunk][group or tile of it]: sums of w A and w B
-    float2* fin;     // [chunk][group]: m1 and m2 of the long sample that begins in the chunk
+    float2* part;    // Parts: sums of w A and w B
     int2* found;     // [chunk]: the long samples with rows in it
 };
 
-// A thread's view of its channels: the parameters, and a sample's statistics.
-template <int E>
+// A thread's view of its channels: the parameters, and a sample's statistics (minus the mean).
+template <int P>
 struct Channels {
-    float w[E], b[E], m[E], rs[E];
+    float2 w[P], b[P], m[P], rs[P];
 };
-
-// dz and xh of a row's values.
-template <typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void row_terms(const Pack<TX, V> (&rx)[U], const Pack<TY, V> (&rg)[U], const Channels<V * U>& ch,
-                                          Activation act, float (&dz)[V * U], float (&xh)[V * U]) {
-    constexpr int E = V * U;
-    Place<V, U>::values(rx, xh);
-    Place<V, U>::values(rg, dz);
+template <int P>
+struct Sums {
+    float2 a[P] = {}, b[P] = {};
+};
+// A thread's sums over all samples that its CTA takes, in shared memory: touched once a sample.
+template <int P>
+struct Totals {
+    float2 (*v)[THREADS];  // [2 P]
+    __device__ void clear() const {
 #pragma unroll
-    for (int e = 0; e < E; ++e) xh[e] = centred(xh[e], ch.m[e], ch.rs[e]);
-    with_act(act, [&](auto a) {
-        if constexpr (decltype(a)::value != Activation::None)
+        for (int e = 0; e < 2 * P; ++e) v[e][threadIdx.x] = make_float2(0.0f, 0.0f);
+    }
+    __device__ void add(const Sums<P>& s) const {
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                dz[e] *= slope_one<sizeof(TY) == 4, decltype(a)::value>(affine(xh[e], ch.w[e], ch.b[e]));
-    });
-}
-
-// Calls f(row, dz, xh) for this thread's rows of [begin, end).
-template <bool CTA, int B, typename TX, typename TY, int V, int U, typename F>
-__device__ __forceinline__ void each_row(const Team<CTA, V, U>& tm, const TX* x, int64_t ldx, const TY* dy, int64_t lddy,
-                                         int64_t begin, int64_t end, const Channels<V * U>& ch, Activation act, F&& f) {
-    for (int64_t r = begin + tm.rl; r < end; r += (int64_t)tm.step * B) {
-        Pack<TX, V> rx[B][U];
-        Pack<TY, V> rg[B][U];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const int64_t row = r + (int64_t)i * tm.step;
-            if (row < end) {
-                tm.at.load(rx[i], x + row * ldx);
-                tm.at.load(rg[i], dy + row * lddy);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const int64_t row = r + (int64_t)i * tm.step;
-            if (row >= end) break;
-            float dz[V * U], xh[V * U];
-            row_terms(rx[i], rg[i], ch, act, dz, xh);
-            f(row, dz, xh);
+        for (int e = 0; e < P; ++e) {
+            v[e][threadIdx.x] = pair_add(v[e][threadIdx.x], s.a[e]);
+            v[P + e][threadIdx.x] = pair_add(v[P + e][threadIdx.x], s.b[e]);
         }
     }
-}
-
-template <int E>
-struct Sums {
-    float a[E] = {}, b[E] = {};
+    __device__ Sums<P> get() const {
+        Sums<P> s;
+#pragma unroll
+        for (int e = 0; e < P; ++e) s.a[e] = v[e][threadIdx.x], s.b[e] = v[P + e][threadIdx.x];
+        return s;
+    }
 };
+
+// Calls f(row, dz, xh) for this thread's rows of [begin, end), counted from the first, or with BACK from the last.
+template <bool CTA, bool BACK, int B, typename TX, typename TY, int V, int U, typename F>
+__device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
+                                         int end, const Channels<V * U / 2>& ch, F&& f) {
+    constexpr int P = V * U / 2;
+    struct Batch {
+        Pack<TX, V> x[B][U];
+        Pack<TY, V> g[B][U];
+    };
+    const int rows = tm.rows(end - begin);
+    const int64_t last = BACK ? max(rows - 1, 0) : 0, step = BACK ? -tm.step : tm.step;
+    const TX* px = tm.first(p.a.x + k.c0, begin, p.a.ldx) + last * tm.step * p.a.ldx;
+    const TY* pg = tm.first(p.dy + k.c0, begin, p.lddy) + last * tm.step * p.lddy;
+    const int64_t nx = step * p.a.ldx, ng = step * p.lddy;
+    batches<B, Batch>(
+        rows,
+        [&](auto full, Batch& t, int i, int n) {
+            const TX* rx = px + i * nx;
+            const TY* rg = pg + i * ng;
+#pragma unroll
+            for (int j = 0; j < B; ++j)
+                if (full || i + j < n) {
+                    tm.at.load(t.x[j], rx + j * nx);
+                    tm.at.load(t.g[j], rg + j * ng);
+                }
+        },
+        [&](auto full, const Batch& t, int i, int n) {
+            with_act(p.a.act, [&](auto act) {
+                constexpr Activation ACT = decltype(act)::value;
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    if (!full && i + j >= n) break;
+                    float2 dz[P], xh[P];
+                    Place<V, U>::values(t.x[j], xh);
+                    Place<V, U>::values(t.g[j], dz);
+#pragma unroll
+                    for (int e = 0; e < P; ++e) xh[e] = centred(xh[e], ch.m[e], ch.rs[e]);
+                    if constexpr (ACT != Activation::None) {
+                        float2 z[P];
+#pragma unroll
+                        for (int e = 0; e < P; ++e) z[e] = affine(xh[e], ch.w[e], ch.b[e]);
+                        act_row<true, sizeof(TY) == 4, ACT>(z);
+#pragma unroll
+                        for (int e = 0; e < P; ++e) dz[e] = pair_mul(dz[e], z[e]);
+                    }
+                    f(i + j, dz, xh);
+                }
+            });
+        });
+}
 
 // This thread's A and B over rows [begin, end), added to `total`, and the groups' sums of w A and w B, which one thread
 // a group hands to f(group of the tile, sum, sum). channels(strips) is called between, once the tile's A and B are
 // there by channel. The strips may be written again after a team_sync.
 template <bool CTA, int B, typename TX, typename TY, int V, int U, typename F, typename C>
-__device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int64_t begin,
-                                           int64_t end, const Channels<V * U>& ch, Sums<V * U>& total, Strips& sh, F&& f,
-                                           C&& channels) {
-    constexpr int E = V * U;
-    Sums<E> s;
-    each_row<CTA, B>(tm, p.a.x + k.c0, p.a.ldx, p.dy + k.c0, p.lddy, begin, end, ch, p.a.act,
-                     [&](int64_t, const float (&dz)[E], const float (&xh)[E]) {
+__device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
+                                           int end, const Channels<V * U / 2>& ch, const Totals<V * U / 2>& total,
+                                           Strips& sh, F&& f, C&& channels) {
+    constexpr int P = V * U / 2;
+    Sums<P> s;
+    each_row<CTA, false, B>(p, tm, k, begin, end, ch, [&](int, const float2 (&dz)[P], const float2 (&xh)[P]) {
 #pragma unroll
-                         for (int e = 0; e < E; ++e) {
-                             s.a[e] += dz[e];
-                             s.b[e] = fmaf(dz[e], xh[e], s.b[e]);
-                         }
-                     });
-#pragma unroll
-    for (int e = 0; e < E; ++e) total.a[e] += s.a[e], total.b[e] += s.b[e];
+        for (int e = 0; e < P; ++e) {
+            s.a[e] = pair_add(s.a[e], dz[e]);
+            s.b[e] = pair_fma(dz[e], xh[e], s.b[e]);
+        }
+    });
+    total.add(s);
     sum_channels<CTA>(s.a, s.b, tm.at, sh);
     const int strip = CTA ? 0 : threadIdx.x >> 5;
     channels(sh.v[strip]);
@@ -126,42 +154,46 @@ __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team
     });
 }
 
-// dx of rows [begin, end) from the groups' m1 and m2.
-template <bool CTA, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int64_t begin,
-                                      int64_t end, const Channels<V * U>& ch, const float* g1, const float* g2) {
-    constexpr int E = V * U;
-    float m1[E], m2[E];
+// dx of rows [begin, end) from the groups' minus m1 and minus m2.
+template <bool CTA, bool BACK, int B, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
+                                      int end, const Channels<V * U / 2>& ch, const float* g1, const float* g2) {
+    constexpr int P = V * U / 2;
+    float2 m1[P], m2[P];
     tm.of_groups(m1, g1, k);
     tm.of_groups(m2, g2, k);
-    each_row<CTA, B>(tm, p.a.x + k.c0, p.a.ldx, p.dy + k.c0, p.lddy, begin, end, ch, p.a.act,
-                     [&](int64_t row, const float (&dz)[E], const float (&xh)[E]) {
-                         float v[E];
+    const int64_t last = BACK ? max(tm.rows(end - begin) - 1, 0) : 0;
+    TY* out = tm.first(p.dx + k.c0, begin, p.lddx) + last * tm.step * p.lddx;
+    const int64_t next = (BACK ? -tm.step : tm.step) * p.lddx;
+    each_row<CTA, BACK, B>(p, tm, k, begin, end, ch, [&](int i, const float2 (&dz)[P], const float2 (&xh)[P]) {
+        float2 v[P];
 #pragma unroll
-                         for (int e = 0; e < E; ++e)
-                             v[e] = ch.rs[e] * (fmaf(-xh[e], m2[e], fmaf(dz[e], ch.w[e], -m1[e])));
-                         tm.at.store(p.dx + k.c0 + row * p.lddx, v);
-                     });
+        for (int e = 0; e < P; ++e) v[e] = pair_mul(ch.rs[e], pair_fma(xh[e], m2[e], pair_fma(dz[e], ch.w[e], m1[e])));
+        tm.at.store(out + i * next, v);
+    });
 }
 
 template <bool CTA, typename TX, typename TY, int V, int U>
 __device__ __forceinline__ void parameters(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k,
-                                           Channels<V * U>& ch) {
+                                           Channels<V * U / 2>& ch) {
     tm.at.param(ch.w, p.a.w, k.c0, 1.0f);
     tm.at.param(ch.b, p.a.b, k.c0, 0.0f);
 }
 template <bool CTA, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void statistics(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int64_t s,
-                                           Channels<V * U>& ch) {
-    tm.of_groups(ch.m, p.mean + s * p.t.groups + k.g0, k);
-    tm.of_groups(ch.rs, p.rstd + s * p.t.groups + k.g0, k);
+__device__ __forceinline__ void statistics(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int s,
+                                           Channels<V * U / 2>& ch) {
+    tm.of_groups(ch.m, p.mean + (int64_t)s * p.t.groups + k.g0, k);
+    tm.of_groups(ch.rs, p.rstd + (int64_t)s * p.t.groups + k.g0, k);
+#pragma unroll
+    for (int e = 0; e < V * U / 2; ++e) ch.m[e] = make_float2(-ch.m[e].x, -ch.m[e].y);
 }
 
 // The CTA's sums of a tile's channels to row `row` of the weights' parts.
 template <typename TX, typename TY, int V, int U>
 __device__ __forceinline__ void leave_weights(const Backward<TX, TY>& p, int64_t row, const Tile& k, const Place<V, U>& at,
-                                              Sums<V * U>& total, Strips& sh) {
-    sum_channels<true>(total.a, total.b, at, sh);
+                                              const Totals<V * U / 2>& total, Strips& sh) {
+    Sums<V * U / 2> s = total.get();
+    sum_channels<true>(s.a, s.b, at, sh);
     if ((int)threadIdx.x < k.cols) {
         float* out = p.weights + row * 2 * p.a.C + k.c0 + threadIdx.x;
         out[0] = sh.v[0][1][threadIdx.x];
@@ -171,8 +203,9 @@ __device__ __forceinline__ void leave_weights(const Backward<TX, TY>& p, int64_t
 
 // A sample by a team. `total` is the CTA's sums where a block is one tile; else they go to the CTA's row.
 template <bool CTA, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int64_t s, Span rows, int block, int64_t row,
-                                             Channels<V * U>& ch, Sums<V * U>& total, Strips& sh, float* g1, float* g2) {
+__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int s, Span rows, int block, int64_t row,
+                                             Channels<V * U / 2>& ch, const Totals<V * U / 2>& total, Strips& sh, float* g1,
+                                             float* g2) {
     const int t0 = block * p.t.tpg;
     const bool one = p.t.tpg == 1;
     for (int j = 0; j < p.t.tpg; ++j) {
@@ -180,7 +213,7 @@ __device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int64_t 
         const Team<CTA, V, U> tm(p.t, k.cols);
         if (!one) parameters(p, tm, k, ch);
         if (one || j == 0) statistics(p, tm, k, s, ch);
-        const float per = 1.0f / ((float)(rows.end - rows.begin) * (float)p.t.width);
+        const float per = -1.0f / ((float)(rows.end - rows.begin) * (float)p.t.width);
         group_sums<CTA, B>(p, tm, k, rows.begin, rows.end, ch, total, sh,
                            [&](int g, float s1, float s2) {
                                if (j > 0) s1 += g1[g], s2 += g2[g];  // the same thread's sums of the tiles before
@@ -202,43 +235,46 @@ __device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int64_t 
         const Tile k = tile_of(p.t, t0 + j);
         const Team<CTA, V, U> tm(p.t, k.cols);
         if (!one) parameters(p, tm, k, ch);
-        apply<CTA, B>(p, tm, k, rows.begin, rows.end, ch, g1, g2);
+        apply<CTA, false, B>(p, tm, k, rows.begin, rows.end, ch, g1, g2);
     }
     team_sync<CTA>();
 }
 
 // CTAs [0, chunks x tiles): sums of the long samples' chunks. The others: short and middle samples.
 template <typename TX, typename TY, int V, int U, int B>
-__global__ void __launch_bounds__(THREADS, 2) group_norm_grad_kernel(const __grid_constant__ Backward<TX, TY> p) {
+__global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_kernel(const __grid_constant__ Backward<TX, TY> p) {
     __shared__ Strips sh;
     __shared__ float g1[WARPS][MAX_TILE], g2[WARPS][MAX_TILE];
+    __shared__ float2 totals[V * U][THREADS];
     cudaGridDependencySynchronize();
     const int chunked = p.ch.count * p.t.tiles, warp = threadIdx.x >> 5;
-    Channels<V * U> ch;
-    Sums<V * U> total;
+    Channels<V * U / 2> ch;
+    const Totals<V * U / 2> total{totals};
+    total.clear();
     if ((int)blockIdx.x < chunked) {
         const int i = blockIdx.x / p.t.tiles, tile = blockIdx.x - i * p.t.tiles;
-        const int2 found = long_samples(p.a.offsets, (int)p.a.samples, p.a.rows, p.ch, i);
+        const int2 found = long_samples(p.a.offsets, (int)p.a.samples, (int)p.a.rows, p.ch, i);
         if (tile == 0 && threadIdx.x == 0) p.found[i] = found;
         const Tile k = tile_of(p.t, tile);
         const Team<true, V, U> tm(p.t, k.cols);
-        const int64_t r0 = i * p.ch.rows, r1 = min(p.a.rows, r0 + p.ch.rows), slots = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
+        const int all = (int)p.a.rows, r0 = i * p.ch.rows, r1 = r0 + min(p.ch.rows, all - r0);
+        const int64_t slots = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
         parameters(p, tm, k, ch);
         for (int slot = 0; slot < 2; ++slot) {
             const int s = slot ? found.y : found.x;
             if (s < 0) continue;
-            const Span sp = span_of(p.a.offsets, s, p.a.rows);
-            float2* out = p.part + ((int64_t)slot * p.ch.count + i) * slots + part_slot(p.t, tile, k);
+            const Span sp = span_of(p.a.offsets, s, all);
+            float2* out = p.part + (slot * slots + part_slot(p.t, tile, k)) * p.ch.count + i;
             statistics(p, tm, k, s, ch);
             group_sums<true, B>(p, tm, k, max(r0, sp.begin), min(r1, sp.end), ch, total, sh,
-                                [&](int g, float s1, float s2) { out[g] = make_float2(s1, s2); },
+                                [&](int g, float s1, float s2) { out[(int64_t)g * p.ch.count] = make_float2(s1, s2); },
                                 [](const float (&)[2][MAX_TILE]) {});
             __syncthreads();
         }
         if (p.weights) leave_weights(p, p.walkers + i, k, tm.at, total, sh);
         return;
     }
-    const int at = blockIdx.x - chunked, block = at % p.t.blocks, walker = at / p.t.blocks;
+    const int at = blockIdx.x - chunked, walker = p.t.blocks == 1 ? at : at / p.t.blocks, block = at - walker * p.t.blocks;
     const Tile k = tile_of(p.t, block * p.t.tpg);
     const Team<true, V, U> tm(p.t, k.cols);
     const bool one = p.t.tpg == 1;
@@ -249,52 +285,28 @@ __global__ void __launch_bounds__(THREADS, 2) group_norm_grad_kernel(const __gri
         for (int c = threadIdx.x; c < p.t.width; c += THREADS) out[c] = out[p.a.C + c] = 0.0f;
         __syncthreads();
     }
-    auto rows_of = [&](int64_t s) { return span_of(p.a.offsets, s, p.a.rows); };
-    for (int64_t s0 = (int64_t)walker * p.each; s0 < p.a.samples; s0 += (int64_t)p.walkers * p.each) {
-        if (p.each > 1) {
-            const int64_t s = s0 + warp;
-            if (s < p.a.samples) {
-                const Span sp = rows_of(s);
-                if (sp.end > sp.begin && sp.end - sp.begin <= p.warp_rows)
-                    whole_sample<false, B, TX, TY, V, U>(p, s, sp, block, walker, ch, total, sh, g1[warp], g2[warp]);
-            }
-            __syncthreads();
+    auto rows_of = [&](int s) { return span_of(p.a.offsets, s, (int)p.a.rows); };
+    const int s0 = walker * p.each, s1 = s0 + min(p.each, (int)p.a.samples - s0);
+    if (p.warp_rows > 0) {
+        for (int s = s0 + warp; s < s1; s += WARPS) {
+            const Span sp = rows_of(s);
+            if (sp.end > sp.begin && sp.end - sp.begin <= p.warp_rows)
+                whole_sample<false, B, TX, TY, V, U>(p, s, sp, block, walker, ch, total, sh, g1[warp], g2[warp]);
         }
-        for (int j = 0; j < p.each && s0 + j < p.a.samples; ++j) {
-            const Span sp = rows_of(s0 + j);
-            const int64_t n = sp.end - sp.begin;
-            if (n > 0 && n <= p.ch.longest && (p.each == 1 || n > p.warp_rows))
-                whole_sample<true, B, TX, TY, V, U>(p, s0 + j, sp, block, walker, ch, total, sh, g1[0], g2[0]);
-        }
+        __syncthreads();
+    }
+    for (int s = s0; s < s1; ++s) {
+        const Span sp = rows_of(s);
+        const int n = sp.end - sp.begin;
+        if (n > p.warp_rows && n <= p.ch.longest)
+            whole_sample<true, B, TX, TY, V, U>(p, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
     }
     if (one && p.weights) leave_weights(p, walker, k, tm.at, total, sh);
 }
 
-// m1 and m2 of the long samples: a warp for each chunk and group. A sample belongs to the chunk it begins in.
-template <typename TX, typename TY>
-__global__ void __launch_bounds__(THREADS) group_norm_grad_join_kernel(const __grid_constant__ Backward<TX, TY> p) {
-    cudaGridDependencySynchronize();
-    const int i = blockIdx.x, s = p.found[i].y, g = blockIdx.y * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (s < 0 || g >= p.t.groups) return;
-    const Span sp = span_of(p.a.offsets, s, p.a.rows);
-    const int last = (int)((sp.end - 1) / p.ch.rows), tpg = p.t.tpg, parts = (last - i + 1) * tpg;
-    const int64_t slots = tpg == 1 ? p.t.groups : p.t.tiles;
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll 4
-    for (int q = lane; q < parts; q += 32) {
-        const int c = i + q / tpg;
-        const float2 v = p.part[((int64_t)(c == i) * p.ch.count + c) * slots + g * tpg + q % tpg];
-        s1 += v.x;
-        s2 += v.y;
-    }
-    s1 = group_sum(s1, 32);
-    s2 = group_sum(s2, 32);
-    const float per = 1.0f / ((float)(sp.end - sp.begin) * (float)p.t.width);
-    if (lane == 0) p.fin[(int64_t)i * p.t.groups + g] = make_float2(s1 * per, s2 * per);
-}
-
+// dx of the long samples' chunks. Every CTA joins the sums of its tile's groups over all of the sample's chunks.
 template <typename TX, typename TY, int V, int U, int B>
-__global__ void __launch_bounds__(THREADS, 2) group_norm_grad_apply_kernel(const __grid_constant__ Backward<TX, TY> p) {
+__global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_apply_kernel(const __grid_constant__ Backward<TX, TY> p) {
     __shared__ float g1[MAX_TILE], g2[MAX_TILE];
     cudaGridDependencySynchronize();
     const int i = p.ch.count - 1 - blockIdx.x / p.t.tiles, tile = blockIdx.x % p.t.tiles;
@@ -302,22 +314,33 @@ __global__ void __launch_bounds__(THREADS, 2) group_norm_grad_apply_kernel(const
     if (found.x < 0 && found.y < 0) return;
     const Tile k = tile_of(p.t, tile);
     const Team<true, V, U> tm(p.t, k.cols);
-    const int64_t r0 = i * p.ch.rows, r1 = min(p.a.rows, r0 + p.ch.rows);
-    Channels<V * U> ch;
+    const int all = (int)p.a.rows, r0 = i * p.ch.rows, r1 = r0 + min(p.ch.rows, all - r0);
+    const int tpg = p.t.tpg, lane = threadIdx.x & 31;
+    Channels<V * U / 2> ch;
     parameters(p, tm, k, ch);
-    for (int slot = 0; slot < 2; ++slot) {
+    for (int slot = 1; slot >= 0; --slot) {
         const int s = slot ? found.y : found.x;
         if (s < 0) continue;
-        const Span sp = span_of(p.a.offsets, s, p.a.rows);
+        const Span sp = span_of(p.a.offsets, s, all);
+        const Parts parts(sp, p.ch, tpg == 1 ? p.t.groups : p.t.tiles);
+        const float per = -1.0f / ((float)(sp.end - sp.begin) * (float)p.t.width);
         __syncthreads();
-        if ((int)threadIdx.x < k.ng) {
-            const float2 v = p.fin[sp.begin / p.ch.rows * p.t.groups + k.g0 + threadIdx.x];
-            g1[threadIdx.x] = v.x;
-            g2[threadIdx.x] = v.y;
+        for (int g = threadIdx.x >> 5; g < k.ng; g += WARPS) {
+            float s1 = 0.0f, s2 = 0.0f;
+            for (int part = 0; part < tpg; ++part)
+#pragma unroll 8
+                for (int c = lane; c < parts.count; c += 32) {
+                    const float2 v = parts.get(p.part, (int64_t)(k.g0 + g) * tpg + part, c);
+                    s1 += v.x;
+                    s2 += v.y;
+                }
+            s1 = group_sum(s1, 32);
+            s2 = group_sum(s2, 32);
+            if (lane == 0) g1[g] = s1 * per, g2[g] = s2 * per;
         }
         __syncthreads();
         statistics(p, tm, k, s, ch);
-        apply<true, B>(p, tm, k, max(r0, sp.begin), min(r1, sp.end), ch, g1, g2);
+        apply<true, true, B>(p, tm, k, max(r0, sp.begin), min(r1, sp.end), ch, g1, g2);
     }
 }
 
@@ -342,18 +365,18 @@ __global__ void __launch_bounds__(1024) group_norm_weights_kernel(const float* p
 template <typename TX, typename TY, int V, int U, int B>
 void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     const int sms = sm_count(h.device);
-    const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), sms);
+    const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), sms, CTAS);
     p.ch = cut.ch;
-    p.each = cut.each;
-    p.warp_rows = cut.warp_rows;
-    const int64_t items = ceil_div(p.a.samples, p.each);
-    p.walkers = cut.only_long ? 0 : (int)std::max<int64_t>(1, std::min(items, ceil_div(2 * sms, p.t.blocks)));
-    DevBuf<float2> ws((size_t)p.ch.count * (2 * part_slots(p.t) + p.t.groups), h.stream);
+    p.warp_rows = cut.by_warp ? cut.warp_rows : 0;
+    // as many samples a CTA as make four waves of them
+    const int64_t items = ceil_div(p.a.samples, cut.by_warp ? WARPS : 1);
+    p.each = (int)std::max<int64_t>(1, items * p.t.blocks / (4 * CTAS * sms)) * (cut.by_warp ? WARPS : 1);
+    p.walkers = cut.only_long ? 0 : (int)std::max<int64_t>(1, ceil_div(p.a.samples, p.each));
+    DevBuf<float2> part((size_t)p.ch.count * 2 * part_slots(p.t), h.stream);
     DevBuf<int2> found((size_t)p.ch.count, h.stream);
-    const int parts = p.walkers + p.ch.count;
-    DevBuf<float> weights(dw || db ? (size_t)parts * 2 * p.a.C : 0, h.stream);
-    p.part = ws.get();
-    p.fin = ws.get() + (int64_t)p.ch.count * 2 * part_slots(p.t);
+    const int rows = p.walkers + p.ch.count;
+    DevBuf<float> weights(dw || db ? (size_t)rows * 2 * p.a.C : 0, h.stream);
+    p.part = part.get();
     p.found = found.get();
     p.weights = weights.get();
     const int64_t chunked = (int64_t)p.ch.count * p.t.tiles, grid = chunked + (int64_t)p.walkers * p.t.blocks;
@@ -361,15 +384,12 @@ void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     launch_dependent(h.stream, group_norm_grad_kernel<TX, TY, V, U, B>, (unsigned)grid, THREADS, 0, 1, p);
     after_launch(h, "group_norm_grad");
     if (p.ch.count > 0 && p.dx) {
-        launch_dependent(h.stream, group_norm_grad_join_kernel<TX, TY>,
-                         dim3((unsigned)p.ch.count, (unsigned)ceil_div(p.t.groups, WARPS)), THREADS, 0, 1, p);
-        after_launch(h, "group_norm_grad_join");
         launch_dependent(h.stream, group_norm_grad_apply_kernel<TX, TY, V, U, B>, (unsigned)chunked, THREADS, 0, 1, p);
         after_launch(h, "group_norm_grad_apply");
     }
     if (p.weights) {
         launch_dependent(h.stream, group_norm_weights_kernel, dim3((unsigned)ceil_div(p.a.C, 32), 2), 1024, 0, 1,
-                         (const float*)p.weights, parts, p.a.C, dw, db);
+                         (const float*)p.weights, rows, p.a.C, dw, db);
         after_launch(h, "group_norm_weights");
     }
 }
@@ -388,18 +408,12 @@ void group_norm_backward(Handle& h, const GroupNormArgs<TX>& a, const TY* dy, in
     p.rstd = rstd;
     p.dx = dx;
     p.lddx = lddx;
-    constexpr int V = 16 / sizeof(TX);
-    constexpr size_t other = std::min<size_t>(16, V * sizeof(TY));
-    const bool wide = a.C % V == 0 && (a.rows <= 1 || (a.ldx % V == 0 && lddy % V == 0 && (!dx || lddx % V == 0))) &&
-                      aligned_to(a.x, 16) && aligned_to(dy, other) && aligned_to(dx, other);
-    if (wide && make_tiling(p.t, a.C, a.groups, V, 1, 32 * V)) return backward<TX, TY, V, 1, 4>(h, p, dw, db);
-    if (a.C <= 32) {
-        make_tiling(p.t, a.C, a.groups, 1, 1, 32);
-        backward<TX, TY, 1, 1, 8>(h, p, dw, db);
-    } else {
-        make_tiling(p.t, a.C, a.groups, 1, 8, MAX_TILE);
-        backward<TX, TY, 1, 8, 2>(h, p, dw, db);
-    }
+    const size_t bx = PER * sizeof(TX), by = PER * sizeof(TY);
+    const bool wide = a.C % PER == 0 && (a.rows <= 1 || (a.ldx % PER == 0 && lddy % PER == 0 && (!dx || lddx % PER == 0))) &&
+                      aligned_to(a.x, bx) && aligned_to(dy, by) && aligned_to(dx, by);
+    if (wide && make_tiling(p.t, a, PER, 1, sm_count(h.device))) return backward<TX, TY, PER, 1, sizeof(TX) == 2 ? 4 : 2>(h, p, dw, db);
+    make_tiling(p.t, a, 1, PER, sm_count(h.device));
+    backward<TX, TY, 1, PER, 2>(h, p, dw, db);
 }
 
 #define XS_INST_GROUP_NORM_GRAD(TX, TY)                                                                          \
