@@ -21,18 +21,16 @@ namespace {
 
 using namespace group;
 
-constexpr int CTAS = 6;  // that an SM should hold: 80 registers a thread
-// Rows of a batch in the second pass, which holds the parameters too: two batches of B fp32 rows would not fit.
-template <typename TX, int B>
-constexpr int apply_rows = sizeof(TX) == 4 && B > 2 ? 2 : B;
+constexpr int CTAS = 4;  // that an SM should hold: 64 registers a thread and
+constexpr int SLOT_BYTES = 152;  // of shared memory a thread for rows
+constexpr int RING_BYTES = 128;  // of them for rows that only pass
 
 template <typename TX, typename TY>
 struct Forward {
     GroupNormArgs<TX> a;
     Tiling t;
     Chunks ch;
-    int each;       // samples that a CTA of short samples takes: WARPS or 1
-    int warp_rows;  // most rows that a warp takes
+    int each;  // samples that a CTA takes: WARPS, one a warp where it can, or 1
     float eps;
     TY* y;
     int64_t ldy;
@@ -47,10 +45,10 @@ struct Moments {
     float2 mean[P] = {}, m2[P] = {};
 };
 
-// Adds a batch of rows: B of them, or with ALL = false the first `count`, the others zeros.
-template <bool ALL, int B, typename TX, int V, int U>
-__device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V> (&raw)[B][U], int count) {
-    constexpr int P = V * U / 2;
+// Adds a batch of rows: BATCH of them, or with ALL = false the first `count`, the others zeros.
+template <bool ALL, typename TX, int V, int U>
+__device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V> (&raw)[BATCH][U], int count) {
+    constexpr int P = V * U / 2, B = BATCH;
     float2 s[P] = {}, q[P] = {}, v[P];
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -89,31 +87,34 @@ __device__ __forceinline__ float join_weights(float na, float nb, float* fb, flo
 }
 
 // Moments of the tile's groups over rows [begin, end) of x (its first channel): f(group of the tile, mean, sum of
-// squares), called by one thread a group. The strips may be written again after a team_sync.
-template <bool CTA, int B, typename TX, int V, int U, typename F>
-__device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const TX* x, int64_t ldx, int begin, int end,
-                                              const Tile& k, Strips& sh, F&& f) {
+// squares), called by one thread a group. KEEP: the rows fit the slots and stay there. The strips may be written again
+// after a team_sync.
+template <bool CTA, bool KEEP, typename TX, int V, int U, typename F>
+__device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const Slots<TX, V, U>& slots, const TX* x, int64_t ldx,
+                                              int begin, int end, const Tile& k, Strips& sh, F&& f) {
     constexpr int P = V * U / 2;
-    struct Batch {
-        Pack<TX, V> raw[B][U];
-    };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = tm.rows(end - begin);
     Moments<P> m;
     const TX* at = tm.first(x, begin, ldx);
     const int64_t next = tm.step * ldx;
-    batches<B, Batch>(
-        tm.rows(end - begin),
-        [&](auto full, Batch& b, int i, int n) {
-            const TX* row = at + i * next;
+    auto fill = [&](int slot, int i) { slots.fill(slot, at + i * next, tm.at); };
+    auto use = [&](auto full, int slot, int i, int n) {
+        Pack<TX, V> raw[BATCH][U];
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                if (full || i + j < n) tm.at.load(b.raw[j], row + j * next);
-                else
+        for (int j = 0; j < BATCH; ++j) {
+            if (full || i + j < n) slots.get(raw[j], slot + j);
+            else
 #pragma unroll
-                    for (int u = 0; u < U; ++u) b.raw[j][u] = Pack<TX, V>{};
-            }
-        },
-        [&](auto full, const Batch& b, int i, int n) { add_rows<decltype(full)::value>(m, b.raw, n - i); });
+                for (int u = 0; u < U; ++u) raw[j][u] = Pack<TX, V>{};
+        }
+        add_rows<decltype(full)::value>(m, raw, n - i);
+    };
+    if constexpr (KEEP) {
+        fill_all(rows, fill);
+        use_all(rows, use);
+    } else {
+        stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(rows, fill, use);
+    }
     for (int o = 16; o >= tm.at.lpr; o >>= 1) {
         // both of a pair take the lower lane's moments first, so that they end with the same numbers
         const bool low = (lane & o) == 0;
@@ -141,15 +142,17 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const T
     if constexpr (CTA) {
         const int c = threadIdx.x;
         if (c < k.cols) {
-            float n = sh.n[0], ma = sh.v[0][0][c], sa = sh.v[0][1][c];
+            const float per = 1.0f / (float)(end - begin);
+            float mean = 0.0f, m2 = 0.0f;
 #pragma unroll
-            for (int w = 1; w < WARPS; ++w) {
-                float fb, g;
-                n = join_weights(n, sh.n[w], &fb, &g);
-                join_moments(ma, sa, sh.v[w][0][c], sh.v[w][1][c], fb, g);
+            for (int w = 0; w < WARPS; ++w) mean = fmaf(sh.n[w] * per, sh.v[w][0][c], mean);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float d = sh.v[w][0][c] - mean;
+                m2 += fmaf(sh.n[w] * d, d, sh.v[w][1][c]);
             }
-            sh.v[0][0][c] = ma;
-            sh.v[0][1][c] = sa;
+            sh.v[0][0][c] = mean;
+            sh.v[0][1][c] = m2;
         }
         __syncthreads();
     }
@@ -173,14 +176,12 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const T
     });
 }
 
-// y of rows [begin, end) from the groups' minus mean and rstd at gm and gr[group of the tile]. BACK: the last rows first.
-template <bool CTA, bool BACK, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void apply(const Forward<TX, TY>& p, const Team<CTA, V, U>& tm, int begin, int end,
-                                      const Tile& k, const float* gm, const float* gr) {
+// y of rows [begin, end) from the groups' minus mean and rstd at gm and gr[group of the tile]. KEPT: the rows are in the
+// slots. BACK: the last rows first.
+template <bool CTA, bool KEPT, bool BACK, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void apply(const Forward<TX, TY>& p, const Team<CTA, V, U>& tm, const Slots<TX, V, U>& slots,
+                                      int begin, int end, const Tile& k, const float* gm, const float* gr) {
     constexpr int P = V * U / 2;
-    struct Batch {
-        Pack<TX, V> raw[B][U];
-    };
     float2 w[P], b[P], m[P], rs[P];
     tm.at.param(w, p.a.w, k.c0, 1.0f);
     tm.at.param(b, p.a.b, k.c0, 0.0f);
@@ -191,29 +192,27 @@ __device__ __forceinline__ void apply(const Forward<TX, TY>& p, const Team<CTA, 
     const TX* from = tm.first(p.a.x + k.c0, begin, p.a.ldx) + last * tm.step * p.a.ldx;
     TY* to = tm.first(p.y + k.c0, begin, p.ldy) + last * tm.step * p.ldy;
     const int64_t fnext = (BACK ? -tm.step : tm.step) * p.a.ldx, tnext = (BACK ? -tm.step : tm.step) * p.ldy;
-    batches<B, Batch>(
-        rows,
-        [&](auto full, Batch& t, int i, int n) {
-            const TX* row = from + i * fnext;
+    auto use = [&](auto act, auto full, int slot, int i, int n) {
+        TY* row = to + i * tnext;
 #pragma unroll
-            for (int j = 0; j < B; ++j)
-                if (full || i + j < n) tm.at.load(t.raw[j], row + j * fnext);
-        },
-        [&](auto full, const Batch& t, int i, int n) {
-            TY* row = to + i * tnext;
-            with_act(p.a.act, [&](auto act) {
+        for (int j = 0; j < BATCH; ++j) {
+            if (!full && i + j >= n) break;
+            Pack<TX, V> raw[U];
+            slots.get(raw, slot + j);
+            float2 v[P];
+            Place<V, U>::values(raw, v);
 #pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    if (!full && i + j >= n) break;
-                    float2 v[P];
-                    Place<V, U>::values(t.raw[j], v);
-#pragma unroll
-                    for (int e = 0; e < P; ++e) v[e] = affine(centred(v[e], m[e], rs[e]), w[e], b[e]);
-                    act_row<false, sizeof(TY) == 4, decltype(act)::value>(v);
-                    tm.at.store(row + j * tnext, v);
-                }
-            });
-        });
+            for (int e = 0; e < P; ++e) v[e] = affine(centred(v[e], m[e], rs[e]), w[e], b[e]);
+            act_row<false, sizeof(TY) == 4, decltype(act)::value>(v);
+            tm.at.store(row + j * tnext, v);
+        }
+    };
+    with_act(p.a.act, [&](auto act) {
+        auto go = [&](auto full, int slot, int i, int n) { use(act, full, slot, i, n); };
+        if constexpr (KEPT) use_all(rows, go);
+        else stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(
+            rows, [&](int slot, int i) { slots.fill(slot, from + i * fnext, tm.at); }, go);
+    });
 }
 
 // A group's statistics: gm and gr take minus the mean and rstd, the caller's arrays the mean and rstd.
@@ -228,16 +227,16 @@ __device__ __forceinline__ void finish(const Forward<TX, TY>& p, int s, int grou
     *gr = rs;
 }
 
-// A sample by a team: all tiles of the block twice.
-template <bool CTA, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void whole_sample(const Forward<TX, TY>& p, int s, Span rows, int block, Strips& sh,
-                                             float* gm, float* gr) {
-    const int t0 = block * p.t.tpg;
+// A sample by a team. KEEP: it is one tile and fits the slots; else all tiles of the block are read twice.
+template <bool CTA, bool KEEP, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void whole_sample(const Forward<TX, TY>& p, const Slots<TX, V, U>& slots, int s, Span rows, int block,
+                                             Strips& sh, float* gm, float* gr) {
+    const int tpg = KEEP ? 1 : p.t.tpg, t0 = block * tpg;
     const float n = (float)(rows.end - rows.begin);
-    for (int j = 0; j < p.t.tpg; ++j) {
+    for (int j = 0; j < tpg; ++j) {
         const Tile k = tile_of(p.t, t0 + j);
         const Team<CTA, V, U> tm(p.t, k.cols);
-        group_moments<CTA, B>(tm, p.a.x + k.c0, p.a.ldx, rows.begin, rows.end, k, sh, [&](int g, float mean, float m2) {
+        group_moments<CTA, KEEP>(tm, slots, p.a.x + k.c0, p.a.ldx, rows.begin, rows.end, k, sh, [&](int g, float mean, float m2) {
             if (j > 0) {  // the same thread's moments of the tiles before
                 float ma = gm[g], sa = gr[g], fb, f;
                 join_weights(n * (float)(j * p.t.max_cols), n * (float)k.lw, &fb, &f);
@@ -247,23 +246,26 @@ __device__ __forceinline__ void whole_sample(const Forward<TX, TY>& p, int s, Sp
             }
             gm[g] = mean;
             gr[g] = m2;
-            if (j + 1 == p.t.tpg) finish(p, s, k.g0 + g, mean, m2, n * (float)p.t.width, true, gm + g, gr + g);
+            if (j + 1 == tpg) finish(p, s, k.g0 + g, mean, m2, n * (float)p.t.width, true, gm + g, gr + g);
         });
         team_sync<CTA>();
     }
-    for (int j = 0; j < p.t.tpg; ++j) {
+    for (int j = 0; j < tpg; ++j) {
         const Tile k = tile_of(p.t, t0 + j);
         const Team<CTA, V, U> tm(p.t, k.cols);
-        apply<CTA, false, apply_rows<TX, B>>(p, tm, rows.begin, rows.end, k, gm, gr);
+        apply<CTA, KEEP, false>(p, tm, slots, rows.begin, rows.end, k, gm, gr);
     }
     team_sync<CTA>();
 }
 
 // CTAs [0, chunks x tiles): moments of the long samples' chunks. The others: short and middle samples.
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 __global__ void __launch_bounds__(THREADS, CTAS) group_norm_kernel(const __grid_constant__ Forward<TX, TY> p) {
     __shared__ Strips sh;
     __shared__ float gm[WARPS][MAX_TILE], gr[WARPS][MAX_TILE];
+    extern __shared__ __align__(16) uint8_t slot_memory[];
+    const Slots<TX, V, U> slots{slot_memory};
+    constexpr int ROWS = SLOT_BYTES / Slots<TX, V, U>::BYTES;  // of a thread in the slots
     cudaGridDependencySynchronize();
     const int chunked = p.ch.count * p.t.tiles;
     if ((int)blockIdx.x < chunked) {
@@ -273,13 +275,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_kernel(const __grid_
         const Tile k = tile_of(p.t, tile);
         const Team<true, V, U> tm(p.t, k.cols);
         const int total = (int)p.a.rows, r0 = i * p.ch.rows, r1 = r0 + min(p.ch.rows, total - r0);
-        const int64_t slots = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
+        const int64_t parts = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
         for (int slot = 0; slot < 2; ++slot) {
             const int s = slot ? found.y : found.x;
             if (s < 0) continue;
             const Span sp = span_of(p.a.offsets, s, total);
-            float2* out = p.part + (slot * slots + part_slot(p.t, tile, k)) * p.ch.count + i;
-            group_moments<true, B>(tm, p.a.x + k.c0, p.a.ldx, max(r0, sp.begin), min(r1, sp.end), k, sh,
+            float2* out = p.part + (slot * parts + part_slot(p.t, tile, k)) * p.ch.count + i;
+            group_moments<true, false>(tm, slots, p.a.x + k.c0, p.a.ldx, max(r0, sp.begin), min(r1, sp.end), k, sh,
                                    [&](int g, float mean, float m2) { out[(int64_t)g * p.ch.count] = make_float2(mean, m2); });
             __syncthreads();
         }
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_kernel(const __grid_
             const Span sp = rows_of(s);
             const int n = sp.end - sp.begin;
             if (n == 0) empty(s);
-            else if (n <= p.warp_rows) whole_sample<false, B, TX, TY, V, U>(p, s, sp, block, sh, gm[warp], gr[warp]);
+            else if (n <= (ROWS << (5 - p.t.lpr_log))) whole_sample<false, true>(p, slots, s, sp, block, sh, gm[warp], gr[warp]);
         }
         __syncthreads();
     }
@@ -312,16 +314,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_kernel(const __grid_
         const Span sp = rows_of(s);
         const int n = sp.end - sp.begin;
         if (n == 0 && p.each == 1 && warp == 0) empty(s);
-        if (n > 0 && n <= p.ch.longest && (p.each == 1 || n > p.warp_rows))
-            whole_sample<true, B, TX, TY, V, U>(p, s, sp, block, sh, gm[0], gr[0]);
+        if (n == 0 || n > p.ch.longest || (p.each > 1 && n <= (ROWS << (5 - p.t.lpr_log)))) continue;
+        if (p.t.tpg == 1 && n <= (ROWS << (5 + WARPS_LOG - p.t.lpr_log)))
+            whole_sample<true, true>(p, slots, s, sp, block, sh, gm[0], gr[0]);
+        else whole_sample<true, false>(p, slots, s, sp, block, sh, gm[0], gr[0]);
     }
 }
 
 // y of the long samples' chunks. Every CTA joins the moments of its tile's groups over all of the sample's chunks, a
 // warp for a group, whose lanes take every 32nd.
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const __grid_constant__ Forward<TX, TY> p) {
     __shared__ float gm[MAX_TILE], gr[MAX_TILE];
+    extern __shared__ __align__(16) uint8_t slot_memory[];
+    const Slots<TX, V, U> slots{slot_memory};
     cudaGridDependencySynchronize();
     const int i = p.ch.count - 1 - blockIdx.x / p.t.tiles, tile = blockIdx.x % p.t.tiles;
     const int2 found = p.found[i];
@@ -362,16 +368,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const _
             if (lane == 0) finish(p, s, k.g0 + g, mean, m2, n, slot == 1 && (tpg == 1 || tile % tpg == 0), gm + g, gr + g);
         }
         __syncthreads();
-        apply<true, true, apply_rows<TX, B>>(p, tm, max(r0, sp.begin), min(r1, sp.end), k, gm, gr);
+        apply<true, false, true>(p, tm, slots, max(r0, sp.begin), min(r1, sp.end), k, gm, gr);
     }
 }
 
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 void forward(Handle& h, Forward<TX, TY>& p) {
     const Cut cut = make_cut(p.a, p.t, (int)sizeof(TX), sm_count(h.device), CTAS);
     p.ch = cut.ch;
     p.each = cut.by_warp ? WARPS : 1;
-    p.warp_rows = cut.warp_rows;
     DevBuf<float2> part((size_t)p.ch.count * 2 * part_slots(p.t), h.stream);
     DevBuf<int2> found((size_t)p.ch.count, h.stream);
     p.part = part.get();
@@ -379,10 +384,11 @@ void forward(Handle& h, Forward<TX, TY>& p) {
     const int64_t chunked = (int64_t)p.ch.count * p.t.tiles;
     const int64_t grid = chunked + (cut.only_long ? 0 : ceil_div(p.a.samples, p.each) * p.t.blocks);
     XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "too many samples and groups");
-    launch_dependent(h.stream, group_norm_kernel<TX, TY, V, U, B>, (unsigned)grid, THREADS, 0, 1, p);
+    allow_smem(group_norm_kernel<TX, TY, V, U>, SLOT_BYTES * THREADS);
+    launch_dependent(h.stream, group_norm_kernel<TX, TY, V, U>, (unsigned)grid, THREADS, SLOT_BYTES * THREADS, 1, p);
     after_launch(h, "group_norm");
     if (p.ch.count == 0) return;
-    launch_dependent(h.stream, group_norm_apply_kernel<TX, TY, V, U, B>, (unsigned)chunked, THREADS, 0, 1, p);
+    launch_dependent(h.stream, group_norm_apply_kernel<TX, TY, V, U>, (unsigned)chunked, THREADS, RING_BYTES * THREADS, 1, p);
     after_launch(h, "group_norm_apply");
 }
 
@@ -401,9 +407,9 @@ void group_norm(Handle& h, const GroupNormArgs<TX>& a, float eps, TY* y, int64_t
     const size_t bx = PER * sizeof(TX), by = PER * sizeof(TY);
     const bool wide = a.C % PER == 0 && (a.rows <= 1 || (a.ldx % PER == 0 && ldy % PER == 0)) && aligned_to(a.x, bx) &&
                       aligned_to(y, by);
-    if (wide && make_tiling(p.t, a, PER, 1, sm_count(h.device))) return forward<TX, TY, PER, 1, 4>(h, p);
+    if (wide && make_tiling(p.t, a, PER, 1, sm_count(h.device))) return forward<TX, TY, PER, 1>(h, p);
     make_tiling(p.t, a, 1, PER, sm_count(h.device));
-    forward<TX, TY, 1, PER, 2>(h, p);
+    forward<TX, TY, 1, PER>(h, p);
 }
 
 #define XS_INST_GROUP_NORM(TX, TY) \

@@ -15,7 +15,9 @@ namespace {
 
 using namespace group;
 
-constexpr int CTAS = 4;  // that an SM should hold: 128 registers a thread
+constexpr int CTAS = 3;  // that an SM should hold: 80 registers a thread and
+constexpr int SLOT_BYTES = 192;  // of shared memory a thread for rows of x and dy
+constexpr int RING = 2;  // batches in flight of rows that only pass
 
 template <typename TX, typename TY>
 struct Backward {
@@ -24,7 +26,7 @@ struct Backward {
     Chunks ch;
     int walkers;        // CTAs a block that walk over samples, 0 where all samples are long
     int each;           // neighbouring samples that one of them takes
-    int warp_rows;      // most rows that a warp takes, 0: none
+    bool by_warp;       // short ones by a warp each
     const TY* dy;
     int64_t lddy;
     const float *mean, *rstd;
@@ -67,67 +69,73 @@ struct Totals {
     }
 };
 
+// A thread's slots for rows of both inputs.
+template <typename TX, typename TY, int V, int U>
+struct Pairs {
+    static constexpr int BYTES = Slots<TX, V, U>::BYTES + Slots<TY, V, U>::BYTES, ROWS = SLOT_BYTES / BYTES;
+    Slots<TX, V, U> x;
+    Slots<TY, V, U> g;
+    __device__ Pairs(uint8_t* memory) : x{memory}, g{memory + ROWS * THREADS * Slots<TX, V, U>::BYTES} {}
+};
+
+enum class Rows { Fill, Kept, Pass };  // to the slots and stay there; there already; through a ring
+
 // Calls f(row, dz, xh) for this thread's rows of [begin, end), counted from the first, or with BACK from the last.
-template <bool CTA, bool BACK, int B, typename TX, typename TY, int V, int U, typename F>
-__device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
-                                         int end, const Channels<V * U / 2>& ch, F&& f) {
+template <bool CTA, Rows HOW, bool BACK, typename TX, typename TY, int V, int U, typename F>
+__device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Pairs<TX, TY, V, U>& slots,
+                                         const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, F&& f) {
     constexpr int P = V * U / 2;
-    struct Batch {
-        Pack<TX, V> x[B][U];
-        Pack<TY, V> g[B][U];
-    };
     const int rows = tm.rows(end - begin);
     const int64_t last = BACK ? max(rows - 1, 0) : 0, step = BACK ? -tm.step : tm.step;
     const TX* px = tm.first(p.a.x + k.c0, begin, p.a.ldx) + last * tm.step * p.a.ldx;
     const TY* pg = tm.first(p.dy + k.c0, begin, p.lddy) + last * tm.step * p.lddy;
     const int64_t nx = step * p.a.ldx, ng = step * p.lddy;
-    batches<B, Batch>(
-        rows,
-        [&](auto full, Batch& t, int i, int n) {
-            const TX* rx = px + i * nx;
-            const TY* rg = pg + i * ng;
+    auto fill = [&](int slot, int i) {
+        slots.x.fill(slot, px + i * nx, tm.at);
+        slots.g.fill(slot, pg + i * ng, tm.at);
+    };
+    if constexpr (HOW == Rows::Fill) fill_all(rows, fill);
+    with_act(p.a.act, [&](auto act) {
+        constexpr Activation ACT = decltype(act)::value;
+        auto use = [&](auto full, int slot, int i, int n) {
 #pragma unroll
-            for (int j = 0; j < B; ++j)
-                if (full || i + j < n) {
-                    tm.at.load(t.x[j], rx + j * nx);
-                    tm.at.load(t.g[j], rg + j * ng);
+            for (int j = 0; j < BATCH; ++j) {
+                if (!full && i + j >= n) break;
+                Pack<TX, V> rx[U];
+                Pack<TY, V> rg[U];
+                slots.x.get(rx, slot + j);
+                slots.g.get(rg, slot + j);
+                float2 dz[P], xh[P];
+                Place<V, U>::values(rx, xh);
+                Place<V, U>::values(rg, dz);
+#pragma unroll
+                for (int e = 0; e < P; ++e) xh[e] = centred(xh[e], ch.m[e], ch.rs[e]);
+                if constexpr (ACT != Activation::None) {
+                    float2 z[P];
+#pragma unroll
+                    for (int e = 0; e < P; ++e) z[e] = affine(xh[e], ch.w[e], ch.b[e]);
+                    act_row<true, sizeof(TY) == 4, ACT>(z);
+#pragma unroll
+                    for (int e = 0; e < P; ++e) dz[e] = pair_mul(dz[e], z[e]);
                 }
-        },
-        [&](auto full, const Batch& t, int i, int n) {
-            with_act(p.a.act, [&](auto act) {
-                constexpr Activation ACT = decltype(act)::value;
-#pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    if (!full && i + j >= n) break;
-                    float2 dz[P], xh[P];
-                    Place<V, U>::values(t.x[j], xh);
-                    Place<V, U>::values(t.g[j], dz);
-#pragma unroll
-                    for (int e = 0; e < P; ++e) xh[e] = centred(xh[e], ch.m[e], ch.rs[e]);
-                    if constexpr (ACT != Activation::None) {
-                        float2 z[P];
-#pragma unroll
-                        for (int e = 0; e < P; ++e) z[e] = affine(xh[e], ch.w[e], ch.b[e]);
-                        act_row<true, sizeof(TY) == 4, ACT>(z);
-#pragma unroll
-                        for (int e = 0; e < P; ++e) dz[e] = pair_mul(dz[e], z[e]);
-                    }
-                    f(i + j, dz, xh);
-                }
-            });
-        });
+                f(i + j, dz, xh);
+            }
+        };
+        if constexpr (HOW == Rows::Pass) stream<Pairs<TX, TY, V, U>::ROWS >= 2 * BATCH ? RING : 1>(rows, fill, use);
+        else use_all(rows, use);
+    });
 }
 
 // This thread's A and B over rows [begin, end), added to `total`, and the groups' sums of w A and w B, which one thread
 // a group hands to f(group of the tile, sum, sum). channels(strips) is called between, once the tile's A and B are
 // there by channel. The strips may be written again after a team_sync.
-template <bool CTA, int B, typename TX, typename TY, int V, int U, typename F, typename C>
-__device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
-                                           int end, const Channels<V * U / 2>& ch, const Totals<V * U / 2>& total,
+template <bool CTA, Rows HOW, typename TX, typename TY, int V, int U, typename F, typename C>
+__device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm,
+                                           const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, const Totals<V * U / 2>& total,
                                            Strips& sh, F&& f, C&& channels) {
     constexpr int P = V * U / 2;
     Sums<P> s;
-    each_row<CTA, false, B>(p, tm, k, begin, end, ch, [&](int, const float2 (&dz)[P], const float2 (&xh)[P]) {
+    each_row<CTA, HOW, false>(p, tm, slots, k, begin, end, ch, [&](int, const float2 (&dz)[P], const float2 (&xh)[P]) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             s.a[e] = pair_add(s.a[e], dz[e]);
@@ -155,9 +163,9 @@ __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team
 }
 
 // dx of rows [begin, end) from the groups' minus m1 and minus m2.
-template <bool CTA, bool BACK, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Tile& k, int begin,
-                                      int end, const Channels<V * U / 2>& ch, const float* g1, const float* g2) {
+template <bool CTA, Rows HOW, bool BACK, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm,
+                                      const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, const float* g1, const float* g2) {
     constexpr int P = V * U / 2;
     float2 m1[P], m2[P];
     tm.of_groups(m1, g1, k);
@@ -165,7 +173,7 @@ __device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA,
     const int64_t last = BACK ? max(tm.rows(end - begin) - 1, 0) : 0;
     TY* out = tm.first(p.dx + k.c0, begin, p.lddx) + last * tm.step * p.lddx;
     const int64_t next = (BACK ? -tm.step : tm.step) * p.lddx;
-    each_row<CTA, BACK, B>(p, tm, k, begin, end, ch, [&](int i, const float2 (&dz)[P], const float2 (&xh)[P]) {
+    each_row<CTA, HOW, BACK>(p, tm, slots, k, begin, end, ch, [&](int i, const float2 (&dz)[P], const float2 (&xh)[P]) {
         float2 v[P];
 #pragma unroll
         for (int e = 0; e < P; ++e) v[e] = pair_mul(ch.rs[e], pair_fma(xh[e], m2[e], pair_fma(dz[e], ch.w[e], m1[e])));
@@ -201,23 +209,24 @@ __device__ __forceinline__ void leave_weights(const Backward<TX, TY>& p, int64_t
     }
 }
 
-// A sample by a team. `total` is the CTA's sums where a block is one tile; else they go to the CTA's row.
-template <bool CTA, int B, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int s, Span rows, int block, int64_t row,
+// A sample by a team. KEEP: it is one tile and fits the slots. `total` is the CTA's sums where a block is one tile; else
+// they go to the CTA's row.
+template <bool CTA, bool KEEP, typename TX, typename TY, int V, int U>
+__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, const Pairs<TX, TY, V, U>& slots, int s, Span rows, int block, int64_t row,
                                              Channels<V * U / 2>& ch, const Totals<V * U / 2>& total, Strips& sh, float* g1,
                                              float* g2) {
-    const int t0 = block * p.t.tpg;
-    const bool one = p.t.tpg == 1;
-    for (int j = 0; j < p.t.tpg; ++j) {
+    const int tpg = KEEP ? 1 : p.t.tpg, t0 = block * tpg;
+    const bool one = tpg == 1;
+    for (int j = 0; j < tpg; ++j) {
         const Tile k = tile_of(p.t, t0 + j);
         const Team<CTA, V, U> tm(p.t, k.cols);
         if (!one) parameters(p, tm, k, ch);
         if (one || j == 0) statistics(p, tm, k, s, ch);
         const float per = -1.0f / ((float)(rows.end - rows.begin) * (float)p.t.width);
-        group_sums<CTA, B>(p, tm, k, rows.begin, rows.end, ch, total, sh,
+        group_sums<CTA, KEEP ? Rows::Fill : Rows::Pass>(p, tm, slots, k, rows.begin, rows.end, ch, total, sh,
                            [&](int g, float s1, float s2) {
                                if (j > 0) s1 += g1[g], s2 += g2[g];  // the same thread's sums of the tiles before
-                               const bool last = j + 1 == p.t.tpg;
+                               const bool last = j + 1 == tpg;
                                g1[g] = last ? s1 * per : s1;
                                g2[g] = last ? s2 * per : s2;
                            },
@@ -231,21 +240,24 @@ __device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, int s, S
         team_sync<CTA>();
     }
     if (!p.dx) return;
-    for (int j = 0; j < p.t.tpg; ++j) {
+    for (int j = 0; j < tpg; ++j) {
         const Tile k = tile_of(p.t, t0 + j);
         const Team<CTA, V, U> tm(p.t, k.cols);
         if (!one) parameters(p, tm, k, ch);
-        apply<CTA, false, B>(p, tm, k, rows.begin, rows.end, ch, g1, g2);
+        apply<CTA, KEEP ? Rows::Kept : Rows::Pass, false>(p, tm, slots, k, rows.begin, rows.end, ch, g1, g2);
     }
     team_sync<CTA>();
 }
 
 // CTAs [0, chunks x tiles): sums of the long samples' chunks. The others: short and middle samples.
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_kernel(const __grid_constant__ Backward<TX, TY> p) {
     __shared__ Strips sh;
     __shared__ float g1[WARPS][MAX_TILE], g2[WARPS][MAX_TILE];
     __shared__ float2 totals[V * U][THREADS];
+    extern __shared__ __align__(16) uint8_t slot_memory[];
+    const Pairs<TX, TY, V, U> slots(slot_memory);
+    constexpr int ROWS = Pairs<TX, TY, V, U>::ROWS;
     cudaGridDependencySynchronize();
     const int chunked = p.ch.count * p.t.tiles, warp = threadIdx.x >> 5;
     Channels<V * U / 2> ch;
@@ -258,15 +270,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_kernel(const __
         const Tile k = tile_of(p.t, tile);
         const Team<true, V, U> tm(p.t, k.cols);
         const int all = (int)p.a.rows, r0 = i * p.ch.rows, r1 = r0 + min(p.ch.rows, all - r0);
-        const int64_t slots = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
+        const int64_t parts = p.t.tpg == 1 ? p.t.groups : p.t.tiles;
         parameters(p, tm, k, ch);
         for (int slot = 0; slot < 2; ++slot) {
             const int s = slot ? found.y : found.x;
             if (s < 0) continue;
             const Span sp = span_of(p.a.offsets, s, all);
-            float2* out = p.part + (slot * slots + part_slot(p.t, tile, k)) * p.ch.count + i;
+            float2* out = p.part + (slot * parts + part_slot(p.t, tile, k)) * p.ch.count + i;
             statistics(p, tm, k, s, ch);
-            group_sums<true, B>(p, tm, k, max(r0, sp.begin), min(r1, sp.end), ch, total, sh,
+            group_sums<true, Rows::Pass>(p, tm, slots, k, max(r0, sp.begin), min(r1, sp.end), ch, total, sh,
                                 [&](int g, float s1, float s2) { out[(int64_t)g * p.ch.count] = make_float2(s1, s2); },
                                 [](const float (&)[2][MAX_TILE]) {});
             __syncthreads();
@@ -287,27 +299,32 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_kernel(const __
     }
     auto rows_of = [&](int s) { return span_of(p.a.offsets, s, (int)p.a.rows); };
     const int s0 = walker * p.each, s1 = s0 + min(p.each, (int)p.a.samples - s0);
-    if (p.warp_rows > 0) {
+    const int warp_rows = p.by_warp ? ROWS << (5 - p.t.lpr_log) : 0;  // most that a warp takes
+    if (p.by_warp) {
         for (int s = s0 + warp; s < s1; s += WARPS) {
             const Span sp = rows_of(s);
-            if (sp.end > sp.begin && sp.end - sp.begin <= p.warp_rows)
-                whole_sample<false, B, TX, TY, V, U>(p, s, sp, block, walker, ch, total, sh, g1[warp], g2[warp]);
+            if (sp.end > sp.begin && sp.end - sp.begin <= warp_rows)
+                whole_sample<false, true>(p, slots, s, sp, block, walker, ch, total, sh, g1[warp], g2[warp]);
         }
         __syncthreads();
     }
     for (int s = s0; s < s1; ++s) {
         const Span sp = rows_of(s);
         const int n = sp.end - sp.begin;
-        if (n > p.warp_rows && n <= p.ch.longest)
-            whole_sample<true, B, TX, TY, V, U>(p, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
+        if (n <= warp_rows || n > p.ch.longest) continue;
+        if (one && n <= (ROWS << (5 + WARPS_LOG - p.t.lpr_log)))
+            whole_sample<true, true>(p, slots, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
+        else whole_sample<true, false>(p, slots, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
     }
     if (one && p.weights) leave_weights(p, walker, k, tm.at, total, sh);
 }
 
 // dx of the long samples' chunks. Every CTA joins the sums of its tile's groups over all of the sample's chunks.
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_apply_kernel(const __grid_constant__ Backward<TX, TY> p) {
     __shared__ float g1[MAX_TILE], g2[MAX_TILE];
+    extern __shared__ __align__(16) uint8_t slot_memory[];
+    const Pairs<TX, TY, V, U> slots(slot_memory);
     cudaGridDependencySynchronize();
     const int i = p.ch.count - 1 - blockIdx.x / p.t.tiles, tile = blockIdx.x % p.t.tiles;
     const int2 found = p.found[i];
@@ -340,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_apply_kernel(co
         }
         __syncthreads();
         statistics(p, tm, k, s, ch);
-        apply<true, true, B>(p, tm, k, max(r0, sp.begin), min(r1, sp.end), ch, g1, g2);
+        apply<true, Rows::Pass, true>(p, tm, slots, k, max(r0, sp.begin), min(r1, sp.end), ch, g1, g2);
     }
 }
 
@@ -362,12 +379,12 @@ __global__ void __launch_bounds__(1024) group_norm_weights_kernel(const float* p
     if (lane == 0 && blockIdx.x * 32ll + warp < C) out[blockIdx.x * 32ll + warp] = s;
 }
 
-template <typename TX, typename TY, int V, int U, int B>
+template <typename TX, typename TY, int V, int U>
 void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     const int sms = sm_count(h.device);
     const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), sms, CTAS);
     p.ch = cut.ch;
-    p.warp_rows = cut.by_warp ? cut.warp_rows : 0;
+    p.by_warp = cut.by_warp;
     // as many samples a CTA as make four waves of them
     const int64_t items = ceil_div(p.a.samples, cut.by_warp ? WARPS : 1);
     p.each = (int)std::max<int64_t>(1, items * p.t.blocks / (4 * CTAS * sms)) * (cut.by_warp ? WARPS : 1);
@@ -381,10 +398,12 @@ void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     p.weights = weights.get();
     const int64_t chunked = (int64_t)p.ch.count * p.t.tiles, grid = chunked + (int64_t)p.walkers * p.t.blocks;
     XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "too many samples and groups");
-    launch_dependent(h.stream, group_norm_grad_kernel<TX, TY, V, U, B>, (unsigned)grid, THREADS, 0, 1, p);
+    allow_smem(group_norm_grad_kernel<TX, TY, V, U>, SLOT_BYTES * THREADS);
+    launch_dependent(h.stream, group_norm_grad_kernel<TX, TY, V, U>, (unsigned)grid, THREADS, SLOT_BYTES * THREADS, 1, p);
     after_launch(h, "group_norm_grad");
     if (p.ch.count > 0 && p.dx) {
-        launch_dependent(h.stream, group_norm_grad_apply_kernel<TX, TY, V, U, B>, (unsigned)chunked, THREADS, 0, 1, p);
+        allow_smem(group_norm_grad_apply_kernel<TX, TY, V, U>, SLOT_BYTES * THREADS);
+        launch_dependent(h.stream, group_norm_grad_apply_kernel<TX, TY, V, U>, (unsigned)chunked, THREADS, SLOT_BYTES * THREADS, 1, p);
         after_launch(h, "group_norm_grad_apply");
     }
     if (p.weights) {
@@ -411,9 +430,9 @@ void group_norm_backward(Handle& h, const GroupNormArgs<TX>& a, const TY* dy, in
     const size_t bx = PER * sizeof(TX), by = PER * sizeof(TY);
     const bool wide = a.C % PER == 0 && (a.rows <= 1 || (a.ldx % PER == 0 && lddy % PER == 0 && (!dx || lddx % PER == 0))) &&
                       aligned_to(a.x, bx) && aligned_to(dy, by) && aligned_to(dx, by);
-    if (wide && make_tiling(p.t, a, PER, 1, sm_count(h.device))) return backward<TX, TY, PER, 1, sizeof(TX) == 2 ? 4 : 2>(h, p, dw, db);
+    if (wide && make_tiling(p.t, a, PER, 1, sm_count(h.device))) return backward<TX, TY, PER, 1>(h, p, dw, db);
     make_tiling(p.t, a, 1, PER, sm_count(h.device));
-    backward<TX, TY, 1, PER, 2>(h, p, dw, db);
+    backward<TX, TY, 1, PER>(h, p, dw, db);
 }
 
 #define XS_INST_GROUP_NORM_GRAD(TX, TY)                                                                          \
