@@ -21,9 +21,9 @@ namespace {
 
 using namespace group;
 
-constexpr int CTAS = 4;  // that an SM should hold: 64 registers a thread and
-constexpr int SLOT_BYTES = 152;  // of shared memory a thread for rows
-constexpr int RING_BYTES = 128;  // of them for rows that only pass
+constexpr int CTAS = 6;  // that an SM should hold: 80 registers a thread and
+constexpr int SLOT_BYTES = 224;  // of shared memory a thread for rows
+constexpr int RING_BYTES = 192;  // of them for rows that only pass
 
 template <typename TX, typename TY>
 struct Forward {
@@ -95,19 +95,18 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const S
     constexpr int P = V * U / 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = tm.rows(end - begin);
     Moments<P> m;
-    const TX* at = tm.first(x, begin, ldx);
-    const int64_t next = tm.step * ldx;
-    auto fill = [&](int slot, int i) { slots.fill(slot, at + i * next, tm.at); };
-    auto use = [&](auto full, int slot, int i, int n) {
+    auto from = tm.template walk<false>(x, begin, rows, ldx);
+    auto fill = [&](int slot) { slots.fill(slot, from.next(), tm.at); };
+    auto use = [&](auto full, int slot, int count) {
         Pack<TX, V> raw[BATCH][U];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            if (full || i + j < n) slots.get(raw[j], slot + j);
+            if (full || j < count) slots.get(raw[j], slot + j);
             else
 #pragma unroll
                 for (int u = 0; u < U; ++u) raw[j][u] = Pack<TX, V>{};
         }
-        add_rows<decltype(full)::value>(m, raw, n - i);
+        add_rows<decltype(full)::value>(m, raw, count);
     };
     if constexpr (KEEP) {
         fill_all(rows, fill);
@@ -188,30 +187,25 @@ __device__ __forceinline__ void apply(const Forward<TX, TY>& p, const Team<CTA, 
     tm.of_groups(m, gm, k);
     tm.of_groups(rs, gr, k);
     const int rows = tm.rows(end - begin);
-    const int64_t last = BACK ? max(rows - 1, 0) : 0;
-    const TX* from = tm.first(p.a.x + k.c0, begin, p.a.ldx) + last * tm.step * p.a.ldx;
-    TY* to = tm.first(p.y + k.c0, begin, p.ldy) + last * tm.step * p.ldy;
-    const int64_t fnext = (BACK ? -tm.step : tm.step) * p.a.ldx, tnext = (BACK ? -tm.step : tm.step) * p.ldy;
-    auto use = [&](auto act, auto full, int slot, int i, int n) {
-        TY* row = to + i * tnext;
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            if (!full && i + j >= n) break;
-            Pack<TX, V> raw[U];
-            slots.get(raw, slot + j);
-            float2 v[P];
-            Place<V, U>::values(raw, v);
-#pragma unroll
-            for (int e = 0; e < P; ++e) v[e] = affine(centred(v[e], m[e], rs[e]), w[e], b[e]);
-            act_row<false, sizeof(TY) == 4, decltype(act)::value>(v);
-            tm.at.store(row + j * tnext, v);
-        }
-    };
+    auto from = tm.template walk<BACK>(p.a.x + k.c0, begin, rows, p.a.ldx);
+    auto to = tm.template walk<BACK>(p.y + k.c0, begin, rows, p.ldy);
     with_act(p.a.act, [&](auto act) {
-        auto go = [&](auto full, int slot, int i, int n) { use(act, full, slot, i, n); };
-        if constexpr (KEPT) use_all(rows, go);
-        else stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(
-            rows, [&](int slot, int i) { slots.fill(slot, from + i * fnext, tm.at); }, go);
+        auto use = [&](auto full, int slot, int count) {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                if (!full && j >= count) break;
+                Pack<TX, V> raw[U];
+                slots.get(raw, slot + j);
+                float2 v[P];
+                Place<V, U>::values(raw, v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) v[e] = affine(centred(v[e], m[e], rs[e]), w[e], b[e]);
+                act_row<false, sizeof(TY) == 4, decltype(act)::value>(v);
+                tm.at.store(to.next(), v);
+            }
+        };
+        if constexpr (KEPT) use_all(rows, use);
+        else stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(rows, [&](int slot) { slots.fill(slot, from.next(), tm.at); }, use);
     });
 }
 

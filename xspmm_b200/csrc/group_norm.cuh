@@ -7,7 +7,7 @@
 namespace xspmm_b200 {
 namespace group {
 
-constexpr int WARPS_LOG = 3, WARPS = 1 << WARPS_LOG, THREADS = 32 * WARPS;
+constexpr int WARPS_LOG = 2, WARPS = 1 << WARPS_LOG, THREADS = 32 * WARPS;
 constexpr int PER = 4;         // channels a thread holds of a row
 constexpr int MAX_TILE = 32 * PER;  // channels of a column tile
 
@@ -183,6 +183,18 @@ __device__ __forceinline__ void team_sync() {
     else __syncwarp();
 }
 
+// A thread's rows in a matrix, walked in order: the next one's first channel and the step to the one after.
+template <typename T>
+struct Walk {
+    T* p;
+    int64_t step;
+    __device__ T* next() {
+        T* r = p;
+        p += step;
+        return r;
+    }
+};
+
 // A team's threads on a tile: thread t takes channels by t mod lpr and rows t / lpr, t / lpr + step, ...
 template <bool CTA, int V, int U>
 struct Team {
@@ -199,10 +211,11 @@ struct Team {
     }
     // This thread's number of rows among n; none where it has no channels.
     __device__ int rows(int n) const { return at.in(0) && rl < n ? (n - rl + step - 1) >> step_log : 0; }
-    // Where its first row and channel are, in a matrix whose row `begin` of the tile is at `p`.
-    template <typename T>
-    __device__ T* first(T* p, int64_t begin, int64_t ld) const {
-        return p + (begin + rl) * ld + at.lane * V;
+    // Its `rows` rows of a matrix whose tile is at `p` and whose rows count from `begin`; BACK: the last ones first.
+    template <bool BACK, typename T>
+    __device__ Walk<T> walk(T* p, int begin, int rows, int64_t ld) const {
+        const int64_t first = begin + rl + (BACK ? max(rows - 1, 0) * (int64_t)step : 0);
+        return {p + first * ld + at.lane * V, (BACK ? -step : step) * ld};
     }
     // The values of the tile's groups at this thread's channels.
     __device__ void of_groups(float2 (&v)[V * U / 2], const float* g, const Tile& k) const {
@@ -258,43 +271,43 @@ struct Slots {
     }
 };
 
-// All n rows to slots 0, 1, ...; fill(slot, row).
+// All n rows to slots 0, 1, ...; fill(slot) takes the next row.
 template <typename F>
 __device__ __forceinline__ void fill_all(int n, F&& fill) {
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) fill(i, i);
+    for (int i = 0; i < n; ++i) fill(i);
     copies_commit();
     copies_wait<0>();
 }
-// use(full, slot, i, n) for batches of rows already in slots 0, 1, ...; full (a constant) says that there are BATCH of
+// use(full, slot, count) for batches of rows already in slots 0, 1, ...; full (a constant) says that there are BATCH of
 // them, which are then one run of instructions without branches.
 template <typename F>
 __device__ __forceinline__ void use_all(int n, F&& use) {
     int i = 0;
-    for (; i + BATCH <= n; i += BATCH) use(std::true_type{}, i, i, n);
-    if (i < n) use(std::false_type{}, i, i, n);
+    for (; i + BATCH <= n; i += BATCH) use(std::true_type{}, i, BATCH);
+    if (i < n) use(std::false_type{}, i, n - i);
 }
 // The same of rows that pass through a ring of RING batches.
 template <int RING, typename F, typename G>
 __device__ __forceinline__ void stream(int n, F&& fill, G&& use) {
-    auto batch = [&](int slot, int i) {
-        if (i + BATCH <= n)
+    auto batch = [&](int slot, int left) {
+        if (left >= BATCH)
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) fill(slot + j, i + j);
+            for (int j = 0; j < BATCH; ++j) fill(slot + j);
         else
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
-                if (i + j < n) fill(slot + j, i + j);
+                if (j < left) fill(slot + j);
         copies_commit();  // a group a batch, empty past the last
     };
 #pragma unroll
-    for (int k = 0; k < RING; ++k) batch(k * BATCH, k * BATCH);
+    for (int k = 0; k < RING; ++k) batch(k * BATCH, n - k * BATCH);
     int slot = 0;
-    for (int i = 0; i < n; i += BATCH) {
+    for (int left = n; left > 0; left -= BATCH) {
         copies_wait<RING - 1>();
-        if (i + BATCH <= n) use(std::true_type{}, slot, i, n);
-        else use(std::false_type{}, slot, i, n);
-        batch(slot, i + RING * BATCH);
+        if (left >= BATCH) use(std::true_type{}, slot, BATCH);
+        else use(std::false_type{}, slot, left);
+        batch(slot, left - RING * BATCH);
         slot = slot == (RING - 1) * BATCH ? 0 : slot + BATCH;
     }
     copies_wait<0>();

@@ -15,9 +15,8 @@ namespace {
 
 using namespace group;
 
-constexpr int CTAS = 3;  // that an SM should hold: 80 registers a thread and
-constexpr int SLOT_BYTES = 192;  // of shared memory a thread for rows of x and dy
-constexpr int RING = 2;  // batches in flight of rows that only pass
+constexpr int CTAS = 4;  // that an SM should hold: 128 registers a thread and
+constexpr int SLOT_BYTES = 336;  // of shared memory a thread for rows of x and dy
 
 template <typename TX, typename TY>
 struct Backward {
@@ -72,7 +71,7 @@ struct Totals {
 // A thread's slots for rows of both inputs.
 template <typename TX, typename TY, int V, int U>
 struct Pairs {
-    static constexpr int BYTES = Slots<TX, V, U>::BYTES + Slots<TY, V, U>::BYTES, ROWS = SLOT_BYTES / BYTES;
+    static constexpr int BYTES = Slots<TX, V, U>::BYTES + Slots<TY, V, U>::BYTES, ROWS = SLOT_BYTES / BYTES, RING = ROWS / BATCH;
     Slots<TX, V, U> x;
     Slots<TY, V, U> g;
     __device__ Pairs(uint8_t* memory) : x{memory}, g{memory + ROWS * THREADS * Slots<TX, V, U>::BYTES} {}
@@ -80,27 +79,25 @@ struct Pairs {
 
 enum class Rows { Fill, Kept, Pass };  // to the slots and stay there; there already; through a ring
 
-// Calls f(row, dz, xh) for this thread's rows of [begin, end), counted from the first, or with BACK from the last.
+// Calls f(dz, xh) for this thread's rows of [begin, end) in order, or with BACK from the last.
 template <bool CTA, Rows HOW, bool BACK, typename TX, typename TY, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm, const Pairs<TX, TY, V, U>& slots,
                                          const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, F&& f) {
     constexpr int P = V * U / 2;
     const int rows = tm.rows(end - begin);
-    const int64_t last = BACK ? max(rows - 1, 0) : 0, step = BACK ? -tm.step : tm.step;
-    const TX* px = tm.first(p.a.x + k.c0, begin, p.a.ldx) + last * tm.step * p.a.ldx;
-    const TY* pg = tm.first(p.dy + k.c0, begin, p.lddy) + last * tm.step * p.lddy;
-    const int64_t nx = step * p.a.ldx, ng = step * p.lddy;
-    auto fill = [&](int slot, int i) {
-        slots.x.fill(slot, px + i * nx, tm.at);
-        slots.g.fill(slot, pg + i * ng, tm.at);
+    auto fx = tm.template walk<BACK>(p.a.x + k.c0, begin, rows, p.a.ldx);
+    auto fg = tm.template walk<BACK>(p.dy + k.c0, begin, rows, p.lddy);
+    auto fill = [&](int slot) {
+        slots.x.fill(slot, fx.next(), tm.at);
+        slots.g.fill(slot, fg.next(), tm.at);
     };
     if constexpr (HOW == Rows::Fill) fill_all(rows, fill);
     with_act(p.a.act, [&](auto act) {
         constexpr Activation ACT = decltype(act)::value;
-        auto use = [&](auto full, int slot, int i, int n) {
+        auto use = [&](auto full, int slot, int count) {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                if (!full && i + j >= n) break;
+                if (!full && j >= count) break;
                 Pack<TX, V> rx[U];
                 Pack<TY, V> rg[U];
                 slots.x.get(rx, slot + j);
@@ -118,10 +115,10 @@ __device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<C
 #pragma unroll
                     for (int e = 0; e < P; ++e) dz[e] = pair_mul(dz[e], z[e]);
                 }
-                f(i + j, dz, xh);
+                f(dz, xh);
             }
         };
-        if constexpr (HOW == Rows::Pass) stream<Pairs<TX, TY, V, U>::ROWS >= 2 * BATCH ? RING : 1>(rows, fill, use);
+        if constexpr (HOW == Rows::Pass) stream<Pairs<TX, TY, V, U>::RING>(rows, fill, use);
         else use_all(rows, use);
     });
 }
@@ -135,7 +132,7 @@ __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team
                                            Strips& sh, F&& f, C&& channels) {
     constexpr int P = V * U / 2;
     Sums<P> s;
-    each_row<CTA, HOW, false>(p, tm, slots, k, begin, end, ch, [&](int, const float2 (&dz)[P], const float2 (&xh)[P]) {
+    each_row<CTA, HOW, false>(p, tm, slots, k, begin, end, ch, [&](const float2 (&dz)[P], const float2 (&xh)[P]) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             s.a[e] = pair_add(s.a[e], dz[e]);
@@ -170,14 +167,12 @@ __device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA,
     float2 m1[P], m2[P];
     tm.of_groups(m1, g1, k);
     tm.of_groups(m2, g2, k);
-    const int64_t last = BACK ? max(tm.rows(end - begin) - 1, 0) : 0;
-    TY* out = tm.first(p.dx + k.c0, begin, p.lddx) + last * tm.step * p.lddx;
-    const int64_t next = (BACK ? -tm.step : tm.step) * p.lddx;
-    each_row<CTA, HOW, BACK>(p, tm, slots, k, begin, end, ch, [&](int i, const float2 (&dz)[P], const float2 (&xh)[P]) {
+    auto to = tm.template walk<BACK>(p.dx + k.c0, begin, tm.rows(end - begin), p.lddx);
+    each_row<CTA, HOW, BACK>(p, tm, slots, k, begin, end, ch, [&](const float2 (&dz)[P], const float2 (&xh)[P]) {
         float2 v[P];
 #pragma unroll
         for (int e = 0; e < P; ++e) v[e] = pair_mul(ch.rs[e], pair_fma(xh[e], m2[e], pair_fma(dz[e], ch.w[e], m1[e])));
-        tm.at.store(out + i * next, v);
+        tm.at.store(to.next(), v);
     });
 }
 
