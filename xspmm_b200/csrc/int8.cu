@@ -7,42 +7,86 @@
 namespace xspmm_b200 {
 namespace {
 
-constexpr int Q_THREADS = 256;
+constexpr int Q_THREADS = 256, Q_HELD = 16;  // elements of a row that a thread holds
 
 // 127 v / most rounded to the nearest, ties to even. inv = 127 / most in fp32 puts the quotient within 2^-22 of
 // itself, so only a product that close to a border can be on its wrong side; those are compared exactly in 64
 // bits (127 v has 31 bits, (2 q + 1) most has 32). inv is infinite for the smallest subnormal `most`: 64 bits.
+__device__ __noinline__ int quantized_exactly(float v, float most) { return (int)rint(127.0 * (double)v / (double)most); }
 __device__ __forceinline__ int quantized(float v, float most, float inv) {
     const float p = v * inv, q = rintf(p);
-    if (fabsf(fabsf(p - q) - 0.5f) > 1e-4f && fabsf(p) < 256.0f) return (int)q;
-    return (int)rint(127.0 * (double)v / (double)most);
+    if (__builtin_expect(fabsf(fabsf(p - q) - 0.5f) > 1e-4f && fabsf(p) < 256.0f, 1)) return (int)q;
+    return quantized_exactly(v, most);
 }
 
-// A CTA per row.
-template <typename T>
-__global__ void __launch_bounds__(Q_THREADS)
-quantize_kernel(int64_t cols, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq, float* scale) {
-    __shared__ float part[Q_THREADS / 32];
-    __shared__ int odd;
-    const int64_t r = blockIdx.x;
-    if (threadIdx.x == 0) odd = 0;
-    __syncthreads();
-    float most = 0.0f;
-    for (int64_t c = threadIdx.x; c < cols; c += Q_THREADS) {
-        const float v = fabsf(to_float(x[r * ldx + c]));
-        if (!(v < INFINITY)) odd = 1;
-        most = fmaxf(most, v);
+// The largest magnitude over a row's threads: part of a warp, or the CTA. As whole numbers, magnitudes compare as the
+// numbers do, infinity above all and NaN above that.
+__device__ __forceinline__ uint32_t row_most(uint32_t v, int tpr) {
+    __shared__ uint32_t part[Q_THREADS / 32];
+    if (tpr >= 32) {
+        v = __reduce_max_sync(0xffffffffu, v);
+    } else {
+        for (int o = tpr >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     }
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+    if (tpr <= 32) return v;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    most = part[0];
-    for (int i = 1; i < Q_THREADS / 32; ++i) most = fmaxf(most, part[i]);
-    const bool zero = odd || most == 0.0f;
-    const float inv = 127.0f / most;
-    for (int64_t c = threadIdx.x; c < cols; c += Q_THREADS)
-        q[r * ldq + c] = zero ? (int8_t)0 : (int8_t)quantized(to_float(x[r * ldx + c]), most, inv);
-    if (threadIdx.x == 0) scale[r] = odd ? NAN : most / 127.0f;
+    for (int i = 0; i < Q_THREADS / 32; ++i) v = max(v, part[i]);
+    return v;
+}
+
+// tpr threads a row, a power of two up to a warp or the whole CTA. A thread takes V consecutive elements at a time, up to
+// Q_HELD in registers (the loads of a row are all in flight together and x is read once); HELD = false: longer rows,
+// read again for the second pass. Bound by memory.
+template <typename T, int V, bool HELD>
+__global__ void __launch_bounds__(Q_THREADS)
+quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+                float* scale) {
+    constexpr int LOADS = Q_HELD / V;
+    cudaGridDependencySynchronize();
+    const int per = Q_THREADS / tpr, t = threadIdx.x & (tpr - 1);
+    const int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / tpr;
+    const bool live = r < rows;
+    const T* from = x + (live ? r : 0) * ldx;
+    int8_t* to = q + (live ? r : 0) * ldq;
+    Pack<T, V> raw[LOADS];
+    uint32_t most = 0;
+    auto look = [&](const Pack<T, V>& k) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) most = max(most, __float_as_uint(to_float(k.v[e])) & 0x7fffffffu);
+    };
+    if constexpr (HELD) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int c = (i * tpr + t) * V;
+            raw[i] = Pack<T, V>{};
+            if (live && c < cols) raw[i] = *reinterpret_cast<const Pack<T, V>*>(from + c);
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) look(raw[i]);
+    } else {
+#pragma unroll 4
+        for (int c = t * V; live && c < cols; c += tpr * V) look(*reinterpret_cast<const Pack<T, V>*>(from + c));
+    }
+    most = row_most(most, tpr);
+    const float top = __uint_as_float(most), inv = 127.0f / top;
+    const bool odd = most >= 0x7f800000u, none = odd || most == 0;
+    if (!live) return;
+    auto put = [&](const Pack<T, V>& k, int c) {
+        Pack<int8_t, V> out;
+#pragma unroll
+        for (int e = 0; e < V; ++e) out.v[e] = none ? (int8_t)0 : (int8_t)quantized(to_float(k.v[e]), top, inv);
+        *reinterpret_cast<Pack<int8_t, V>*>(to + c) = out;
+    };
+    if constexpr (HELD) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            if ((i * tpr + t) * V < cols) put(raw[i], (i * tpr + t) * V);
+    } else {
+#pragma unroll 4
+        for (int c = t * V; c < cols; c += tpr * V) put(*reinterpret_cast<const Pack<T, V>*>(from + c), c);
+    }
+    if (t == 0) scale[r] = odd ? __uint_as_float(0x7fc00000u) : top / 127.0f;
 }
 
 // 16 bytes from anywhere in a matrix (bytes [begin, end)): the two aligned 16-byte words that hold them, shifted
@@ -244,8 +288,21 @@ template <typename T>
 void quantize_rows(Handle& h, int64_t rows, int64_t cols, const T* x, int64_t ldx, int8_t* q, int64_t ldq,
                    float* scale) {
     if (rows == 0) return;
-    XS_REQUIRE(rows < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "rows pass 2^31");
-    quantize_kernel<T><<<(unsigned)rows, Q_THREADS, 0, h.stream>>>(cols, x, ldx, q, ldq, scale);
+    XS_REQUIRE(cols < INT32_MAX - 2 * Q_THREADS * Q_HELD, XSPMM_STATUS_UNSUPPORTED, "columns pass 2^31");
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = cols % V == 0 && aligned_to(x, 16) && aligned_to(q, V) && (rows == 1 || (ldx % V == 0 && ldq % V == 0));
+    const int64_t threads = ceil_div(cols, wide ? V : 1);  // that would have one load each
+    // enough threads to hold the row, more while their loads are few and the row is split in a warp for nothing
+    int tpr = 1;
+    while (tpr < Q_THREADS && tpr < threads && (tpr * (int64_t)Q_HELD < cols || (wide && tpr < 32 && tpr * 2 * V <= cols && rows < 4096)))
+        tpr *= 2;
+    if (tpr > 32) tpr = Q_THREADS;
+    const bool held = tpr * (int64_t)Q_HELD >= cols;
+    const int64_t grid = ceil_div(rows, Q_THREADS / tpr);
+    XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "rows pass 2^31");
+    auto kern = wide ? (held ? quantize_kernel<T, V, true> : quantize_kernel<T, V, false>)
+                     : (held ? quantize_kernel<T, 1, true> : quantize_kernel<T, 1, false>);
+    launch_dependent(h.stream, kern, (unsigned)grid, Q_THREADS, 0, 1, rows, (int)cols, tpr, x, ldx, q, ldq, scale);
     after_launch(h, "quantize_rows");
 }
 

@@ -76,6 +76,177 @@ scaled_kernel(int64_t rows, int64_t cols, const TX* g, int64_t ldg, const double
         y[i / cols * ldy + i % cols] = from_float<TY>((float)(to_float(g[i / cols * ldg + i % cols]) * inv));
 }
 
+// ---- small matrices: all steps in one CTA -----------------------------------------------------------
+// A side of at most 128 and another of at most 256: X (as a matrix of at most 128 rows, transposed if need be) and A
+// stay in shared memory in two parts, in the SWIZZLE_128B layout: 64-column chunks of 128 rows of 128 bytes. Read along
+// its rows a chunk is a K-major operand, along its columns an MN-major one, so X serves both products. A is replaced by
+// B' in place and X by its successor, each after the MMAs that read it. Bound by the latency of 3 products a step, their
+// MMAs on 1 of 148 SMs and the epilogues between (128 x 128, 5 steps: 17 launches of the large path took 107 us).
+constexpr int SMALL_THREADS = 512, SMALL_ROWS = 128, SMALL_COLS = 256;
+constexpr int SMALL_CHUNK = SMALL_ROWS * 128;
+
+__device__ __forceinline__ uint64_t small_desc_mn(uint32_t saddr) {  // 64-column chunks SMALL_CHUNK apart
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(SMALL_CHUNK >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Where 8 elements of row r from column c (a multiple of 8) on are.
+__device__ __forceinline__ int small_at(int r, int c) {
+    return (c >> 6) * SMALL_CHUNK + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4);
+}
+
+template <typename TX, typename TY>
+__global__ void __launch_bounds__(SMALL_THREADS, 1)
+small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, float eps, TY* y, int64_t ldy,
+                    uint32_t square, uint32_t wide, unsigned* err) {  // descriptors: 128 x 128, 128 x X's columns
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ double red[SMALL_THREADS / 32];
+    __shared__ uint64_t done;
+    __shared__ uint32_t tmem_slot;
+    const bool turned = rows > cols;
+    const int m = min(rows, cols), n = max(rows, cols), chunks = (n + 63) / 64;
+    uint8_t *xh = smem, *xl = xh + chunks * SMALL_CHUNK, *ah = xl + chunks * SMALL_CHUNK, *al = ah + 2 * SMALL_CHUNK;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc_all<1>(&tmem_slot);
+    cudaGridDependencySynchronize();
+    double s = 0.0;
+    for (int i = threadIdx.x; i < rows * cols; i += SMALL_THREADS) {
+        const int r = i / cols;
+        const double v = to_float(g[r * ldg + i - r * cols]);
+        s += v * v;
+    }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < SMALL_THREADS / 32; ++i) s += red[i];
+    const double inv = 1.0 / (sqrt(s) + (double)eps);
+    for (int i = threadIdx.x; i < SMALL_ROWS * chunks * 32; i += SMALL_THREADS) {  // two columns of X, zeros outside
+        const int r = i % SMALL_ROWS, c = i / SMALL_ROWS * 2;  // neighbouring threads: rows of X
+        float v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const bool in = r < m && c + e < n;
+            const int64_t from = turned ? (c + e) * ldg + r : r * ldg + c + e;
+            v[e] = in ? (float)(to_float(g[from]) * inv) * SPLIT_SCALE : 0.0f;
+        }
+        uint32_t hi, lo;
+        split2(v[0], v[1], &hi, &lo);
+        const int at = small_at(r, c & ~7) + (c & 7) * 2;
+        *reinterpret_cast<uint32_t*>(xh + at) = hi;
+        *reinterpret_cast<uint32_t*>(xl + at) = lo;
+    }
+    int phase = 0;
+    uint32_t tmem = 0;
+    // What was written to shared memory and read from TMEM before is done; `issue` runs in one thread, and its MMAs have
+    // finished on return.
+    auto products = [&](auto&& issue) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = tmem_slot;
+        if (threadIdx.x == 0) {
+            issue();
+            tc_commit(&done);
+        }
+        mbar_wait(&done, phase, err);
+        phase ^= 1;
+        __syncwarp();
+        tc_fence_after();
+    };
+    auto three = [&](uint64_t da, uint64_t la, uint64_t db, uint64_t lb, uint32_t idesc, bool more) {
+        tc_mma(tmem, da, db, idesc, more);
+        tc_mma(tmem + ACC_COLS, da, lb, idesc, more);
+        tc_mma(tmem + ACC_COLS, la, db, idesc, 1);
+    };
+    // f(row, first column, sums) for 32 columns at a time of the accumulators' `width`: four warps a quarter of the rows
+    auto results = [&](int width, auto&& f) {
+        for (int c = (warp >> 2) * 32; c < width; c += SMALL_THREADS / 128 * 32) {
+            uint32_t v[32], u[32];
+            const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c;
+            tmem_ld32(at, v);
+            tmem_ld32(at + ACC_COLS, u);
+            tmem_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(u[e]));
+            f((warp & 3) * 32 + lane, c, v);
+        }
+    };
+    auto put = [&](uint8_t* hi, uint8_t* lo, int r, int c, const float (&v)[8]) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], &h[e], &l[e]);
+        *reinterpret_cast<uint4*>(hi + small_at(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(lo + small_at(r, c)) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+    const int km = (m + 15) / 16, kn = (n + 15) / 16;  // MMAs that a sum over rows, or columns, of X takes
+    auto along = [](const uint8_t* p, int k) { return desc_k(smem_u32(p) + (k >> 2) * SMALL_CHUNK) + (k & 3) * 2; };
+    auto down = [](const uint8_t* p, int k) { return small_desc_mn(smem_u32(p)) + k * 128; };
+    for (int i = 0; i < steps; ++i) {
+        products([&] {  // A = X X^T
+            for (int k = 0; k < kn; ++k) three(along(xh, k), along(xl, k), along(xh, k), along(xl, k), square, k > 0);
+        });
+        results(SMALL_ROWS, [&](int r, int c, const uint32_t (&v)[32]) {
+#pragma unroll
+            for (int b = 0; b < 32; b += 8) {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Gram>(__uint_as_float(v[b + e]), 0.0f, false);
+                put(ah, al, r, c + b, t);
+            }
+        });
+        products([&] {  // A A
+            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), along(ah, k), along(al, k), square, k > 0);
+        });
+        results(SMALL_ROWS, [&](int r, int c, const uint32_t (&v)[32]) {
+#pragma unroll
+            for (int b = 0; b < 32; b += 8) {
+                const uint4 h = *reinterpret_cast<const uint4*>(ah + small_at(r, c + b));
+                const uint4 l = *reinterpret_cast<const uint4*>(al + small_at(r, c + b));
+                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 fh = unpack2(hw[e / 2], __half()), fl = unpack2(lw[e / 2], __half());
+                    t[e] = finish<Epi::Poly>(__uint_as_float(v[b + e]), fh.x + fl.x, r == c + b + e);
+                    t[e + 1] = finish<Epi::Poly>(__uint_as_float(v[b + e + 1]), fh.y + fl.y, r == c + b + e + 1);
+                }
+                put(ah, al, r, c + b, t);
+            }
+        });
+        products([&] {  // B' X
+            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), down(xh, k), down(xl, k), wide, k > 0);
+        });
+        results(chunks * 64, [&](int r, int c, const uint32_t (&v)[32]) {
+            if (i + 1 < steps) {
+#pragma unroll
+                for (int b = 0; b < 32; b += 8) {
+                    float t[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Next>(__uint_as_float(v[b + e]), 0.0f, false);
+                    put(xh, xl, r, c + b, t);
+                }
+            } else if (r < m) {
+                TY* to = turned ? y + c * ldy + r : y + r * ldy + c;
+                const int64_t next = turned ? ldy : 1;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (c + e < n) to[e * next] = from_float<TY>(__uint_as_float(v[e]) * (SPLIT_INV * SPLIT_INV));
+            }
+        });
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_free_all<1>(tmem_slot);
+}
+
 // A matrix in two parts, rows padded to whole 16-byte words.
 struct Parts {
     __half *hi, *lo;
@@ -124,6 +295,17 @@ void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t l
     if (rows == 0 || cols == 0) return;
     const int64_t limit = (int64_t(1) << 31) - 512;  // TMA coordinates are 32 bits
     XS_REQUIRE(rows < limit && cols < limit, XSPMM_STATUS_UNSUPPORTED, "a dimension of the update passes 2^31");
+    if (steps > 0 && std::min(rows, cols) <= SMALL_ROWS && std::max(rows, cols) <= SMALL_COLS) {
+        auto kern = small_update_kernel<TX, TY>;
+        allow_smem(kern);
+        const int chunks = (int)ceil_div(std::max(rows, cols), 64);
+        const size_t smem = 1024 + (size_t)(2 * chunks + 4) * SMALL_CHUNK;
+        launch_dependent(h.stream, kern, 1, SMALL_THREADS, smem, 1, (int)rows, (int)cols, g, ldg, steps, eps, y, ldy,
+                         make_idesc(false, false, false, SMALL_ROWS, SMALL_ROWS),
+                         make_idesc(false, false, true, SMALL_ROWS, chunks * 64), h.d_err);
+        after_launch(h, "update_small");
+        return;
+    }
     const int parts = (int)std::min<int64_t>(ceil_div(rows * cols, 4096), sm_count(h.device));
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * cols, 512), 8 * sm_count(h.device));
     DevBuf<double> part((size_t)parts, h.stream);
