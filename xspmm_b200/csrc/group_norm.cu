@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const _
 
 template <typename TX, typename TY, int V, int U>
 void forward(Handle& h, Forward<TX, TY>& p) {
-    const Cut cut = make_cut(p.a, p.t, (int)sizeof(TX), sm_count(h.device), CTAS);
+    const Cut cut = make_cut(p.a, p.t, (int)sizeof(TX), V > 1, sm_count(h.device), CTAS);
     p.ch = cut.ch;
     p.each = cut.by_warp ? WARPS : 1;
     DevBuf<float2> part((size_t)p.ch.count * 2 * part_slots(p.t), h.stream);

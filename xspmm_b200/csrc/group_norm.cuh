@@ -538,7 +538,8 @@ bool make_tiling(Tiling& t, const GroupNormArgs<TX>& a, int vec, int places, int
 }
 
 // Who takes which samples. Chunks: one for each CTA of a wave (per_sm an SM), at least 64 rows. `longest`: 512 KB of a
-// tile's columns, or a chunk. Samples of less than 4 KB of a tile on the average go to warps, up to 16 KB each: a CTA's
+// tile's columns but no more rows than a thread can take one after the other in about 20 us (which are fewer in
+// single elements), or a chunk. Samples of less than 4 KB of a tile on the average go to warps, up to 16 KB each: a CTA's
 // threads would have a row or two.
 struct Cut {
     Chunks ch;
@@ -546,10 +547,11 @@ struct Cut {
     bool only_long;  // all rows are one sample, and it is long
 };
 template <typename TX>
-Cut make_cut(const GroupNormArgs<TX>& a, const Tiling& t, int bytes, int sms, int per_sm) {
+Cut make_cut(const GroupNormArgs<TX>& a, const Tiling& t, int bytes, bool vector, int sms, int per_sm) {
     Cut c = {};
     const int64_t row = (int64_t)t.max_cols * bytes, share = std::max<int64_t>(64, ceil_div(a.rows * t.tiles, per_sm * sms));
-    c.ch.longest = (int)std::max(share, (512 << 10) / row);
+    const int64_t step = THREADS / t.lpr;  // rows that a CTA takes at a time
+    c.ch.longest = (int)std::max(share, std::min((512 << 10) / row, step * (vector ? 256 : 48)));
     if (a.rows > c.ch.longest) {
         c.ch.rows = (int)share;
         c.ch.count = (int)ceil_div(a.rows, share);

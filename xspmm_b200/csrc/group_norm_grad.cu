@@ -32,6 +32,7 @@ struct Backward {
     TY* dx;  // or null
     int64_t lddx;
     float* weights;  // [walker, then chunk][2][channel]: sums of dz * xh and dz, or null
+    float *dw, *db;  // not null: the only walker's, which leaves its sums there at once
     float2* part;    // Parts: sums of w A and w B
     int2* found;     // [chunk]: the long samples with rows in it
 };
@@ -191,16 +192,21 @@ __device__ __forceinline__ void statistics(const Backward<TX, TY>& p, const Team
     for (int e = 0; e < V * U / 2; ++e) ch.m[e] = make_float2(-ch.m[e].x, -ch.m[e].y);
 }
 
-// The CTA's sums of a tile's channels to row `row` of the weights' parts.
+// The CTA's sums of a tile's channels to row `row` of the weights' parts, or to their place.
 template <typename TX, typename TY, int V, int U>
 __device__ __forceinline__ void leave_weights(const Backward<TX, TY>& p, int64_t row, const Tile& k, const Place<V, U>& at,
                                               const Totals<V * U / 2>& total, Strips& sh) {
     Sums<V * U / 2> s = total.get();
     sum_channels<true>(s.a, s.b, at, sh);
-    if ((int)threadIdx.x < k.cols) {
-        float* out = p.weights + row * 2 * p.a.C + k.c0 + threadIdx.x;
+    if ((int)threadIdx.x >= k.cols) return;
+    const int c = k.c0 + threadIdx.x;
+    if (p.weights) {
+        float* out = p.weights + row * 2 * p.a.C + c;
         out[0] = sh.v[0][1][threadIdx.x];
         out[p.a.C] = sh.v[0][0][threadIdx.x];
+    } else {
+        if (p.dw) p.dw[c] = sh.v[0][1][threadIdx.x];
+        if (p.db) p.db[c] = sh.v[0][0][threadIdx.x];
     }
 }
 
@@ -311,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_kernel(const __
             whole_sample<true, true>(p, slots, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
         else whole_sample<true, false>(p, slots, s, sp, block, walker, ch, total, sh, g1[0], g2[0]);
     }
-    if (one && p.weights) leave_weights(p, walker, k, tm.at, total, sh);
+    if (one && (p.weights || p.dw || p.db)) leave_weights(p, walker, k, tm.at, total, sh);
 }
 
 // dx of the long samples' chunks. Every CTA joins the sums of its tile's groups over all of the sample's chunks.
@@ -377,7 +383,7 @@ __global__ void __launch_bounds__(1024) group_norm_weights_kernel(const float* p
 template <typename TX, typename TY, int V, int U>
 void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     const int sms = sm_count(h.device);
-    const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), sms, CTAS);
+    const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), V > 1, sms, CTAS);
     p.ch = cut.ch;
     p.by_warp = cut.by_warp;
     // as many samples a CTA as make four waves of them
@@ -387,7 +393,9 @@ void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     DevBuf<float2> part((size_t)p.ch.count * 2 * part_slots(p.t), h.stream);
     DevBuf<int2> found((size_t)p.ch.count, h.stream);
     const int rows = p.walkers + p.ch.count;
-    DevBuf<float> weights(dw || db ? (size_t)rows * 2 * p.a.C : 0, h.stream);
+    const bool direct = p.walkers == 1 && p.ch.count == 0 && p.t.tpg == 1;  // nothing to add up
+    DevBuf<float> weights((dw || db) && !direct ? (size_t)rows * 2 * p.a.C : 0, h.stream);
+    if (direct) p.dw = dw, p.db = db;
     p.part = part.get();
     p.found = found.get();
     p.weights = weights.get();

@@ -9,14 +9,41 @@ namespace {
 
 constexpr int Q_THREADS = 256, Q_HELD = 16;  // elements of a row that a thread holds
 
-// 127 v / most rounded to the nearest, ties to even. inv = 127 / most in fp32 puts the quotient within 2^-22 of
-// itself, so only a product that close to a border can be on its wrong side; those are compared exactly in 64
-// bits (127 v has 31 bits, (2 q + 1) most has 32). inv is infinite for the smallest subnormal `most`: 64 bits.
+// 127 v / most rounded to the nearest, ties to even, of V values. inv = 127 / most in fp32 puts the quotient within 2^-22
+// of itself, so only one that close to a border can be on its wrong side; where there is such a one, all are compared
+// exactly in 64 bits (127 v has 31 bits, (2 q + 1) most has 32). inv is infinite for the smallest subnormal `most`: 64
+// bits too. Adding 1.5 * 2^23 rounds to whole numbers and leaves them in the low bits.
 __device__ __noinline__ int quantized_exactly(float v, float most) { return (int)rint(127.0 * (double)v / (double)most); }
-__device__ __forceinline__ int quantized(float v, float most, float inv) {
-    const float p = v * inv, q = rintf(p);
-    if (__builtin_expect(fabsf(fabsf(p - q) - 0.5f) > 1e-4f && fabsf(p) < 256.0f, 1)) return (int)q;
-    return quantized_exactly(v, most);
+template <int V>
+__device__ __forceinline__ void quantized(Pack<int8_t, V>& out, const float (&v)[V], float most, float inv) {
+    constexpr float WHOLE = 12582912.0f;
+    bool clear = true;
+    uint32_t t[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float p = v[e] * inv, w = p + WHOLE;
+        clear = clear && fabsf(p - (w - WHOLE)) <= 0.4999f;
+        t[e] = __float_as_uint(w);
+    }
+    if (__builtin_expect(!clear, 0))
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) {
+            float one = v[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) one = j == e ? v[j] : one;
+            const uint32_t q = (uint32_t)quantized_exactly(one, most);
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[j] = j == e ? q : t[j];
+        }
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4)  // the low bytes
+            reinterpret_cast<uint32_t*>(&out)[e / 4] =
+                __byte_perm(__byte_perm(t[e], t[e + 1], 0x0040), __byte_perm(t[e + 2], t[e + 3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out.v[e] = (int8_t)(t[e] & 0xff);
+    }
 }
 
 // The largest magnitude over a row's threads: part of a warp, or the CTA. As whole numbers, magnitudes compare as the
@@ -31,20 +58,21 @@ __device__ __forceinline__ uint32_t row_most(uint32_t v, int tpr) {
     if (tpr <= 32) return v;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    for (int i = 0; i < Q_THREADS / 32; ++i) v = max(v, part[i]);
+    for (int i = 0; i < tpr / 32; ++i) v = max(v, part[i]);
     return v;
 }
 
-// tpr threads a row, a power of two up to a warp or the whole CTA. A thread takes V consecutive elements at a time, up to
-// Q_HELD in registers (the loads of a row are all in flight together and x is read once); HELD = false: longer rows,
-// read again for the second pass. Bound by memory.
+// tpr threads a row, a power of two: part of a warp, or a CTA of that many. A thread takes V consecutive elements at a
+// time, up to Q_HELD in registers (the loads of a row are all in flight together and x is read once); HELD = false:
+// longer rows, read again for the second pass. Bound by memory where rows start on 16 bytes (2^20 x 128 fp32: 153 us, 103
+// at the copy bandwidth); by the instructions of narrow loads and stores elsewhere.
 template <typename T, int V, bool HELD>
 __global__ void __launch_bounds__(Q_THREADS)
 quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
                 float* scale) {
     constexpr int LOADS = Q_HELD / V;
     cudaGridDependencySynchronize();
-    const int per = Q_THREADS / tpr, t = threadIdx.x & (tpr - 1);
+    const int per = blockDim.x / tpr, t = threadIdx.x & (tpr - 1);
     const int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / tpr;
     const bool live = r < rows;
     const T* from = x + (live ? r : 0) * ldx;
@@ -73,9 +101,12 @@ quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_
     const bool odd = most >= 0x7f800000u, none = odd || most == 0;
     if (!live) return;
     auto put = [&](const Pack<T, V>& k, int c) {
-        Pack<int8_t, V> out;
-#pragma unroll
-        for (int e = 0; e < V; ++e) out.v[e] = none ? (int8_t)0 : (int8_t)quantized(to_float(k.v[e]), top, inv);
+        Pack<int8_t, V> out = {};
+        if (!none) {
+            float v[V];
+            unpack<T, V>(k, v);
+            quantized<V>(out, v, top, inv);
+        }
         *reinterpret_cast<Pack<int8_t, V>*>(to + c) = out;
     };
     if constexpr (HELD) {
@@ -121,7 +152,7 @@ __device__ __forceinline__ uint4 load_bytes(const int8_t* src, int64_t valid, ui
 // straight to registers as the A operand of mma.sync m16n8k32 (16 features; the tokens are the 8 columns). The
 // sum's order is free, so a lane loads 32 contiguous bytes of a weight row (four lanes: a 128-byte line) and hands
 // them to four MMAs as if they were the k positions the fragment layout asks for; x is loaded in the same order.
-constexpr int FEW_WARPS = 4;
+constexpr int FEW_WARPS = 8;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -289,21 +320,26 @@ void quantize_rows(Handle& h, int64_t rows, int64_t cols, const T* x, int64_t ld
                    float* scale) {
     if (rows == 0) return;
     XS_REQUIRE(cols < INT32_MAX - 2 * Q_THREADS * Q_HELD, XSPMM_STATUS_UNSUPPORTED, "columns pass 2^31");
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = cols % V == 0 && aligned_to(x, 16) && aligned_to(q, V) && (rows == 1 || (ldx % V == 0 && ldq % V == 0));
-    const int64_t threads = ceil_div(cols, wide ? V : 1);  // that would have one load each
-    // enough threads to hold the row, more while their loads are few and the row is split in a warp for nothing
-    int tpr = 1;
-    while (tpr < Q_THREADS && tpr < threads && (tpr * (int64_t)Q_HELD < cols || (wide && tpr < 32 && tpr * 2 * V <= cols && rows < 4096)))
-        tpr *= 2;
-    if (tpr > 32) tpr = Q_THREADS;
-    const bool held = tpr * (int64_t)Q_HELD >= cols;
-    const int64_t grid = ceil_div(rows, Q_THREADS / tpr);
-    XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "rows pass 2^31");
-    auto kern = wide ? (held ? quantize_kernel<T, V, true> : quantize_kernel<T, V, false>)
-                     : (held ? quantize_kernel<T, 1, true> : quantize_kernel<T, 1, false>);
-    launch_dependent(h.stream, kern, (unsigned)grid, Q_THREADS, 0, 1, rows, (int)cols, tpr, x, ldx, q, ldq, scale);
-    after_launch(h, "quantize_rows");
+    auto launch = [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        // enough threads to hold the row; in a small call as many as a warp can use
+        int tpr = 1;
+        while (tpr < Q_THREADS && (tpr * (int64_t)Q_HELD < cols || (tpr < 32 && tpr * V < cols && rows < 4096))) tpr *= 2;
+        const int threads = tpr > 32 ? tpr : Q_THREADS;
+        const int64_t grid = ceil_div(rows, threads / tpr);
+        XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "rows pass 2^31");
+        auto kern = tpr * (int64_t)Q_HELD >= cols ? quantize_kernel<T, V, true> : quantize_kernel<T, V, false>;
+        launch_dependent(h.stream, kern, (unsigned)grid, threads, 0, 1, rows, (int)cols, tpr, x, ldx, q, ldq, scale);
+        after_launch(h, "quantize_rows");
+    };
+    // the widest loads that every row's start allows
+    auto fits = [&](int v) {
+        return cols % v == 0 && aligned_to(x, v * sizeof(T)) && aligned_to(q, v) && (rows == 1 || (ldx % v == 0 && ldq % v == 0));
+    };
+    constexpr int WIDE = 16 / sizeof(T);
+    if (fits(WIDE)) launch(std::integral_constant<int, WIDE>{});
+    else if (fits(WIDE / 2)) launch(std::integral_constant<int, WIDE / 2>{});
+    else launch(std::integral_constant<int, 1>{});
 }
 
 template <typename T>
