@@ -7,34 +7,31 @@
 namespace xspmm_b200 {
 namespace {
 
-constexpr int Q_THREADS = 256, Q_HELD = 16;  // elements of a row that a thread holds
+constexpr int Q_THREADS = 256;  // of a CTA of several rows
 
-// 127 v / most rounded to the nearest, ties to even, of V values. inv = 127 / most in fp32 puts the quotient within 2^-22
-// of itself, so only one that close to a border can be on its wrong side; where there is such a one, all are compared
-// exactly in 64 bits (127 v has 31 bits, (2 q + 1) most has 32). inv is infinite for the smallest subnormal `most`: 64
-// bits too. Adding 1.5 * 2^23 rounds to whole numbers and leaves them in the low bits.
-__device__ __noinline__ int quantized_exactly(float v, float most) { return (int)rint(127.0 * (double)v / (double)most); }
+// 127 v / most rounded to the nearest, ties to even, of V values. inv = 127 / most in fp32 puts the quotient p, at most
+// 127.0001, within 2^-23 of itself, 1.6e-5, so only one that close to a border can be on its wrong side; such ones (one of
+// 25000) are decided in 64 bits (127 v has 31 bits, (2 q + 1) most has 32). inv is infinite for the smallest subnormal
+// `most`: 64 bits too. Adding 1.5 * 2^23 rounds to whole numbers and leaves them in the low bits.
+__device__ __noinline__ uint32_t quantized_exactly(float v, float most) {
+    return (uint32_t)(int)rint(127.0 * (double)v / (double)most);
+}
 template <int V>
 __device__ __forceinline__ void quantized(Pack<int8_t, V>& out, const float (&v)[V], float most, float inv) {
     constexpr float WHOLE = 12582912.0f;
     bool clear = true;
     uint32_t t[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
+    auto off = [&](int e) {  // NaN where p is infinite
         const float p = v[e] * inv, w = p + WHOLE;
-        clear = clear && fabsf(p - (w - WHOLE)) <= 0.4999f;
         t[e] = __float_as_uint(w);
-    }
+        return fabsf(p - (w - WHOLE));
+    };
+#pragma unroll
+    for (int e = 0; e < V; ++e) clear = clear && off(e) <= 0.49998f;
     if (__builtin_expect(!clear, 0))
-#pragma unroll 1
-        for (int e = 0; e < V; ++e) {
-            float one = v[0];
 #pragma unroll
-            for (int j = 1; j < V; ++j) one = j == e ? v[j] : one;
-            const uint32_t q = (uint32_t)quantized_exactly(one, most);
-#pragma unroll
-            for (int j = 0; j < V; ++j) t[j] = j == e ? q : t[j];
-        }
+        for (int e = 0; e < V; ++e)
+            if (!(off(e) <= 0.49998f)) t[e] = quantized_exactly(v[e], most);
     if constexpr (V % 4 == 0) {
 #pragma unroll
         for (int e = 0; e < V; e += 4)  // the low bytes
@@ -49,7 +46,7 @@ __device__ __forceinline__ void quantized(Pack<int8_t, V>& out, const float (&v)
 // The largest magnitude over a row's threads: part of a warp, or the CTA. As whole numbers, magnitudes compare as the
 // numbers do, infinity above all and NaN above that.
 __device__ __forceinline__ uint32_t row_most(uint32_t v, int tpr) {
-    __shared__ uint32_t part[Q_THREADS / 32];
+    __shared__ uint32_t part[32];
     if (tpr >= 32) {
         v = __reduce_max_sync(0xffffffffu, v);
     } else {
@@ -63,17 +60,17 @@ __device__ __forceinline__ uint32_t row_most(uint32_t v, int tpr) {
 }
 
 // tpr threads a row, a power of two: part of a warp, or a CTA of that many. A thread takes V consecutive elements at a
-// time, up to Q_HELD in registers (the loads of a row are all in flight together and x is read once); HELD = false:
-// longer rows, read again for the second pass. Bound by memory where rows start on 16 bytes (2^20 x 128 fp32: 153 us, 103
+// time, HELD in registers (the loads of a row are all in flight together and x is read once; with 8 instead of 16 what a
+// thread does once a row weighs more: 2^20 x 128 fp16 203 us); HELD = 0: longer rows, read again for the second pass. Bound by memory where rows start on 16 bytes (2^20 x 128 fp32: 153 us, 103
 // at the copy bandwidth); by the instructions of narrow loads and stores elsewhere.
-template <typename T, int V, bool HELD>
-__global__ void __launch_bounds__(Q_THREADS)
-quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+template <typename T, int V, int HELD>
+__global__ void __launch_bounds__(HELD == 16 ? Q_THREADS : 512)
+quantize_kernel(int64_t rows, int cols, int tpr_log, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
                 float* scale) {
-    constexpr int LOADS = Q_HELD / V;
+    constexpr int LOADS = HELD > V ? HELD / V : 1;
     cudaGridDependencySynchronize();
-    const int per = blockDim.x / tpr, t = threadIdx.x & (tpr - 1);
-    const int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / tpr;
+    const int tpr = 1 << tpr_log, t = threadIdx.x & (tpr - 1);
+    const int64_t r = (int64_t)blockIdx.x * (blockDim.x >> tpr_log) + (threadIdx.x >> tpr_log);
     const bool live = r < rows;
     const T* from = x + (live ? r : 0) * ldx;
     int8_t* to = q + (live ? r : 0) * ldq;
@@ -83,7 +80,7 @@ quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_
 #pragma unroll
         for (int e = 0; e < V; ++e) most = max(most, __float_as_uint(to_float(k.v[e])) & 0x7fffffffu);
     };
-    if constexpr (HELD) {
+    if constexpr (HELD > 0) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int c = (i * tpr + t) * V;
@@ -109,7 +106,7 @@ quantize_kernel(int64_t rows, int cols, int tpr, const T* __restrict__ x, int64_
         }
         *reinterpret_cast<Pack<int8_t, V>*>(to + c) = out;
     };
-    if constexpr (HELD) {
+    if constexpr (HELD > 0) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             if ((i * tpr + t) * V < cols) put(raw[i], (i * tpr + t) * V);
@@ -319,17 +316,18 @@ template <typename T>
 void quantize_rows(Handle& h, int64_t rows, int64_t cols, const T* x, int64_t ldx, int8_t* q, int64_t ldq,
                    float* scale) {
     if (rows == 0) return;
-    XS_REQUIRE(cols < INT32_MAX - 2 * Q_THREADS * Q_HELD, XSPMM_STATUS_UNSUPPORTED, "columns pass 2^31");
+    XS_REQUIRE(cols < INT32_MAX - 65536, XSPMM_STATUS_UNSUPPORTED, "columns pass 2^31");
     auto launch = [&](auto vec) {
         constexpr int V = decltype(vec)::value;
+        const int held = cols <= 16 * Q_THREADS ? 16 : cols <= 32 * 512 ? 32 : 0;
         // enough threads to hold the row; in a small call as many as a warp can use
-        int tpr = 1;
-        while (tpr < Q_THREADS && (tpr * (int64_t)Q_HELD < cols || (tpr < 32 && tpr * V < cols && rows < 4096))) tpr *= 2;
-        const int threads = tpr > 32 ? tpr : Q_THREADS;
-        const int64_t grid = ceil_div(rows, threads / tpr);
+        int log = 0;
+        while (log < 9 && ((held ? (int64_t)held << log < cols : true) || (log < 5 && V << log < cols && rows < 4096))) ++log;
+        const int threads = log > 5 ? 1 << log : Q_THREADS;
+        const int64_t grid = ceil_div(rows, threads >> log);
         XS_REQUIRE(grid < INT32_MAX, XSPMM_STATUS_UNSUPPORTED, "rows pass 2^31");
-        auto kern = tpr * (int64_t)Q_HELD >= cols ? quantize_kernel<T, V, true> : quantize_kernel<T, V, false>;
-        launch_dependent(h.stream, kern, (unsigned)grid, threads, 0, 1, rows, (int)cols, tpr, x, ldx, q, ldq, scale);
+        auto kern = held == 16 ? quantize_kernel<T, V, 16> : held ? quantize_kernel<T, V, 32> : quantize_kernel<T, V, 0>;
+        launch_dependent(h.stream, kern, (unsigned)grid, threads, 0, 1, rows, (int)cols, log, x, ldx, q, ldq, scale);
         after_launch(h, "quantize_rows");
     };
     // the widest loads that every row's start allows
