@@ -16,16 +16,30 @@ namespace {
 
 using namespace product;
 
-// Sum of squares in fp64: one partial per CTA, added in order by the next kernel.
-template <typename T>
+// A matrix is walked in pieces of PIECE columns of a row, one a warp, V elements a lane at a time: f(row, first column).
+constexpr int PIECE = 1024;
+template <int V, typename F>
+__device__ __forceinline__ void each_piece(int64_t rows, int64_t cols, F&& f) {
+    const int64_t per = (cols + PIECE - 1) / PIECE, warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < rows * per; i += warps) {
+        const int64_t r = i / per, c0 = (i - r * per) * PIECE, end = min(cols, c0 + PIECE);
+#pragma unroll 4
+        for (int64_t c = c0 + (threadIdx.x & 31) * V; c < end; c += 32 * V) f(r, c);
+    }
+}
+
+// Sum of squares in fp64: one partial per CTA, added in a fixed order by the next kernel.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) squares_kernel(int64_t rows, int64_t cols, const T* g, int64_t ldg, double* part) {
     __shared__ double red[8];
     cudaGridDependencySynchronize();
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256) {
-        const double v = to_float(g[i / cols * ldg + i % cols]);
-        s += v * v;
-    }
+    each_piece<V>(rows, cols, [&](int64_t r, int64_t c) {
+        float v[V];
+        load_pack<T, V>(g + r * ldg + c, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += (double)v[e] * (double)v[e];
+    });
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
     __syncthreads();
@@ -35,34 +49,44 @@ __global__ void __launch_bounds__(256) squares_kernel(int64_t rows, int64_t cols
     }
 }
 
-// The inverse of the norm, from the partial sums in their order; the same in all threads.
+// The inverse of the norm, from the partial sums; the same in all threads of the CTA and in all CTAs.
 __device__ __forceinline__ double inverse_norm(const double* part, int parts, float eps) {
     __shared__ double inv;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 32) {
         double s = 0.0;
-        for (int i = 0; i < parts; ++i) s += part[i];
-        inv = 1.0 / (sqrt(s) + (double)eps);
+        for (int i = threadIdx.x; i < parts; i += 32) s += part[i];
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x == 0) inv = 1.0 / (sqrt(s) + (double)eps);
     }
     __syncthreads();
     return inv;
 }
 
 // X_0 in two parts; the padding of its rows becomes zeros.
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 start_kernel(int64_t rows, int64_t cols, const T* g, int64_t ldg, const double* part, int parts, float eps, __half* hi,
              __half* lo, int64_t ld) {
     cudaGridDependencySynchronize();
     const double inv = inverse_norm(part, parts, eps);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * (ld / 2); i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / (ld / 2), c = (i - r * (ld / 2)) * 2;
-        const float v0 = c < cols ? (float)(to_float(g[r * ldg + c]) * inv) * SPLIT_SCALE : 0.0f;
-        const float v1 = c + 1 < cols ? (float)(to_float(g[r * ldg + c + 1]) * inv) * SPLIT_SCALE : 0.0f;
-        uint32_t h, l;
-        split2(v0, v1, &h, &l);
-        *reinterpret_cast<uint32_t*>(hi + r * ld + c) = h;
-        *reinterpret_cast<uint32_t*>(lo + r * ld + c) = l;
-    }
+    each_piece<4>(rows, ld, [&](int64_t r, int64_t c) {
+        float v[4] = {};
+        const T* from = g + r * ldg + c;
+        if constexpr (V == 4) {
+            if (c < cols) load_pack<T, 4>(from, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) v[e] = to_float(from[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)(v[e] * inv) * SPLIT_SCALE;
+        uint2 h, l;
+        split2(v[0], v[1], &h.x, &l.x);
+        split2(v[2], v[3], &h.y, &l.y);
+        *reinterpret_cast<uint2*>(hi + r * ld + c) = h;
+        *reinterpret_cast<uint2*>(lo + r * ld + c) = l;
+    });
 }
 
 // y = X_0: no steps.
@@ -306,10 +330,12 @@ void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t l
         after_launch(h, "update_small");
         return;
     }
-    const int parts = (int)std::min<int64_t>(ceil_div(rows * cols, 4096), sm_count(h.device));
+    const int parts = (int)std::min<int64_t>(ceil_div(rows * ceil_div(cols, PIECE), 8), 8 * sm_count(h.device));
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * cols, 512), 8 * sm_count(h.device));
+    const bool wide = cols % 4 == 0 && aligned_to(g, 4 * sizeof(TX)) && (rows == 1 || ldg % 4 == 0);
     DevBuf<double> part((size_t)parts, h.stream);
-    launch_dependent(h.stream, squares_kernel<TX>, (unsigned)parts, 256, 0, 1, rows, cols, g, ldg, part.get());
+    launch_dependent(h.stream, wide ? squares_kernel<TX, 4> : squares_kernel<TX, 1>, (unsigned)parts, 256, 0, 1, rows, cols, g,
+                     ldg, part.get());
     after_launch(h, "update_squares");
     if (steps == 0) {
         launch_dependent(h.stream, scaled_kernel<TX, TY>, grid, 256, 0, 1, rows, cols, g, ldg, part.get(), parts, eps, y, ldy);
@@ -326,7 +352,8 @@ void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t l
         return p;
     };
     Parts X = take(rows, cols, ldx), next = take(rows, cols, ldx), A = take(m, m, lda), B = take(m, m, lda);
-    launch_dependent(h.stream, start_kernel<TX>, grid, 256, 0, 1, rows, cols, g, ldg, part.get(), parts, eps, X.hi, X.lo, ldx);
+    launch_dependent(h.stream, wide ? start_kernel<TX, 4> : start_kernel<TX, 1>, (unsigned)parts, 256, 0, 1, rows, cols, g, ldg,
+                     part.get(), parts, eps, X.hi, X.lo, ldx);
     after_launch(h, "update_start");
     for (int i = 0; i < steps; ++i) {
         if (tall) multiply<Epi::Gram, __half, true, true>(h, m, m, rows, X, X, &A);

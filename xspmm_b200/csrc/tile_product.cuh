@@ -402,62 +402,73 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
     if (warp == 2) tmem_free_all<CG>(tmem);
 }
 
-// Adds the slices of the split tiles and finishes them, as gated::join_kernel does: a CTA takes 4 rows x 32
-// columns, its eight warps every eighth slice, and the eight sums are added in order.
+// Adds the slices of the split tiles in their order and finishes them. A CTA takes 32 x 32 elements: summed with a row a
+// lane, as the slices lie (512 bytes a load), and through shared memory stored with a column a lane, and for the mirror
+// image with a row a lane. (Stored from the sums' own places, 2 bytes here and there, the joining of a 1341 x 1341 product
+// took 35 us, twice the product's time.)
 template <Epi E, typename T, int CG>
 __global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ Args p) {
-    __shared__ uint4 red[8][32];
+    __shared__ float tile[32][33];
     cudaGridDependencySynchronize();
     const int rest = tiles_of<E>(p) - p.whole, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int groups = (p.bn + 31) / 32;
+    const int groups = (p.bn + 31) / 32, slab = (int)(blockIdx.x % (TM / 32)), grp = (int)(blockIdx.x / (TM / 32) % groups);
+    const int part = (int)(blockIdx.x / (TM / 32) / groups), rank = part % CG;
     const int64_t slice = (int64_t)rest * CG * (ACC_COLS / 4) * TM;
-    const int slab = (int)(blockIdx.x % (TM / 4)), grp = (int)(blockIdx.x / (TM / 4) % groups);
-    const int part = (int)(blockIdx.x / (TM / 4) / groups), rank = part % CG;
     int mi, ni;
     place<E>(p, p.whole + part / CG, &mi, &ni);
-    const int r = slab * 4 + (lane & 3), c4 = grp * 8 + (lane >> 2);
-    const int64_t row = (int64_t)(mi * CG + rank) * TM + r, col = (int64_t)ni * p.bn + c4 * 4;
-    const bool in = row < p.M && col < p.N && c4 * 4 < p.bn;
-    const uint4* src = reinterpret_cast<const uint4*>(p.partial) + (int64_t)part * (ACC_COLS / 4) * TM + r;
-    auto add = [](uint4& s, uint4 v) {
-        auto one = [](uint32_t& a, uint32_t b) {
-            if constexpr (split(E)) a = __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-            else a += b;
-        };
-        one(s.x, v.x), one(s.y, v.y), one(s.z, v.z), one(s.w, v.w);
-    };
-    uint4 s = make_uint4(0, 0, 0, 0);
-    if (in)
+    const int64_t row0 = (int64_t)(mi * CG + rank) * TM + slab * 32, col0 = (int64_t)ni * p.bn + grp * 32;
+    const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
+    const int cols = (int)max((int64_t)0, min((int64_t)min(32, p.bn - grp * 32), p.N - col0));
+    if (rows == 0 || cols == 0) return;  // the same in all threads
+    if (warp * 4 < cols) {  // a row a lane, 4 columns a warp
+        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + ((int64_t)part * (ACC_COLS / 4) + grp * 8 + warp) * TM +
+                           slab * 32 + lane;
+        uint4 s = src[0];
 #pragma unroll 4
-        for (int i = warp; i < p.splits; i += 8) add(s, src[(int64_t)c4 * TM + i * slice]);
-    red[warp][lane] = s;
+        for (int i = 1; i < p.splits; ++i) {
+            const uint4 v = src[i * slice];
+            auto one = [](uint32_t& a, uint32_t b) {
+                if constexpr (split(E)) a = __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+                else a += b;
+            };
+            one(s.x, v.x), one(s.y, v.y), one(s.z, v.z), one(s.w, v.w);
+        }
+        const uint32_t v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[lane][warp * 4 + e] = split(E) ? __uint_as_float(v[e]) : (float)(int)v[e];
+    }
     __syncthreads();
-    if (warp > 0 || !in) return;
+    const int64_t col = col0 + lane;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) add(s, red[i][lane]);
-    const uint32_t v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (col + e >= p.N) break;
+    for (int i = 0; i < 4; ++i) {
+        const int r = warp * 4 + i;
+        const int64_t row = row0 + r;
+        if (r >= rows || lane >= cols) continue;
+        const float v = tile[r][lane];
         if constexpr (E == Epi::Int8) {
-            const float f = fmaf((float)(int)v[e] * p.xs[row], p.ws[col + e], p.bias ? p.bias[col + e] : 0.0f);
-            static_cast<T*>(p.out[0])[row * p.ld[0] + col + e] = from_float<T>(f);
+            static_cast<T*>(p.out[0])[row * p.ld[0] + col] =
+                from_float<T>(fmaf(v * p.xs[row], p.ws[col], p.bias ? p.bias[col] : 0.0f));
         } else if constexpr (E == Epi::Last) {
-            static_cast<T*>(p.out[0])[row * p.ld[0] + col + e] =
-                from_float<T>(__uint_as_float(v[e]) * (SPLIT_INV * SPLIT_INV));
+            static_cast<T*>(p.out[0])[row * p.ld[0] + col] = from_float<T>(v * (SPLIT_INV * SPLIT_INV));
         } else {
             float a = 0.0f;
-            if constexpr (E == Epi::Poly)
-                a = to_float(p.ah[row * p.lda + col + e]) + to_float(p.al[row * p.lda + col + e]);
-            const float f = finish<E>(__uint_as_float(v[e]), a, row == col + e);
-            const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
-            __half *oh = static_cast<__half*>(p.out[0]), *ol = static_cast<__half*>(p.out[1]);
-            oh[row * p.ld[0] + col + e] = hi;
-            ol[row * p.ld[1] + col + e] = lo;
-            if (symmetric(E) && mi != ni && col + e < p.M) {
-                oh[(col + e) * p.ld[0] + row] = hi;
-                ol[(col + e) * p.ld[1] + row] = lo;
-            }
+            if constexpr (E == Epi::Poly) a = to_float(p.ah[row * p.lda + col]) + to_float(p.al[row * p.lda + col]);
+            const float f = finish<E>(v, a, row == col);
+            const __half hi = __float2half_rn(f);
+            static_cast<__half*>(p.out[0])[row * p.ld[0] + col] = hi;
+            static_cast<__half*>(p.out[1])[row * p.ld[1] + col] = __float2half_rn(f - __half2float(hi));
+            if constexpr (symmetric(E)) tile[r][lane] = f;
+        }
+    }
+    if constexpr (symmetric(E)) {
+        if (mi == ni) return;  // the same in all threads
+        __syncthreads();
+        for (int c = warp; c < cols && col0 + c < p.M; c += 8) {  // without the padding
+            if (lane >= rows) continue;
+            const float f = tile[lane][c];
+            const __half hi = __float2half_rn(f);
+            static_cast<__half*>(p.out[0])[(col0 + c) * p.ld[0] + row0 + lane] = hi;
+            static_cast<__half*>(p.out[1])[(col0 + c) * p.ld[1] + row0 + lane] = __float2half_rn(f - __half2float(hi));
         }
     }
 }
@@ -529,7 +540,7 @@ void launch(Handle& h, Args& t) {
     launch_dependent(h.stream, kern, grid, THREADS, smem, CG, t);
     after_launch(h, "tile_product");
     if (rest > 0) {
-        const int64_t blocks = rest * CG * ((t.bn + 31) / 32) * (TM / 4);
+        const int64_t blocks = rest * CG * ((t.bn + 31) / 32) * (TM / 32);
         launch_dependent(h.stream, tile_join_kernel<E, T, CG>, (unsigned)blocks, 256, 0, 1, t);
         after_launch(h, "tile_join");
     }
