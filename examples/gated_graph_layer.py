@@ -5,9 +5,11 @@
 A is the graph (rows normalised by degree) as a plan for the sparse product, whose fp32 output the layer
 norm turns into the 16-bit operand of the projections; the backward pass ends in the 16-bit operand of
 the transposed product. The loss is the mean squared distance to a target; the weights take one step of
-gradient descent, and the loss before and after is printed.
+gradient descent, or with --update orthogonal the projections take the orthogonalised update of their momentum,
+and the loss before and after is printed.
 
     python examples/gated_graph_layer.py [--nodes-log2 14] [--steps 5] [--dtype fp16|bf16]
+                                         [--update descent|orthogonal]
 """
 import argparse
 import os
@@ -56,6 +58,7 @@ class GatedGraphLayer:
         self.dh, self.dn, self.dagg, self.dx = buf(), buf(), buf(), buf(torch.float32)
         self.dwg, self.dwu = torch.empty_like(self.wg), torch.empty_like(self.wu)
         self.dnw, self.dnb = torch.empty_like(self.norm_w), torch.empty_like(self.norm_b)
+        self.momentum = None
 
     def forward(self, x):
         ex = self.ex
@@ -77,6 +80,19 @@ class GatedGraphLayer:
         self.graph_t.execute(self.dagg, self.dx, self.width)
         return self.dx
 
+    def orthogonal_step(self, lr, momentum=0.95):
+        """The projections move by the orthogonalised momentum (fp32) of their gradients, the norm's
+        parameters by gradient descent of the same rate."""
+        if self.momentum is None:
+            self.momentum = [torch.zeros_like(w, dtype=torch.float32) for w in (self.wg, self.wu)]
+            self.update = torch.empty_like(self.wg)
+        for w, d, m in zip((self.wg, self.wu), (self.dwg, self.dwu), self.momentum):
+            m.mul_(momentum).add_(d)
+            xs.orthogonalize(self.ex, m, self.update)
+            w.sub_(self.update, alpha=lr)
+        for w, d in ((self.norm_w, self.dnw), (self.norm_b, self.dnb)):
+            w.sub_(d, alpha=lr)
+
     def step(self, lr):
         for w, d in ((self.wg, self.dwg), (self.wu, self.dwu), (self.norm_w, self.dnw), (self.norm_b, self.dnb)):
             w.sub_(d, alpha=lr)
@@ -88,6 +104,7 @@ def main(argv=None):
     ap.add_argument("--width", type=int, default=128)
     ap.add_argument("--steps", type=int, default=5)
     ap.add_argument("--dtype", choices=("fp16", "bf16"), default="bf16")
+    ap.add_argument("--update", choices=("descent", "orthogonal"), default="descent")
     a = ap.parse_args(argv)
     dtype = {"fp16": torch.float16, "bf16": torch.bfloat16}[a.dtype]
     ex = xs.CudaExecutor(0)
@@ -104,7 +121,10 @@ def main(argv=None):
         # the mean's gradient, scaled up by `scale` so that it does not vanish in fp16
         scale = 1024.0 * a.width
         layer.backward((diff * (2.0 / diff.numel() * scale)).to(dtype))
-        layer.step(lr=0.05 * a.width / scale)
+        if a.update == "orthogonal":
+            layer.orthogonal_step(lr=0.01)
+        else:
+            layer.step(lr=0.05 * a.width / scale)
     print(f"nodes={P.M} nnz={P.nnz} width={a.width} loss " + " ".join(f"{v:.6f}" for v in losses))
     return losses
 

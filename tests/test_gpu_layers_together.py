@@ -1,0 +1,171 @@
+"""GPU tests of the layer operators as they are used together: a training step of a norm over the graphs of a batch,
+gated projections and their orthogonalised update, and the same layer served in 8 bits; calls from several threads at
+once; a call on tensors that another device's context is not current for; long offsets.
+
+The run's tolerance is that of its 16-bit roundings: an intermediate is off by U = 2^-11 (fp16) of itself, a sum of n
+products of two rounded factors by 2 U sqrt(n) of its terms' root mean square sum where the roundings are independent;
+the bounds below take 8 times that.
+"""
+import os
+import subprocess
+import sys
+import threading
+
+import pytest
+import torch
+
+import xspmm_b200 as xs
+
+pytestmark = pytest.mark.gpu
+
+f16, bf16, f32 = torch.float16, torch.bfloat16, torch.float32
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def rand(seed, *shape, dtype=f32, scale=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def near(got, ref, rel):
+    ref = ref.double()
+    off = torch.linalg.vector_norm(got.double() - ref).item()
+    assert off <= rel * torch.linalg.vector_norm(ref).item(), off / torch.linalg.vector_norm(ref).item()
+
+
+def norm64(x, off, groups, w, b, eps):
+    parts = []
+    for lo, hi in zip(off[:-1], off[1:]):
+        v = x[lo:hi].double().reshape(hi - lo, groups, x.shape[1] // groups)
+        if hi > lo:
+            m = v.mean((0, 2), keepdim=True)
+            v = (v - m) / torch.sqrt(((v - m) ** 2).mean((0, 2), keepdim=True) + eps)
+        parts.append(v.reshape(hi - lo, x.shape[1]))
+    return torch.cat(parts) * w.double() + b.double()
+
+
+@pytest.mark.parametrize("rows,cols,inner,groups", [(700, 128, 160, 8), (333, 90, 77, 9)])
+def test_training_step(executor, rows, cols, inner, groups):
+    """group norm with silu -> gated projections, back through both, and the weights' orthogonalised updates."""
+    U = 2.0 ** -11
+    off = [0, 100, 100, 101, rows]
+    dev = torch.tensor(off, device="cuda")
+    x, dy = rand(1, rows, cols), rand(2, rows, inner, dtype=f16)
+    w, b = 1.0 + rand(3, cols, scale=0.2), rand(4, cols, scale=0.1)
+    wg, wu = rand(5, inner, cols, dtype=f16, scale=cols ** -0.5), rand(6, inner, cols, dtype=f16, scale=cols ** -0.5)
+    n, y = torch.empty(rows, cols, dtype=f16, device="cuda"), torch.empty(rows, inner, dtype=f16, device="cuda")
+    gate, up, dn = torch.empty_like(y), torch.empty_like(y), torch.empty_like(n)
+    mean, rstd = torch.empty(4, groups, device="cuda"), torch.empty(4, groups, device="cuda")
+    dwg, dwu, dx = torch.empty_like(wg), torch.empty_like(wu), torch.empty_like(n)
+    dw, db, step = torch.empty_like(w), torch.empty_like(b), torch.empty_like(wg)
+    xs.group_norm(executor, x, groups, w, b, 1e-5, n, offsets=dev, activation="silu", mean=mean, rstd=rstd)
+    xs.gated_ffn(executor, n, wg, wu, y, "silu", gate, up)
+    xs.gated_ffn_backward(executor, dy, n, wg, wu, gate, up, dn, dwg, dwu)
+    xs.group_norm_backward(executor, dn, x, groups, w, b, mean, rstd, dx, dw, db, offsets=dev, activation="silu")
+    xs.orthogonalize(executor, dwg, step)
+
+    leaves = [t.double().requires_grad_() for t in (x, w, b, wg, wu)]
+    z = norm64(leaves[0], off, groups, leaves[1], leaves[2], 1e-5)
+    h = torch.nn.functional.silu(z)
+    out = torch.nn.functional.silu(h @ leaves[3].t()) * (h @ leaves[4].t())
+    out.backward(dy.double())
+    near(y, out.detach(), 8 * U)
+    for got, leaf, deep in ((dwg, leaves[3], 2), (dwu, leaves[4], 2), (dx, leaves[0], 3), (dw, leaves[1], 3), (db, leaves[2], 3)):
+        near(got, leaf.grad, 8 * deep * U)
+    u, _, v = torch.linalg.svd(dwg.double(), full_matrices=False)  # the update's directions are the gradient's
+    s = torch.diagonal(u.t() @ step.double() @ v.t())
+    assert s.min().item() > 0 and s.max().item() < 1.21
+    rest = u.t() @ step.double() @ v.t() - torch.diag(s)
+    assert torch.linalg.vector_norm(rest).item() <= 8 * U * len(s) ** 0.5 * 2
+
+
+@pytest.mark.parametrize("rows", [1, 12, 100, 400])
+def test_served_in_8_bits(executor, rows):
+    """group norm -> 8-bit rows -> product with an 8-bit weight: within the steps of both, 1 / 254 of a row's largest."""
+    cols, inner = 256, 300
+    x, w = rand(1, rows, cols, dtype=bf16), rand(2, inner, cols, dtype=bf16)
+    wq, ws = torch.empty(inner, cols, dtype=torch.int8, device="cuda"), torch.empty(inner, device="cuda")
+    xs.quantize_rows(executor, w, wq, ws)
+    n = torch.empty_like(x)
+    q, s = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    y = torch.empty(rows, inner, device="cuda")
+    xs.group_norm(executor, x, 8, None, None, 1e-5, n, activation="gelu")
+    xs.quantize_rows(executor, n, q, s)
+    xs.linear_int8(executor, q, s, wq, ws, y)
+    ref = n.double() @ w.double().t()
+    # each factor is off by half a step at most
+    ex, ew = s.double()[:, None] / 2, ws.double() / 2
+    bound = ex * w.double().abs().sum(1) + ew * n.double().abs().sum(1, keepdim=True) + cols * ex * ew
+    assert ((y.double() - ref).abs() <= bound * 1.001).all()
+
+
+def test_the_example_with_orthogonal_updates():
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "gated_graph_layer.py"), "--nodes-log2", "10", "--steps", "2",
+                        "--update", "orthogonal"], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "loss" in r.stdout, r.stderr[-2000:]
+
+
+def test_threads_with_their_own_executors(executor):
+    """Calls of every operator from several threads at once, each with its executor, stream and tensors."""
+    failures = []
+
+    def work(seed):
+        ex, stream = xs.CudaExecutor(0), torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            rows, cols = 300 + 37 * seed, 64 + 32 * seed
+            x = rand(seed, rows, cols, dtype=f16)
+            off = torch.tensor([0, 10, rows], device="cuda")
+
+            def call():
+                y, u = torch.empty_like(x), torch.empty_like(x)
+                q, s = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+                p = torch.empty(rows, rows, dtype=f16, device="cuda")
+                dw = torch.empty(cols, device="cuda")
+                mean, rstd = torch.empty(2, 8, device="cuda"), torch.empty(2, 8, device="cuda")
+                xs.group_norm(ex, x, 8, None, None, 1e-5, y, offsets=off, activation="silu", mean=mean, rstd=rstd)
+                xs.group_norm_backward(ex, y, x, 8, None, None, mean, rstd, None, dw, offsets=off, activation="silu")
+                xs.quantize_rows(ex, y, q, s)
+                xs.linear_int8(ex, q, s, q, s, p)
+                xs.orthogonalize(ex, x, u)
+                return y, dw, q, s, p, u
+
+            first = call()
+            for _ in range(30):
+                if not all(torch.equal(a, b) for a, b in zip(first, call())):
+                    failures.append(seed)
+                    break
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
+def test_offsets_past_32_bits(executor):
+    """Element offsets above 2^31: the last rows of a matrix of 2^31 + elements."""
+    cols = 4096
+    rows = (1 << 31) // cols + 300
+    x = torch.zeros(rows, cols, dtype=f16, device="cuda")
+    tail = rand(1, 300, cols, dtype=f16)
+    x[-300:] = tail
+    y = torch.zeros_like(x)
+    off = torch.tensor([rows - 300, rows], device="cuda")
+    xs.group_norm(executor, x, 64, None, None, 1e-5, y, offsets=off, activation="relu")
+    small = torch.empty_like(tail)
+    xs.group_norm(executor, tail, 64, None, None, 1e-5, small, activation="relu")
+    near(y[-300:], small, 2.0 ** -10)
+    assert not y[:rows - 300].any()
+    q, s = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    xs.quantize_rows(executor, x, q, s)
+    q2, s2 = torch.empty(300, cols, dtype=torch.int8, device="cuda"), torch.empty(300, device="cuda")
+    xs.quantize_rows(executor, tail, q2, s2)
+    assert torch.equal(q[-300:], q2) and torch.equal(s[-300:], s2) and not s[:rows - 300].any()
+    w, ws = q2[:64].contiguous(), s2[:64].contiguous()
+    p, p2 = torch.empty(rows, 64, dtype=f16, device="cuda"), torch.empty(300, 64, dtype=f16, device="cuda")
+    xs.linear_int8(executor, q, s, w, ws, p)
+    xs.linear_int8(executor, q2, s2, w, ws, p2)
+    assert torch.equal(p[-300:], p2) and not p[:rows - 300].any()
