@@ -45,10 +45,10 @@ struct Moments {
     float2 mean[P] = {}, m2[P] = {};
 };
 
-// Adds a batch of rows: BATCH of them, or with ALL = false the first `count`, the others zeros.
-template <bool ALL, typename TX, int V, int U>
-__device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V> (&raw)[BATCH][U], int count) {
-    constexpr int P = V * U / 2, B = BATCH;
+// Adds B rows.
+template <int B, typename TX, int V, int U>
+__device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V> (&raw)[B][U]) {
+    constexpr int P = V * U / 2;
     float2 s[P] = {}, q[P] = {}, v[P];
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -56,19 +56,19 @@ __device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V
 #pragma unroll
         for (int e = 0; e < P; ++e) s[e] = pair_add(s[e], v[e]);
     }
-    const float n = ALL ? (float)B : (float)count, per = ALL ? -1.0f / B : -1.0f / n;
 #pragma unroll
-    for (int e = 0; e < P; ++e) s[e] = pair_mul(s[e], both(per));  // minus the mean
+    for (int e = 0; e < P; ++e) s[e] = pair_mul(s[e], both(-1.0f / B));  // minus the mean
+    if constexpr (B > 1)
 #pragma unroll
-    for (int i = 0; i < B; ++i) {
-        Place<V, U>::values(raw[i], v);
+        for (int i = 0; i < B; ++i) {
+            Place<V, U>::values(raw[i], v);
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-            const float2 d = pair_add(v[e], s[e]);
-            if (ALL || i < count) q[e] = pair_fma(d, d, q[e]);
+            for (int e = 0; e < P; ++e) {
+                const float2 d = pair_add(v[e], s[e]);
+                q[e] = pair_fma(d, d, q[e]);
+            }
         }
-    }
-    const float total = m.n + n, fb = __fdividef(n, total), f = -m.n * fb;
+    const float total = m.n + (float)B, fb = __fdividef((float)B, total), f = -m.n * fb;
 #pragma unroll
     for (int e = 0; e < P; ++e) {
         const float2 d = pair_add(s[e], m.mean[e]);  // the batch's mean and the rows' before it, apart; minus that
@@ -97,16 +97,12 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const S
     Moments<P> m;
     auto from = tm.template walk<false>(x, begin, rows, ldx);
     auto fill = [&](int slot) { slots.fill(slot, from.next(), tm.at); };
-    auto use = [&](auto full, int slot, int count) {
-        Pack<TX, V> raw[BATCH][U];
+    auto use = [&](auto full, int slot) {
+        constexpr int B = decltype(full)::value ? BATCH : 1;
+        Pack<TX, V> raw[B][U];
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            if (full || j < count) slots.get(raw[j], slot + j);
-            else
-#pragma unroll
-                for (int u = 0; u < U; ++u) raw[j][u] = Pack<TX, V>{};
-        }
-        add_rows<decltype(full)::value>(m, raw, count);
+        for (int j = 0; j < B; ++j) slots.get(raw[j], slot + j);
+        add_rows<B>(m, raw);
     };
     if constexpr (KEEP) {
         fill_all(rows, fill);
@@ -190,10 +186,9 @@ __device__ __forceinline__ void apply(const Forward<TX, TY>& p, const Team<CTA, 
     auto from = tm.template walk<BACK>(p.a.x + k.c0, begin, rows, p.a.ldx);
     auto to = tm.template walk<BACK>(p.y + k.c0, begin, rows, p.ldy);
     with_act(p.a.act, [&](auto act) {
-        auto use = [&](auto full, int slot, int count) {
+        auto use = [&](auto full, int slot) {
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                if (!full && j >= count) break;
+            for (int j = 0; j < (decltype(full)::value ? BATCH : 1); ++j) {
                 Pack<TX, V> raw[U];
                 slots.get(raw, slot + j);
                 float2 v[P];

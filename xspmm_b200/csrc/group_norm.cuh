@@ -279,13 +279,16 @@ __device__ __forceinline__ void fill_all(int n, F&& fill) {
     copies_commit();
     copies_wait<0>();
 }
-// use(full, slot, count) for batches of rows already in slots 0, 1, ...; full (a constant) says that there are BATCH of
-// them, which are then one run of instructions without branches.
+// use(full, slot) for rows already in slots 0, 1, ...: with full (a constant) BATCH of them, one run of instructions without
+// branches; else one. Warps at different places of the code have to share the instruction cache, where misses are what
+// they wait for most: what is done once a sample is not unrolled.
 template <typename F>
 __device__ __forceinline__ void use_all(int n, F&& use) {
     int i = 0;
-    for (; i + BATCH <= n; i += BATCH) use(std::true_type{}, i, BATCH);
-    if (i < n) use(std::false_type{}, i, n - i);
+#pragma unroll 1
+    for (; i + BATCH <= n; i += BATCH) use(std::true_type{}, i);
+#pragma unroll 1
+    for (; i < n; ++i) use(std::false_type{}, i);
 }
 // The same of rows that pass through a ring of RING batches.
 template <int RING, typename F, typename G>
@@ -295,18 +298,20 @@ __device__ __forceinline__ void stream(int n, F&& fill, G&& use) {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) fill(slot + j);
         else
-#pragma unroll
-            for (int j = 0; j < BATCH; ++j)
-                if (j < left) fill(slot + j);
+#pragma unroll 1
+            for (int j = 0; j < left; ++j) fill(slot + j);
         copies_commit();  // a group a batch, empty past the last
     };
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < RING; ++k) batch(k * BATCH, n - k * BATCH);
     int slot = 0;
+#pragma unroll 1
     for (int left = n; left > 0; left -= BATCH) {
         copies_wait<RING - 1>();
-        if (left >= BATCH) use(std::true_type{}, slot, BATCH);
-        else use(std::false_type{}, slot, left);
+        if (left >= BATCH) use(std::true_type{}, slot);
+        else
+#pragma unroll 1
+            for (int j = 0; j < left; ++j) use(std::false_type{}, slot + j);
         batch(slot, left - RING * BATCH);
         slot = slot == (RING - 1) * BATCH ? 0 : slot + BATCH;
     }

@@ -95,10 +95,9 @@ __device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<C
     if constexpr (HOW == Rows::Fill) fill_all(rows, fill);
     with_act(p.a.act, [&](auto act) {
         constexpr Activation ACT = decltype(act)::value;
-        auto use = [&](auto full, int slot, int count) {
+        auto use = [&](auto full, int slot) {
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                if (!full && j >= count) break;
+            for (int j = 0; j < (decltype(full)::value ? BATCH : 1); ++j) {
                 Pack<TX, V> rx[U];
                 Pack<TY, V> rg[U];
                 slots.x.get(rx, slot + j);
