@@ -508,8 +508,8 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   an odd polynomial of the singular values that drives them to about 1 (0.68 to 1.2 after 5 steps,
  *   where they were not tiny). g fp16, bf16 or fp32; y fp16 or bf16 (the type of a 16-bit g). Products
  *   of 22-bit operands (two fp16 parts each) with fp32 sums: the error is a small part of y's rounding.
- *   0 <= steps <= 100; steps = 0: y = X_0. An infinity or NaN in g makes y NaN (steps >= 1). y may be g
- *   (same type and stride).
+ *   0 <= steps <= 100; steps = 0: y = X_0. A g of zeros gives zeros (with eps = 0: NaN). An infinity or
+ *   NaN in g makes y NaN (steps >= 1). y may be g (same type and stride).
  * ------------------------------------------------------------------------------------------- */
 typedef enum xspmm_activation {
     XSPMM_ACT_SILU = 0,

@@ -8,6 +8,11 @@
 // Who takes which samples is decided as in the forward pass (group_norm.cu). The sums for the weights' gradients are
 // kept for each thread over all samples that its CTA takes and leave as one row a CTA (or chunk), added in order by the
 // last kernel; a block of several tiles has no room for them and adds them to its CTA's row as it goes.
+//
+// 2^20 x 128 fp16, relu: 246 us (206 for both inputs read twice at the copy bandwidth), DRAM at 5.1 and 5.3 TB/s. 4096 samples
+// of 2^18 x 256 bf16, silu: 215 to 230 us (62), bound by instructions: 44 for each value of a lane, issue in 46 % of the cycles,
+// misses of the instruction cache the most frequent wait. The slope is computed in both passes: dz would take half as much
+// shared memory again, and fewer samples would stay there.
 #include "group_norm.cuh"
 
 namespace xspmm_b200 {

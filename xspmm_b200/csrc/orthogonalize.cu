@@ -9,6 +9,9 @@
 // would add to those directions with them. X, A and B' are therefore held as two fp16 parts (22 bits), and the
 // products are those of the parts with fp32 sums (tile_product.cuh). A and B' are symmetric: half of their tiles
 // are computed. The norm is summed in fp64: squares of any fp32 gradient are in its range.
+//
+// 11008 x 4096: 7.75 ms; the three products of the parts' 3.1 TFLOP are 6.73 ms at the sustained bf16 rate. Below about 1000
+// the launches and latencies of fifteen products (768 x 1232: 208 us).
 #include "tile_product.cuh"
 
 namespace xspmm_b200 {
@@ -105,7 +108,7 @@ scaled_kernel(int64_t rows, int64_t cols, const TX* g, int64_t ldg, const double
 // stay in shared memory in two parts, in the SWIZZLE_128B layout: 64-column chunks of 128 rows of 128 bytes. Read along
 // its rows a chunk is a K-major operand, along its columns an MN-major one, so X serves both products. A is replaced by
 // B' in place and X by its successor, each after the MMAs that read it. Bound by the latency of 3 products a step, their
-// MMAs on 1 of 148 SMs and the epilogues between (128 x 128, 5 steps: 17 launches of the large path took 107 us).
+// MMAs on 1 of 148 SMs and the epilogues between (128 x 128, 5 steps: 61 us; 17 launches of the large path took 107).
 constexpr int SMALL_THREADS = 512, SMALL_ROWS = 128, SMALL_COLS = 256;
 constexpr int SMALL_CHUNK = SMALL_ROWS * 128;
 
