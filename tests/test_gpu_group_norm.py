@@ -420,3 +420,37 @@ def test_long_samples(executor, rows, cols, groups, offsets, tx, ty):
     check_forward(executor, x, groups, w, b, 1e-5, y, offsets, "gelu", ybuf)
     dx, dbuf = guarded(rows, cols, ty)
     check_backward(executor, dy, x, groups, w, b, offsets, "gelu", dx, dbuf)
+
+
+@pytest.mark.parametrize("cols,groups", [(32, 4), (474, 2), (21, 3)])
+def test_relu_slope_is_that_of_z_rounded_step_by_step(executor, cols, groups):
+    """z is 0 where the rounded product is exactly -bias, and its slope is 0 there: dbias counts the rows with z > 0."""
+    rows = 3000
+    x, b = rand(41, rows, cols), rand(42, cols, scale=0.1)
+    w = 1.0 + rand(43, cols, scale=0.2)
+    mean, rstd = rand(44, 1, groups, scale=0.1), rand(45, 1, groups).abs() + 0.5
+    width = cols // groups
+    m, r = mean[0].repeat_interleave(width), rstd[0].repeat_interleave(width)
+    rounded = ((x - m) * r) * w  # separate kernels: each operation rounded
+    b = -rounded[torch.arange(cols, device="cuda") % rows, torch.arange(cols, device="cuda")]  # a zero in every column
+    z = rounded + b
+    assert int((z == 0).sum()) >= cols
+    db = torch.empty(cols, device="cuda")
+    xs.group_norm_backward(executor, torch.ones_like(x), x, groups, w, b, mean, rstd, None, None, db, activation="relu")
+    assert torch.equal(db.long(), (z > 0).sum(0))
+
+
+@pytest.mark.parametrize("tx,ty", TYPES)
+@pytest.mark.parametrize("cols", [16, 23])
+def test_gradient_of_groups_of_one_value_is_zero(executor, cols, tx, ty):
+    """One row and one channel a group: y does not depend on x, and rstd (316 for eps 1e-5) multiplies no rounding."""
+    rows = 40
+    off = torch.arange(rows + 1, device="cuda")
+    x, dy = rand(51, rows, cols, dtype=tx), rand(52, rows, cols, dtype=ty)
+    w, b = rand(53, cols, shift=1.0, scale=0.2), rand(54, cols, scale=0.1)
+    mean, rstd = torch.empty(rows, cols, device="cuda"), torch.empty(rows, cols, device="cuda")
+    y, dx = torch.empty(rows, cols, dtype=ty, device="cuda"), torch.empty(rows, cols, dtype=ty, device="cuda")
+    xs.group_norm(executor, x, cols, w, b, 1e-5, y, offsets=off, activation="silu", mean=mean, rstd=rstd)
+    assert torch.equal(mean, x.float())
+    xs.group_norm_backward(executor, dy, x, cols, w, b, mean, rstd, dx, offsets=off, activation="silu")
+    assert not dx.any()

@@ -17,6 +17,11 @@ constexpr int MAX_TILE = 32 * PER;  // channels of a column tile
 __device__ __forceinline__ float2 pair_add(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 pair_mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 pair_fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// A product that is rounded by itself whatever is added to it: a packed one and an addition are joined to one operation,
+// as the results show, .rn or not.
+__device__ __forceinline__ float2 pair_mul_alone(float2 a, float2 b) {
+    return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y));
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // Channels are cut into column tiles: whole groups side by side (gpt of them), or, where a group is wider than a
@@ -395,7 +400,7 @@ __device__ __forceinline__ float group_sum(float v, int l) {
 // z, each operation rounded by itself: the sign of z, which decides relu's slope, is then the same in the forward
 // and the backward pass and however the compiler orders the code around it.
 __device__ __forceinline__ float2 centred(float2 x, float2 neg_mean, float2 rstd) { return pair_mul(pair_add(x, neg_mean), rstd); }
-__device__ __forceinline__ float2 affine(float2 xh, float2 w, float2 b) { return pair_add(pair_mul(xh, w), b); }
+__device__ __forceinline__ float2 affine(float2 xh, float2 w, float2 b) { return pair_add(pair_mul_alone(xh, w), b); }
 
 // act(z) of a row's values and its slope. 16-bit outputs take the gated block's approximate forms (errors far below
 // their rounding), fp32 ones CUDA's accurate functions.

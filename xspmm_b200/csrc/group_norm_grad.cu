@@ -176,7 +176,8 @@ __device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA,
     each_row<CTA, HOW, BACK>(p, tm, slots, k, begin, end, ch, [&](const float2 (&dz)[P], const float2 (&xh)[P]) {
         float2 v[P];
 #pragma unroll
-        for (int e = 0; e < P; ++e) v[e] = pair_mul(ch.rs[e], pair_fma(xh[e], m2[e], pair_fma(dz[e], ch.w[e], m1[e])));
+        for (int e = 0; e < P; ++e)  // t rounded by itself: a group's only value has dx = 0, not a rounding times rstd
+            v[e] = pair_mul(ch.rs[e], pair_fma(xh[e], m2[e], pair_add(pair_mul_alone(dz[e], ch.w[e]), m1[e])));
         tm.at.store(to.next(), v);
     });
 }
