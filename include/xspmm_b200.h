@@ -487,7 +487,9 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   is at most 16384. Over a sample's rows and a group's n values,
  *   mean = sum(x) / n, rstd = 1 / sqrt(sum((x - mean)^2) / n + eps) (no values: 0 and 1 / sqrt(eps)),
  *   z = ((x - mean) * rstd) * weight + bias, y = act(z); activation as below or XSPMM_ACT_NONE (y = z).
- *   All in fp32, z with each operation rounded by itself. Types as for the layer norm; weight, bias
+ *   All in fp32, z with each operation rounded by itself; features of any finite size have a finite mean
+ *   where they differ by no more than fp32's largest number, and rstd is 0 where their squares' sum about
+ *   it passes that. Types as for the layer norm; weight, bias
  *   (cols, fp32; NULL: 1 and 0); mean, rstd (samples x groups, fp32) are written where not NULL. y may
  *   be x (same type and stride).
  * Its gradient. dz = dy * act'(z) with z as above (relu: 1 where z > 0), t = dz * weight,

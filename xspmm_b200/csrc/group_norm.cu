@@ -47,19 +47,18 @@ struct Moments {
     float2 mean[P] = {}, m2[P] = {};
 };
 
-// Adds B rows.
+// Adds B rows. Their mean is the sum of parts of them, and a weight is multiplied to one deviation before the other: no sum
+// of values leaves fp32's range, and where no rows were before (weight 0) no infinite square becomes NaN.
 template <int B, typename TX, int V, int U>
 __device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V> (&raw)[B][U]) {
     constexpr int P = V * U / 2;
-    float2 s[P] = {}, q[P] = {}, v[P];
+    float2 s[P] = {}, q[P] = {}, v[P];  // s: minus the mean
 #pragma unroll
     for (int i = 0; i < B; ++i) {
         Place<V, U>::values(raw[i], v);
 #pragma unroll
-        for (int e = 0; e < P; ++e) s[e] = pair_add(s[e], v[e]);
+        for (int e = 0; e < P; ++e) s[e] = pair_fma(v[e], both(-1.0f / B), s[e]);
     }
-#pragma unroll
-    for (int e = 0; e < P; ++e) s[e] = pair_mul(s[e], both(-1.0f / B));  // minus the mean
     if constexpr (B > 1)
 #pragma unroll
         for (int i = 0; i < B; ++i) {
@@ -75,7 +74,7 @@ __device__ __forceinline__ void add_rows(Moments<V * U / 2>& m, const Pack<TX, V
     for (int e = 0; e < P; ++e) {
         const float2 d = pair_add(s[e], m.mean[e]);  // the batch's mean and the rows' before it, apart; minus that
         m.mean[e] = pair_fma(d, both(-fb), m.mean[e]);
-        m.m2[e] = pair_add(m.m2[e], pair_fma(pair_mul(d, d), both(-f), q[e]));
+        m.m2[e] = pair_add(m.m2[e], pair_fma(pair_mul(d, both(-f)), d, q[e]));
     }
     m.n = total;
 }
@@ -139,10 +138,12 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const S
     if constexpr (CTA) {
         const int c = threadIdx.x;
         if (c < k.cols) {
-            const float per = 1.0f / (float)(end - begin);
+            // means about one of them: equal ones give that value, and no sum of them leaves the range
+            const float per = 1.0f / (float)(end - begin), base = sh.v[0][0][c];
             float mean = 0.0f, m2 = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) mean = fmaf(sh.n[w] * per, sh.v[w][0][c], mean);
+            for (int w = 1; w < WARPS; ++w) mean = fmaf(sh.n[w] * per, sh.v[w][0][c] - base, mean);
+            mean += base;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float d = sh.v[w][0][c] - mean;
@@ -159,9 +160,10 @@ __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const S
     const float n = (float)(end - begin), per = 1.0f / (float)k.lw;
     each_group<CTA>(k.ng, [&](int g, int j, int l, bool live) {
         float s = 0.0f;
+        const float base = live ? cm[g * k.lw] : 0.0f;
         if (live)
-            for (int c = j; c < k.lw; c += l) s += cm[g * k.lw + c];
-        const float mean = group_sum(s, l) * per;
+            for (int c = j; c < k.lw; c += l) s = fmaf(cm[g * k.lw + c] - base, per, s);
+        const float mean = base + group_sum(s, l);
         s = 0.0f;
         if (live)
             for (int c = j; c < k.lw; c += l) {
@@ -348,9 +350,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const _
                     }
                 }
             };
+            const float base = parts.get(p.part, (int64_t)(k.g0 + g) * tpg, 0).x, per = 1.0f / n;
             float mean = 0.0f, m2 = 0.0f;
-            each_part([&](float count, float2 v) { mean = fmaf(count, v.x, mean); });
-            mean = group_sum(mean, 32) / n;
+            each_part([&](float count, float2 v) { mean = fmaf(count * per, v.x - base, mean); });
+            mean = base + group_sum(mean, 32);
             each_part([&](float count, float2 v) {
                 const float d = v.x - mean;
                 m2 += fmaf(count * d, d, v.y);

@@ -330,11 +330,12 @@ struct Strips {
 };
 
 // Joins (nb, mb, sb) into (na, ma, sa): counts, means and sums of squares about the mean (Chan, Golub and LeVeque,
-// 1979). fb = nb / (na + nb) and f = na nb / (na + nb) are the same for all channels of a row.
+// 1979). fb = nb / (na + nb) and f = na nb / (na + nb) are the same for all channels of a row. f, 0 where one side has no
+// values, comes before the second d: 0 times an infinite square would be NaN.
 __device__ __forceinline__ void join_moments(float& ma, float& sa, float mb, float sb, float fb, float f) {
     const float d = mb - ma;
     ma = fmaf(d, fb, ma);
-    sa += fmaf(d * d, f, sb);
+    sa += fmaf(d * f, d, sb);
 }
 
 // A thread's two values a channel to a warp's strips.
