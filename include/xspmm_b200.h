@@ -482,8 +482,10 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   device) cuts the rows into samples, sample i being rows [offsets[i], offsets[i + 1]): the graphs of
  *   a packed batch. offsets NULL (samples = 1): one sample of all rows. Rows before the first offset and
  *   behind the last are not read and their outputs are left as they were; a sample may have no rows.
- *   Offsets must not decrease and lie in [0, rows]; others are taken as the nearest that does (samples
- *   then overlap or are empty, and nothing out of range is touched). groups divides cols, cols / groups
+ *   Offsets must not decrease and lie in [0, rows]. Of others nothing out of range is touched: each is
+ *   taken as the nearest in [0, rows], and a sample that ends before it begins has no rows. Where offsets
+ *   decrease, samples may overlap; their rows and statistics may then be left as they were, hold NaN, or
+ *   hold any one sample's values. groups divides cols, cols / groups
  *   is at most 16384. Over a sample's rows and a group's n values,
  *   mean = sum(x) / n, rstd = 1 / sqrt(sum((x - mean)^2) / n + eps) (no values: 0 and 1 / sqrt(eps)),
  *   z = ((x - mean) * rstd) * weight + bias, y = act(z); activation as below or XSPMM_ACT_NONE (y = z).

@@ -1,11 +1,11 @@
-"""GPU tests of the group norm at the ends of its range: features of large magnitude."""
+"""GPU tests of the group norm at the ends of its range: features of large magnitude, offsets that decrease."""
 import math
 
 import pytest
 import torch
 
 import xspmm_b200 as xs
-from test_gpu_group_norm import U, bf16, check_forward, f16, f32, guarded, rand, value
+from test_gpu_group_norm import U, bf16, check_forward, f16, f32, guarded, outside_untouched, rand, value
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,44 @@ def test_squares_past_the_range(executor, rows, cols, groups, offsets, tx, ty):
     assert torch.isfinite(mean).all() and not rstd.any()
     inner = slice(0, rows) if offsets is None else slice(offsets[0], offsets[-1])
     assert torch.equal(y[inner], b.clamp(min=0).to(ty).expand(rows, cols)[inner])
+
+
+# of 50000 rows: long samples that no or not every chunk finds, since a short or empty one hides them
+DECREASING = [[0, 50000, 100, 200], [100, 200, 0, 50000], [0, 30000, 20000, 50000], [50000, 0, 50000], [0, 50000, 0, 50000],
+              [0, 20000, 49000, 10000, 50000], [1 << 40, -5, 1 << 40, 7]]
+
+
+@pytest.mark.parametrize("cols,groups", [(128, 32), (33, 3), (300, 1)])
+@pytest.mark.parametrize("offsets", DECREASING)
+def test_decreasing_offsets_take_nothing_from_earlier_calls(executor, offsets, cols, groups):
+    """What is written is the same after calls that left different sums in the pool's memory, and nothing outside is."""
+    rows = 50000
+    x, dy = rand(1, rows, cols, dtype=bf16), rand(2, rows, cols, dtype=bf16)
+    off, fine = torch.tensor(offsets, device="cuda"), torch.tensor([0] * (len(offsets) - 1) + [rows], device="cuda")
+    samples = len(offsets) - 1
+    got = []
+    for scale in (1.0, 3.0):
+        spare, dw, db = torch.empty_like(x), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+        mean, rstd = torch.zeros(samples, groups, device="cuda"), torch.ones(samples, groups, device="cuda")
+        torch.cuda.synchronize()
+        xs.group_norm(executor, x * scale, groups, None, None, 1e-5, spare, offsets=fine, mean=mean, rstd=rstd)
+        y, ybuf = guarded(rows, cols, bf16)
+        mean, rstd = torch.full((samples, groups), 7.0, device="cuda"), torch.full((samples, groups), 7.0, device="cuda")
+        xs.group_norm(executor, x, groups, None, None, 1e-5, y, offsets=off, activation="silu", mean=mean, rstd=rstd)
+        one, zero = torch.ones(samples, groups, device="cuda"), torch.zeros(samples, groups, device="cuda")
+        xs.group_norm_backward(executor, dy * scale, x, groups, None, None, zero, one, spare, dw, db, offsets=fine)
+        dx, dbuf = guarded(rows, cols, bf16)
+        dw, db = torch.full((cols,), 7.0, device="cuda"), torch.full((cols,), 7.0, device="cuda")
+        xs.group_norm_backward(executor, dy, x, groups, None, None, zero, one, dx, dw, db, offsets=off)
+        outside_untouched(y, ybuf)
+        outside_untouched(dx, dbuf)
+        got.append((y, mean, rstd, dx, dw, db))
+    for a, b in zip(*got):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_a_sample_that_a_later_one_hides_has_no_statistics(executor):
+    x = rand(1, 50000, 128, dtype=f16)
+    y, mean = torch.zeros_like(x), torch.zeros(3, 32, device="cuda")
+    xs.group_norm(executor, x, 32, None, None, 1e-5, y, offsets=torch.tensor([0, 50000, 100, 200], device="cuda"), mean=mean)
+    assert mean[0].isnan().all() and not mean[1].any() and mean[2].isfinite().all()

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const _
         if (s < 0) continue;
         const Span sp = span_of(p.a.offsets, s, total);
         const Parts parts(sp, p.ch, tpg == 1 ? p.t.groups : p.t.tiles);
-        __syncthreads();
+        const bool lost = not_found(p.found, parts, s);
         for (int g = threadIdx.x >> 5; g < k.ng; g += WARPS) {
             // the mean of the parts' means, then the squares about it
             const int n_rows = sp.end - sp.begin;
@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_apply_kernel(const _
                 m2 += fmaf(count * d, d, v.y);
             });
             m2 = group_sum(m2, 32);
+            if (lost) mean = m2 = __uint_as_float(0x7fc00000u);
             if (lane == 0) finish(p, s, k.g0 + g, mean, m2, n, slot == 1 && (tpg == 1 || tile % tpg == 0), gm + g, gr + g);
         }
         __syncthreads();

@@ -81,7 +81,7 @@ __device__ __forceinline__ Span span_of(const int64_t* offsets, int s, int rows)
     return {b, max(b, (int)max((int64_t)0, min((int64_t)rows, offsets[s + 1])))};
 }
 // The last sample that begins at or before row r, -1 if none does. A warp's threads call it together and probe 32
-// offsets at a time.
+// offsets at a time. Offsets that decrease give some sample or -1.
 __device__ __forceinline__ int last_begun(const int64_t* offsets, int samples, int64_t r) {
     if (!offsets) return 0;
     int lo = 0, n = samples;  // the answer is lo - 1 + (how many of the next n begin by r)
@@ -124,6 +124,17 @@ __device__ __forceinline__ int2 long_samples(const int64_t* offsets, int samples
     }
     __syncthreads();
     return make_int2(found[0], found[1]);
+}
+
+// Whether a chunk of long sample s, its parts being `parts`, does not have it: the offsets decrease, and what parts[] holds
+// for it is in part not of this call. Called by the whole CTA; the same in all threads.
+__device__ __forceinline__ bool not_found(const int2* found, const Parts& parts, int s) {
+    bool lost = false;
+    for (int i = threadIdx.x; i < parts.count; i += THREADS) {
+        const int2 f = found[parts.first + i];
+        lost = lost || (i == 0 ? f.y : f.x) != s;
+    }
+    return __syncthreads_or(lost);
 }
 
 // A thread's channels of a tile: V consecutive ones at each of U places, lpr * V apart. Pointers to rows are at the

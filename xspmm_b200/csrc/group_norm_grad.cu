@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_apply_kernel(co
         if (s < 0) continue;
         const Span sp = span_of(p.a.offsets, s, all);
         const Parts parts(sp, p.ch, tpg == 1 ? p.t.groups : p.t.tiles);
-        const float per = -1.0f / ((float)(sp.end - sp.begin) * (float)p.t.width);
-        __syncthreads();
+        const bool lost = not_found(p.found, parts, s);
+        const float per = lost ? __uint_as_float(0x7fc00000u) : -1.0f / ((float)(sp.end - sp.begin) * (float)p.t.width);
         for (int g = threadIdx.x >> 5; g < k.ng; g += WARPS) {
             float s1 = 0.0f, s2 = 0.0f;
             for (int part = 0; part < tpg; ++part)
