@@ -1,11 +1,13 @@
-"""GPU tests of the group norm at the ends of its range: features of large magnitude, offsets that decrease."""
+"""GPU tests of the group norm at the ends of its range: features of large magnitude, offsets that decrease,
+sums of many terms."""
 import math
 
 import pytest
 import torch
 
+import test_gpu_group_norm
 import xspmm_b200 as xs
-from test_gpu_group_norm import U, bf16, check_forward, f16, f32, guarded, outside_untouched, rand, value
+from test_gpu_group_norm import U, bf16, check_backward, check_forward, f16, f32, guarded, outside_untouched, rand, value
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +107,44 @@ def test_a_sample_that_a_later_one_hides_has_no_statistics(executor):
     y, mean = torch.zeros_like(x), torch.zeros(3, 32, device="cuda")
     xs.group_norm(executor, x, 32, None, None, 1e-5, y, offsets=torch.tensor([0, 50000, 100, 200], device="cuda"), mean=mean)
     assert mean[0].isnan().all() and not mean[1].any() and mean[2].isfinite().all()
+
+
+@pytest.mark.parametrize("rows,cols,samples", [(1 << 24, 128, 1), (1 << 26, 8, 1 << 26)])
+def test_sums_of_equal_terms(executor, rows, cols, samples):
+    """dy = 1 + 2^-13 - 2^-20 and xh = 1 everywhere: added up one after the other, every term past the 2048th loses its
+    fraction, 7000 in a row 8.6e-5 of the sum. 1024 + 32 roundings of half a step are 6.3e-5."""
+    term = 1.0 + 2.0 ** -13 - 2.0 ** -20
+    x, dy = torch.ones(rows, cols, device="cuda"), torch.full((rows, cols), term, device="cuda")
+    mean, rstd = torch.zeros(samples, 1, device="cuda"), torch.ones(samples, 1, device="cuda")
+    off = None if samples == 1 else torch.arange(samples + 1, device="cuda")
+    dw, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    xs.group_norm_backward(executor, dy, x, 1, None, None, mean, rstd, None, dw, db, offsets=off)
+    want = rows * term
+    for got in (dw, db):
+        assert (got.double() - want).abs().max().item() <= 1.01 * (1024 + 32) * 2.0 ** -24 * want
+
+
+class EqualLengths(test_gpu_group_norm.Ref):
+    """The 64-bit sums of samples of one length, all at once."""
+
+    def mean_of(self, v):
+        return v.reshape(len(self.spans), -1, self.groups, self.width).sum((1, 3)) * self.per
+
+    def spread(self, v, rows):
+        v = v.expand(len(self.spans), self.groups).repeat_interleave(self.width, 1)
+        return v.repeat_interleave(rows // len(self.spans), 0)
+
+
+@pytest.mark.parametrize("tx,ty", [(f16, f16), (f32, f32), (f32, bf16)])
+@pytest.mark.parametrize("samples,length,cols,groups", [(40000, 3, 64, 8), (40000, 2, 21, 3), (3000, 40, 640, 5), (6000, 1, 300, 1)])
+def test_walks_over_many_samples(executor, monkeypatch, samples, length, cols, groups, tx, ty):
+    """So many samples that every warp, or CTA, of the gradient takes several in turn."""
+    monkeypatch.setattr(test_gpu_group_norm, "Ref", EqualLengths)
+    rows = samples * length
+    offsets = list(range(0, rows + 1, length))
+    x, dy = rand(21, rows, cols, dtype=tx, shift=0.5), rand(22, rows, cols, dtype=ty, shift=0.5)
+    w, b = rand(23, cols, scale=0.2, shift=1.0), rand(24, cols, scale=0.1)
+    y, ybuf = guarded(rows, cols, ty)
+    check_forward(executor, x, groups, w, b, 1e-5, y, offsets, "silu", ybuf)
+    dx, dbuf = guarded(rows, cols, ty)
+    check_backward(executor, dy, x, groups, w, b, offsets, "silu", dx, dbuf)

@@ -94,22 +94,42 @@ template <bool CTA, bool KEEP, typename TX, int V, int U, typename F>
 __device__ __forceinline__ void group_moments(const Team<CTA, V, U>& tm, const Slots<TX, V, U>& slots, const TX* x, int64_t ldx,
                                               int begin, int end, const Tile& k, Strips& sh, F&& f) {
     constexpr int P = V * U / 2;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = tm.rows(end - begin);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Moments<P> m;
-    auto from = tm.template walk<false>(x, begin, rows, ldx);
-    auto fill = [&](int slot) { slots.fill(slot, from.next(), tm.at); };
-    auto use = [&](auto full, int slot) {
-        constexpr int B = decltype(full)::value ? BATCH : 1;
-        Pack<TX, V> raw[B][U];
+    auto add = [&](Moments<P>& to, int b, int e) {
+        const int rows = tm.rows(e - b);
+        auto from = tm.template walk<false>(x, b, rows, ldx);
+        auto fill = [&](int slot) { slots.fill(slot, from.next(), tm.at); };
+        auto use = [&](auto full, int slot) {
+            constexpr int B = decltype(full)::value ? BATCH : 1;
+            Pack<TX, V> raw[B][U];
 #pragma unroll
-        for (int j = 0; j < B; ++j) slots.get(raw[j], slot + j);
-        add_rows<B>(m, raw);
+            for (int j = 0; j < B; ++j) slots.get(raw[j], slot + j);
+            add_rows<B>(to, raw);
+        };
+        if constexpr (KEEP) {
+            fill_all(rows, fill);
+            use_all(rows, use);
+        } else {
+            stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(rows, fill, use);
+        }
     };
     if constexpr (KEEP) {
-        fill_all(rows, fill);
-        use_all(rows, use);
+        add(m, begin, end);
     } else {
-        stream<RING_BYTES / Slots<TX, V, U>::BYTES / BATCH>(rows, fill, use);
+        const int most = TERMS * BATCH << tm.step_log;
+#pragma unroll 1
+        for (int b = begin; b < end; b += most) {
+            Moments<P> part;
+            add(part, b, min(end, b + most));
+            float fb, f;
+            m.n = join_weights(m.n, part.n, &fb, &f);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                join_moments(m.mean[e].x, m.m2[e].x, part.mean[e].x, part.m2[e].x, fb, f);
+                join_moments(m.mean[e].y, m.m2[e].y, part.mean[e].y, part.m2[e].y, fb, f);
+            }
+        }
     }
     for (int o = 16; o >= tm.at.lpr; o >>= 1) {
         // both of a pair take the lower lane's moments first, so that they end with the same numbers

@@ -255,6 +255,9 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
 constexpr int BATCH = 4;  // rows that are worked on together
+// Terms that a thread adds up one after the other: sums of more are joined from such ones, so that the rounding of a sum
+// does not grow with its length (7000 of 1 + 2^-13 in a row lose 2^-13.5 of it).
+constexpr int TERMS = 1024;
 
 // One thread's slots for rows of T.
 template <typename T, int V, int U>

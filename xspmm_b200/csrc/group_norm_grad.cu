@@ -6,8 +6,9 @@
 // for A and B serves the weights and the groups, and a second one gives dx.
 //
 // Who takes which samples is decided as in the forward pass (group_norm.cu). The sums for the weights' gradients are
-// kept for each thread over all samples that its CTA takes and leave as one row a CTA (or chunk), added in order by the
-// last kernel; a block of several tiles has no room for them and adds them to its CTA's row as it goes.
+// kept for each thread over all samples that its CTA takes (at most TERMS) and leave as one row a CTA (or chunk), added in
+// order and in 64 bits by the last kernel; a block of several tiles has no room for them and adds them to its CTA's row
+// as it goes.
 //
 // 2^20 x 128 fp16, relu: 246 us (206 for both inputs read twice at the copy bandwidth), DRAM at 5.1 and 5.3 TB/s. 4096 samples
 // of 2^18 x 256 bf16, silu: 215 to 230 us (62), bound by instructions: 44 for each value of a lane, issue in 46 % of the cycles,
@@ -50,6 +51,10 @@ struct Channels {
 template <int P>
 struct Sums {
     float2 a[P] = {}, b[P] = {};
+    __device__ void add(const Sums& o) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) a[e] = pair_add(a[e], o.a[e]), b[e] = pair_add(b[e], o.b[e]);
+    }
 };
 // A thread's sums over all samples that its CTA takes, in shared memory: touched once a sample.
 template <int P>
@@ -137,13 +142,24 @@ __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team
                                            Strips& sh, F&& f, C&& channels) {
     constexpr int P = V * U / 2;
     Sums<P> s;
-    each_row<CTA, HOW, false>(p, tm, slots, k, begin, end, ch, [&](const float2 (&dz)[P], const float2 (&xh)[P]) {
+    auto add = [&](int b, int e) {
+        Sums<P> part;
+        each_row<CTA, HOW, false>(p, tm, slots, k, b, e, ch, [&](const float2 (&dz)[P], const float2 (&xh)[P]) {
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-            s.a[e] = pair_add(s.a[e], dz[e]);
-            s.b[e] = pair_fma(dz[e], xh[e], s.b[e]);
-        }
-    });
+            for (int i = 0; i < P; ++i) {
+                part.a[i] = pair_add(part.a[i], dz[i]);
+                part.b[i] = pair_fma(dz[i], xh[i], part.b[i]);
+            }
+        });
+        s.add(part);
+    };
+    if constexpr (HOW == Rows::Pass) {
+        const int most = TERMS << tm.step_log;
+#pragma unroll 1
+        for (int b = begin; b < end; b += most) add(b, min(end, b + most));
+    } else {
+        add(begin, end);
+    }
     total.add(s);
     sum_channels<CTA>(s.a, s.b, tm.at, sh);
     const int strip = CTA ? 0 : threadIdx.x >> 5;
@@ -367,22 +383,24 @@ __global__ void __launch_bounds__(THREADS, CTAS) group_norm_grad_apply_kernel(co
     }
 }
 
-// dw and db: the rows of parts added in order, 32 channels a CTA; its warps take every 32nd row.
+// dw and db: the rows of parts added in order, 32 channels a CTA; its warps take every 32nd. In 64 bits: there may be as
+// many rows as samples.
 __global__ void __launch_bounds__(1024) group_norm_weights_kernel(const float* part, int rows, int64_t C, float* dw, float* db) {
-    __shared__ float red[32][33];
+    __shared__ double red[32][33];
     cudaGridDependencySynchronize();
     float* out = blockIdx.y ? db : dw;
     if (!out) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = blockIdx.x * 32ll + lane;
-    float s = 0.0f;
+    double s = 0.0;
     if (c < C)
 #pragma unroll 8
-        for (int r = warp; r < rows; r += 32) s += part[((int64_t)r * 2 + blockIdx.y) * C + c];
+        for (int r = warp; r < rows; r += 32) s += (double)part[((int64_t)r * 2 + blockIdx.y) * C + c];
     red[warp][lane] = s;
     __syncthreads();
-    s = group_sum(red[lane][warp], 32);  // of channel blockIdx.x * 32 + warp
-    if (lane == 0 && blockIdx.x * 32ll + warp < C) out[blockIdx.x * 32ll + warp] = s;
+    s = red[lane][warp];  // of channel blockIdx.x * 32 + warp
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0 && blockIdx.x * 32ll + warp < C) out[blockIdx.x * 32ll + warp] = (float)s;
 }
 
 template <typename TX, typename TY, int V, int U>
@@ -391,9 +409,9 @@ void backward(Handle& h, Backward<TX, TY>& p, float* dw, float* db) {
     const Cut cut = make_cut(p.a, p.t, (int)(sizeof(TX) + sizeof(TY)), V > 1, sms, CTAS);
     p.ch = cut.ch;
     p.by_warp = cut.by_warp;
-    // as many samples a CTA as make four waves of them
+    // as many samples a CTA as make four waves of them, but no more than TERMS a thread
     const int64_t items = ceil_div(p.a.samples, cut.by_warp ? WARPS : 1);
-    p.each = (int)std::max<int64_t>(1, items * p.t.blocks / (4 * CTAS * sms)) * (cut.by_warp ? WARPS : 1);
+    p.each = (int)std::clamp<int64_t>(items * p.t.blocks / (4 * CTAS * sms), 1, TERMS) * (cut.by_warp ? WARPS : 1);
     p.walkers = cut.only_long ? 0 : (int)std::max<int64_t>(1, ceil_div(p.a.samples, p.each));
     DevBuf<float2> part((size_t)p.ch.count * 2 * part_slots(p.t), h.stream);
     DevBuf<int2> found((size_t)p.ch.count, h.stream);
