@@ -14,6 +14,10 @@
 // are summed in an accumulator of their own and joined with the large one in fp32 afterwards: an addition in the
 // tensor core truncates, and small terms on top of a large sum would triple the truncations of it. The two
 // accumulators fill TMEM, so a tile's epilogue does not run under the next one's MMAs as it does for Int8.
+// The large accumulator holds the sum of DRAIN stages at most: then the epilogue's warps add it to sums in their
+// registers, where additions round, while the tensor core is at the cross products of the stages on both sides. An update
+// of 11008 x 4096 normal numbers is 5e-6 off before its rounding, the iteration in fp32 8e-6; with all of the sum in the
+// accumulator it was 1e-4 (at 1 % less time; DRAIN = 4: 9e-6; 768 x 1232: 3e-6 in 228 us, 5e-6 in 221, 7e-6 in 210).
 //
 // The entries of X, A and B' (orthogonalize.cu) are below 4 in magnitude, so 2^14 times them fits fp16, and parts
 // down to 2^-38 are held.
@@ -31,6 +35,8 @@ using namespace gated;
 enum class Epi { Int8, Gram, Poly, Next, Last };
 constexpr bool symmetric(Epi e) { return e == Epi::Gram || e == Epi::Poly; }
 constexpr bool split(Epi e) { return e != Epi::Int8; }
+
+constexpr int DRAIN = 2;  // stages: 128 summed elements, 8 truncated additions
 
 constexpr float SPLIT_SCALE = 16384.0f, SPLIT_INV = 1.0f / 16384.0f;
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
@@ -164,6 +170,71 @@ __device__ __forceinline__ void store_mirror(__half* out, int64_t ld, const uint
         if (c < cols) at[c * ld] = (uint16_t)(w[c / 2] >> (c % 2 * 16));
 }
 
+// A warp has read its part of an accumulator.
+template <int CG>
+__device__ __forceinline__ void taken(uint64_t* acc_empty) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        if constexpr (CG == 2) arrive_cluster(first_cta_addr(acc_empty));
+        else mbar_arrive(acc_empty);
+    }
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+        "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+
+// Takes a work item's large accumulator as often as it is filled, the u-th filling of all first, and returns with the last
+// filling's wait done and the sum of all in the accumulator, false where a wait ran out. acc: the warp's lanes; it takes
+// the 32-column groups half, half + 2, ... below ncols.
+template <int CG>
+__device__ __forceinline__ bool drain(const TileArgs& p, uint32_t acc, int half, int ncols, int stages, uint64_t* acc_full,
+                                      uint64_t* acc_empty, int& u) {
+    constexpr int GROUPS = ACC_COLS / 64;
+    if (stages <= DRAIN) return mbar_wait(acc_full, u & 1, p.err);
+    float sum[GROUPS][32] = {};
+#pragma unroll 1
+    for (int left = stages;; left -= DRAIN) {
+        if (!mbar_wait(acc_full, u & 1, p.err)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            if (half * 32 + g * 64 >= ncols) continue;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {  // 16 columns: the sums leave no room for more
+                uint32_t v[16];
+                tmem_ld16(acc + (uint32_t)(half * 32 + g * 64 + h), v);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    asm volatile("" : "+r"(v[e]));  // not before the wait
+                    sum[g][h + e] += __uint_as_float(v[e]);
+                }
+            }
+        }
+        if (left <= DRAIN) break;
+        taken<CG>(acc_empty);
+        ++u;
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        if (half * 32 + g * 64 >= ncols) continue;
+        uint32_t v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(sum[g][e]);
+        tmem_st32(acc + (uint32_t)(half * 32 + g * 64), v);
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    return true;
+}
+
 // AMN, BMN: the operand's output index is contiguous in memory, not the summed one (Split only).
 template <Epi E, typename T, int CG, bool AMN, bool BMN, bool ANY>
 __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_constant__ Args p) {
@@ -212,9 +283,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
         if (lane == 0 && rank == 0) {
             int s = 0, phase = 0;  // the next stage, and whether its ring has come round an odd number of times
             bool ok = true;
-            for (int t = group, i = 0; t < work && ok; t += groups, ++i) {
-                const int b = i % BUFFERS;
-                if (i >= BUFFERS && !mbar_wait(&acc_empty[b], (i / BUFFERS - 1) & 1, p.err)) break;
+            int u = 0;  // accumulators filled
+            for (int t = group; t < work && ok; t += groups, ++u) {
+                const int b = u % BUFFERS;
+                if (u >= BUFFERS && !mbar_wait(&acc_empty[b], (u / BUFFERS - 1) & 1, p.err)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + (uint32_t)(b * ACC_COLS), cross = tmem + ACC_COLS;
                 const Item it = item<E>(p, t);
@@ -229,15 +301,36 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
                     }
                     tc_fence_after();
                     // an MMA's summed elements: 32 bytes along a K-major row, 2 KB of MN-major rows, in units of 16
+                    auto each = [&](auto&& f) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t more = k > it.k0 || q > 0;
-                        const uint64_t oa = q * (AMN ? 128 : 2), ob = q * (BMN ? 128 : 2);
-                        issue<E, CG>(acc, da + oa, db + ob, p.idesc, more);
-                        if constexpr (SPLIT) {
-                            issue<E, CG>(cross, da + oa, lb + ob, p.idesc, more);
+                        for (int q = 0; q < 4; ++q) f(q, (uint64_t)(q * (AMN ? 128 : 2)), (uint64_t)(q * (BMN ? 128 : 2)));
+                    };
+                    const int in = SPLIT ? (k - it.k0) % DRAIN : k - it.k0;  // stages in the accumulator
+                    auto large = [&] {
+                        each([&](int q, uint64_t oa, uint64_t ob) { issue<E, CG>(acc, da + oa, db + ob, p.idesc, in > 0 || q > 0); });
+                    };
+                    auto small = [&] {
+                        each([&](int q, uint64_t oa, uint64_t ob) {
+                            issue<E, CG>(cross, da + oa, lb + ob, p.idesc, k > it.k0 || q > 0);
                             issue<E, CG>(cross, la + oa, db + ob, p.idesc, 1);
+                        });
+                    };
+                    // the accumulator is drained under the cross products before its first stage and after its last
+                    if constexpr (!SPLIT) {
+                        large();
+                    } else if (in > 0 || k == it.k0) {
+                        large();
+                        if (in == DRAIN - 1 && k + 1 < it.k1) pair_commit<CG>(&acc_full[b]);
+                        small();
+                    } else {
+                        small();
+                        if (!mbar_wait(&acc_empty[b], u & 1, p.err)) {
+                            ok = false;
+                            break;
                         }
+                        ++u;
+                        tc_fence_after();
+                        large();
                     }
                     pair_commit<CG>(&empty[s]);
                     if (++s == p.stages) s = 0, phase ^= 1;
@@ -293,8 +386,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
         uint8_t* my_turn = turn + (warp - FIRST_EPI) * (turn_bytes<T>() / EPI_WARPS);
         float* my_columns = columns + (warp - FIRST_EPI) * 64;
         int piece = 0;
-        for (int t = group, i = 0; t < work; t += groups, ++i) {
-            const int b = i % BUFFERS;
+        bool ok = true;
+        for (int t = group, u = 0; t < work; t += groups, ++u) {
+            const int b = u % BUFFERS;
             const Item it = item<E>(p, t);
             const int64_t row0 = (int64_t)(it.mi * CG + rank) * TM + quarter * 32, n0 = (int64_t)it.ni * p.bn;
             const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
@@ -302,7 +396,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
             float scale = 0.0f;
             if constexpr (E == Epi::Int8)
                 if (lane < rows) scale = p.xs[row0 + lane];
-            if (!mbar_wait(&acc_full[b], (i / BUFFERS) & 1, p.err)) break;
+            if constexpr (SPLIT)
+                ok = drain<CG>(p, tmem + ((uint32_t)(quarter * 32) << 16), half, ncols, it.k1 - it.k0, acc_full, acc_empty, u);
+            else ok = mbar_wait(&acc_full[b], (u / BUFFERS) & 1, p.err);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * ACC_COLS);
             float4* partial = p.partial + ((int64_t)it.part * CG + rank) * (ACC_COLS / 4) * TM + quarter * 32 + lane;
@@ -383,12 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
                         }
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2) arrive_cluster(first_cta_addr(&acc_empty[b]));
-                else mbar_arrive(&acc_empty[b]);
-            }
+            taken<CG>(&acc_empty[b]);
         }
         // the stores have read the shared memory they come from before the CTA gives it up
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
