@@ -133,6 +133,19 @@ def test_orthogonalize():
     refused("overlap", xs.orthogonalize, g[:1].expand(4, 8), y)
 
 
+def test_eps_past_fp32():
+    """eps becomes float32 on its way: what is infinite there is refused like an infinity."""
+    x, g, w = t(6, 8), t(4, 8, dtype=f32), t(8, dtype=f32)
+    for eps in (1e39, 1e308, float("inf"), float("nan"), -1e-300):
+        refused("eps must", xs.layer_norm, x, w, w, eps, x)
+        refused("eps must", xs.group_norm, x, 4, w, w, eps, x)
+        refused("eps must", xs.orthogonalize, g, t(4, 8), eps=eps)
+    for eps in (0, 1, 1e-300, 3.4e38):
+        reached(xs.layer_norm, x, w, w, eps, x)
+        reached(xs.group_norm, x, 4, w, w, eps, x)
+        reached(xs.orthogonalize, g, t(4, 8), eps=eps)
+
+
 def test_c_entries_reject_a_null_handle():
     L = _lib.lib()
     for suf in ("f16f16", "bf16bf16", "f32f32", "f32f16", "f32bf16"):

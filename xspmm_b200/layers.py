@@ -11,8 +11,6 @@ before anything runs.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ._lib import check, lib
@@ -70,6 +68,12 @@ def _needed(exec: CudaExecutor, t, name: str, shape, dtype):
     return _dense(exec, t, name, shape, dtype)
 
 
+def _check_eps(eps):
+    """eps is passed on in float32."""
+    if not 0.0 <= eps <= torch.finfo(torch.float32).max:
+        raise ValueError("eps must be finite and non-negative")
+
+
 def _norm_rows(exec: CudaExecutor, t: torch.Tensor, name: str):
     """Checks the first matrix of a layer norm, which has to have features; returns _matrix's."""
     found = _matrix(exec, t, name)
@@ -91,8 +95,7 @@ def layer_norm(exec: CudaExecutor, x: torch.Tensor, weight, bias, eps: float, y:
     y 16 bits. weight and bias: float32 (cols) or None. mean, rstd: float32 (rows), written where
     given. y may be x."""
     suffix = _norm_suffix(x, y)
-    if not (math.isfinite(eps) and eps >= 0):
-        raise ValueError("eps must be finite and non-negative")
+    _check_eps(eps)
     px, ldx = _norm_rows(exec, x, "x")
     rows, cols = x.shape
     py, ldy = _matrix(exec, y, "y", rows, cols)
@@ -229,8 +232,7 @@ def group_norm(exec: CudaExecutor, x: torch.Tensor, groups: int, weight, bias, e
     header for what those out of order mean."""
     suffix, sizes, (px, ldx), (py, ldy), wb, shape = _group_norm(
         exec, x, y, "y", groups, weight, bias, offsets, activation)
-    if not (math.isfinite(eps) and eps >= 0):
-        raise ValueError("eps must be finite and non-negative")
+    _check_eps(eps)
     pm = _dense(exec, mean, "mean", shape, torch.float32)
     pr = _dense(exec, rstd, "rstd", shape, torch.float32)
     check(getattr(lib(), "xspmm_group_norm_" + suffix)(
@@ -302,8 +304,7 @@ def orthogonalize(exec: CudaExecutor, g: torch.Tensor, y: torch.Tensor, steps: i
         raise ValueError(f"orthogonalize takes {g.dtype} to no {y.dtype}")
     if not (isinstance(steps, int) and 0 <= steps <= 100):
         raise ValueError("steps must be a whole number in [0, 100]")
-    if not (math.isfinite(eps) and eps >= 0):
-        raise ValueError("eps must be finite and non-negative")
+    _check_eps(eps)
     pg, ldg = _matrix(exec, g, "g")
     rows, cols = g.shape
     py, ldy = _matrix(exec, y, "y", rows, cols)
