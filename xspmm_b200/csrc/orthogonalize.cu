@@ -187,16 +187,16 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
         __syncwarp();
         tc_fence_after();
     };
-    // The k-th MMAs of a sum. A sum of more than 128 terms (of 128 columns then) goes to two accumulators side by side: an
-    // addition in the tensor core truncates (tile_product.cuh).
-    auto three = [&](uint64_t da, uint64_t la, uint64_t db, uint64_t lb, uint32_t idesc, int k) {
-        tc_mma(tmem + (k < 8 ? 0 : SMALL_ROWS), da, db, idesc, k % 8 > 0);
+    // The k-th MMAs of a sum. With up to 128 columns its second half goes to an accumulator of its own: an addition in the
+    // tensor core truncates (tile_product.cuh).
+    auto three = [&](uint64_t da, uint64_t la, uint64_t db, uint64_t lb, uint32_t idesc, int k, int half) {
+        tc_mma(tmem + (k < half ? 0 : SMALL_ROWS), da, db, idesc, k != 0 && k != half);
         tc_mma(tmem + ACC_COLS, da, lb, idesc, k > 0);
         tc_mma(tmem + ACC_COLS, la, db, idesc, 1);
     };
     // f(row, first column, sums of MMAs' results) for 32 columns at a time of the accumulators' `width`: four warps a
     // quarter of the rows
-    auto results = [&](int width, int mmas, auto&& f) {
+    auto results = [&](int width, bool two, auto&& f) {
         for (int c = (warp >> 2) * 32; c < width; c += SMALL_THREADS / 128 * 32) {
             uint32_t v[32], u[32];
             const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c;
@@ -205,7 +205,7 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
             tmem_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(u[e]));
-            if (mmas > 8) {
+            if (two) {
                 tmem_ld32(at + SMALL_ROWS, u);
                 tmem_wait();
 #pragma unroll
@@ -226,9 +226,9 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
     auto down = [](const uint8_t* p, int k) { return small_desc_mn(smem_u32(p)) + k * 128; };
     for (int i = 0; i < steps; ++i) {
         products([&] {  // A = X X^T
-            for (int k = 0; k < kn; ++k) three(along(xh, k), along(xl, k), along(xh, k), along(xl, k), square, k);
+            for (int k = 0; k < kn; ++k) three(along(xh, k), along(xl, k), along(xh, k), along(xl, k), square, k, (kn + 1) / 2);
         });
-        results(SMALL_ROWS, kn, [&](int r, int c, const uint32_t (&v)[32]) {
+        results(SMALL_ROWS, kn > 1, [&](int r, int c, const uint32_t (&v)[32]) {
 #pragma unroll
             for (int b = 0; b < 32; b += 8) {
                 float t[8];
@@ -238,9 +238,9 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
             }
         });
         products([&] {  // A A
-            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), along(ah, k), along(al, k), square, k);
+            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), along(ah, k), along(al, k), square, k, (km + 1) / 2);
         });
-        results(SMALL_ROWS, km, [&](int r, int c, const uint32_t (&v)[32]) {
+        results(SMALL_ROWS, km > 1, [&](int r, int c, const uint32_t (&v)[32]) {
 #pragma unroll
             for (int b = 0; b < 32; b += 8) {
                 const uint4 h = *reinterpret_cast<const uint4*>(ah + small_at(r, c + b));
@@ -257,9 +257,9 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
             }
         });
         products([&] {  // B' X
-            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), down(xh, k), down(xl, k), wide, k);
+            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), down(xh, k), down(xl, k), wide, k, chunks > 2 ? km : (km + 1) / 2);
         });
-        results(chunks * 64, km, [&](int r, int c, const uint32_t (&v)[32]) {
+        results(chunks * 64, km > 1 && chunks <= 2, [&](int r, int c, const uint32_t (&v)[32]) {
             if (i + 1 < steps) {
 #pragma unroll
                 for (int b = 0; b < 32; b += 8) {
