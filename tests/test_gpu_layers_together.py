@@ -15,6 +15,7 @@ import pytest
 import torch
 
 import xspmm_b200 as xs
+from xspmm_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +170,111 @@ def test_offsets_past_32_bits(executor):
     xs.linear_int8(executor, q, s, w, ws, p)
     xs.linear_int8(executor, q2, s2, w, ws, p2)
     assert torch.equal(p[-300:], p2) and not p[:rows - 300].any()
+
+
+def _calls(ex):
+    """A call of each operator through the C ABI with kernels of every kind, and its outputs; call() returns the statuses."""
+    device, L, h = ex.device, _lib.lib(), ex.handle
+    x = rand(1, 300, 160, dtype=f16).to(device)
+    off = torch.tensor([0, 7, 300], device=device)
+    y, dx, u = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x)
+    q, s = torch.zeros(300, 160, dtype=torch.int8, device=device), torch.zeros(300, device=device)
+    p = torch.zeros(300, 300, dtype=f16, device=device)
+    mean, rstd, dw = (torch.zeros(*n, device=device) for n in ((2, 8), (2, 8), (160,)))
+    a = lambda t: t.data_ptr()  # noqa: E731
+    torch.cuda.synchronize(device)
+
+    def call():
+        return [L.xspmm_group_norm_f16f16(h, 300, 160, 8, 2, a(off), a(x), 160, None, None, 1e-5, 0, a(y), 160, a(mean), a(rstd)),
+                L.xspmm_group_norm_backward_f16f16(h, 300, 160, 8, 2, a(off), a(y), 160, a(x), 160, None, None, a(mean), a(rstd), 0,
+                                                   a(dx), 160, a(dw), None),
+                L.xspmm_quantize_rows_f16(h, 300, 160, a(y), 160, a(q), 160, a(s)),
+                L.xspmm_linear_int8_f16(h, 300, 160, 300, a(q), 160, a(s), a(q), 160, a(s), None, a(p), 300),
+                L.xspmm_orthogonalize_f16f16(h, 300, 160, a(x), 160, 5, 1e-7, a(u), 160)]
+
+    return call, (y, dx, q, s, p, u, mean, rstd, dw, x, off)
+
+
+def test_a_threads_first_cuda_calls(executor):
+    """A host thread that has not touched the GPU has no device's context current; every operator runs from it."""
+    call, here = _calls(executor)
+    other, there = _calls(executor)
+    assert call() == [0] * 5
+    statuses = []
+    thread = threading.Thread(target=lambda: statuses.extend(other()))
+    thread.start()
+    thread.join()
+    assert statuses == [0] * 5, _lib.lib().xspmm_last_error()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(here, there))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_of_another_device_than_the_current_one(executor):
+    call, here = _calls(executor)
+    assert torch.cuda.current_device() == 0
+    other, there = _calls(xs.CudaExecutor(1))
+    assert call() == [0] * 5 and other() == [0] * 5
+    assert torch.cuda.current_device() == 0
+    torch.cuda.synchronize(0)
+    torch.cuda.synchronize(1)
+    assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(here, there))
+
+
+def test_offsets_past_32_bits_in_the_gradient(executor):
+    """The gradient of the last rows of matrices of 2^31 + elements; the rows before are in no sample and stay."""
+    cols, tail = 4096, 300
+    rows = (1 << 31) // cols + tail
+    x, dy = (torch.zeros(rows, cols, dtype=f16, device="cuda") for _ in range(2))
+    small = [rand(k, tail, cols, dtype=f16) for k in (1, 2)]
+    x[-tail:], dy[-tail:] = small
+    mean, rstd = rand(3, 1, 64, scale=0.1), rand(4, 1, 64).abs() + 0.5
+    outs = []
+    for xx, dd, off in ((x, dy, torch.tensor([rows - tail, rows], device="cuda")), (small[0], small[1], None)):
+        dx, dw, db = torch.zeros_like(xx), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+        xs.group_norm_backward(executor, dd, xx, 64, None, None, mean, rstd, dx, dw, db, offsets=off, activation="silu")
+        outs.append((dx, dw, db))
+    (dx, dw, db), (sdx, sdw, sdb) = outs
+    near(dx[-tail:], sdx, 2.0 ** -10)
+    near(dw, sdw, 2.0 ** -18)
+    near(db, sdb, 2.0 ** -18)
+    assert not dx[:rows - tail].any()
+
+
+def test_product_of_more_than_32_bits_of_elements(executor):
+    """y of 2^31 + elements: its last rows are those of the product of the last rows alone."""
+    K, F = 16, 66000
+    rows = (1 << 31) // F + 500
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x, w = (torch.randint(-128, 128, (n, K), generator=g, device="cuda", dtype=torch.int8) for n in (rows, F))
+    s, ws = rand(2, rows), rand(3, F)
+    y, part = torch.empty(rows, F, dtype=f16, device="cuda"), torch.empty(400, F, dtype=f16, device="cuda")
+    xs.linear_int8(executor, x, s, w, ws, y)
+    xs.linear_int8(executor, x[-400:], s[-400:], w, ws, part)
+    assert torch.equal(y[-400:], part)
+
+
+def test_update_of_more_than_32_bits_of_elements(executor):
+    """20 rows of 2^31 / 20 + columns: y = P g with a 20 x 20 matrix P, from g's products with itself."""
+    m, n, slab = 20, (1 << 31) // 20 + 1000, 1 << 22
+    g = torch.empty(m, n, dtype=f16, device="cuda")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    for c in range(0, n, slab):
+        g[:, c:c + slab] = torch.randn(m, min(slab, n - c), generator=gen, device="cuda") * (1.0 + torch.arange(m, device="cuda"))[:, None]
+    y = torch.zeros_like(g)
+    xs.orthogonalize(executor, g, y)
+    a = torch.zeros(m, m, dtype=torch.float64, device="cuda")
+    for c in range(0, n, slab):
+        v = g[:, c:c + slab].double()
+        a += v @ v.t()
+    norm = torch.sqrt(torch.diagonal(a).sum())
+    a /= norm * norm
+    p = torch.eye(m, dtype=torch.float64, device="cuda") / norm
+    for _ in range(5):
+        step = 3.4445 * torch.eye(m, dtype=torch.float64, device="cuda") - 4.7750 * a + 2.0315 * (a @ a)
+        p, a = step @ p, step @ a @ step
+    for c in (0, n // 2, n - 100_000):
+        ref = p @ g[:, c:c + 100_000].double()
+        near(y[:, c:c + 100_000], ref, 2.0 ** -11 + 2.0 ** -13)
