@@ -511,7 +511,9 @@ xspmm_status_t xspmm_dist_plan_destroy(xspmm_dist_plan_t plan);
  *   squares, X_{i+1} = a X_i + (b A + c A A) X_i, A = X_i X_i^T, (a, b, c) = (3.4445, -4.7750, 2.0315):
  *   an odd polynomial of the singular values that drives them to about 1 (0.68 to 1.2 after 5 steps,
  *   where they were not tiny). g fp16, bf16 or fp32; y fp16 or bf16 (the type of a 16-bit g). Products
- *   of 22-bit operands (two fp16 parts each) with fp32 sums: the error is a small part of y's rounding.
+ *   of 22-bit operands (two fp16 parts each) with fp32 sums: the error before y's rounding is about that
+ *   of the steps in fp32 (1.5e-6 of |y| for 128 x 128, 5e-6 for 11008 x 4096), also where |g| is far
+ *   below eps, down to 2^-100 of it.
  *   0 <= steps <= 100; steps = 0: y = X_0. A g of zeros gives zeros (with eps = 0: NaN). An infinity or
  *   NaN in g makes y NaN (steps >= 1). y may be g (same type and stride).
  * ------------------------------------------------------------------------------------------- */

@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import xspmm_b200 as xs
-from test_gpu_orthogonalize import f16, rand, reference
+from test_gpu_orthogonalize import bf16, check, f16, rand, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,14 @@ def test_error_before_the_rounding(executor, rows, cols, strong):
     rounding = square(ref.half().double() - ref)
     error = max(0.0, square(y.double() - ref) - rounding) / square(ref)
     assert error ** 0.5 <= 16.1 * 3 * 2.0 ** -21, error ** 0.5
+
+
+@pytest.mark.parametrize("rows,cols", [(100, 100), (64, 200), (300, 200), (200, 700), (900, 260)])
+@pytest.mark.parametrize("halvings,steps", [(1, 5), (10, 5), (20, 5), (20, 16), (45, 5), (90, 5), (90, 1)])
+def test_gradients_far_below_eps(executor, rows, cols, halvings, steps):
+    """|g| = eps 2^-halvings: X_0 is as small, and every step multiplies it by 3.4445 until it is near 1."""
+    base = rand(4, rows, cols).double()
+    g = (base / torch.linalg.matrix_norm(base) * (1e-7 * 2.0 ** -halvings)).float()
+    y = torch.empty(rows, cols, dtype=bf16, device="cuda")
+    xs.orthogonalize(executor, g, y, steps=steps)
+    check(y, reference(g, steps))

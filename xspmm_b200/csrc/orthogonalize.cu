@@ -8,7 +8,9 @@
 // Precision. A step multiplies small singular values by 3.4445, 485 in five steps, and what rounding X to 16 bits
 // would add to those directions with them. X, A and B' are therefore held as two fp16 parts (22 bits), and the
 // products are those of the parts with fp32 sums, joined from runs of 128 terms (tile_product.cuh). A and B' are symmetric: half of their tiles
-// are computed. The norm is summed in fp64: squares of any fp32 gradient are in its range.
+// are computed. The norm is summed in fp64: squares of any fp32 gradient are in its range. A gradient far below eps makes
+// an X_0 far below 1, of which 2^14 times would lose bits of the parts, or all: step i holds 2^(14 + e_i) X_i, e_i from the
+// bound a^i |X_0| on its entries, 0 as soon as that passes 1/2. A X_0 of norm 2^-100 still has all its bits.
 //
 // 11008 x 4096: 7.75 ms; the three products of the parts' 3.1 TFLOP are 6.73 ms at the sustained bf16 rate. Below about 1000
 // the launches and latencies of fifteen products (768 x 1232: 208 us).
@@ -52,26 +54,43 @@ __global__ void __launch_bounds__(256) squares_kernel(int64_t rows, int64_t cols
     }
 }
 
-// The inverse of the norm, from the partial sums; the same in all threads of the CTA and in all CTAs.
-__device__ __forceinline__ double inverse_norm(const double* part, int parts, float eps) {
-    __shared__ double inv;
+// The norm and 1 / (norm + eps), from the partial sums; the same in all threads of the CTA and in all CTAs.
+__device__ __forceinline__ double2 norm_of(const double* part, int parts, float eps) {
+    __shared__ double norm;
     if (threadIdx.x < 32) {
         double s = 0.0;
         for (int i = threadIdx.x; i < parts; i += 32) s += part[i];
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (threadIdx.x == 0) inv = 1.0 / (sqrt(s) + (double)eps);
+        if (threadIdx.x == 0) norm = sqrt(s);
     }
     __syncthreads();
-    return inv;
+    return make_double2(norm, 1.0 / (norm + (double)eps));
 }
 
-// X_0 in two parts; the padding of its rows becomes zeros.
+// e_i from a^i |X_0|, and the bound of the next step.
+__device__ __forceinline__ int exponent(double* bound) {
+    int x;
+    frexp(*bound, &x);  // below 2^x; 0 and what is not finite: no matter
+    *bound *= (double)NS_A;
+    return max(0, min(100, -x));
+}
+
+// X_0 in two parts; the padding of its rows becomes zeros. mul[i]: what step i's A and its X or y are multiplied by.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 start_kernel(int64_t rows, int64_t cols, const T* g, int64_t ldg, const double* part, int parts, float eps, __half* hi,
-             __half* lo, int64_t ld) {
+             __half* lo, int64_t ld, int steps, float2* mul) {
     cudaGridDependencySynchronize();
-    const double inv = inverse_norm(part, parts, eps);
+    const double2 norm = norm_of(part, parts, eps);
+    double bound = norm.x * norm.y;
+    int at = exponent(&bound);
+    const double inv = norm.y * (double)(ldexpf(SPLIT_SCALE, at));
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        for (int i = 0; i < steps; ++i) {
+            const int next = i + 1 < steps ? exponent(&bound) : 0;
+            mul[i] = make_float2(ldexpf(1.0f, -2 * at), ldexpf(1.0f, next - at));
+            at = next;
+        }
     each_piece<4>(rows, ld, [&](int64_t r, int64_t c) {
         float v[4] = {};
         const T* from = g + r * ldg + c;
@@ -83,7 +102,7 @@ start_kernel(int64_t rows, int64_t cols, const T* g, int64_t ldg, const double* 
                 if (c + e < cols) v[e] = to_float(from[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)(v[e] * inv) * SPLIT_SCALE;
+        for (int e = 0; e < 4; ++e) v[e] = (float)(v[e] * inv);
         uint2 h, l;
         split2(v[0], v[1], &h.x, &l.x);
         split2(v[2], v[3], &h.y, &l.y);
@@ -98,7 +117,7 @@ __global__ void __launch_bounds__(256)
 scaled_kernel(int64_t rows, int64_t cols, const TX* g, int64_t ldg, const double* part, int parts, float eps, TY* y,
               int64_t ldy) {
     cudaGridDependencySynchronize();
-    const double inv = inverse_norm(part, parts, eps);
+    const double inv = norm_of(part, parts, eps).y;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256)
         y[i / cols * ldy + i % cols] = from_float<TY>((float)(to_float(g[i / cols * ldg + i % cols]) * inv));
 }
@@ -152,7 +171,11 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
     s = 0.0;
 #pragma unroll
     for (int i = 0; i < SMALL_THREADS / 32; ++i) s += red[i];
-    const double inv = 1.0 / (sqrt(s) + (double)eps);
+    double bound = sqrt(s);
+    double inv = 1.0 / (bound + (double)eps);
+    bound *= inv;
+    int at = exponent(&bound);
+    inv *= (double)ldexpf(SPLIT_SCALE, at);
     for (int i = threadIdx.x; i < SMALL_ROWS * chunks * 32; i += SMALL_THREADS) {  // two columns of X, zeros outside
         const int r = i % SMALL_ROWS, c = i / SMALL_ROWS * 2;  // neighbouring threads: rows of X
         float v[2];
@@ -160,13 +183,13 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
         for (int e = 0; e < 2; ++e) {
             const bool in = r < m && c + e < n;
             const int64_t from = turned ? (c + e) * ldg + r : r * ldg + c + e;
-            v[e] = in ? (float)(to_float(g[from]) * inv) * SPLIT_SCALE : 0.0f;
+            v[e] = in ? (float)(to_float(g[from]) * inv) : 0.0f;
         }
         uint32_t hi, lo;
         split2(v[0], v[1], &hi, &lo);
-        const int at = small_at(r, c & ~7) + (c & 7) * 2;
-        *reinterpret_cast<uint32_t*>(xh + at) = hi;
-        *reinterpret_cast<uint32_t*>(xl + at) = lo;
+        const int place = small_at(r, c & ~7) + (c & 7) * 2;
+        *reinterpret_cast<uint32_t*>(xh + place) = hi;
+        *reinterpret_cast<uint32_t*>(xl + place) = lo;
     }
     int phase = 0;
     uint32_t tmem = 0;
@@ -225,6 +248,9 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
     auto along = [](const uint8_t* p, int k) { return desc_k(smem_u32(p) + (k >> 2) * SMALL_CHUNK) + (k & 3) * 2; };
     auto down = [](const uint8_t* p, int k) { return small_desc_mn(smem_u32(p)) + k * 128; };
     for (int i = 0; i < steps; ++i) {
+        const int next = i + 1 < steps ? exponent(&bound) : 0;
+        const float square_mul = ldexpf(1.0f, -2 * at), mul = ldexpf(1.0f, next - at);
+        at = next;
         products([&] {  // A = X X^T
             for (int k = 0; k < kn; ++k) three(along(xh, k), along(xl, k), along(xh, k), along(xl, k), square, k, (kn + 1) / 2);
         });
@@ -233,7 +259,7 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
             for (int b = 0; b < 32; b += 8) {
                 float t[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Gram>(__uint_as_float(v[b + e]), 0.0f, false);
+                for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Gram>(__uint_as_float(v[b + e]), 0.0f, false, square_mul);
                 put(ah, al, r, c + b, t);
             }
         });
@@ -250,8 +276,8 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     const float2 fh = unpack2(hw[e / 2], __half()), fl = unpack2(lw[e / 2], __half());
-                    t[e] = finish<Epi::Poly>(__uint_as_float(v[b + e]), fh.x + fl.x, r == c + b + e);
-                    t[e + 1] = finish<Epi::Poly>(__uint_as_float(v[b + e + 1]), fh.y + fl.y, r == c + b + e + 1);
+                    t[e] = finish<Epi::Poly>(__uint_as_float(v[b + e]), fh.x + fl.x, r == c + b + e, 1.0f);
+                    t[e + 1] = finish<Epi::Poly>(__uint_as_float(v[b + e + 1]), fh.y + fl.y, r == c + b + e + 1, 1.0f);
                 }
                 put(ah, al, r, c + b, t);
             }
@@ -265,7 +291,7 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
                 for (int b = 0; b < 32; b += 8) {
                     float t[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Next>(__uint_as_float(v[b + e]), 0.0f, false);
+                    for (int e = 0; e < 8; ++e) t[e] = finish<Epi::Next>(__uint_as_float(v[b + e]), 0.0f, false, mul);
                     put(xh, xl, r, c + b, t);
                 }
             } else if (r < m) {
@@ -273,7 +299,7 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
                 const int64_t next = turned ? ldy : 1;
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                    if (c + e < n) to[e * next] = from_float<TY>(__uint_as_float(v[e]) * (SPLIT_INV * SPLIT_INV));
+                    if (c + e < n) to[e * next] = from_float<TY>(finish<Epi::Last>(__uint_as_float(v[e]), 0.0f, false, mul));
             }
         });
     }
@@ -295,9 +321,10 @@ struct Parts {
 
 // out = the product of P and Q (P Q^T, with AMN P^T, with BMN Q) finished by E; y instead of `out` for Last.
 template <Epi E, typename T, int CG, bool AMN, bool BMN>
-void multiply(Handle& h, int64_t M, int64_t N, int64_t K, const Parts& P, const Parts& Q, const Parts* out,
+void multiply(Handle& h, int64_t M, int64_t N, int64_t K, const Parts& P, const Parts& Q, const float* mul, const Parts* out,
               const Parts* A, T* y, int64_t ldy) {
     Args t = {};
+    t.mul = mul;
     t.M = M;
     t.N = out ? out->ld : N;
     t.ksteps = (int)ceil_div(K, 64);
@@ -317,10 +344,10 @@ void multiply(Handle& h, int64_t M, int64_t N, int64_t K, const Parts& P, const 
     launch<E, T, CG, AMN, BMN>(h, t);
 }
 template <Epi E, typename T, bool AMN, bool BMN>
-void multiply(Handle& h, int64_t M, int64_t N, int64_t K, const Parts& P, const Parts& Q, const Parts* out,
+void multiply(Handle& h, int64_t M, int64_t N, int64_t K, const Parts& P, const Parts& Q, const float* mul, const Parts* out,
               const Parts* A = nullptr, T* y = nullptr, int64_t ldy = 0) {
-    if (M > TM) multiply<E, T, 2, AMN, BMN>(h, M, N, K, P, Q, out, A, y, ldy);
-    else multiply<E, T, 1, AMN, BMN>(h, M, N, K, P, Q, out, A, y, ldy);
+    if (M > TM) multiply<E, T, 2, AMN, BMN>(h, M, N, K, P, Q, mul, out, A, y, ldy);
+    else multiply<E, T, 1, AMN, BMN>(h, M, N, K, P, Q, mul, out, A, y, ldy);
 }
 
 }  // namespace
@@ -356,6 +383,7 @@ void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t l
     }
     const bool tall = rows > cols;
     const int64_t m = std::min(rows, cols), ldx = ceil_div(cols, 8) * 8, lda = ceil_div(m, 8) * 8;
+    DevBuf<float2> muls((size_t)steps, h.stream);
     DevBuf<__half> buf((size_t)(4 * rows * ldx + 4 * m * lda), h.stream);
     __half* at = buf.get();
     auto take = [&](int64_t r, int64_t c, int64_t ld) {
@@ -365,19 +393,20 @@ void orthogonalize(Handle& h, int64_t rows, int64_t cols, const TX* g, int64_t l
     };
     Parts X = take(rows, cols, ldx), next = take(rows, cols, ldx), A = take(m, m, lda), B = take(m, m, lda);
     launch_dependent(h.stream, wide ? start_kernel<TX, 4> : start_kernel<TX, 1>, (unsigned)parts, 256, 0, 1, rows, cols, g, ldg,
-                     part.get(), parts, eps, X.hi, X.lo, ldx);
+                     part.get(), parts, eps, X.hi, X.lo, ldx, steps, muls.get());
     after_launch(h, "update_start");
     for (int i = 0; i < steps; ++i) {
-        if (tall) multiply<Epi::Gram, __half, true, true>(h, m, m, rows, X, X, &A);
-        else multiply<Epi::Gram, __half, false, false>(h, m, m, cols, X, X, &A);
-        multiply<Epi::Poly, __half, false, false>(h, m, m, m, A, A, &B, &A);
+        const float *square = reinterpret_cast<const float*>(muls.get() + i), *mul = square + 1;
+        if (tall) multiply<Epi::Gram, __half, true, true>(h, m, m, rows, X, X, square, &A);
+        else multiply<Epi::Gram, __half, false, false>(h, m, m, cols, X, X, square, &A);
+        multiply<Epi::Poly, __half, false, false>(h, m, m, m, A, A, nullptr, &B, &A);
         if (i + 1 == steps) {
-            if (tall) multiply<Epi::Last, TY, false, false>(h, rows, m, m, X, B, nullptr, nullptr, y, ldy);
-            else multiply<Epi::Last, TY, false, true>(h, m, cols, m, B, X, nullptr, nullptr, y, ldy);
+            if (tall) multiply<Epi::Last, TY, false, false>(h, rows, m, m, X, B, mul, nullptr, nullptr, y, ldy);
+            else multiply<Epi::Last, TY, false, true>(h, m, cols, m, B, X, mul, nullptr, nullptr, y, ldy);
         } else if (tall) {
-            multiply<Epi::Next, __half, false, false>(h, rows, m, m, X, B, &next);
+            multiply<Epi::Next, __half, false, false>(h, rows, m, m, X, B, mul, &next);
         } else {
-            multiply<Epi::Next, __half, false, true>(h, m, cols, m, B, X, &next);
+            multiply<Epi::Next, __half, false, true>(h, m, cols, m, B, X, mul, &next);
         }
         std::swap(X, next);
     }

@@ -20,7 +20,7 @@
 // accumulator it was 1e-4 (at 1 % less time; DRAIN = 4: 9e-6; 768 x 1232: 3e-6 in 228 us, 5e-6 in 221, 7e-6 in 210).
 //
 // The entries of X, A and B' (orthogonalize.cu) are below 4 in magnitude, so 2^14 times them fits fp16, and parts
-// down to 2^-38 are held.
+// down to 2^-38 are held. An X of small norm is held with a larger power of two.
 #pragma once
 
 #include "gated_tc.cuh"
@@ -47,6 +47,7 @@ struct Args : TileArgs {
     const float *xs, *ws, *bias;  // Int8
     const __half *ah, *al;        // Poly: A's parts, row stride lda
     int64_t lda;
+    const float* mul;             // the others of Split: a power of two that the results are multiplied by
 };
 
 constexpr int COLUMN_BYTES = EPI_WARPS * 64 * 4;  // Int8: a warp's 32 column scales and biases
@@ -118,12 +119,14 @@ __device__ __forceinline__ void split2(float v0, float v1, uint32_t* hi, uint32_
     *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// An accumulator's value (2^28 times the product's) as 2^14 times the result; `a` is 2^14 times A's entry.
+// An accumulator's value (2^28 times the product's, before `mul`) as 2^14 times the result, for Last as the result itself;
+// `a` is 2^14 times A's entry.
 template <Epi E>
-__device__ __forceinline__ float finish(float acc, float a, bool diagonal) {
+__device__ __forceinline__ float finish(float acc, float a, bool diagonal, float mul) {
     if constexpr (E == Epi::Poly)
         return fmaf(NS_B, a, NS_C * (acc * SPLIT_INV)) + (diagonal ? NS_A * SPLIT_SCALE : 0.0f);
-    else return acc * SPLIT_INV;
+    else if constexpr (E == Epi::Last) return acc * (SPLIT_INV * SPLIT_INV) * mul;
+    else return acc * SPLIT_INV * mul;
 }
 
 // fp32 results (lane = row, 32 columns) to `out`, through a staging piece of 32 rows of 128 bytes.
@@ -387,6 +390,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
         float* my_columns = columns + (warp - FIRST_EPI) * 64;
         int piece = 0;
         bool ok = true;
+        float mul = 1.0f;
+        if constexpr (SPLIT && E != Epi::Poly) mul = *p.mul;
         for (int t = group, u = 0; t < work; t += groups, ++u) {
             const int b = u % BUFFERS;
             const Item it = item<E>(p, t);
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
                 } else if constexpr (E == Epi::Last) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * (SPLIT_INV * SPLIT_INV));
+                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(finish<E>(__uint_as_float(v[e]), 0.0f, false, mul));
                     pack_words<T>(w, v);
                     store_group<T, ANY>(p, 0, my_turn, piece, w, row0, n0 + c, rows, cols);
                 } else {
@@ -467,8 +472,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_product_kernel(const __grid_c
                         float2 a = make_float2(0.0f, 0.0f);
                         if constexpr (E == Epi::Poly) a = add2(unpack2(hi[e], __half()), unpack2(lo[e], __half()));
                         const int64_t d = row - (n0 + c + 2 * e);
-                        split2(finish<E>(__uint_as_float(v[2 * e]), a.x, d == 0),
-                               finish<E>(__uint_as_float(v[2 * e + 1]), a.y, d == 1), &hi[e], &lo[e]);
+                        split2(finish<E>(__uint_as_float(v[2 * e]), a.x, d == 0, mul),
+                               finish<E>(__uint_as_float(v[2 * e + 1]), a.y, d == 1, mul), &hi[e], &lo[e]);
                     }
                     store_group<__half, false>(p, 0, my_turn, piece, hi, row0, n0 + c, rows, cols);
                     store_group<__half, false>(p, 1, my_turn, piece, lo, row0, n0 + c, rows, cols);
@@ -541,11 +546,11 @@ __global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ 
             static_cast<T*>(p.out[0])[row * p.ld[0] + col] =
                 from_float<T>(fmaf(v * p.xs[row], p.ws[col], p.bias ? p.bias[col] : 0.0f));
         } else if constexpr (E == Epi::Last) {
-            static_cast<T*>(p.out[0])[row * p.ld[0] + col] = from_float<T>(v * (SPLIT_INV * SPLIT_INV));
+            static_cast<T*>(p.out[0])[row * p.ld[0] + col] = from_float<T>(finish<E>(v, 0.0f, false, *p.mul));
         } else {
             float a = 0.0f;
             if constexpr (E == Epi::Poly) a = to_float(p.ah[row * p.lda + col]) + to_float(p.al[row * p.lda + col]);
-            const float f = finish<E>(v, a, row == col);
+            const float f = finish<E>(v, a, row == col, E == Epi::Poly ? 1.0f : *p.mul);
             const __half hi = __float2half_rn(f);
             static_cast<__half*>(p.out[0])[row * p.ld[0] + col] = hi;
             static_cast<__half*>(p.out[1])[row * p.ld[1] + col] = __float2half_rn(f - __half2float(hi));
