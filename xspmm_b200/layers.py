@@ -259,7 +259,7 @@ def group_norm_backward(exec: CudaExecutor, dy: torch.Tensor, x: torch.Tensor, g
 
 
 def quantize_rows(exec: CudaExecutor, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
-    """Rows of x in 8-bit integers: scale = max|x| / 127 of each row (float32), q = x / scale rounded to
+    """Rows of x in 8-bit integers: scale = max|x| / 127 of each row (float32), q = 127 x / max|x| rounded to
     the nearest (int8, of x's shape). A row of zeros has scale 0, one with an infinity or NaN scale NaN."""
     if x.dtype not in _VAL:
         raise ValueError(f"quantize_rows takes no {x.dtype}")
@@ -274,8 +274,10 @@ def quantize_rows(exec: CudaExecutor, x: torch.Tensor, q: torch.Tensor, scale: t
 def linear_int8(exec: CudaExecutor, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor,
                 w_scale: torch.Tensor, y: torch.Tensor, bias=None) -> None:
     """y = (x @ w.T) * x_scale[:, None] * w_scale + bias: x (rows x K) and w (F x K) int8, as
-    quantize_rows makes them of activations and of a weight; the sum is exact. y (rows x F) float16,
-    bfloat16 or float32; x_scale (rows), w_scale (F) and bias (F, or None) float32."""
+    quantize_rows makes them of activations and of a weight; the sum is exact. Operands whose rows start on
+    16 bytes (the first row and the stride) are read in place, others of more than 16 rows of x are copied
+    in every call: a weight with K no multiple of 16 is best kept as a slice of padded rows. y (rows x F)
+    float16, bfloat16 or float32; x_scale (rows), w_scale (F) and bias (F, or None) float32."""
     if y.dtype not in _VAL:
         raise ValueError(f"linear_int8 gives no {y.dtype}")
     px, ldx = _matrix(exec, x, "x", None, None, torch.int8)
