@@ -1,5 +1,6 @@
 // capi_layers.cu -- extern "C" entry points of the layer operators (include/xspmm_b200.h): layer
-// norm, group norm, dropout, gated feed-forward, 8-bit rows and their product, orthogonalised updates. Validates arguments; the kernels see only valid ones.
+// norm, group norm, dropout, gated feed-forward, 8-bit rows and their product, orthogonalised updates.
+// Validates arguments; the kernels see only valid ones.
 #include "layers.cuh"
 
 #include <cmath>

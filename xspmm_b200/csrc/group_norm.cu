@@ -12,10 +12,11 @@
 //     is not launched where no sample can be long.
 // Long samples are bound by DRAM in the first pass (2^20 x 128 fp32: 88 us, 6.1 TB/s) and by the activation's instructions
 // and their latency in the second (silu, to fp16: 165 us for 786 MB; issue in 43 % of the cycles). Short ones are bound by
-// instructions (4096 samples of 2^18 x 256 bf16, gelu: 113 us, 41 at the copy bandwidth; 33 warp instructions for each value
+// instructions (4096 samples of 2^18 x 256 bf16, gelu: 117 us, 41 at the copy bandwidth; 33 warp instructions for each value
 // of a lane, issue in 63 % of the cycles). More CTAs of fewer registers an SM, or fewer of more slots, were not faster.
 // Moments are joined from those of batches of rows that a thread holds in registers, each taken about its own mean, so
-// neither a large mean nor rows far from the others cost accuracy; all orders are fixed by the sizes and offsets.
+// neither a large mean nor rows far from the others cost accuracy; means are joined about one of them, so equal values have
+// that mean exactly, of any size. All orders are fixed by the sizes and offsets.
 #include "group_norm.cuh"
 
 namespace xspmm_b200 {

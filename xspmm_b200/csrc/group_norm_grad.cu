@@ -10,8 +10,8 @@
 // order and in 64 bits by the last kernel; a block of several tiles has no room for them and adds them to its CTA's row
 // as it goes.
 //
-// 2^20 x 128 fp16, relu: 246 us (206 for both inputs read twice at the copy bandwidth), DRAM at 5.1 and 5.3 TB/s. 4096 samples
-// of 2^18 x 256 bf16, silu: 215 to 230 us (62), bound by instructions: 44 for each value of a lane, issue in 46 % of the cycles,
+// 2^20 x 128 fp16, relu: 256 us (206 for both inputs read twice at the copy bandwidth), DRAM at 5.1 and 5.3 TB/s. 4096 samples
+// of 2^18 x 256 bf16, silu: 223 to 228 us (62), bound by instructions: 44 for each value of a lane, issue in 46 % of the cycles,
 // misses of the instruction cache the most frequent wait. The slope is computed in both passes: dz would take half as much
 // shared memory again, and fewer samples would stay there.
 #include "group_norm.cuh"
@@ -138,7 +138,8 @@ __device__ __forceinline__ void each_row(const Backward<TX, TY>& p, const Team<C
 // there by channel. The strips may be written again after a team_sync.
 template <bool CTA, Rows HOW, typename TX, typename TY, int V, int U, typename F, typename C>
 __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm,
-                                           const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, const Totals<V * U / 2>& total,
+                                           const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end,
+                                           const Channels<V * U / 2>& ch, const Totals<V * U / 2>& total,
                                            Strips& sh, F&& f, C&& channels) {
     constexpr int P = V * U / 2;
     Sums<P> s;
@@ -183,7 +184,8 @@ __device__ __forceinline__ void group_sums(const Backward<TX, TY>& p, const Team
 // dx of rows [begin, end) from the groups' minus m1 and minus m2.
 template <bool CTA, Rows HOW, bool BACK, typename TX, typename TY, int V, int U>
 __device__ __forceinline__ void apply(const Backward<TX, TY>& p, const Team<CTA, V, U>& tm,
-                                      const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end, const Channels<V * U / 2>& ch, const float* g1, const float* g2) {
+                                      const Pairs<TX, TY, V, U>& slots, const Tile& k, int begin, int end,
+                                      const Channels<V * U / 2>& ch, const float* g1, const float* g2) {
     constexpr int P = V * U / 2;
     float2 m1[P], m2[P];
     tm.of_groups(m1, g1, k);
@@ -234,7 +236,8 @@ __device__ __forceinline__ void leave_weights(const Backward<TX, TY>& p, int64_t
 // A sample by a team. KEEP: it is one tile and fits the slots. `total` is the CTA's sums where a block is one tile; else
 // they go to the CTA's row.
 template <bool CTA, bool KEEP, typename TX, typename TY, int V, int U>
-__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, const Pairs<TX, TY, V, U>& slots, int s, Span rows, int block, int64_t row,
+__device__ __forceinline__ void whole_sample(const Backward<TX, TY>& p, const Pairs<TX, TY, V, U>& slots, int s, Span rows, int block,
+                                             int64_t row,
                                              Channels<V * U / 2>& ch, const Totals<V * U / 2>& total, Strips& sh, float* g1,
                                              float* g2) {
     const int tpg = KEEP ? 1 : p.t.tpg, t0 = block * tpg;

@@ -3,7 +3,7 @@
 // Quantisation: scale = max|x| / 127, q = 127 x / max|x| rounded to the nearest whole number, ties to even, of
 // the exact quotient. Product: y[r, f] = xs[r] * ws[f] * sum_k x[r, k] w[f, k] + bias[f], the sum exact in 32 bits.
 //
-// 2048 rows of 4096 -> 11008, to bf16: 77 us (2.4 POP/s; the library's product without scales 65), bound by the loads into
+// 2048 rows of 4096 -> 11008, to bf16: 78 us (2.4 POP/s; the library's product without scales 65), bound by the loads into
 // each SM, 64 bytes a clock. One row: 9.4 us, 73 % of the copy bandwidth.
 #include "tile_product.cuh"
 
@@ -64,8 +64,9 @@ __device__ __forceinline__ uint32_t row_most(uint32_t v, int tpr) {
 
 // tpr threads a row, a power of two: part of a warp, or a CTA of that many. A thread takes V consecutive elements at a
 // time, HELD in registers (the loads of a row are all in flight together and x is read once; with 8 instead of 16 what a
-// thread does once a row weighs more: 2^20 x 128 fp16 163 us, with 16 108); HELD = 0: longer rows, read again for the second pass. Bound by memory where rows start on 16 bytes (2^20 x 128 fp32: 132 us, 103
-// at the copy bandwidth); by the instructions of narrow loads and stores elsewhere.
+// thread does once a row weighs more: 2^20 x 128 fp16 163 us, with 16 108); HELD = 0: longer rows, read again for the
+// second pass. Bound by memory where rows start on 16 bytes (2^20 x 128 fp32: 132 to 146 us, 103 at the copy bandwidth);
+// by the instructions of narrow loads and stores elsewhere.
 template <typename T, int V, int HELD>
 __global__ void __launch_bounds__(HELD == 16 ? Q_THREADS : 512)
 quantize_kernel(int64_t rows, int cols, int tpr_log, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
@@ -148,7 +149,7 @@ __device__ __forceinline__ uint4 load_bytes(const int8_t* src, int64_t valid, ui
 }
 
 // ---- a few rows: the weight's bytes, each used once ------------------------------------------------
-// A CTA takes 16 features, its four warps interleaved 128-byte slices of the sum. The weight goes from memory
+// A CTA takes 16 features, its eight warps interleaved 128-byte slices of the sum. The weight goes from memory
 // straight to registers as the A operand of mma.sync m16n8k32 (16 features; the tokens are the 8 columns). The
 // sum's order is free, so a lane loads 32 contiguous bytes of a weight row (four lanes: a 128-byte line) and hands
 // them to four MMAs as if they were the k positions the fragment layout asks for; x is loaded in the same order.
@@ -352,13 +353,13 @@ void linear_int8(Handle& h, const Int8Args& a, T* y, int64_t ldy) {
         const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.rows * a.F, 256), 8 * sm_count(h.device));
         launch_dependent(h.stream, bias_kernel<T>, grid, 256, 0, 1, a.rows, a.F, a.bias, y, ldy);
         after_launch(h, "int8_bias");
-    } else if (a.rows <= 16) {
+    } else if (a.rows <= 16) {  // 4096 -> 11008: 16 rows 15.0 us (tiles 20.2), 9 rows 13.1 (19.1), 17 rows by tiles 20.3
         const bool vec = a.K % 16 == 0 && tma_bytes(a.w, a.F > 1 ? a.ldw : 0) && tma_bytes(a.x, a.rows > 1 ? a.ldx : 0);
         auto kern = a.rows <= 8 ? (vec ? few_rows_int8_kernel<T, 1, true> : few_rows_int8_kernel<T, 1, false>)
                                 : (vec ? few_rows_int8_kernel<T, 2, true> : few_rows_int8_kernel<T, 2, false>);
         launch_dependent(h.stream, kern, (unsigned)ceil_div(a.F, 16), 32 * FEW_WARPS, 0, 1, a, y, ldy);
         after_launch(h, "int8_few_rows");
-    } else if (a.rows <= product::TM) {
+    } else if (a.rows <= product::TM) {  // 128 rows 15.3 us (pairs 17.5), 129 rows by pairs 17.5 (single CTAs 16.1)
         tiles<T, 1>(h, a, y, ldy);
     } else {
         tiles<T, 2>(h, a, y, ldy);

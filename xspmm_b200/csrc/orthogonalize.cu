@@ -1,19 +1,21 @@
 // orthogonalize.cu -- the orthogonalised update of a weight matrix by Newton-Schulz steps.
 //
 // X = g / (|g| + eps), then `steps` times X <- B' X, B' = a I + b A + c A A, A = X X^T, taken on the smaller side:
-// for more rows than columns X <- X B' with A = X^T X. The polynomial p(s) = a s + b s^3 + c s^5 acts on the
+// for more rows than columns X <- X B' with A = X^T X. The coefficients (a, b, c) = (3.4445, -4.7750, 2.0315) were
+// published by K. Jordan and others in 2024 with this use of the iteration. The polynomial p(s) = a s + b s^3 + c s^5 acts on the
 // singular values, which start in [0, 1]; it is at most 1.2025 there (at s = 0.5545) and maps [0, 1.2025] into
 // itself, so every entry of X stays below 1.21, of A below 1.45 and of B' (eigenvalues in [0.63, 3.4445]) below 3.45.
 //
 // Precision. A step multiplies small singular values by 3.4445, 485 in five steps, and what rounding X to 16 bits
 // would add to those directions with them. X, A and B' are therefore held as two fp16 parts (22 bits), and the
-// products are those of the parts with fp32 sums, joined from runs of 128 terms (tile_product.cuh). A and B' are symmetric: half of their tiles
-// are computed. The norm is summed in fp64: squares of any fp32 gradient are in its range. A gradient far below eps makes
-// an X_0 far below 1, of which 2^14 times would lose bits of the parts, or all: step i holds 2^(14 + e_i) X_i, e_i from the
-// bound a^i |X_0| on its entries, 0 as soon as that passes 1/2. A X_0 of norm 2^-100 still has all its bits.
+// products are those of the parts with fp32 sums, joined from runs of at most 128 terms (tile_product.cuh): the error
+// before y's rounding is about that of the steps in fp32. A and B' are symmetric: half of their tiles are computed. The
+// norm is summed in fp64: squares of any fp32 gradient are in its range. A gradient far below eps makes an X_0 far below
+// 1, of which 2^14 times would lose bits of the parts, or all: step i holds 2^(14 + e_i) X_i, e_i from the bound
+// a^i |X_0| on its entries, 0 as soon as that passes 1/2. An X_0 of norm 2^-100 still has all its bits.
 //
-// 11008 x 4096: 7.75 ms; the three products of the parts' 3.1 TFLOP are 6.73 ms at the sustained bf16 rate. Below about 1000
-// the launches and latencies of fifteen products (768 x 1232: 208 us).
+// 11008 x 4096: 7.8 to 8.1 ms; the three products of the parts' 3.1 TFLOP are 6.73 ms at the sustained bf16 rate. Below about 1000
+// the launches and latencies of fifteen products (768 x 1232: 228 us).
 #include "tile_product.cuh"
 
 namespace xspmm_b200 {
@@ -127,7 +129,8 @@ scaled_kernel(int64_t rows, int64_t cols, const TX* g, int64_t ldg, const double
 // stay in shared memory in two parts, in the SWIZZLE_128B layout: 64-column chunks of 128 rows of 128 bytes. Read along
 // its rows a chunk is a K-major operand, along its columns an MN-major one, so X serves both products. A is replaced by
 // B' in place and X by its successor, each after the MMAs that read it. Bound by the latency of 3 products a step, their
-// MMAs on 1 of 148 SMs and the epilogues between (128 x 128, 5 steps: 61 us; 17 launches of the large path took 107).
+// MMAs on 1 of 148 SMs and the epilogues between (128 x 128, 5 steps: 64 us, on the large path 111; 100 x 200 75 and 121;
+// 128 x 256, the largest that fits, 107 and 121).
 constexpr int SMALL_THREADS = 512, SMALL_ROWS = 128, SMALL_COLS = 256;
 constexpr int SMALL_CHUNK = SMALL_ROWS * 128;
 
@@ -283,7 +286,8 @@ small_update_kernel(int rows, int cols, const TX* g, int64_t ldg, int steps, flo
             }
         });
         products([&] {  // B' X
-            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), down(xh, k), down(xl, k), wide, k, chunks > 2 ? km : (km + 1) / 2);
+            const int half = chunks > 2 ? km : (km + 1) / 2;
+            for (int k = 0; k < km; ++k) three(along(ah, k), along(al, k), down(xh, k), down(xl, k), wide, k, half);
         });
         results(chunks * 64, km > 1 && chunks <= 2, [&](int r, int c, const uint32_t (&v)[32]) {
             if (i + 1 < steps) {

@@ -113,7 +113,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// ---- host: 2-D tensor maps, of 16-bit elements unless another type is given -------------------------------------------------------
+// ---- host: 2-D tensor maps, of 16-bit elements unless another type is given ------------------------
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
