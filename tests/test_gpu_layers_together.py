@@ -278,3 +278,41 @@ def test_update_of_more_than_32_bits_of_elements(executor):
     for c in (0, n // 2, n - 100_000):
         ref = p @ g[:, c:c + 100_000].double()
         near(y[:, c:c + 100_000], ref, 2.0 ** -11 + 2.0 ** -13)
+
+
+def test_two_captured_graphs_at_once(executor):
+    """Graphs of the same calls on different inputs, replayed side by side on two streams: each has its own scratch."""
+    jobs = []
+    for seed in (1, 2):
+        x = rand(seed, 30000, 64, dtype=f16)
+        g = rand(seed + 2, 400, 530, dtype=f16)
+        off = torch.tensor([0, 7, 20000, 29990], device="cuda")
+        y, dx, u = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(g)
+        q, s = torch.empty(400, 530, dtype=torch.int8, device="cuda"), torch.empty(400, device="cuda")
+        p = torch.empty(400, 400, dtype=f16, device="cuda")
+        mean, rstd, dw = torch.zeros(3, 8, device="cuda"), torch.zeros(3, 8, device="cuda"), torch.zeros(64, device="cuda")
+
+        def call(x=x, g=g, off=off, y=y, dx=dx, u=u, q=q, s=s, p=p, mean=mean, rstd=rstd, dw=dw):
+            xs.group_norm(executor, x, 8, None, None, 1e-5, y, offsets=off, activation="silu", mean=mean, rstd=rstd)
+            xs.group_norm_backward(executor, y, x, 8, None, None, mean, rstd, dx, dw, offsets=off, activation="silu")
+            xs.quantize_rows(executor, g, q, s)
+            xs.linear_int8(executor, q, s, q, s, p)
+            xs.orthogonalize(executor, g, u)
+
+        call()
+        outs = (y, dx, u, q, s, p, mean, rstd, dw)
+        want = [t.clone() for t in outs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        for t in outs:
+            t.zero_()
+        jobs.append((graph, torch.cuda.Stream(), outs, want, call))  # call keeps the inputs that the graph reads
+    torch.cuda.synchronize()
+    for _ in range(40):
+        for graph, stream, _, _, _ in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, outs, want, _ in jobs:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
